@@ -2,6 +2,7 @@
 // Every op runs on the caller's current CUDA stream and raises on a launch or
 // argument error, so a missing or failing kernel is never silently replaced.
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
 #include <cstring>
@@ -502,6 +503,196 @@ void paged_prefill(const at::Tensor& q, at::Tensor& out, const at::Tensor& arena
   }
 }
 
+// ------------------------------------------------------------------ 8-bit KV arena
+void check_same_device(const at::Tensor& t, const at::Tensor& ref, const char* name) {
+  TORCH_CHECK(t.is_cuda() && t.device() == ref.device(), name, " must be on ", ref.device(), ", got ", t.device());
+}
+
+void check_kv8_arena(const at::Tensor& arena, int64_t layer, int64_t n_kv_heads) {
+  TORCH_CHECK(arena.is_cuda() && arena.scalar_type() == at::kByte && arena.dim() == 5 && arena.is_contiguous(),
+              "an 8-bit KV arena is a contiguous uint8 CUDA tensor [blocks, layers, kv_heads, 2, 2064]");
+  TORCH_CHECK(arena.size(3) == 2 && arena.size(4) == 2064,
+              "8-bit KV arena: head_dim must be 128 and pages 16 tokens (last sizes 2, 2064)");
+  TORCH_CHECK(arena.size(2) == n_kv_heads, "kv heads mismatch: ", n_kv_heads, " for an arena of ", arena.size(2));
+  TORCH_CHECK(layer >= 0 && layer < arena.size(1), "layer ", layer, " of an arena of ", arena.size(1));
+  check_aligned(arena, "arena");
+}
+
+lakeb::Kv8RowArgs kv8_row_args(const at::Tensor& k, const at::Tensor& v, const at::Tensor& slots,
+                               const at::Tensor& arena, int64_t layer, const c10::optional<at::Tensor>& status) {
+  check_bf16_2d(k, "k");
+  check_bf16_2d(v, "v");
+  TORCH_CHECK(k.size(1) % 128 == 0 && k.sizes() == v.sizes(), "k and v are [rows, kv_heads * 128], got ", k.sizes(),
+              " and ", v.sizes());
+  check_kv8_arena(arena, layer, k.size(1) / 128);
+  TORCH_CHECK(slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.is_contiguous() &&
+                  slots.size(0) == k.size(0),
+              "slots int64 [rows]");
+  check_same_device(k, arena, "k");
+  check_same_device(v, arena, "v");
+  check_same_device(slots, arena, "slots");
+  TORCH_CHECK(k.size(0) < (int64_t(1) << 31), "too many rows");
+  lakeb::Kv8RowArgs a;
+  a.k_stride = k.stride(0);
+  a.v_stride = v.stride(0);
+  a.slots = slots.data_ptr<int64_t>();
+  a.arena = arena.data_ptr<uint8_t>();
+  a.num_blocks = arena.size(0);
+  a.block_bytes = arena.stride(0);
+  a.layer_offset = layer * arena.stride(1);
+  a.rows = static_cast<int>(k.size(0));
+  a.heads = static_cast<int>(arena.size(2));
+  a.status = status_ptr(status);
+  return a;
+}
+
+void kv8_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& slots, at::Tensor& arena, int64_t layer,
+               c10::optional<at::Tensor> status) {
+  lakeb::Kv8RowArgs a = kv8_row_args(k, v, slots, arena, layer, status);
+  a.k = bf(k);
+  a.v = bf(v);
+  const c10::cuda::CUDAGuard guard(arena.device());
+  LAKEB_CHECK_RC(lakeb::kv8_write(a, cur_stream()), "kv8_write");
+}
+
+void kv8_read(const at::Tensor& arena, int64_t layer, const at::Tensor& slots, at::Tensor& k_out, at::Tensor& v_out,
+              c10::optional<at::Tensor> status) {
+  lakeb::Kv8RowArgs a = kv8_row_args(k_out, v_out, slots, arena, layer, status);
+  a.k_out = bfm(k_out);
+  a.v_out = bfm(v_out);
+  const c10::cuda::CUDAGuard guard(arena.device());
+  LAKEB_CHECK_RC(lakeb::kv8_read(a, cur_stream()), "kv8_read");
+}
+
+lakeb::Kv8AttnArgs kv8_attn_args(const at::Tensor& q, const at::Tensor& out, const at::Tensor& arena, int64_t layer,
+                                 const at::Tensor& block_tables, const at::Tensor& seq_lens, int64_t n_q_heads,
+                                 int64_t n_kv_heads, double scale, const c10::optional<at::Tensor>& status) {
+  check_bf16_2d(q, "q");
+  check_bf16_2d(out, "out");
+  check_kv8_arena(arena, layer, n_kv_heads);
+  TORCH_CHECK(n_q_heads > 0 && n_q_heads % n_kv_heads == 0, "q heads (", n_q_heads, ") must be a multiple of kv heads (",
+              n_kv_heads, ")");
+  TORCH_CHECK(q.size(1) == n_q_heads * 128 && out.size(1) == n_q_heads * 128 && out.size(0) >= q.size(0),
+              "q and out are [rows, n_q_heads * 128]");
+  TORCH_CHECK(block_tables.scalar_type() == at::kInt && block_tables.dim() == 2 && block_tables.stride(1) == 1,
+              "block_tables int32 [seqs, max_blocks]");
+  TORCH_CHECK(seq_lens.scalar_type() == at::kInt && seq_lens.dim() == 1 && seq_lens.is_contiguous() &&
+                  seq_lens.size(0) <= block_tables.size(0),
+              "seq_lens int32 [seqs], a block table row for each");
+  check_same_device(q, arena, "q");
+  check_same_device(out, arena, "out");
+  check_same_device(block_tables, arena, "block_tables");
+  check_same_device(seq_lens, arena, "seq_lens");
+  lakeb::Kv8AttnArgs p;
+  p.q = bf(q);
+  p.q_stride = q.stride(0);
+  p.out = bfm(out);
+  p.out_stride = out.stride(0);
+  p.arena = arena.data_ptr<uint8_t>();
+  p.num_blocks = arena.size(0);
+  p.block_bytes = arena.stride(0);
+  p.layer_offset = layer * arena.stride(1);
+  p.n_q_heads = static_cast<int>(n_q_heads);
+  p.n_kv_heads = static_cast<int>(n_kv_heads);
+  p.block_tables = block_tables.data_ptr<int>();
+  p.bt_stride = block_tables.stride(0);
+  p.max_blocks = static_cast<int>(block_tables.size(1));
+  p.seq_lens = seq_lens.data_ptr<int>();
+  p.num_seqs = static_cast<int>(seq_lens.size(0));
+  p.num_rows = static_cast<int>(q.size(0));
+  p.scale = static_cast<float>(scale);
+  p.status = status_ptr(status);
+  return p;
+}
+
+void kv8_decode(const at::Tensor& q, at::Tensor& out, const at::Tensor& arena, int64_t layer,
+                const at::Tensor& block_tables, const at::Tensor& seq_lens, int64_t n_q_heads, int64_t n_kv_heads,
+                double scale, c10::optional<at::Tensor> status) {
+  lakeb::Kv8AttnArgs p =
+      kv8_attn_args(q, out, arena, layer, block_tables, seq_lens, n_q_heads, n_kv_heads, scale, status);
+  TORCH_CHECK(q.size(0) >= p.num_seqs, "one query row per sequence");
+  const c10::cuda::CUDAGuard guard(arena.device());
+  p.num_rows = p.num_seqs;
+  p.splits = lakeb::paged_decode_splits(p.num_seqs, p.n_kv_heads, p.max_blocks);
+  at::Tensor ws;
+  if (p.splits > 1) {
+    const int64_t parts = static_cast<int64_t>(p.num_rows) * n_q_heads * p.splits;
+    ws = at::empty({parts * 132}, q.options().dtype(at::kFloat));
+    p.ws_o = ws.data_ptr<float>();
+    p.ws_ml = p.ws_o + parts * 128;
+  }
+  LAKEB_CHECK_RC(lakeb::kv8_attention(p, cur_stream()), "kv8_decode");
+}
+
+void kv8_prefill(const at::Tensor& q, at::Tensor& out, const at::Tensor& arena, int64_t layer,
+                 const at::Tensor& block_tables, const at::Tensor& seq_lens, const at::Tensor& tiles, int64_t n_q_heads,
+                 int64_t n_kv_heads, double scale, c10::optional<at::Tensor> status) {
+  lakeb::Kv8AttnArgs p =
+      kv8_attn_args(q, out, arena, layer, block_tables, seq_lens, n_q_heads, n_kv_heads, scale, status);
+  TORCH_CHECK(tiles.scalar_type() == at::kInt && tiles.dim() == 2 && tiles.size(1) == 4 && tiles.is_contiguous(),
+              "tiles int32 [n, 4]");
+  check_aligned(tiles, "tiles");
+  check_same_device(tiles, arena, "tiles");
+  p.tiles = reinterpret_cast<const int4*>(tiles.data_ptr<int>());
+  p.num_tiles = static_cast<int>(tiles.size(0));
+  const c10::cuda::CUDAGuard guard(arena.device());
+  LAKEB_CHECK_RC(lakeb::kv8_attention(p, cur_stream()), "kv8_prefill");
+}
+
+// ------------------------------------------------------------------ step tables
+void step_tables(const at::Tensor& pages, const at::Tensor& rows, const at::Tensor& context_lens,
+                 const at::Tensor& new_lens, int64_t n_decode, int64_t block_size, int64_t tile,
+                 at::Tensor& block_tables, at::Tensor& seq_lens, at::Tensor& query_start, at::Tensor& positions,
+                 at::Tensor& slots, at::Tensor& tiles, at::Tensor& counts, c10::optional<at::Tensor> status) {
+  TORCH_CHECK(pages.is_cuda() && pages.scalar_type() == at::kInt && pages.dim() == 2 &&
+                  (pages.size(1) <= 1 || pages.stride(1) == 1),
+              "pages int32 [request rows, max_blocks] with unit inner stride");
+  const int64_t n = rows.numel();
+  const std::pair<const at::Tensor*, const char*> ints[] = {
+      {&rows, "rows"},           {&context_lens, "context_lens"}, {&new_lens, "new_lens"},
+      {&block_tables, "block_tables"}, {&seq_lens, "seq_lens"},   {&query_start, "query_start"},
+      {&positions, "positions"}, {&tiles, "tiles"},               {&counts, "counts"}};
+  for (const auto& [t, name] : ints) {
+    TORCH_CHECK(t->scalar_type() == at::kInt && t->is_contiguous(), name, " must be contiguous int32");
+    check_same_device(*t, pages, name);
+  }
+  TORCH_CHECK(slots.scalar_type() == at::kLong && slots.is_contiguous(), "slots must be contiguous int64");
+  check_same_device(slots, pages, "slots");
+  TORCH_CHECK(context_lens.numel() == n && new_lens.numel() == n, "one context and one new length per sequence");
+  TORCH_CHECK(n <= lakeb::kStepTableMaxSeqs, "at most ", lakeb::kStepTableMaxSeqs, " sequences, got ", n);
+  TORCH_CHECK(n_decode >= 0 && n_decode <= n, "n_decode ", n_decode, " of ", n, " sequences");
+  TORCH_CHECK(block_size > 0 && tile > 0, "block_size and tile must be positive");
+  TORCH_CHECK(block_tables.dim() == 2 && block_tables.size(0) == n && block_tables.size(1) == pages.size(1) &&
+                  seq_lens.numel() == n && query_start.numel() == n + 1 && positions.numel() == slots.numel() &&
+                  tiles.dim() == 2 && tiles.size(1) == 4 && counts.numel() == 2,
+              "output sizes");
+  check_aligned(tiles, "tiles");
+  lakeb::StepTableArgs a;
+  a.pages = pages.data_ptr<int>();
+  a.pages_stride = pages.stride(0);
+  a.num_rows = static_cast<int>(pages.size(0));
+  a.max_blocks = static_cast<int>(pages.size(1));
+  a.rows = rows.data_ptr<int>();
+  a.context_lens = context_lens.data_ptr<int>();
+  a.new_lens = new_lens.data_ptr<int>();
+  a.num_seqs = static_cast<int>(n);
+  a.num_decode = static_cast<int>(n_decode);
+  a.max_tokens = static_cast<int>(positions.numel());
+  a.max_tiles = static_cast<int>(tiles.size(0));
+  a.block_size = static_cast<int>(block_size);
+  a.tile = static_cast<int>(tile);
+  a.block_tables = block_tables.data_ptr<int>();
+  a.seq_lens = seq_lens.data_ptr<int>();
+  a.query_start = query_start.data_ptr<int>();
+  a.positions = positions.data_ptr<int>();
+  a.slots = slots.data_ptr<int64_t>();
+  a.tiles = reinterpret_cast<int4*>(tiles.data_ptr<int>());
+  a.counts = counts.data_ptr<int>();
+  a.status = status_ptr(status);
+  const c10::cuda::CUDAGuard guard(pages.device());
+  LAKEB_CHECK_RC(lakeb::step_tables(a, cur_stream()), "step_tables");
+}
+
 void rmsnorm(const at::Tensor& x, const at::Tensor& w, at::Tensor& out, double eps) {
   check_bf16_2d(x, "x");
   check_bf16_2d(out, "out");
@@ -755,6 +946,20 @@ PYBIND11_MODULE(LAKEB_MODULE, m) {
   m.def("paged_prefill", &paged_prefill, py::arg("q"), py::arg("out"), py::arg("arena"), py::arg("layer"),
         py::arg("block_tables"), py::arg("seq_lens"), py::arg("tiles"), py::arg("n_q_heads"), py::arg("n_kv_heads"),
         py::arg("scale"), py::arg("status") = py::none(), py::arg("tensor_core") = true);
+  m.def("kv8_write", &kv8_write, py::arg("k"), py::arg("v"), py::arg("slots"), py::arg("arena"), py::arg("layer"),
+        py::arg("status") = py::none());
+  m.def("kv8_read", &kv8_read, py::arg("arena"), py::arg("layer"), py::arg("slots"), py::arg("k_out"),
+        py::arg("v_out"), py::arg("status") = py::none());
+  m.def("kv8_decode", &kv8_decode, py::arg("q"), py::arg("out"), py::arg("arena"), py::arg("layer"),
+        py::arg("block_tables"), py::arg("seq_lens"), py::arg("n_q_heads"), py::arg("n_kv_heads"), py::arg("scale"),
+        py::arg("status") = py::none());
+  m.def("kv8_prefill", &kv8_prefill, py::arg("q"), py::arg("out"), py::arg("arena"), py::arg("layer"),
+        py::arg("block_tables"), py::arg("seq_lens"), py::arg("tiles"), py::arg("n_q_heads"), py::arg("n_kv_heads"),
+        py::arg("scale"), py::arg("status") = py::none());
+  m.def("step_tables", &step_tables, py::arg("pages"), py::arg("rows"), py::arg("context_lens"), py::arg("new_lens"),
+        py::arg("n_decode"), py::arg("block_size"), py::arg("tile"), py::arg("block_tables"), py::arg("seq_lens"),
+        py::arg("query_start"), py::arg("positions"), py::arg("slots"), py::arg("tiles"), py::arg("counts"),
+        py::arg("status") = py::none());
   m.def("rmsnorm", &rmsnorm);
   m.def("embedding", &embedding, py::arg("ids"), py::arg("table"), py::arg("out"), py::arg("status") = py::none());
   m.def("argmax", &argmax);

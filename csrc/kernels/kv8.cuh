@@ -1,0 +1,60 @@
+// The 8-bit KV arena: uint8 [num_blocks, layers, kv_heads, 2 (K, V), 16 * 128 + 16].
+//
+// For one page, layer, head and side: 16 rows of 128 e4m3 codes, then the page's scale line, one
+// power-of-two byte b per token (E8M0): value = code * 2^(b - 127); b = 255 marks a row that held
+// an infinity or a NaN (its codes are 0, it reads back as NaN).
+//
+//  * A row's bytes are a function of the row alone (no scale shared between tokens that could
+//    grow as a page fills): pages are content-addressed by their tokens and shared by prefix, so a
+//    page filled token by token, in one chunk, or after a rejected draft has the same bytes.
+//  * Powers of two: dequantising is exact in fp16 and bf16 products, nothing is rounded twice.
+//  * Row t keeps its 16-byte chunk c at chunk c ^ (t & 7), so the bytes as they lie in memory are
+//    free of bank conflicts for ldmatrix, and K, V and both scale lines of a page and head arrive
+//    in shared memory with one bulk copy of 4128 contiguous bytes (129 sectors of 32 bytes).
+#pragma once
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace lakeb {
+
+constexpr int kKv8Page = 16;
+constexpr int kKv8Dim = 128;
+constexpr int kKv8Side = kKv8Page * kKv8Dim + kKv8Page;  // 2064 bytes: codes, scale line
+constexpr int kKv8Head = 2 * kKv8Side;                   // K and V of one page and head
+
+// Byte offset of 16-byte chunk `c` of token `t` inside one side.
+__host__ __device__ __forceinline__ int kv8_chunk(int t, int c) { return t * kKv8Dim + ((c ^ (t & 7)) << 4); }
+
+// Scale byte of a row from the largest |x| bit pattern of its elements (as integers, so that NaN
+// and infinity sort above every finite value): the smallest e >= -126 with amax <= 448 * 2^e.
+__device__ __forceinline__ int kv8_scale_byte(uint32_t amax_bits) {
+  if (amax_bits >= 0x7f800000u) return 255;
+  const int e = static_cast<int>(amax_bits >> 23) - 127 - 8 + ((amax_bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return max(e, -126) + 127;
+}
+// 2^(127 - b): the factor that brings a row into e4m3's range (0 for a NaN row: codes 0).
+__device__ __forceinline__ float kv8_inv_scale(int b) {
+  return b == 255 ? 0.f : __uint_as_float(static_cast<uint32_t>(254 - b) << 23);
+}
+// 2^(b - 127); NaN for b = 255 (b = 0 counts as 0: an arena that was never written reads as zeros).
+__device__ __forceinline__ float kv8_scale(int b) {
+  return __uint_as_float(b == 255 ? 0x7fffffffu : static_cast<uint32_t>(b) << 23);
+}
+
+// Two fp32 -> two e4m3 codes (round to nearest even), lo in the low byte.
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// Two e4m3 codes (low half of x) -> f16x2, exact.
+__device__ __forceinline__ uint32_t f16x2_of_e4m3(uint16_t x) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t f16x2_lo(uint32_t x) { return f16x2_of_e4m3(static_cast<uint16_t>(x)); }
+__device__ __forceinline__ uint32_t f16x2_hi(uint32_t x) { return f16x2_of_e4m3(static_cast<uint16_t>(x >> 16)); }
+
+}  // namespace lakeb

@@ -194,6 +194,72 @@ void set_prefill_variant(int v);    // softmax variant of the ping-pong kernel (
 int prefill_trace_enable(int on);
 int prefill_trace_read(long long* host, int n);
 
+// ----------------------------------------------------------------- 8-bit KV arena
+// Rows in and out of the arena (kv8.cuh). k/v (write) or k_out/v_out (read): bf16 rows of
+// heads * 128 elements, v_stride and k_stride elements apart; slots < 0 are skipped (write) or
+// read as zeros.
+struct Kv8RowArgs {
+  const __nv_bfloat16* k = nullptr;
+  const __nv_bfloat16* v = nullptr;
+  __nv_bfloat16* k_out = nullptr;
+  __nv_bfloat16* v_out = nullptr;
+  int64_t k_stride = 0, v_stride = 0;
+  const int64_t* slots = nullptr;  // [rows]
+  uint8_t* arena = nullptr;
+  int64_t num_blocks = 0, block_bytes = 0, layer_offset = 0;  // bytes
+  int rows = 0, heads = 0;
+  int* status = nullptr;
+};
+int kv8_write(const Kv8RowArgs& a, cudaStream_t stream);
+int kv8_read(const Kv8RowArgs& a, cudaStream_t stream);
+
+// Attention over the 8-bit arena. tiles == nullptr: one query row per sequence (decode).
+struct Kv8AttnArgs {
+  const __nv_bfloat16* q = nullptr;
+  int64_t q_stride = 0;
+  __nv_bfloat16* out = nullptr;
+  int64_t out_stride = 0;
+  const uint8_t* arena = nullptr;
+  int64_t num_blocks = 0, block_bytes = 0, layer_offset = 0;  // bytes
+  int n_q_heads = 0, n_kv_heads = 0;
+  const int* block_tables = nullptr;  // [num_seqs, bt_stride], max_blocks entries used
+  int64_t bt_stride = 0;
+  int max_blocks = 0;
+  const int* seq_lens = nullptr;
+  int num_seqs = 0;
+  int num_rows = 0;  // rows of q
+  float scale = 0.f;
+  const int4* tiles = nullptr;  // (seq, first query row, number of queries, position of the first)
+  int num_tiles = 0;
+  int splits = 1;
+  float* ws_o = nullptr;   // [num_rows, n_q_heads, splits, 128]
+  float* ws_ml = nullptr;  // [num_rows, n_q_heads, splits, 4]
+  int* status = nullptr;
+};
+int kv8_attention(const Kv8AttnArgs& a, cudaStream_t stream);
+
+// ----------------------------------------------------------------- step tables
+constexpr int kStepTableMaxSeqs = 8192;
+struct StepTableArgs {
+  const int* pages = nullptr;  // [num_rows, pages_stride] page ids of every request row
+  int64_t pages_stride = 0;
+  int num_rows = 0, max_blocks = 0;
+  const int* rows = nullptr;          // [num_seqs] request row of each sequence of the step
+  const int* context_lens = nullptr;  // [num_seqs] tokens in the cache before the step
+  const int* new_lens = nullptr;      // [num_seqs] tokens of the step
+  int num_seqs = 0, num_decode = 0;   // the first num_decode sequences get no query tiles
+  int max_tokens = 0, max_tiles = 0, block_size = 16, tile = 128;
+  int* block_tables = nullptr;  // [num_seqs, max_blocks]
+  int* seq_lens = nullptr;      // [num_seqs]
+  int* query_start = nullptr;   // [num_seqs + 1]
+  int* positions = nullptr;     // [max_tokens]
+  int64_t* slots = nullptr;     // [max_tokens]
+  int4* tiles = nullptr;        // [max_tiles]
+  int* counts = nullptr;        // tokens, tiles
+  int* status = nullptr;
+};
+int step_tables(const StepTableArgs& a, cudaStream_t stream);
+
 // ----------------------------------------------------------------- misc
 int rmsnorm_bf16(const __nv_bfloat16* x, int64_t sx, const __nv_bfloat16* w, __nv_bfloat16* out, int64_t so, int rows,
                  int dim, float eps, cudaStream_t stream);

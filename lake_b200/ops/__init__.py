@@ -19,5 +19,7 @@ from .core import (  # noqa: F401
     resolve_tokens,
     rms_norm,
 )
+from .kv8 import is_kv8, kv8_arena, kv8_read, kv8_write  # noqa: F401
+from .step import StepTables, build_step_tables  # noqa: F401
 from ..oracle.ops_ref import interleave_gate_up, rope_cache  # noqa: F401
 from ._ext import available as native_available  # noqa: F401

@@ -122,7 +122,7 @@ def linear_qkv(a: torch.Tensor, w_qkv: torch.Tensor, q_out: torch.Tensor, rope_c
         return q_out
     acc = ref.linear(a, _dense(w_qkv))
     t = a.shape[0]
-    d = arena.shape[-1]
+    d = ref.arena_head_dim(arena)
     q = acc[:, : n_q_heads * d].view(t, n_q_heads, d)
     k = acc[:, n_q_heads * d:(n_q_heads + n_kv_heads) * d].view(t, n_kv_heads, d)
     v = acc[:, (n_q_heads + n_kv_heads) * d:].view(t, n_kv_heads, d)
@@ -172,10 +172,18 @@ def paged_decode_attention(q: torch.Tensor, arena: torch.Tensor, layer: int, blo
                            seq_lens: torch.Tensor, n_q_heads: int, n_kv_heads: int, scale: float,
                            out: torch.Tensor | None = None, splits: int | None = None,
                            ws_o: torch.Tensor | None = None, ws_ml: torch.Tensor | None = None) -> torch.Tensor:
-    """One query row per sequence; row s attends to keys [0, seq_lens[s])."""
+    """One query row per sequence; row s attends to keys [0, seq_lens[s]) (none: a row of zeros).
+
+    With an 8-bit arena (ops.kv8_arena) the sequences' pages are cut over the whole GPU by their
+    lengths, so `splits`, `ws_o` and `ws_ml` have no effect there."""
     n = seq_lens.shape[0]
     if out is None:
-        out = torch.empty(q.shape[0], n_q_heads * arena.shape[-1], dtype=q.dtype, device=q.device)
+        out = torch.empty(q.shape[0], n_q_heads * ref.arena_head_dim(arena), dtype=q.dtype, device=q.device)
+    if q.is_cuda and ref.is_kv8(arena):
+        native().kv8_decode(q, out, arena, layer, block_tables, seq_lens, n_q_heads, n_kv_heads, scale,
+                            status_word(q.device))
+        LAUNCHES[0] += 1
+        return out
     if q.is_cuda:
         if splits is None:
             splits = decode_splits(n, n_kv_heads, block_tables.shape[1])
@@ -217,12 +225,18 @@ def paged_prefill_attention(q: torch.Tensor, arena: torch.Tensor, layer: int, bl
                             seq_lens: torch.Tensor, tiles: torch.Tensor, query_start: torch.Tensor,
                             positions: torch.Tensor, n_q_heads: int, n_kv_heads: int, scale: float,
                             out: torch.Tensor | None = None, tensor_core: bool = True) -> torch.Tensor:
-    """Causal attention of packed query rows against each sequence's paged context.
+    """Causal attention of packed query rows against each sequence's paged context (bf16 arena, or
+    the 8-bit one of ops.kv8_arena).
 
     tensor_core=True runs the tcgen05 kernel (tiles of up to PREFILL_TILE rows);
     False runs the warp-MMA kernel (tiles of up to 64 rows)."""
     if out is None:
-        out = torch.empty(q.shape[0], n_q_heads * arena.shape[-1], dtype=q.dtype, device=q.device)
+        out = torch.empty(q.shape[0], n_q_heads * ref.arena_head_dim(arena), dtype=q.dtype, device=q.device)
+    if q.is_cuda and ref.is_kv8(arena):
+        native().kv8_prefill(q, out, arena, layer, block_tables, seq_lens, tiles, n_q_heads, n_kv_heads, scale,
+                             status_word(q.device))
+        LAUNCHES[0] += 1
+        return out
     if q.is_cuda:
         native().paged_prefill(q, out, arena, layer, block_tables, seq_lens, tiles, n_q_heads, n_kv_heads, scale,
                                status_word(q.device), tensor_core)

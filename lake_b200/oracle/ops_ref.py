@@ -79,11 +79,76 @@ def rms_norm(x: torch.Tensor, w: torch.Tensor, eps: float) -> torch.Tensor:
     return xf * torch.rsqrt(xf.pow(2).mean(-1, keepdim=True) + eps) * w.float()
 
 
+# ------------------------------------------------------------------ 8-bit KV arena
+def is_kv8(arena: torch.Tensor) -> bool:
+    """Whether `arena` is an 8-bit KV arena (uint8 [blocks, layers, kv_heads, 2, 16 * D + 16])."""
+    return arena.dtype == torch.uint8
+
+
+def arena_head_dim(arena: torch.Tensor) -> int:
+    return arena.shape[-1] // PAGE - 1 if is_kv8(arena) else arena.shape[-1]
+
+
+def kv8_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows [..., D] -> (e4m3 codes uint8 [..., D], scale bytes uint8 [...]): the scale is 2^(b - 127)
+    with the smallest b >= 1 that keeps the row's largest element within 448; b = 255 and codes 0 for a
+    row with an infinity or a NaN."""
+    x = x.float()
+    fine = torch.isfinite(x).all(-1)
+    x = torch.where(fine[..., None], x, torch.zeros_like(x))
+    amax = x.abs().amax(-1)
+    m, e = torch.frexp(amax)  # amax = m * 2^e, m in [0.5, 1); 448 = 0.875 * 2^9
+    e = torch.where(amax > 0, (e - 9 + (m > 0.875).to(e.dtype)).clamp_min(-126), torch.full_like(e, -126))
+    q = torch.ldexp(x, -e[..., None]).to(torch.float8_e4m3fn).view(torch.uint8)
+    return q, torch.where(fine, e + 127, torch.full_like(e, 255)).to(torch.uint8)
+
+
+def kv8_scale(b: torch.Tensor) -> torch.Tensor:
+    """Scale bytes -> fp32 2^(b - 127); 255 -> NaN, 0 (never written) -> 0."""
+    return torch.where(b == 255, torch.full(b.shape, float("nan"), device=b.device),
+                       (b.to(torch.int32) << 23).view(torch.float32))
+
+
+def _kv8_cols(tok: torch.Tensor, d: int) -> torch.Tensor:
+    """Byte offsets [N, d] of the codes of tokens `tok` (offsets in the page): 16-byte chunk c of
+    token t lies at chunk c ^ (t & (p - 1)), p the power of two in the row's chunks, at most 8."""
+    n = d // 16
+    c = torch.arange(n, device=tok.device)[None, :] ^ (tok[:, None] & (min(n & -n, 8) - 1))
+    return (tok[:, None, None] * d + c[:, :, None] * 16 + torch.arange(16, device=tok.device)).reshape(-1, d)
+
+
+def kv8_rows(arena: torch.Tensor, layer: int, slots: torch.Tensor) -> torch.Tensor:
+    """fp32 values [N, Hkv, 2 (K, V), D] of cached tokens (negative slots: zeros)."""
+    d = arena_head_dim(arena)
+    sl = slots.long().clamp_min(0)
+    blk, tok = sl // PAGE, sl % PAGE
+    raw = arena[blk, layer]  # [N, Hkv, 2, 16 * D + 16]
+    at = _kv8_cols(tok, d)[:, None, None, :].expand(-1, raw.shape[1], 2, -1)
+    q = raw.gather(-1, at).view(torch.float8_e4m3fn).float()
+    b = raw.gather(-1, (PAGE * d + tok)[:, None, None, None].expand(-1, raw.shape[1], 2, 1))
+    x = q * kv8_scale(b)
+    return torch.where((slots >= 0)[:, None, None, None], x, torch.zeros_like(x))
+
+
+def _kv8_put(arena: torch.Tensor, layer: int, slots: torch.Tensor, x: torch.Tensor) -> None:
+    """x [N, Hkv, 2, D] into the arena at slots [N] (all >= 0)."""
+    d = arena_head_dim(arena)
+    q, b = kv8_quantize(x)
+    blk, tok = slots // PAGE, slots % PAGE
+    h = torch.arange(arena.shape[2], device=slots.device)[None, :, None]
+    kv = torch.arange(2, device=slots.device)[None, None, :]
+    arena[blk[:, None, None, None], layer, h[..., None], kv[..., None], _kv8_cols(tok, d)[:, None, None, :]] = q
+    arena[blk[:, None, None], layer, h, kv, (PAGE * d + tok)[:, None, None]] = b
+
+
 def write_kv(arena: torch.Tensor, layer: int, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
     """k, v [T, Hkv, D]; slots [T] (block*16+offset, <0 skipped)."""
     sl = slots.long()
     keep = sl >= 0
     sl = sl[keep]
+    if is_kv8(arena):
+        _kv8_put(arena, layer, sl, torch.stack([k[keep].float(), v[keep].float()], dim=2))
+        return
     page = arena.shape[4]
     blk, off = sl // page, sl % page
     arena[blk, layer, 0, :, off, :] = k[keep].to(arena.dtype)
@@ -92,6 +157,10 @@ def write_kv(arena: torch.Tensor, layer: int, slots: torch.Tensor, k: torch.Tens
 
 def gather_kv(arena: torch.Tensor, layer: int, block_table: torch.Tensor, length: int):
     """Return K, V [length, Hkv, D] fp32 for one sequence."""
+    if is_kv8(arena):
+        j = torch.arange(length, device=arena.device)
+        x = kv8_rows(arena, layer, block_table.long()[j // PAGE] * PAGE + j % PAGE)
+        return x[:, :, 0], x[:, :, 1]
     page = arena.shape[4]
     nb = (length + page - 1) // page
     ids = block_table[:nb].long()
@@ -120,7 +189,7 @@ def paged_attention(q: torch.Tensor, arena: torch.Tensor, layer: int, block_tabl
                     seq_lens: torch.Tensor, query_start: torch.Tensor, positions: torch.Tensor,
                     n_q_heads: int, n_kv_heads: int, scale: float) -> torch.Tensor:
     """Generic paged attention: rows [query_start[s], query_start[s+1]) belong to sequence s."""
-    d = arena.shape[-1]
+    d = arena_head_dim(arena)
     out = torch.zeros(q.shape[0], n_q_heads * d, dtype=torch.float32, device=q.device)
     qs = query_start.tolist()
     lens = seq_lens.tolist()
@@ -133,6 +202,51 @@ def paged_attention(q: torch.Tensor, arena: torch.Tensor, layer: int, block_tabl
         o = attention_one(qq, k, v, positions[a:b], scale)
         out[a:b] = o.reshape(b - a, -1)
     return out
+
+
+def step_tables(pages: torch.Tensor, rows: torch.Tensor, context_lens: torch.Tensor, new_lens: torch.Tensor,
+                max_tokens: int, max_tiles: int, n_decode: int = 0, block_size: int = PAGE, tile: int = 128):
+    """Tables of an engine step by plain loops (see ops.build_step_tables); raises ValueError where
+    the kernel reports through the status word."""
+    r, ctx, new = rows.tolist(), context_lens.tolist(), new_lens.tolist()
+    n, maxb = len(r), pages.shape[1]
+    if len(ctx) != n or len(new) != n:
+        raise ValueError("one context and one new length per sequence")
+    if not 0 <= n_decode <= n:
+        raise ValueError(f"n_decode {n_decode} of {n} sequences")
+    if any(x < 0 for x in new) or any(x < 0 for x in ctx):
+        raise ValueError("negative length")
+    if any(not 0 <= x < pages.shape[0] for x in r):
+        raise ValueError("request row outside the page table")
+    bt = torch.zeros(n, maxb, dtype=torch.int32)
+    start, positions, slots, tiles = [0], [], [], []
+    for s in range(n):
+        nb = (ctx[s] + new[s] + block_size - 1) // block_size
+        if nb > maxb:
+            raise ValueError(f"sequence {s} needs {nb} pages, its row has {maxb}")
+        own = pages[r[s], :nb]
+        if bool((own < 0).any()):
+            raise ValueError(f"sequence {s} has a token without a page")
+        bt[s, :nb] = own
+        ids = own.tolist()
+        for j in range(new[s]):
+            p = ctx[s] + j
+            positions.append(p)
+            slots.append(ids[p // block_size] * block_size + p % block_size)
+        if s >= n_decode:
+            for at in range(0, new[s], tile):
+                tiles.append((s, start[-1] + at, min(tile, new[s] - at), ctx[s] + at))
+        start.append(start[-1] + new[s])
+    if start[-1] > max_tokens or len(tiles) > max_tiles:
+        raise ValueError(f"{start[-1]} tokens and {len(tiles)} tiles, room for {max_tokens} and {max_tiles}")
+    counts = [start[-1], len(tiles)]
+    positions += [0] * (max_tokens - len(positions))
+    slots += [-1] * (max_tokens - len(slots))
+    tiles += [(0, 0, 0, 0)] * (max_tiles - len(tiles))
+    i32 = torch.int32
+    return (bt, torch.tensor([a + b for a, b in zip(ctx, new)], dtype=i32), torch.tensor(start, dtype=i32),
+            torch.tensor(positions, dtype=i32), torch.tensor(slots, dtype=torch.int64),
+            torch.tensor(tiles, dtype=i32).reshape(max_tiles, 4), torch.tensor(counts, dtype=i32))
 
 
 def greedy(logits: torch.Tensor, bitmask: torch.Tensor | None = None) -> torch.Tensor:

@@ -1,0 +1,594 @@
+"""8-bit KV arena: rows in and out, decode and prefill attention over it, against 64-bit results
+computed here from the format's definition."""
+import math
+
+import pytest
+import torch
+
+from lake_b200 import ops
+from lake_b200.oracle import ops_ref as ref
+
+BF = torch.bfloat16
+PAGE = 16
+
+
+# ------------------------------------------------------------------ definitions in 64 bits
+def quantize64(x):
+    """The value that a cached row stands for, element by element in 64 bits ([..., D])."""
+    x = x.double()
+    fine = torch.isfinite(x).all(-1, keepdim=True)
+    x0 = torch.where(fine, x, torch.zeros_like(x))
+    top = x0.abs().amax(-1, keepdim=True)
+    e = torch.full_like(top, -126.0)
+    for k in range(-126, 129):  # the smallest e with top <= 448 * 2^e
+        e = torch.where((top > 448.0 * 2.0 ** (k - 1)) & (top <= 448.0 * 2.0 ** k) & (k > -126),
+                        torch.full_like(e, float(k)), e)
+    y = x0 * torch.exp2(-e)
+    step = torch.exp2(torch.floor(torch.log2(y.abs().clamp_min(2.0 ** -6))) - 3)  # e4m3: 3 bits, 2^-9 at least
+    y = torch.round(y / step) * step * torch.exp2(e)
+    return torch.where(fine, y, torch.full_like(y, float("nan")))
+
+
+def stored64(arena, layer, page, tok):
+    """[heads, 2, D] of one cached token, byte by byte from the layout."""
+    d = arena.shape[-1] // PAGE - 1
+    n = d // 16
+    swz = min(n & -n, 8) - 1
+    raw = arena[page, layer].cpu()
+    out = torch.empty(raw.shape[0], 2, d, dtype=torch.float64)
+    for c in range(n):
+        at = tok * d + (c ^ (tok & swz)) * 16
+        out[:, :, 16 * c:16 * c + 16] = raw[:, :, at:at + 16].contiguous().view(torch.float8_e4m3fn).double()
+    b = raw[:, :, PAGE * d + tok].double()
+    scale = torch.where(b == 255, torch.full_like(b, float("nan")), torch.exp2(b - 127))
+    scale = torch.where(b == 0, torch.zeros_like(b), scale)
+    return out * scale[..., None]
+
+
+def attend64(q, k, v, lim, scale):
+    """q [n, hq, D], k/v [L, hkv, D] in 64 bits, row i sees keys [0, lim[i]): the result, the mean of
+    |v| under the same weights, and the largest sum of |q_d k_d| * scale of a row."""
+    g = q.shape[1] // k.shape[1]
+    k, v = k.repeat_interleave(g, 1), v.repeat_interleave(g, 1)
+    z = torch.einsum("nhd,lhd->nhl", q, k) * scale
+    mask = torch.arange(k.shape[0], device=q.device)[None, :] >= lim[:, None]
+    z = z.masked_fill(mask[:, None], float("-inf"))
+    none = (lim <= 0)[:, None, None]
+    p = torch.where(none, torch.zeros_like(z), torch.softmax(z.masked_fill(none, 0.0), -1))
+    p = torch.where(mask[:, None], torch.zeros_like(p), p)
+    # a key that a row does not see counts for nothing, whatever it holds
+    o = torch.stack([torch.einsum("hl,lhd->hd", p[i, :, :int(lim[i])], v[:int(lim[i])]) for i in range(len(lim))])
+    w = torch.stack([torch.einsum("hl,lhd->hd", p[i, :, :int(lim[i])], v[:int(lim[i])].abs())
+                     for i in range(len(lim))])
+    size = torch.einsum("nhd,lhd->nhl", q.abs(), k.abs()) * scale
+    size = size.masked_fill(mask[:, None], 0.0).amax(-1) if k.shape[0] else torch.zeros_like(o[..., 0])
+    return o, w, size
+
+
+def attention_tolerance(o, w, size, vmax):
+    """How far a kernel's bf16 result may be from o:
+    the final rounding, half a bf16 step: 2^-8 |o|;
+    P rounded to fp16, half a step each: 2^-11 of the mean |v|;
+    scores: fp32 sums of 128 exact products and their scaling, at most (128 + 4) 2^-24 of
+    sum |q_d k_d| each, which moves p by that part in the numerator and in the denominator: 2^-15 size;
+    ex2.approx (2^-22) and the rounding of its argument (2^-24 of at most ~2 size / ln 2): within 2^-15 (1 + size);
+    P below fp16's normal range, or V below it where the kernel scales V by tile: 2^-17 of the largest |v|."""
+    return 2.0 ** -8 * o.abs() + (2.0 ** -11 + 2.0 ** -14 * (1 + size[..., None])) * w + 2.0 ** -17 * vmax
+
+
+# ------------------------------------------------------------------ inputs
+def rows(n, heads, d, g, spread=0.3):
+    x = torch.randn(n, heads, d, generator=g, dtype=torch.float32)
+    return x * torch.exp(spread * torch.randn(n, heads, 1, generator=g))
+
+
+def special_rows(heads, d, g):
+    """Rows at the edges of the format (each repeated over the heads with another order of elements)."""
+    f = torch.finfo(BF)
+    out = []
+    for kind in ("zero", "one", "top448", "over448", "tiny", "subnormal", "huge", "ties", "wide", "inf", "nan",
+                 "negative"):
+        x = torch.zeros(heads, d)
+        if kind == "one":
+            x[:, 3] = 1.0
+        elif kind == "top448":
+            x[:] = 448.0 * torch.sign(torch.randn(heads, d, generator=g))
+        elif kind == "over448":
+            x[:, 0] = 450.0
+            x[:, 1:] = torch.randn(heads, d - 1, generator=g)
+        elif kind == "tiny":
+            x[:] = torch.randn(heads, d, generator=g) * f.tiny
+        elif kind == "subnormal":
+            x[:, ::2] = 2.0 ** -133
+            x[:, 1] = 2.0 ** -128
+        elif kind == "huge":
+            x[:] = torch.randn(heads, d, generator=g).clamp(-2, 2) * 2.0 ** 125
+        elif kind == "ties":  # halfway between two codes
+            x[:] = (torch.arange(d) % 8 + 8 + 0.5)[None] * 16.0
+        elif kind == "wide":
+            x[:] = torch.exp2(-torch.arange(d).float() / 4)[None]
+        elif kind == "inf":
+            x[:] = torch.randn(heads, d, generator=g)
+            x[:, d // 2] = float("-inf")
+        elif kind == "nan":
+            x[:] = torch.randn(heads, d, generator=g)
+            x[:, d - 1] = float("nan")
+        elif kind == "negative":
+            x[:] = -torch.rand(heads, d, generator=g)
+        out.append(x)
+    return torch.stack(out).to(BF).float()
+
+
+def same(a, b):
+    return torch.equal(torch.nan_to_num(a, nan=12345.0), torch.nan_to_num(b, nan=12345.0)) \
+        and torch.equal(torch.isnan(a), torch.isnan(b))
+
+
+def build(lens, hq, hkv, layers, layer, g, device, d=128, spread=0.3, garbage=True, extra_cols=0):
+    """An arena with shuffled pages holding the sequences' random K and V, bytes past their ends
+    random (garbage) where asked; the block tables and the cached values in 64 bits per sequence."""
+    nb = [-(-x // PAGE) for x in lens]
+    blocks = sum(nb) + 3
+    arena = ops.kv8_arena(blocks, layers, hkv, head_dim=d, device="cpu")
+    if garbage:
+        arena.copy_(torch.randint(0, 256, arena.shape, generator=g, dtype=torch.uint8))
+    perm = torch.randperm(blocks, generator=g)
+    bt = torch.full((len(lens), max(nb + [1]) + extra_cols), blocks - 1, dtype=torch.int32)
+    cached, at = [], 0
+    for s, n in enumerate(lens):
+        bt[s, :nb[s]] = perm[at:at + nb[s]].to(torch.int32)
+        at += nb[s]
+        k, v = rows(n, hkv, d, g, spread).to(BF), rows(n, hkv, d, g, spread).to(BF)
+        j = torch.arange(n)
+        ops.kv8_write(k.reshape(n, hkv * d), v.reshape(n, hkv * d), bt[s].long()[j // PAGE] * PAGE + j % PAGE, arena, layer)
+        cached.append((quantize64(k), quantize64(v)))
+    return arena.to(device), bt.to(device), cached
+
+
+# ------------------------------------------------------------------ rows, CPU
+@pytest.mark.parametrize("d", [16, 48, 64, 128, 256])
+def test_rows_round_trip_cpu(d):
+    g = torch.Generator().manual_seed(d)
+    heads = 3
+    x = torch.cat([special_rows(heads, d, g), rows(30, heads, d, g).to(BF).float()])
+    y = torch.cat([rows(30, heads, d, g).to(BF).float(), special_rows(heads, d, g)])
+    t = x.shape[0]
+    arena = ops.kv8_arena(6, 2, heads, head_dim=d, device="cpu")
+    slots = torch.randperm(6 * PAGE, generator=g)[:t]
+    slots[4] = -1
+    ops.kv8_write(x.reshape(t, -1), y.reshape(t, -1), slots, arena, 1)
+    k, v = ops.kv8_read(arena, 1, slots)
+    keep = slots >= 0
+    assert same(k.view(t, heads, d).double()[keep], quantize64(x)[keep].to(BF).double())
+    assert same(v.view(t, heads, d).double()[keep], quantize64(y)[keep].to(BF).double())
+    assert not k[4].any() and not v[4].any()
+    for i in (0, 7, 12, 40):
+        if slots[i] >= 0:
+            got = stored64(arena, 1, int(slots[i]) // PAGE, int(slots[i]) % PAGE)
+            assert same(got[:, 0], quantize64(x)[i]) and same(got[:, 1], quantize64(y)[i])
+    assert not arena[:, 0].any()  # the other layer is left as it was
+    fresh = ops.kv8_read(ops.kv8_arena(2, 1, heads, head_dim=d, device="cpu"), 0, torch.arange(5))
+    assert not fresh[0].any()
+
+
+def test_quantisation_error_is_half_a_step():
+    g = torch.Generator().manual_seed(0)
+    x = rows(200, 2, 128, g).to(BF)
+    err = (quantize64(x) - x.double()).abs()
+    top = x.double().abs().amax(-1, keepdim=True)
+    # e4m3 rounds by at most 2^-4 of the value, or by half of its smallest step, 2^-10 * 2^e, 2^e < top / 224
+    assert bool((err <= torch.maximum(2.0 ** -4 * x.double().abs(), 2.0 ** -10 * top / 224)).all())
+
+
+def test_row_bytes_do_not_depend_on_the_page():
+    """Token by token, in one chunk, and after rows that were overwritten: the same bytes."""
+    g = torch.Generator().manual_seed(1)
+    k, v = rows(16, 2, 128, g).to(BF).reshape(16, -1), rows(16, 2, 128, g).to(BF).reshape(16, -1)
+    big = 1000 * k
+    a, b, c = (ops.kv8_arena(1, 1, 2, device="cpu") for _ in range(3))
+    ops.kv8_write(k, v, torch.arange(16), a, 0)
+    for i in range(16):
+        ops.kv8_write(k[i:i + 1], v[i:i + 1], torch.tensor([i]), b, 0)
+    ops.kv8_write(big, big, torch.arange(16), c, 0)
+    ops.kv8_write(k, v, torch.arange(16), c, 0)
+    assert torch.equal(a, b) and torch.equal(a, c)
+
+
+def test_arena_refusals_cpu():
+    with pytest.raises(ValueError):
+        ops.kv8_arena(2, 1, 1, head_dim=100, device="cpu")
+    a = ops.kv8_arena(2, 1, 1, device="cpu")
+    with pytest.raises(IndexError):
+        ops.kv8_write(torch.zeros(1, 128), torch.zeros(1, 128), torch.tensor([99]), a, 0)
+
+
+# ------------------------------------------------------------------ attention, CPU
+@pytest.mark.parametrize("d", [64, 128])
+def test_decode_and_prefill_cpu(d):
+    g = torch.Generator().manual_seed(2)
+    lens, hq, hkv = [0, 1, 16, 17, 50], 4, 2
+    arena, bt, cached = build(lens, hq, hkv, 2, 1, g, "cpu", d=d, garbage=False)
+    scale = 1 / math.sqrt(d)
+    q = torch.randn(len(lens), hq * d, generator=g)
+    out = ops.paged_decode_attention(q, arena, 1, bt, torch.tensor(lens, dtype=torch.int32), hq, hkv, scale)
+    for s, n in enumerate(lens):
+        o, _, _ = attend64(q[s:s + 1].double().view(1, hq, d), *cached[s], torch.tensor([n]), scale)
+        assert torch.allclose(out[s].double(), o.flatten(), atol=1e-5, rtol=1e-5)
+    new = [0, 1, 5, 3, 20]
+    qs = torch.tensor([0, 0, 1, 6, 9, 29], dtype=torch.int32)
+    pos = torch.cat([torch.arange(n - m, n, dtype=torch.int32) for n, m in zip(lens, new)])
+    q = torch.randn(29, hq * d, generator=g)
+    out = ops.paged_prefill_attention(q, arena, 1, bt, torch.tensor(lens, dtype=torch.int32), None, qs, pos, hq, hkv,
+                                      scale)
+    for s in range(len(lens)):
+        a, b = int(qs[s]), int(qs[s + 1])
+        if b > a:
+            o, _, _ = attend64(q[a:b].double().view(b - a, hq, d), *cached[s], pos[a:b].long() + 1, scale)
+            assert torch.allclose(out[a:b].double(), o.reshape(b - a, -1), atol=1e-5, rtol=1e-5)
+
+
+def test_linear_qkv_cpu_writes_the_8bit_arena():
+    g = torch.Generator().manual_seed(3)
+    t, hid, hq, hkv, d = 5, 32, 4, 2, 64
+    a, w = torch.randn(t, hid, generator=g), torch.randn((hq + 2 * hkv) * d, hid, generator=g)
+    cs = ref.rope_cache(64, 10000.0, d)
+    pos = torch.tensor([3, 4, 5, 0, 9], dtype=torch.int32)
+    slots = torch.tensor([3, 4, 5, -1, 25])
+    arena = ops.kv8_arena(2, 1, hkv, head_dim=d, device="cpu")
+    dense = torch.zeros(2, 1, 2, hkv, PAGE, d)
+    qa, qb = torch.empty(t, hq * d), torch.empty(t, hq * d)
+    ops.linear_qkv(a, w, qa, cs, pos, slots, arena, 0, hq, hkv)
+    ops.linear_qkv(a, w, qb, cs, pos, slots, dense, 0, hq, hkv)
+    assert torch.equal(qa, qb)
+    k, v = ref.gather_kv(arena, 0, torch.tensor([0, 1]), 32)
+    kd, vd = ref.gather_kv(dense, 0, torch.tensor([0, 1]), 32)
+    at = slots[slots >= 0]
+    assert same(k[at].double(), quantize64(kd[at])) and same(v[at].double(), quantize64(vd[at]))
+
+
+# ------------------------------------------------------------------ rows, GPU
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads", [1, 2, 8])
+def test_rows_round_trip_gpu(cuda_dev, heads):
+    g = torch.Generator().manual_seed(heads)
+    x = torch.cat([special_rows(heads, 128, g), rows(70, heads, 128, g).to(BF).float()]).to(BF)
+    y = torch.cat([rows(70, heads, 128, g).to(BF).float(), special_rows(heads, 128, g)]).to(BF)
+    t = x.shape[0]
+    slots = torch.randperm(8 * PAGE, generator=g)[:t]
+    slots[3] = -1
+    base = torch.randint(0, 255, (8, 3, heads, 2, 2064), generator=g, dtype=torch.uint8)
+    want = base.clone()
+    ops.kv8_write(x.reshape(t, -1).float(), y.reshape(t, -1).float(), slots, want, 1)
+    # K and V as strided views of one packed projection, behind q columns
+    packed = torch.zeros(t, (4 + 2 * heads) * 128, dtype=BF)
+    packed[:, 512:512 + heads * 128] = x.reshape(t, -1)
+    packed[:, 512 + heads * 128:] = y.reshape(t, -1)
+    packed = packed.to(cuda_dev)
+    arena = base.to(cuda_dev)
+    ops.kv8_write(packed[:, 512:512 + heads * 128], packed[:, 512 + heads * 128:], slots.to(cuda_dev), arena, 1)
+    assert torch.equal(arena.cpu(), want)  # the same bytes, and nothing else touched
+    k, v = ops.kv8_read(arena, 1, slots.to(cuda_dev))
+    kc, vc = ops.kv8_read(want, 1, slots)
+    assert same(k.cpu().float(), kc.float()) and same(v.cpu().float(), vc.float())
+    keep = slots >= 0
+    assert same(k.cpu().view(t, heads, 128).double()[keep], quantize64(x)[keep].to(BF).double())
+    assert not k[3].any() and not v[3].any()
+    wide = torch.full((t, heads * 256), 7.0, dtype=BF, device=cuda_dev)
+    ops.kv8_read(arena, 1, slots.to(cuda_dev), k_out=wide[:, :heads * 128], v_out=wide[:, heads * 128:])
+    assert same(wide[:, :heads * 128].float(), k.float()) and same(wide[:, heads * 128:].float(), v.float())
+    empty = torch.empty(0, heads * 128, dtype=BF, device=cuda_dev)
+    ops.kv8_write(empty, empty, torch.empty(0, dtype=torch.int64, device=cuda_dev), arena, 1)
+    assert ops.kv8_read(arena, 1, torch.empty(0, dtype=torch.int64, device=cuda_dev))[0].shape == (0, heads * 128)
+    ops.core.check_status(cuda_dev)
+
+
+@pytest.mark.gpu
+def test_all_codes_and_scales_read_exactly(cuda_dev):
+    arena = ops.kv8_arena(16, 1, 1, device=cuda_dev)
+    codes = torch.arange(256, dtype=torch.uint8).view(2, 128)
+    for page in range(16):
+        for t in range(PAGE):
+            at = ref._kv8_cols(torch.tensor([t]), 128)[0].to(cuda_dev)
+            arena[page, 0, 0, 0, at] = codes[0].to(cuda_dev)
+            arena[page, 0, 0, 1, at] = codes[1].to(cuda_dev)
+            arena[page, 0, 0, :, 2048 + t] = page * 16 + t
+    slots = torch.arange(256, device=cuda_dev)
+    k, v = ops.kv8_read(arena, 0, slots)
+    kc, vc = ops.kv8_read(arena.cpu(), 0, slots.cpu())
+    assert same(k.cpu().float(), kc.float()) and same(v.cpu().float(), vc.float())
+
+
+@pytest.mark.gpu
+def test_rows_refusals_gpu(cuda_dev):
+    a = ops.kv8_arena(2, 1, 2, device=cuda_dev)
+    x = torch.zeros(3, 256, dtype=BF, device=cuda_dev)
+    s = torch.tensor([0, 40, 1], device=cuda_dev)  # 40: past the arena's 32 slots
+    for bad in (dict(k=x.float()), dict(k=x[:, :128]), dict(slots=s.int()), dict(slots=s[:2]), dict(layer=1),
+                dict(layer=-1), dict(arena=a[:, :, :1]), dict(arena=a.view(torch.int8)), dict(k=x.cpu()),
+                dict(slots=s.cpu())):
+        kw = dict(k=x, v=x, slots=s, arena=a, layer=0) | bad
+        with pytest.raises(RuntimeError):
+            ops.kv8_write(**kw)
+    odd = ops.kv8_arena(2, 1, 2, head_dim=64, device=cuda_dev)
+    with pytest.raises(RuntimeError, match="head_dim"):
+        ops.kv8_write(x[:, :128], x[:, :128], s, odd, 0)
+    ops.core.check_status(cuda_dev)
+    ops.kv8_write(x + 1, x + 2, s, a, 0)
+    with pytest.raises(ops.core.KernelError, match="out of bounds"):
+        ops.core.check_status(cuda_dev)
+    k, v = ops.kv8_read(a, 0, s)
+    with pytest.raises(ops.core.KernelError, match="out of bounds"):
+        ops.core.check_status(cuda_dev)
+    assert k[0, 0] == 1 and v[2, 5] == 2 and not k[1].any()
+
+
+# ------------------------------------------------------------------ decode, GPU
+def check_decode(dev, lens, hq, hkv, seed, layers=2, layer=1, spread=0.3, qscale=1.5, **kw):
+    g = torch.Generator().manual_seed(seed)
+    arena, bt, cached = build(lens, hq, hkv, layers, layer, g, dev, spread=spread, **kw)
+    scale = 1 / math.sqrt(128)
+    q = (torch.randn(len(lens), hq * 128, generator=g) * qscale).to(BF)
+    sl = torch.tensor(lens, dtype=torch.int32, device=dev)
+    out = ops.paged_decode_attention(q.to(dev), arena, layer, bt, sl, hq, hkv, scale)
+    ops.core.check_status(dev)
+    again = ops.paged_decode_attention(q.to(dev), arena, layer, bt, sl, hq, hkv, scale)
+    assert torch.equal(out, again)
+    for s, n in enumerate(lens):
+        k, v = (x.to(dev) for x in cached[s])
+        o, w, size = attend64(q[s:s + 1].to(dev).double().view(1, hq, 128), k, v, torch.tensor([n], device=dev), scale)
+        vmax = v.abs().amax() if n else torch.zeros((), device=dev)
+        err = (out[s].double().view(1, hq, 128) - o).abs()
+        tol = attention_tolerance(o, w, size, vmax)
+        assert bool((err <= tol).all()), (s, n, float((err - tol).amax()), float(err.amax()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv", [(1, 1), (4, 4), (4, 2), (8, 2), (6, 2), (16, 2), (7, 1), (24, 2), (40, 1)])
+def test_decode_heads(cuda_dev, hq, hkv):
+    check_decode(cuda_dev, [1, 33, 200], hq, hkv, 10 + hq)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens", [[0], [1], [0, 0, 5, 0], [15, 16, 17], [63, 64, 65], [320, 321, 319], [1000], [4097],
+                                  [3] * 70, [1, 5000, 2, 700, 0, 64], [257] * 40 + [0] * 9])
+def test_decode_lengths(cuda_dev, lens):
+    check_decode(cuda_dev, lens, 8, 2, 100 + len(lens) + lens[0], extra_cols=3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("spread,qscale", [(3.0, 1.0), (0.3, 40.0), (8.0, 0.01), (0.0, 1e-20)])
+def test_decode_values(cuda_dev, spread, qscale):
+    """Rows whose scales differ by many octaves, sharp and flat softmax, tiny queries."""
+    check_decode(cuda_dev, [90, 700], 8, 2, 7, spread=spread, qscale=qscale)
+
+
+@pytest.mark.gpu
+def test_decode_strided_rows_and_unseen_pages(cuda_dev):
+    """q and out as views of wider rows; table entries past a sequence's pages name no page at all."""
+    g = torch.Generator().manual_seed(5)
+    lens, hq, hkv = [40, 0, 7], 8, 2
+    arena, bt, cached = build(lens, hq, hkv, 1, 0, g, cuda_dev, extra_cols=2)
+    sl = torch.tensor(lens, dtype=torch.int32, device=cuda_dev)
+    for s, n in enumerate(lens):
+        bt[s, -(-n // PAGE):] = -7
+    wide = torch.randn(4, 3 * hq * 128, generator=g).to(BF).to(cuda_dev)
+    q = wide[:, hq * 128:2 * hq * 128]
+    res = torch.full((5, 2 * hq * 128), 3.0, dtype=BF, device=cuda_dev)
+    ops.paged_decode_attention(q, arena, 0, bt, sl, hq, hkv, 0.1, out=res[:, :hq * 128])
+    ops.core.check_status(cuda_dev)
+    plain = ops.paged_decode_attention(q[:3].contiguous(), arena, 0, bt, sl, hq, hkv, 0.1)
+    assert torch.equal(res[:3, :hq * 128], plain) and not plain[1].any()
+    assert bool((res[3:] == 3.0).all()) and bool((res[:, hq * 128:] == 3.0).all())
+
+
+@pytest.mark.gpu
+def test_decode_non_finite_rows(cuda_dev):
+    """A NaN or infinite row reaches what sees it and nothing else."""
+    g = torch.Generator().manual_seed(6)
+    lens, hq, hkv = [50, 50, 50], 8, 2
+    arena, bt, cached = build(lens, hq, hkv, 1, 0, g, cuda_dev)
+    q = torch.randn(3, hq * 128, generator=g).to(BF).to(cuda_dev)
+    sl = torch.tensor(lens, dtype=torch.int32, device=cuda_dev)
+    clean = ops.paged_decode_attention(q, arena, 0, bt, sl, hq, hkv, 0.1)
+    at = int(bt[1, 2]) * PAGE + 5
+    k, v = ops.kv8_read(arena, 0, torch.tensor([at], device=cuda_dev))
+    v[0, 130] = float("inf")  # KV head 1
+    ops.kv8_write(k, v, torch.tensor([at], device=cuda_dev), arena, 0)
+    out = ops.paged_decode_attention(q, arena, 0, bt, sl, hq, hkv, 0.1)
+    assert torch.equal(out[0], clean[0]) and torch.equal(out[2], clean[2]) and torch.equal(out[1, :512], clean[1, :512])
+    assert bool(torch.isnan(out[1, 512:]).all())
+    sl[1] = 37  # the row is no longer seen
+    short = ops.paged_decode_attention(q, arena, 0, bt, sl, hq, hkv, 0.1)
+    assert bool(torch.isfinite(short.float()).all())
+
+
+@pytest.mark.gpu
+def test_decode_refusals_and_bad_pages(cuda_dev):
+    g = torch.Generator().manual_seed(8)
+    arena, bt, _ = build([40, 20], 8, 2, 1, 0, g, cuda_dev)
+    q = torch.zeros(2, 1024, dtype=BF, device=cuda_dev)
+    sl = torch.tensor([40, 20], dtype=torch.int32, device=cuda_dev)
+    for bad in (dict(q=q.float()), dict(q=q[:1]), dict(q=q[:, :512]), dict(layer=3), dict(block_tables=bt.long()),
+                dict(block_tables=bt[:1]), dict(seq_lens=sl.long()), dict(n_kv_heads=4), dict(n_q_heads=7),
+                dict(block_tables=bt.cpu()), dict(seq_lens=sl.cpu()), dict(n_q_heads=0)):
+        kw = dict(q=q, arena=arena, layer=0, block_tables=bt, seq_lens=sl, n_q_heads=8, n_kv_heads=2, scale=0.1) | bad
+        with pytest.raises(RuntimeError):
+            ops.paged_decode_attention(**kw, out=torch.empty(2, 1024, dtype=BF, device=cuda_dev))
+    ops.core.check_status(cuda_dev)
+    good = ops.paged_decode_attention(q, arena, 0, bt, sl, 8, 2, 0.1)
+    for page in (arena.shape[0], -1, 2 ** 31 - 1):
+        worse = bt.clone()
+        worse[0, 1] = page
+        out = ops.paged_decode_attention(q, arena, 0, worse, sl, 8, 2, 0.1)
+        with pytest.raises(ops.core.KernelError, match="out of bounds"):
+            ops.core.check_status(cuda_dev)
+        assert torch.equal(out[1], good[1])
+
+
+# ------------------------------------------------------------------ prefill, GPU
+def check_prefill(dev, lens, new, hq, hkv, seed, layers=2, layer=1, tile=128, spread=0.3, qscale=1.5, pad_tiles=0):
+    g = torch.Generator().manual_seed(seed)
+    arena, bt, cached = build(lens, hq, hkv, layers, layer, g, dev, spread=spread)
+    scale = 1 / math.sqrt(128)
+    starts = [0]
+    for n in new:
+        starts.append(starts[-1] + n)
+    t = starts[-1]
+    q = (torch.randn(t + 2, hq * 128, generator=g) * qscale).to(BF).to(dev)
+    pos = torch.cat([torch.arange(n - m, n, dtype=torch.int32) for n, m in zip(lens, new)]).to(dev)
+    qs = torch.tensor(starts, dtype=torch.int32, device=dev)
+    sl = torch.tensor(lens, dtype=torch.int32, device=dev)
+    tiles = ops.build_prefill_tiles(starts, [n - m for n, m in zip(lens, new)], tile=tile, device=dev)
+    if pad_tiles:
+        tiles = torch.cat([tiles, torch.zeros(pad_tiles, 4, dtype=torch.int32, device=dev)])
+    out = torch.full((t + 2, hq * 128), 5.0, dtype=BF, device=dev)
+    ops.paged_prefill_attention(q, arena, layer, bt, sl, tiles, qs, pos, hq, hkv, scale, out=out)
+    ops.core.check_status(dev)
+    assert bool((out[t:] == 5.0).all())  # rows behind the last sequence
+    again = torch.full_like(out, 5.0)
+    ops.paged_prefill_attention(q, arena, layer, bt, sl, tiles, qs, pos, hq, hkv, scale, out=again)
+    assert torch.equal(out, again)
+    for s, n in enumerate(lens):
+        a, b = starts[s], starts[s + 1]
+        if b == a:
+            continue
+        k, v = (x.to(dev) for x in cached[s])
+        o, w, size = attend64(q[a:b].double().view(b - a, hq, 128), k, v, pos[a:b].long() + 1, scale)
+        err = (out[a:b].double().view(b - a, hq, 128) - o).abs()
+        tol = attention_tolerance(o, w, size, v.abs().amax())
+        assert bool((err <= tol).all()), (s, n, float((err - tol).amax()), float(err.amax()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv", [(1, 1), (4, 4), (4, 2), (8, 2), (6, 2), (16, 2), (5, 1), (24, 2), (40, 1)])
+def test_prefill_heads(cuda_dev, hq, hkv):
+    check_prefill(cuda_dev, [140, 33], [140, 7], hq, hkv, 20 + hq)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,new", [([1], [1]), ([16], [16]), ([17], [1]), ([127], [127]), ([128], [128]),
+                                      ([129], [129]), ([300], [172]), ([700, 5, 90], [300, 5, 1]),
+                                      ([40, 0, 60], [5, 0, 5]), ([513], [257]), ([1030, 2, 2], [6, 2, 1]),
+                                      ([1500], [640]), ([200] * 12, [5] * 12), ([256, 2000], [256, 3])])
+def test_prefill_lengths(cuda_dev, lens, new):
+    check_prefill(cuda_dev, lens, new, 8, 2, 200 + lens[0], pad_tiles=2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("spread,qscale", [(1.5, 1.0), (0.3, 40.0), (0.0, 1e-20)])
+def test_prefill_values(cuda_dev, spread, qscale):
+    check_prefill(cuda_dev, [400, 150], [300, 9], 8, 2, 9, spread=spread, qscale=qscale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tile", [5, 64])
+def test_prefill_smaller_tiles(cuda_dev, tile):
+    check_prefill(cuda_dev, [150, 70], [150, 33], 8, 2, 11, tile=tile)
+
+
+@pytest.mark.gpu
+def test_prefill_non_finite_rows(cuda_dev):
+    """A row that is not finite reaches the rows that see it: those before it in the chunk stay as they were."""
+    g = torch.Generator().manual_seed(12)
+    n, hq, hkv = 200, 8, 2
+    arena, bt, _ = build([n], hq, hkv, 1, 0, g, cuda_dev)
+    q = torch.randn(n, hq * 128, generator=g).to(BF).to(cuda_dev)
+    sl = torch.tensor([n], dtype=torch.int32, device=cuda_dev)
+    qs, pos = torch.tensor([0, n], dtype=torch.int32, device=cuda_dev), torch.arange(n, dtype=torch.int32, device=cuda_dev)
+    tiles = ops.build_prefill_tiles([0, n], [0], device=cuda_dev)
+    args = (bt, sl, tiles, qs, pos, hq, hkv, 0.1)
+    clean = ops.paged_prefill_attention(q, arena, 0, *args)
+    for side in (0, 1):
+        for tok in (37, 150):
+            a2 = arena.clone()
+            at = torch.tensor([int(bt[0, tok // PAGE]) * PAGE + tok % PAGE], device=cuda_dev)
+            kv = ops.kv8_read(arena, 0, at)
+            kv[side][0, 5] = float("nan")  # KV head 0
+            ops.kv8_write(*kv, at, a2, 0)
+            out = ops.paged_prefill_attention(q, a2, 0, *args)
+            assert torch.equal(out[:tok], clean[:tok]) and torch.equal(out[:, 512:], clean[:, 512:])
+            assert bool(torch.isnan(out[tok:, :512]).all())
+
+
+@pytest.mark.gpu
+def test_prefill_refusals(cuda_dev):
+    g = torch.Generator().manual_seed(13)
+    arena, bt, _ = build([40], 8, 2, 1, 0, g, cuda_dev)
+    q = torch.zeros(40, 1024, dtype=BF, device=cuda_dev)
+    sl = torch.tensor([40], dtype=torch.int32, device=cuda_dev)
+    tiles = ops.build_prefill_tiles([0, 40], [0], device=cuda_dev)
+    for bad in (dict(q=q.float()), dict(tiles=tiles.long()), dict(tiles=tiles[:, :3]), dict(tiles=tiles.cpu()),
+                dict(layer=1), dict(n_kv_heads=1), dict(n_q_heads=4)):
+        kw = dict(q=q, arena=arena, layer=0, block_tables=bt, seq_lens=sl, tiles=tiles, query_start=None,
+                  positions=None, n_q_heads=8, n_kv_heads=2, scale=0.1) | bad
+        with pytest.raises(RuntimeError):
+            ops.paged_prefill_attention(**kw, out=torch.empty(40, 1024, dtype=BF, device=cuda_dev))
+    bt[0, 1] = arena.shape[0] + 3
+    ops.paged_prefill_attention(q, arena, 0, bt, sl, tiles, None, None, 8, 2, 0.1)
+    with pytest.raises(ops.core.KernelError, match="out of bounds"):
+        ops.core.check_status(cuda_dev)
+    none = ops.paged_prefill_attention(q[:0], arena, 0, bt, sl, tiles[:0], None, None, 8, 2, 0.1)
+    assert none.shape == (0, 1024)
+
+
+# ------------------------------------------------------------------ streams, graphs, sizes
+@pytest.mark.gpu
+def test_two_streams_and_a_replayed_graph(cuda_dev):
+    """Calls on two streams at once and a captured call replayed with other lengths give what single
+    calls give."""
+    g = torch.Generator().manual_seed(14)
+    lens, hq, hkv = [700, 90, 1500, 1], 8, 2
+    arena, bt, _ = build(lens, hq, hkv, 1, 0, g, cuda_dev)
+    sl = torch.tensor(lens, dtype=torch.int32, device=cuda_dev)
+    qs = [torch.randn(4, 1024, generator=g).to(BF).to(cuda_dev) for _ in range(4)]
+    want = [ops.paged_decode_attention(q, arena, 0, bt, sl, hq, hkv, 0.1) for q in qs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[] for _ in qs]
+    for _ in range(20):
+        for i, q in enumerate(qs):
+            with torch.cuda.stream(streams[i % 2]):
+                got[i].append(ops.paged_decode_attention(q, arena, 0, bt, sl, hq, hkv, 0.1))
+    torch.cuda.synchronize()
+    for i in range(4):
+        assert all(torch.equal(x, want[i]) for x in got[i])
+    q, lens_buf = qs[0].clone(), sl.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.paged_decode_attention(q, arena, 0, bt, lens_buf, hq, hkv, 0.1)
+    graph.replay()
+    assert torch.equal(out, want[0])
+    q.copy_(qs[1])
+    lens_buf.copy_(torch.tensor([3, 0, 1499, 1], device=cuda_dev))
+    graph.replay()
+    assert torch.equal(out, ops.paged_decode_attention(qs[1], arena, 0, bt, lens_buf, hq, hkv, 0.1))
+    ops.core.check_status(cuda_dev)
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits(cuda_dev):
+    """Pages beyond 4 GiB of the arena are written, read and attended to."""
+    blocks = (1 << 32) // (4128 * 2) + 64
+    arena = torch.zeros(blocks, 1, 2, 2, 2064, dtype=torch.uint8, device=cuda_dev)
+    g = torch.Generator().manual_seed(15)
+    n, hq = 50, 8
+    k, v = (rows(n, 2, 128, g).to(BF).reshape(n, -1).to(cuda_dev) for _ in range(2))
+    small = ops.kv8_arena(4, 1, 2, device=cuda_dev)
+    j = torch.arange(n, device=cuda_dev)
+    far = (blocks - 4) * PAGE + j
+    ops.kv8_write(k, v, far, arena, 0)
+    ops.kv8_write(k, v, j, small, 0)
+    assert torch.equal(arena[blocks - 4:], small)
+    assert torch.equal(ops.kv8_read(arena, 0, far)[0], ops.kv8_read(small, 0, j)[0])
+    q = torch.randn(n, hq * 128, generator=g).to(BF).to(cuda_dev)
+    sl = torch.tensor([n], dtype=torch.int32, device=cuda_dev)
+    near = torch.arange(4, dtype=torch.int32, device=cuda_dev)[None]
+    args = (sl, hq, 2, 0.1)
+    assert torch.equal(ops.paged_decode_attention(q[:1], arena, 0, near + (blocks - 4), *args),
+                       ops.paged_decode_attention(q[:1], small, 0, near, *args))
+    tiles = ops.build_prefill_tiles([0, n], [0], device=cuda_dev)
+    a = ops.paged_prefill_attention(q, arena, 0, near + (blocks - 4), sl, tiles, None, None, hq, 2, 0.1)
+    b = ops.paged_prefill_attention(q, small, 0, near, sl, tiles, None, None, hq, 2, 0.1)
+    assert torch.equal(a, b)
+    ops.core.check_status(cuda_dev)
