@@ -636,7 +636,8 @@ void kv8_prefill(const at::Tensor& q, at::Tensor& out, const at::Tensor& arena, 
   p.tiles = reinterpret_cast<const int4*>(tiles.data_ptr<int>());
   p.num_tiles = static_cast<int>(tiles.size(0));
   const c10::cuda::CUDAGuard guard(arena.device());
-  LAKEB_CHECK_RC(lakeb::kv8_attention(p, cur_stream()), "kv8_prefill");
+  const bool tc = p.num_rows > 8 * p.num_tiles;
+  LAKEB_CHECK_RC(tc ? lakeb::kv8_prefill_tc(p, cur_stream()) : lakeb::kv8_attention(p, cur_stream()), "kv8_prefill");
 }
 
 // ------------------------------------------------------------------ step tables

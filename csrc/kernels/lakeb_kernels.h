@@ -237,6 +237,8 @@ struct Kv8AttnArgs {
   int* status = nullptr;
 };
 int kv8_attention(const Kv8AttnArgs& a, cudaStream_t stream);
+// Query tiles of <= 128 rows on the tcgen05 tensor cores.
+int kv8_prefill_tc(const Kv8AttnArgs& a, cudaStream_t stream);
 
 // ----------------------------------------------------------------- step tables
 constexpr int kStepTableMaxSeqs = 8192;
