@@ -1,18 +1,21 @@
 // Causal prefill attention over the 8-bit KV arena on tcgen05 tensor cores (sm_100a).
 //
 // A CTA owns up to 128 query rows of two query heads A and B of one KV head (the last head of an
-// odd group runs alone), so each K/V tile that it brings in and converts serves both. Per tile of
-// 128 keys:
-//   S_h   = Q_h K_j^T           tcgen05.mma fp16 (M=128, N=128, K=128), fp32 in tensor memory
+// odd group runs alone), so each K/V tile of 128 keys that it brings in and converts serves both.
+// Per step of 64 keys:
+//   S_h   = Q_h K_i^T           tcgen05.mma fp16 (M=128, N=64, K=128), fp32 in tensor memory
 //   P_h   = 2^(S_h c + e_j - b) softmax warpgroup h: thread = query row; fp16 over S_h's columns
-//   O_h  += P_h V_j             tcgen05.mma, A = P_h from tensor memory, V_j MN-major in shared memory
-// The MMA warp issues PV_A(j), S_A(j+1), PV_B(j), S_B(j+1): one head's products run while the
-// other head's softmax does.
+//   O_h  += P_h V_i             tcgen05.mma, A = P_h from tensor memory, V_i MN-major in shared memory
+// A head has two S buffers of 64 columns: S(i+1) is there when the softmax of step i ends, so the
+// softmax warps never wait for a product, and PV(i) and S(i+2) run behind them. With one buffer of
+// 128 columns (tensor memory holds no more beside the two O) softmax and products of a head take
+// turns: 5.1k cycles per 128 keys and two heads, against 2.0k of products and 2.0k of exponentials.
 //
-// 8-bit operands become fp16 ones in shared memory: bulk copies bring the tile's eight pages
-// (4128 bytes each, K, V and scales) into a staging buffer, a warpgroup of converters turns codes
-// into fp16 rows of the 128-byte swizzle (thread = key; e4m3 -> fp16 is exact). The tensor cores'
-// own fp8 products would need Q and P in 8 bits as well, or twice the products. A tile is scaled
+// 8-bit operands become fp16 ones in shared memory: bulk copies bring the K and the V sides of the
+// tile's eight pages (2064 bytes each, scales included) into a staging buffer each, a warpgroup for
+// each side turns codes into fp16 rows of the 128-byte swizzle (thread = key; e4m3 -> fp16 is
+// exact). The tensor cores' own fp8
+// products would need Q and P in 8 bits as well, or twice the products. A tile is scaled
 // against its own largest K scale and V scale: a row keeps code * 2^(e_row - e_tile), exact while
 // e_tile - e_row <= 15 (a code's last bit is 2^-9, fp16's 2^-24), and e_tile itself is one
 // multiplier of the tile's scores, or one addend of its exponents, not work per element. Where
@@ -23,10 +26,11 @@
 // row lazily (it moves when w grows by more than 2^8), P = 2^(w - b + 7) <= 2^15. The row sum is
 // kept in fp32 over sum_j 2^(e_0 - e_j) rowsum(P_j), so O / sum needs 2^(e_0) at the end.
 //
-// Warps: 0 = loads, 1 = tensor memory and MMA issue, 2-3 idle, 4-7 = converters, 8-11 and 12-15 =
-// softmax of head A and B. Registers are moved from the first two warpgroups to the softmax ones,
-// which hold a row of 128 scores. Every wait is bounded; a role whose wait ran out goes on through
-// its loop without work, so that the converters' named barrier is always reached by all of them.
+// Warps: 0 = loads, 1 = tensor memory and MMA issue, 2-3 idle, 4-7 = converters of K, 8-11 = of V,
+// 12-15 and 16-19 = softmax of head A and B. Registers move from the first three warpgroups to the
+// softmax ones.
+// Every wait is bounded; a role whose wait ran out goes on through its loop without work, so that
+// the converters' named barriers are always reached by all of their warps.
 #include <math_constants.h>
 
 #include "common.cuh"
@@ -44,16 +48,16 @@ constexpr int kOperand = 2 * kHalf;   // 32 KB: both 64-dim halves
 constexpr int kQ = 0;                 // Q of head A, B
 constexpr int kK = 2 * kOperand;      // fp16 K, 2 stages
 constexpr int kV = kK + 2 * kOperand; // fp16 V, 2 stages
-constexpr int kRaw = kV + 2 * kOperand;              // staging: 8 pages as they lie in the arena
+constexpr int kRaw = kV + 2 * kOperand;              // staging: the K and the V sides of 8 pages
 constexpr int kBars = kRaw + 8 * kKv8Head;           // 229,632
-constexpr int kParams = kBars + 192;                 // [4] TileParams
-constexpr int kRed = kParams + 4 * 32;               // [2][4] converter warps' maxima and flags
-constexpr int kSmem = kRed + 2 * 4 * 16 + 1024;      // + the 1024-byte alignment
-constexpr int kThreads = 512;
+constexpr int kParams = kBars + 256;                 // [4] TileParams
+constexpr int kRed = kParams + 4 * 32;               // [2 tiles][K, V][4] converter warps' maxima and flags
+constexpr int kSmem = kRed + 2 * 2 * 4 * 8;
+constexpr int kThreads = 640;
+constexpr int kStep = 64;                            // keys per softmax step
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.0f;
 constexpr float kPBias = 7.0f;
-constexpr int kConvBar = 1;
 
 // e_tile of K and V, and the keys whose V row is NaN (their codes are 0: the softmax makes the
 // scores of rows that see them NaN, so that rows that do not stay clean).
@@ -85,6 +89,33 @@ __device__ __forceinline__ uint32_t f16x2_exp2(int d) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
+// One lane of the warp (the same each time).
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t r;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(r));
+  return r;
+}
+// Products and commits that take effect in the lane with lead != 0.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t lead) {
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(lead));
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t lead) {
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(lead));
+}
+__device__ __forceinline__ void commit(uint64_t* bar, uint32_t lead) {
+  asm volatile(
+      "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(smem_u32(bar)),
+      "r"(lead)
+      : "memory");
+}
+
 // One row of 128 codes (chunk c at kv8_chunk) -> fp16 row `row` of a swizzled two-half tile.
 __device__ __forceinline__ void convert_row(const uint8_t* side, int t, uint8_t* dst, int row, uint32_t f) {
 #pragma unroll
@@ -106,28 +137,31 @@ __device__ __forceinline__ void zero_row(uint8_t* dst, int row) {
 
 __global__ void __launch_bounds__(kThreads, 1)
     kv8_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const Kv8AttnArgs a) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kBars);
-  uint64_t* q_full = bars + 0;    // Q in shared memory as bf16
-  uint64_t* q_ready = bars + 1;   // Q converted to fp16
-  uint64_t* raw_full = bars + 2;
-  uint64_t* raw_empty = bars + 3;
-  uint64_t* k_full = bars + 4;    // [2 stages]
-  uint64_t* k_empty = bars + 6;   // [2]
-  uint64_t* v_full = bars + 8;    // [2]
-  uint64_t* v_empty = bars + 10;  // [2]
-  uint64_t* s_full = bars + 12;   // [2 heads]
-  uint64_t* p_full = bars + 14;   // [2 heads]
-  uint64_t* o_done = bars + 16;   // [2 heads]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 18);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 19);
+  uint64_t* q_full = bars + 0;      // Q in shared memory as bf16
+  uint64_t* q_ready = bars + 1;     // Q converted to fp16
+  uint64_t* raw_full = bars + 2;    // [K, V]
+  uint64_t* raw_empty = bars + 4;   // [K, V]
+  uint64_t* k_full = bars + 6;      // [2 stages]
+  uint64_t* k_empty = bars + 8;     // [2]
+  uint64_t* v_full = bars + 10;     // [2]
+  uint64_t* v_empty = bars + 12;    // [2]
+  uint64_t* s_full = bars + 14;     // [2 heads][2 buffers]
+  uint64_t* p_full = bars + 18;     // [2 heads][2 buffers]
+  uint64_t* o_done = bars + 22;     // [2 heads]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 25);
   TileParams* params = reinterpret_cast<TileParams*>(smem + kParams);
 
   // heavy (late) query tiles first: the grid runs in reverse tile order
   const int4 tile = a.tiles[a.num_tiles - 1 - static_cast<int>(blockIdx.x)];
   const int seq = tile.x, qrow0 = tile.y, nq = tile.z, pos0 = tile.w;
   if (nq <= 0) return;
+  if (smem_u32(smem) & 1023) {  // the swizzled tiles need it; the launch gives it
+    if (threadIdx.x == 0) record_error(a.status, kErrBadArg);
+    return;
+  }
   const int G = a.n_q_heads / a.n_kv_heads, pairs = (G + 1) / 2;
   const int kvh = static_cast<int>(blockIdx.y) / pairs, pair = static_cast<int>(blockIdx.y) % pairs;
   const int qh0 = kvh * G + 2 * pair;
@@ -135,21 +169,24 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int len = min(a.seq_lens[seq], a.max_blocks * kKv8Page);
   const int max_pos = min(pos0 + nq - 1, len - 1);
-  const int n_tiles = max_pos < 0 ? 0 : max_pos / kTile + 1;
+  const int n_steps = max_pos < 0 ? 0 : max_pos / kStep + 1;
+  const int n_tiles = (n_steps + 1) / 2;
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
     mbar_init(q_ready, 128 * heads);
-    mbar_init(raw_full, 1);
-    mbar_init(raw_empty, 128);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&raw_full[i], 1);
+      mbar_init(&raw_empty[i], 128);
       mbar_init(&k_full[i], 128);
       mbar_init(&k_empty[i], 1);
       mbar_init(&v_full[i], 128);
       mbar_init(&v_empty[i], 1);
+      mbar_init(&o_done[i], 1);
+    }
+    for (int i = 0; i < 4; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 128);
-      mbar_init(&o_done[i], 1);
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -159,11 +196,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const uint32_t t_s[2] = {tmem, tmem + 128};        // S of head A, B (P overwrites its first 64 columns)
+  const uint32_t t_s[2] = {tmem, tmem + 128};        // S of head A, B: two buffers of 64 columns (P over the first 32)
   const uint32_t t_o[2] = {tmem + 256, tmem + 384};  // O of head A, B
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 0 && n_tiles > 0) {
       // ------------------------------------------------------------ loads
       if (lane == 0) {
@@ -185,141 +222,146 @@ __global__ void __launch_bounds__(kThreads, 1)
           record_error(a.status, kErrBounds);
           page = 0;
         }
-        ok = __all_sync(0xffffffffu, mbar_wait(raw_empty, (j & 1) ^ 1, abort_flag, a.status));
-        if (ok && lane == 0) mbar_expect_tx(raw_full, n * kKv8Head);
-        __syncwarp();
-        if (ok && lane < n) bulk_load(smem + kRaw + lane * kKv8Head, base + page * a.block_bytes, kKv8Head, raw_full);
+        for (int kv = 0; kv < 2; ++kv) {
+          ok = __all_sync(0xffffffffu, ok && mbar_wait(&raw_empty[kv], (j & 1) ^ 1, abort_flag, a.status));
+          if (ok && lane == 0) mbar_expect_tx(&raw_full[kv], n * kKv8Side);
+          __syncwarp();
+          if (ok && lane < n)
+            bulk_load(smem + kRaw + (kv * 8 + lane) * kKv8Side, base + page * a.block_bytes + kv * kKv8Side, kKv8Side,
+                      &raw_full[kv]);
+        }
       }
       // the release arrivals of the last two tiles must land before the CTA exits
       for (int j = max(0, n_tiles - 2); j < n_tiles && ok; ++j)
         ok = mbar_wait(&k_empty[j & 1], (j >> 1) & 1, abort_flag, a.status) &&
              mbar_wait(&v_empty[j & 1], (j >> 1) & 1, abort_flag, a.status);
-    } else if (warp == 1 && lane == 0 && n_tiles > 0) {
+    } else if (warp == 1 && n_tiles > 0) {
       // ------------------------------------------------------------ MMA issue
-      constexpr uint32_t idesc_s = idesc_f16(128, 128, false);
+      // The whole warp runs this loop and one elected lane's instructions take effect: descriptors stay
+      // in uniform registers (from a branch of one lane each product cost ~120 cycles of issue, twice
+      // its run time).
+      constexpr uint32_t idesc_s = idesc_f16(128, kStep, false);
       constexpr uint32_t idesc_o = idesc_f16(128, 128, true);
-      auto issue_s = [&](int h, int j) {
-        const uint32_t q_base = smem_u32(smem + kQ + h * kOperand);
-        const uint32_t k_base = smem_u32(smem + kK + (j & 1) * kOperand);
+      const uint32_t lead = elect_one();
+      const uint64_t q_desc = umma_desc_sw128(smem_u32(smem + kQ)), k_desc = umma_desc_sw128(smem_u32(smem + kK));
+      const uint64_t v_desc = desc_sw128_mn(smem_u32(smem + kV), kHalf);
+      auto issue_s = [&](int h, int i) {
+        const uint64_t qd = q_desc + h * (kOperand >> 4);
+        const uint64_t kd = k_desc + ((i >> 1) & 1) * (kOperand >> 4) + (i & 1) * (kStep * 128 >> 4);
+        const uint32_t d = tmem + h * 128 + (i & 1) * kStep;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const uint32_t off = (k >> 2) * kHalf + (k & 3) * 32;
-          umma_f16(t_s[h], umma_desc_sw128(q_base + off), umma_desc_sw128(k_base + off), idesc_s, k > 0);
+          constexpr int kNext = kHalf >> 4;
+          const int off = (k >> 2) * kNext + (k & 3) * 2;
+          mma_ss(d, qd + off, kd + off, idesc_s, k > 0, lead);
         }
-        umma_commit(&s_full[h]);
+        commit(&s_full[2 * h + (i & 1)], lead);
       };
-      auto issue_pv = [&](int h, int j) {
-        const uint32_t v_base = smem_u32(smem + kV + (j & 1) * kOperand);
+      auto issue_pv = [&](int h, int i) {  // 16 keys per product: 8 columns of P, 16 rows of V
+        const uint64_t vd = v_desc + ((i >> 1) & 1) * (kOperand >> 4) + (i & 1) * (kStep * 128 >> 4);
+        const uint32_t d = tmem + 256 + h * 128, p = tmem + h * 128 + (i & 1) * kStep;
 #pragma unroll
-        for (int k = 0; k < 8; ++k)  // 16 keys per step: P columns 8k..8k+7, V rows 16k..16k+15
-          umma_f16_ts(t_o[h], t_s[h] + 8 * k, desc_sw128_mn(v_base + k * 2048, kHalf), idesc_o, (j > 0) || (k > 0));
-        umma_commit(&o_done[h]);
+        for (int k = 0; k < 4; ++k) mma_ts(d, p + 8 * k, vd + k * 128, idesc_o, i > 0 || k > 0, lead);
+        commit(&o_done[h], lead);
       };
       bool ok = mbar_wait(q_ready, 0, abort_flag, a.status) && mbar_wait(&k_full[0], 0, abort_flag, a.status);
+      ok = __all_sync(0xffffffffu, ok);
       if (ok) {
         tc_fence_after();
-        for (int h = 0; h < heads; ++h) issue_s(h, 0);
-        umma_commit(&k_empty[0]);
+        for (int i = 0; i < min(2, n_steps); ++i)
+          for (int h = 0; h < heads; ++h) issue_s(h, i);
+        commit(&k_empty[0], lead);
       }
-      for (int j = 0; j < n_tiles && ok; ++j) {
-        const int s = j & 1, sn = (j + 1) & 1;
-        const bool more = j + 1 < n_tiles;
-        ok = mbar_wait(&v_full[s], (j >> 1) & 1, abort_flag, a.status);
+      auto wait = [&](uint64_t* bar, int parity) {
+        return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, a.status));
+      };
+      // S(h, i) goes over P(h, i - 2): PV(h, i - 2) has to be done with it, not just issued (products of
+      // different shapes may overlap). It is issued behind the other head's next PV, so that the wait
+      // for o_done finds it done.
+      auto next_s = [&](int h, int i) {
+        if (i < 2 || i >= n_steps) return true;
+        if (h == 0 && (i & 1) == 0 && !wait(&k_full[(i >> 1) & 1], (i >> 2) & 1)) return false;
+        if (!wait(&o_done[h], i & 1)) return false;
+        tc_fence_after();
+        issue_s(h, i);
+        if (h == heads - 1 && ((i & 1) || i + 1 == n_steps)) commit(&k_empty[(i >> 1) & 1], lead);
+        return true;
+      };
+      for (int i = 0; i < n_steps && ok; ++i) {
+        const int j = i >> 1;
+        if ((i & 1) == 0) ok = wait(&v_full[j & 1], (j >> 1) & 1);
         for (int h = 0; h < heads && ok; ++h) {
-          if (!mbar_wait(&p_full[h], j & 1, abort_flag, a.status)) {
-            ok = false;
-            break;
-          }
+          ok = wait(&p_full[2 * h + (i & 1)], j & 1);
+          if (!ok) break;
           tc_fence_after();
-          issue_pv(h, j);
-          if (h == heads - 1) umma_commit(&v_empty[s]);
-          if (more) {
-            if (h == 0) {
-              if (!mbar_wait(&k_full[sn], ((j + 1) >> 1) & 1, abort_flag, a.status)) {
-                ok = false;
-                break;
-              }
-              tc_fence_after();
-            }
-            issue_s(h, j + 1);  // after PV(h, j) in issue order: P's columns are read before S overwrites them
-          }
+          issue_pv(h, i);
+          if (h == heads - 1 && ((i & 1) || i + 1 == n_steps)) commit(&v_empty[j & 1], lead);
+          ok = heads == 1 ? next_s(0, i + 2) : h == 0 ? next_s(1, i + 1) : next_s(0, i + 2);
         }
-        if (ok && more) umma_commit(&k_empty[sn]);
       }
     }
-  } else if (warp < 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-    // -------------------------------------------------------------- converters: thread = key of the tile
-    const int row = threadIdx.x - 128, t = row & 15;
-    const uint8_t* page = smem + kRaw + (row >> 4) * kKv8Head;
-    int* red = reinterpret_cast<int*>(smem + kRed);  // [2 tiles][4 warps][K max, V max, NaN keys]
+  } else if (warp < 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    // ------------------------------- converters of K (kv = 0) and of V (kv = 1): thread = key of the tile
+    const int kv = (warp - 4) >> 2, row = (threadIdx.x - 128) & 127, t = row & 15;
+    const uint8_t* side = smem + kRaw + (kv * 8 + (row >> 4)) * kKv8Side;
     constexpr int kNone = -1000;
     int ev_last = kNone, ev_top = kNone;
     bool ok = true;
     for (int j = 0; j < n_tiles; ++j) {
       const int s = j & 1;
-      const uint32_t ph = ((j >> 1) & 1) ^ 1;
-      ok = ok && mbar_wait(raw_full, j & 1, abort_flag, a.status);
+      int2* red = reinterpret_cast<int2*>(smem + kRed) + (s * 2 + kv) * 4;  // largest scale, NaN keys of each warp
+      // tile j - 4's was read before PV(j - 4) and S(j - 3), which the waits of tile j - 1 waited for
+      TileParams& p = params[j & 3];
+      ok = ok && mbar_wait(&raw_full[kv], j & 1, abort_flag, a.status);
       const bool real = ok && j * kTile + row < len;
-      const int kb = real ? page[kKv8Page * kKv8Dim + t] : 0, vb = real ? page[kKv8Side + kKv8Page * kKv8Dim + t] : 0;
+      const int b = real ? side[kKv8Page * kKv8Dim + t] : 0;
       // rows of zeros (b <= 1) and NaN rows (255) say nothing about the tile's scale
-      const int km = __reduce_max_sync(0xffffffffu, kb > 1 && kb < 255 ? kb - 127 : kNone);
-      const int vm = __reduce_max_sync(0xffffffffu, vb > 1 && vb < 255 ? vb - 127 : kNone);
-      const uint32_t nan = __ballot_sync(0xffffffffu, vb == 255);
-      if (lane == 0) {
-        int* r = red + (s * 4 + (warp - 4)) * 4;
-        r[0] = km, r[1] = vm, r[2] = static_cast<int>(nan);
-      }
-      asm volatile("bar.sync %0, 128;" ::"n"(kConvBar) : "memory");
-      int ek = kNone, et = kNone;
+      const int top = __reduce_max_sync(0xffffffffu, b > 1 && b < 255 ? b - 127 : kNone);
+      const uint32_t nan = __ballot_sync(0xffffffffu, b == 255);
+      if (lane == 0) red[warp & 3] = make_int2(top, static_cast<int>(nan));
+      asm volatile("bar.sync %0, 128;" ::"r"(1 + kv) : "memory");
+      int e = max(max(red[0].x, red[1].x), max(red[2].x, red[3].x));
+      if (kv == 0) {
+        if (e == kNone) e = 0;
+        if (row == 0) p.ek = e;
+      } else {
+        // V's reference may fall by 15 per tile (what fp16 holds exactly) and to 2^-80 of the largest
+        // so far, so that the sum's factor 2^(e_0 - e_j) stays within fp32
+        e = e == kNone ? (ev_last == kNone ? -30 : ev_last) : max(e, -90);
+        if (ev_last != kNone) e = max(e, max(ev_last - 15, ev_top - 80));
+        ev_last = e;
+        ev_top = max(ev_top, e);
+        if (row == 0) {
+          p.ev = e;
+          p.any_nan = 0;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        ek = max(ek, red[(s * 4 + w) * 4]);
-        et = max(et, red[(s * 4 + w) * 4 + 1]);
-      }
-      if (ek == kNone) ek = 0;
-      // V's reference may fall by 15 per tile (what fp16 holds exactly) and to 2^-80 of the largest so
-      // far, so that the sum's factor 2^(e_0 - e_j) stays within fp32
-      int ev = et == kNone ? (ev_last == kNone ? -30 : ev_last) : max(et, -90);
-      if (ev_last != kNone) ev = max(ev, max(ev_last - 15, ev_top - 80));
-      ev_last = ev;
-      ev_top = max(ev_top, ev);
-      if (row == 0) {
-        TileParams& p = params[j & 3];  // tile j - 4's was read before PV(j - 4), which v_empty below waited for
-        p.ek = ek;
-        p.ev = ev;
-        int any = 0;
-        for (int w = 0; w < 4; ++w) {
-          p.nan[w] = static_cast<uint32_t>(red[(s * 4 + w) * 4 + 2]);
-          any |= red[(s * 4 + w) * 4 + 2];
+          for (int w = 0; w < 4; ++w) {
+            p.nan[w] = static_cast<uint32_t>(red[w].y);
+            p.any_nan |= red[w].y;
+          }
         }
-        p.any_nan = any;
       }
-      ok = ok && mbar_wait(&k_empty[s], ph, abort_flag, a.status);
+      ok = ok && mbar_wait(kv ? &v_empty[s] : &k_empty[s], ((j >> 1) & 1) ^ 1, abort_flag, a.status);
       if (ok) {
-        uint8_t* kd = smem + kK + s * kOperand;
-        if (real) convert_row(page, t, kd, row, kb == 255 ? 0x7fff7fffu : f16x2_exp2(min(kb - 127 - ek, 0)));
-        else zero_row(kd, row);
+        uint8_t* dst = smem + (kv ? kV : kK) + s * kOperand;
+        // a NaN row of K gives NaN scores; one of V becomes zeros, its NaNs come through P
+        if (real && !(kv && b == 255))
+          convert_row(side, t, dst, row, b == 255 ? 0x7fff7fffu : f16x2_exp2(min(b - 127 - e, 0)));
+        else
+          zero_row(dst, row);
         fence_proxy_async_smem();
-        mbar_arrive(&k_full[s]);
-      }
-      ok = ok && mbar_wait(&v_empty[s], ph, abort_flag, a.status);
-      if (ok) {
-        uint8_t* vd = smem + kV + s * kOperand;
-        if (real && vb != 255) convert_row(page + kKv8Side, t, vd, row, f16x2_exp2(min(vb - 127 - ev, 0)));
-        else zero_row(vd, row);
-        fence_proxy_async_smem();
-        mbar_arrive(&v_full[s]);
-        mbar_arrive(raw_empty);
+        mbar_arrive(kv ? &v_full[s] : &k_full[s]);
+        mbar_arrive(&raw_empty[kv]);
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
     // -------------------------------------------------------------- softmax + epilogue: thread = query row
-    const int h = (warp - 8) >> 2;
+    const int h = (warp - 12) >> 2;
     const int r = (warp & 3) * 32 + lane;  // query row in the tile = TMEM lane
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    if (h < heads && n_tiles > 0) {
+    if (h < heads && n_steps > 0) {
       const int kmax = min(pos0 + r, len - 1);  // last key this row may see
       bool ok = __all_sync(0xffffffffu, mbar_wait(q_full, 0, abort_flag, a.status));
       // Q: bf16 -> fp16 in place, times a power of two that brings the row's largest element to [2^14, 2^15)
@@ -344,73 +386,75 @@ __global__ void __launch_bounds__(kThreads, 1)
           return pack_f16x2(__uint_as_float(u << 16) * f, __uint_as_float(u & 0xffff0000u) * f);
         };
 #pragma unroll
-        for (int c = 0; c < 16; ++c)
-          *at(c) = make_uint4(two(x[c].x), two(x[c].y), two(x[c].z), two(x[c].w));
+        for (int c = 0; c < 16; ++c) *at(c) = make_uint4(two(x[c].x), two(x[c].y), two(x[c].z), two(x[c].w));
       }
       fence_proxy_async_smem();
       if (ok) mbar_arrive(q_ready);
       float bo = -CUDART_INF_F;  // base of w, at most kSlack below the largest w so far
-      float l = 0.f;
+      float l = 0.f, c = 0.f, ev = 0.f, unscale = 0.f;
       int e0 = 0;
-      for (int j = 0; j < n_tiles; ++j) {
-        if (!__all_sync(0xffffffffu, ok && mbar_wait(&s_full[h], j & 1, abort_flag, a.status))) {
+      for (int i = 0; i < n_steps; ++i) {
+        const int j = i >> 1, buf = i & 1;
+        const TileParams& tp = params[j & 3];
+        ok = ok && mbar_wait(&s_full[2 * h + buf], j & 1, abort_flag, a.status);
+        if (buf == 0) ok = ok && mbar_wait(&v_full[j & 1], (j >> 1) & 1, abort_flag, a.status);  // e_j of V
+        if (!__all_sync(0xffffffffu, ok)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        const int k0 = j * kTile;
-        const TileParams& tp = params[j & 3];
-        uint32_t sv[128];
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          tmem_ld32(t_s[h] + lane_off + c * 32, *reinterpret_cast<uint32_t(*)[32]>(sv + 32 * c));
-        const float ev = static_cast<float>(tp.ev);
-        const float c = cr * __uint_as_float(static_cast<uint32_t>(127 + tp.ek) << 23);
-        if (j == 0) e0 = tp.ev;
-        const float unscale = exp2f(static_cast<float>(e0 - tp.ev));
+        const uint32_t t_mine = t_s[h] + lane_off + kStep * buf;
+        uint32_t sv[64];
+        tmem_ld32(t_mine, *reinterpret_cast<uint32_t(*)[32]>(sv));
+        tmem_ld32(t_mine + 32, *reinterpret_cast<uint32_t(*)[32]>(sv + 32));
+        if (buf == 0) {
+          if (j == 0) e0 = tp.ev;
+          ev = static_cast<float>(tp.ev);
+          c = cr * __uint_as_float(static_cast<uint32_t>(127 + tp.ek) << 23);
+          unscale = ex2(static_cast<float>(e0 - tp.ev));
+        }
+        const int k0 = i * kStep;
         const bool nan = tp.any_nan != 0;
         tmem_ld_wait();
-        if (k0 + kTile - 1 > kmax) {  // the diagonal or the sequence end: keys past this row's last
+        if (k0 + kStep - 1 > kmax) {  // the diagonal or the sequence end: keys past this row's last
 #pragma unroll
-          for (int i = 0; i < 128; ++i)
-            if (k0 + i > kmax) sv[i] = __float_as_uint(-CUDART_INF_F);
+          for (int k = 0; k < 64; ++k)
+            if (k0 + k > kmax) sv[k] = __float_as_uint(-CUDART_INF_F);
         }
         if (nan) {
 #pragma unroll
-          for (int i = 0; i < 128; ++i)
-            if (((tp.nan[i >> 5] >> (i & 31)) & 1u) && k0 + i <= kmax) sv[i] = 0x7fffffffu;
+          for (int k = 0; k < 64; ++k)
+            if (((tp.nan[buf * 2 + (k >> 5)] >> (k & 31)) & 1u) && k0 + k <= kmax) sv[k] = 0x7fffffffu;
         }
-        // row max: eight independent three-input chains, then a short tree
-        float mv[8];
+        // row max: four independent three-input chains, then a short tree
+        float mv[4];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) mv[q] = max3f(__uint_as_float(sv[q]), __uint_as_float(sv[8 + q]), -CUDART_INF_F);
+        for (int q = 0; q < 4; ++q) mv[q] = max3f(__uint_as_float(sv[q]), __uint_as_float(sv[4 + q]), -CUDART_INF_F);
 #pragma unroll
-        for (int i = 16; i < 128; i += 16)
+        for (int k = 8; k < 64; k += 8)
 #pragma unroll
-          for (int q = 0; q < 8; ++q) mv[q] = max3f(mv[q], __uint_as_float(sv[i + q]), __uint_as_float(sv[i + 8 + q]));
-        const float mx =
-            fmaf(max3f(max3f(mv[0], mv[1], mv[2]), max3f(mv[3], mv[4], mv[5]), fmaxf(mv[6], mv[7])), c, ev);
+          for (int q = 0; q < 4; ++q) mv[q] = max3f(mv[q], __uint_as_float(sv[k + q]), __uint_as_float(sv[k + 4 + q]));
+        const float mx = fmaf(fmaxf(max3f(mv[0], mv[1], mv[2]), mv[3]), c, ev);
         const bool grow = mx > bo + kSlack;
         const float old = bo;
         if (grow) bo = mx;
         const float add = bo == -CUDART_INF_F ? 0.f : ev - bo + kPBias;
-        float2 rs[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        float2 rs[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         const float2 cv = make_float2(c, c), av = make_float2(add, add);
 #pragma unroll
-        for (int k = 0; k < 64; ++k) {  // key pair k -> packed column k (written over consumed scores)
+        for (int k = 0; k < 32; ++k) {  // key pair k -> packed column k (written over consumed scores)
           const float2 z = fma2(make_float2(__uint_as_float(sv[2 * k]), __uint_as_float(sv[2 * k + 1])), cv, av);
           const float2 p = make_float2(ex2(z.x), ex2(z.y));
-          rs[k & 3] = add2(rs[k & 3], p);
+          rs[k & 1] = add2(rs[k & 1], p);
           sv[k] = pack_f16x2(p.x, p.y);
-          if (k == 31) tmem_st32(t_s[h] + lane_off, *reinterpret_cast<uint32_t(*)[32]>(sv));
         }
-        tmem_st32(t_s[h] + lane_off + 32, *reinterpret_cast<uint32_t(*)[32]>(sv + 32));
-        rs[0] = add2(add2(rs[0], rs[1]), add2(rs[2], rs[3]));
+        tmem_st32(t_mine, *reinterpret_cast<uint32_t(*)[32]>(sv));
+        rs[0] = add2(rs[0], rs[1]);
         // O and l still hold sums against the old base. tcgen05.ld/st are warp-collective: the whole
         // warp rescales when any of its rows needs it (rows that do not keep alpha = 1).
         float alpha = 1.f;
-        if (__any_sync(0xffffffffu, grow && j > 0)) {
-          if (!__all_sync(0xffffffffu, mbar_wait(&o_done[h], (j - 1) & 1, abort_flag, a.status))) {
+        if (__any_sync(0xffffffffu, grow && i > 0)) {
+          if (!__all_sync(0xffffffffu, mbar_wait(&o_done[h], (i - 1) & 1, abort_flag, a.status))) {
             ok = false;
             break;
           }
@@ -422,28 +466,32 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_ld32(t_o[h] + lane_off + q * 32, ov);
             tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha);
+            for (int k = 0; k < 32; ++k) ov[k] = __float_as_uint(__uint_as_float(ov[k]) * alpha);
             tmem_st32(t_o[h] + lane_off + q * 32, ov);
           }
         }
         l = fmaf(l, alpha, (rs[0].x + rs[0].y) * unscale);
         tmem_st_wait();
         tc_fence_before();
-        mbar_arrive(&p_full[h]);
+        mbar_arrive(&p_full[2 * h + buf]);
       }
-      if (ok && __all_sync(0xffffffffu, mbar_wait(&o_done[h], (n_tiles - 1) & 1, abort_flag, a.status))) {
+      // This warp may have ended its last step before another one's arrival let PV(n_steps - 2) go: both
+      // phases in turn (one wait for the last could be met by the phase two before it).
+      ok = ok && (n_steps < 2 || mbar_wait(&o_done[h], n_steps & 1, abort_flag, a.status)) &&
+           mbar_wait(&o_done[h], (n_steps - 1) & 1, abort_flag, a.status);
+      if (__all_sync(0xffffffffu, ok)) {
         tc_fence_after();
         const float inv = l == 0.f ? 0.f : exp2f(static_cast<float>(e0)) / l;
         __nv_bfloat16* orow = a.out + static_cast<int64_t>(qrow0 + r) * a.out_stride + (qh0 + h) * 128;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int q = 0; q < 4; ++q) {
           uint32_t ov[32];
-          tmem_ld32(t_o[h] + lane_off + c * 32, ov);
+          tmem_ld32(t_o[h] + lane_off + q * 32, ov);
           tmem_ld_wait();
           if (r < nq) {
-            uint4* dst = reinterpret_cast<uint4*>(orow + c * 32);
-            auto two = [&](int i) {
-              return pack_bf16x2(__uint_as_float(ov[i]) * inv, __uint_as_float(ov[i + 1]) * inv);
+            uint4* dst = reinterpret_cast<uint4*>(orow + q * 32);
+            auto two = [&](int k) {
+              return pack_bf16x2(__uint_as_float(ov[k]) * inv, __uint_as_float(ov[k + 1]) * inv);
             };
 #pragma unroll
             for (int v = 0; v < 4; ++v) dst[v] = make_uint4(two(8 * v), two(8 * v + 2), two(8 * v + 4), two(8 * v + 6));
