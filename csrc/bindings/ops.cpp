@@ -605,6 +605,17 @@ lakeb::Kv8AttnArgs kv8_attn_args(const at::Tensor& q, const at::Tensor& out, con
   return p;
 }
 
+// Workspace (this call's own, so calls on several streams and captured graphs share none) and launch.
+void kv8_few_rows(lakeb::Kv8AttnArgs& p, const at::Tensor& q) {
+  at::Tensor ws;
+  if (const int64_t n = lakeb::kv8_attention_ws_floats(p)) {
+    ws = at::empty({n}, q.options().dtype(at::kFloat));
+    p.ws_o = ws.data_ptr<float>();
+    p.ws_ml = p.ws_o + n / 132 * 128;
+  }
+  LAKEB_CHECK_RC(lakeb::kv8_attention(p, cur_stream()), "kv8_attention");
+}
+
 void kv8_decode(const at::Tensor& q, at::Tensor& out, const at::Tensor& arena, int64_t layer,
                 const at::Tensor& block_tables, const at::Tensor& seq_lens, int64_t n_q_heads, int64_t n_kv_heads,
                 double scale, c10::optional<at::Tensor> status) {
@@ -613,15 +624,7 @@ void kv8_decode(const at::Tensor& q, at::Tensor& out, const at::Tensor& arena, i
   TORCH_CHECK(q.size(0) >= p.num_seqs, "one query row per sequence");
   const c10::cuda::CUDAGuard guard(arena.device());
   p.num_rows = p.num_seqs;
-  p.splits = lakeb::paged_decode_splits(p.num_seqs, p.n_kv_heads, p.max_blocks);
-  at::Tensor ws;
-  if (p.splits > 1) {
-    const int64_t parts = static_cast<int64_t>(p.num_rows) * n_q_heads * p.splits;
-    ws = at::empty({parts * 132}, q.options().dtype(at::kFloat));
-    p.ws_o = ws.data_ptr<float>();
-    p.ws_ml = p.ws_o + parts * 128;
-  }
-  LAKEB_CHECK_RC(lakeb::kv8_attention(p, cur_stream()), "kv8_decode");
+  kv8_few_rows(p, q);
 }
 
 void kv8_prefill(const at::Tensor& q, at::Tensor& out, const at::Tensor& arena, int64_t layer,
@@ -636,8 +639,11 @@ void kv8_prefill(const at::Tensor& q, at::Tensor& out, const at::Tensor& arena, 
   p.tiles = reinterpret_cast<const int4*>(tiles.data_ptr<int>());
   p.num_tiles = static_cast<int>(tiles.size(0));
   const c10::cuda::CUDAGuard guard(arena.device());
-  const bool tc = p.num_rows > 8 * p.num_tiles;
-  LAKEB_CHECK_RC(tc ? lakeb::kv8_prefill_tc(p, cur_stream()) : lakeb::kv8_attention(p, cur_stream()), "kv8_prefill");
+  if (p.num_rows > 8 * p.num_tiles) {
+    LAKEB_CHECK_RC(lakeb::kv8_prefill_tc(p, cur_stream()), "kv8_prefill");
+  } else {
+    kv8_few_rows(p, q);
+  }
 }
 
 // ------------------------------------------------------------------ step tables

@@ -16,6 +16,16 @@
 // above them, so a page costs one vote instead of six shuffles and 32 multiplications. The two
 // bases keep p = 2^(z-m) (summed in fp32) and P = 2^(w-bo+7) <= 2^15 (fp16, what the product
 // needs) in range whatever the tokens' scales are.
+//
+// Work is cut by pages, not by sequences: the pages of every (sequence, KV head, column group) are
+// laid end to end and each CTA takes an equal run of them, whatever the lengths are (two CTAs per
+// SM, all resident). A segment that lies within one CTA's run goes straight to the output; a CTA
+// has at most two pieces of segments (its first and its last) that go to the workspace, and a
+// second kernel joins them in the order of the CTAs, so results do not depend on timing. When no
+// block table is wider than kWholePages, a CTA takes a whole segment and there is no second kernel.
+//
+// In a CTA one warp copies pages into a ring (bulk copies of 4128 bytes, page ids fetched 32 at a
+// time, queries of the next segment ahead) and four warps take the pages in turn.
 #include <math_constants.h>
 
 #include "common.cuh"
@@ -27,19 +37,26 @@
 namespace lakeb {
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kSlots = 20;  // pages in flight per CTA: 82,560 bytes, two CTAs per SM
-constexpr int kCols = 8;
+constexpr int kWarps = 4;                     // consumers; warp 4 loads
+constexpr int kThreads = kWarps * 32 + 32;
+constexpr int kWholePages = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.f;  // a base trails the true maximum by at most this
 constexpr float kPBias = 7.f;  // P = 2^(w - bo + 7): fp16 subnormals begin at 2^-21 of the base
 
-constexpr int kMergeFloats = kWarps * kCols * kKv8Dim;
-constexpr int kRingBytes = kSlots * kKv8Head;
-constexpr int kMergeOff = (kRingBytes + 15) / 16 * 16;
-constexpr int kStatOff = kMergeOff + kMergeFloats * 4;
-constexpr int kBarOff = kStatOff + kWarps * kCols * 3 * 4;
-constexpr int kSmem = kBarOff + kSlots * 8;
+// Shared memory of a CTA with NT groups of 8 columns: ring of pages, two query buffers, the
+// consumers' sums for the join at a segment's end. Two CTAs fit an SM (113 KB each).
+template <int NT>
+struct Smem {
+  static constexpr int kCols = 8 * NT;
+  static constexpr int kSlots = NT == 1 ? 20 : 16;  // pages; a multiple of kWarps
+  static constexpr int kQ = kSlots * kKv8Head;
+  static constexpr int kO = kQ + 2 * kCols * 256;
+  static constexpr int kStat = kO + kWarps * kCols * kKv8Dim * 4;  // [warp][col][m, bo, l]
+  static constexpr int kBar = kStat + kWarps * kCols * 3 * 4;
+  static constexpr int kBytes = kBar + (2 * kSlots + 4) * 8;
+  static_assert(kQ % 16 == 0 && kO % 16 == 0 && kBar % 8 == 0 && kBytes <= 113 * 1024, "");
+};
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -72,24 +89,35 @@ struct ColState {
   float m[2], bo[2], l[2];  // bases and this lane's part of the sum of p
 };
 
-// Adds one page (16 tokens from tok0) to the state. lim[e]: keys of column 2t+e end before lim[e];
-// len: tokens from len on are not the sequence's (their bytes may be anything).
-__device__ __forceinline__ void page_step(const uint8_t* page, int tok0, int len, const int (&lim)[2],
-                                          const uint32_t (&qf)[8][2], const float (&cq)[2], int lane, ColState& st) {
+// Adds one page (16 tokens from tok0) to the states. lim[n][e]: keys of column 8n+2t+e end before
+// it; len: tokens from len on are not the sequence's (their bytes may be anything).
+template <int NT>
+__device__ __forceinline__ void page_step(const uint8_t* page, int tok0, int len, const int (&lim)[NT][2],
+                                          const uint32_t (&qf)[NT][8][2], const float (&cq)[NT][2], int lane,
+                                          ColState (&st)[NT]) {
   const int g = lane >> 2, j = lane >> 3, r8 = lane & 7;
   const int tok = (j & 1) * 8 + r8;
   const uint32_t kb = smem_u32(page), vb = kb + kKv8Side;
-  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  float s[NT][4];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
 #pragma unroll
   for (int c2 = 0; c2 < 4; ++c2) {
     uint32_t m0, m1, m2, m3;
     ldsm_x4(kb + kv8_chunk(tok, 2 * c2 + (j >> 1)), m0, m1, m2, m3);
-    mma_f16_16816(s, f16x2_lo(m0), f16x2_lo(m1), f16x2_hi(m0), f16x2_hi(m1), qf[2 * c2][0], qf[2 * c2][1]);
-    mma_f16_16816(s, f16x2_lo(m2), f16x2_lo(m3), f16x2_hi(m2), f16x2_hi(m3), qf[2 * c2 + 1][0], qf[2 * c2 + 1][1]);
+    const uint32_t a0 = f16x2_lo(m0), a1 = f16x2_lo(m1), a2 = f16x2_hi(m0), a3 = f16x2_hi(m1);
+    const uint32_t b0 = f16x2_lo(m2), b1 = f16x2_lo(m3), b2 = f16x2_hi(m2), b3 = f16x2_hi(m3);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      mma_f16_16816(s[n], a0, a1, a2, a3, qf[n][2 * c2][0], qf[n][2 * c2][1]);
+      mma_f16_16816(s[n], b0, b1, b2, b3, qf[n][2 * c2 + 1][0], qf[n][2 * c2 + 1][1]);
+    }
   }
   const uint8_t* sk = page + kKv8Page * kKv8Dim;
   const uint8_t* sv = sk + kKv8Side;
-  float z[4], w[4];
+  float w[NT][4];
   bool grow = false;
 #pragma unroll
   for (int hi = 0; hi < 2; ++hi) {
@@ -98,49 +126,59 @@ __device__ __forceinline__ void page_step(const uint8_t* page, int tok0, int len
     const int b = sv[tk];
     const float ev = b == 255 ? CUDART_NAN_F : static_cast<float>(b - 127);
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const bool see = tok0 + tk < lim[e];
-      z[2 * hi + e] = see ? s[2 * hi + e] * (ks * cq[e]) : -CUDART_INF_F;
-      w[2 * hi + e] = see ? z[2 * hi + e] + ev : -CUDART_INF_F;
-      grow |= z[2 * hi + e] > st.m[e] + kSlack || w[2 * hi + e] > st.bo[e] + kSlack;
-    }
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const bool see = tok0 + tk < lim[n][e];
+        float& z = s[n][2 * hi + e];
+        z = see ? z * (ks * cq[n][e]) : -CUDART_INF_F;
+        w[n][2 * hi + e] = see ? z + ev : -CUDART_INF_F;
+        grow |= z > st[n].m[e] + kSlack || w[n][2 * hi + e] > st[n].bo[e] + kSlack;
+      }
   }
   if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float zm = fmaxf(s[n][e], s[n][2 + e]), wm = fmaxf(w[n][e], w[n][2 + e]);
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) {
+          zm = fmaxf(zm, __shfl_xor_sync(0xffffffffu, zm, o));
+          wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, o));
+        }
+        ColState& c = st[n];
+        const float mn = fmaxf(c.m[e], zm), bn = fmaxf(c.bo[e], wm);
+        const float al = mn == -CUDART_INF_F ? 1.f : ex2(c.m[e] - mn);
+        const float be = bn == -CUDART_INF_F ? 1.f : ex2(c.bo[e] - bn);
+        c.m[e] = mn;
+        c.bo[e] = bn;
+        c.l[e] *= al;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          c.o[k][e] *= be;
+          c.o[k][2 + e] *= be;
+        }
+      }
+  }
+  uint32_t p0[NT], p1[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    float P[4];
+#pragma unroll
     for (int e = 0; e < 2; ++e) {
-      float zm = fmaxf(z[e], z[2 + e]), wm = fmaxf(w[e], w[2 + e]);
-#pragma unroll
-      for (int o = 4; o < 32; o <<= 1) {
-        zm = fmaxf(zm, __shfl_xor_sync(0xffffffffu, zm, o));
-        wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, o));
-      }
-      const float mn = fmaxf(st.m[e], zm), bn = fmaxf(st.bo[e], wm);
-      const float al = mn == -CUDART_INF_F ? 1.f : ex2(st.m[e] - mn);
-      const float be = bn == -CUDART_INF_F ? 1.f : ex2(st.bo[e] - bn);
-      st.m[e] = mn;
-      st.bo[e] = bn;
-      st.l[e] *= al;
-#pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        st.o[c][e] *= be;
-        st.o[c][2 + e] *= be;
-      }
+      const float mb = st[n].m[e] == -CUDART_INF_F ? 0.f : st[n].m[e];
+      const float bb = st[n].bo[e] == -CUDART_INF_F ? 0.f : st[n].bo[e] - kPBias;
+      st[n].l[e] += ex2(s[n][e] - mb) + ex2(s[n][2 + e] - mb);
+      P[e] = ex2(w[n][e] - bb);
+      P[2 + e] = ex2(w[n][2 + e] - bb);
     }
+    p0[n] = movmatrix_t(pack_f16x2(P[0], P[1]));
+    p1[n] = movmatrix_t(pack_f16x2(P[2], P[3]));
   }
-  float P[4];
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const float mb = st.m[e] == -CUDART_INF_F ? 0.f : st.m[e];
-    const float bb = st.bo[e] == -CUDART_INF_F ? 0.f : st.bo[e] - kPBias;
-    st.l[e] += ex2(z[e] - mb) + ex2(z[2 + e] - mb);
-    P[e] = ex2(w[e] - bb);
-    P[2 + e] = ex2(w[2 + e] - bb);
-  }
-  const uint32_t b0 = movmatrix_t(pack_f16x2(P[0], P[1])), b1 = movmatrix_t(pack_f16x2(P[2], P[3]));
-  const bool tail = tok0 + kKv8Page > len;
   const int t2 = (lane & 3) * 2;
   uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
-  if (tail) {  // codes past the sequence's end may be NaNs: P is 0 there, but 0 * NaN is not
+  if (tok0 + kKv8Page > len) {  // codes past the sequence's end may be NaNs: P is 0 there, but 0 * NaN is not
     keep0 = (tok0 + t2 < len ? 0x00ff00ffu : 0u) | (tok0 + t2 + 1 < len ? 0xff00ff00u : 0u);
     keep1 = (tok0 + t2 + 8 < len ? 0x00ff00ffu : 0u) | (tok0 + t2 + 9 < len ? 0xff00ff00u : 0u);
   }
@@ -153,26 +191,26 @@ __device__ __forceinline__ void page_step(const uint8_t* page, int tok0, int len
     m1 = __byte_perm(m1, 0, 0x3120) & keep1;
     m2 = __byte_perm(m2, 0, 0x3120) & keep0;
     m3 = __byte_perm(m3, 0, 0x3120) & keep1;
-    mma_f16_16816(st.o[2 * c2], f16x2_lo(m0), f16x2_hi(m0), f16x2_lo(m1), f16x2_hi(m1), b0, b1);
-    mma_f16_16816(st.o[2 * c2 + 1], f16x2_lo(m2), f16x2_hi(m2), f16x2_lo(m3), f16x2_hi(m3), b0, b1);
+    const uint32_t a0 = f16x2_lo(m0), a1 = f16x2_hi(m0), a2 = f16x2_lo(m1), a3 = f16x2_hi(m1);
+    const uint32_t b0 = f16x2_lo(m2), b1 = f16x2_hi(m2), b2 = f16x2_lo(m3), b3 = f16x2_hi(m3);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      mma_f16_16816(st[n].o[2 * c2], a0, a1, a2, a3, p0[n], p1[n]);
+      mma_f16_16816(st[n].o[2 * c2 + 1], b0, b1, b2, b3, p0[n], p1[n]);
+    }
   }
 }
 
-// Columns c = row * G + head-in-group of one tile: column base + g as this lane's B fragment.
-// q is scaled by a power of two so that the column's largest element is in [2^14, 2^15).
-__device__ __forceinline__ void load_columns(const Kv8AttnArgs& a, int row0, int kvh, int G, int ncols, int base,
-                                             int lane, uint32_t (&qf)[8][2], float (&cq)[2]) {
+// Column g of `q` (bf16 rows of 128 in shared memory, `real` of them) as this lane's B fragment,
+// times a power of two that brings the column's largest element to [2^14, 2^15).
+__device__ __forceinline__ void load_columns(const uint8_t* q, int real, float scale, int lane, uint32_t (&qf)[8][2],
+                                             float (&cq)[2]) {
   const int g = lane >> 2, t = lane & 3;
-  const int col = base + g;
   float x[32];
   float top = 0.f;
-  const bool real = col < ncols;
-  const int c = real ? col : 0;
-  const __nv_bfloat16* q =
-      a.q + static_cast<int64_t>(row0 + c / G) * a.q_stride + (static_cast<int64_t>(kvh) * G + c % G) * kKv8Dim + 4 * t;
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
-    const uint2 u = real ? *reinterpret_cast<const uint2*>(q + 16 * k) : make_uint2(0, 0);
+    const uint2 u = g < real ? *reinterpret_cast<const uint2*>(q + g * 256 + k * 32 + t * 8) : make_uint2(0, 0);
     x[4 * k] = __uint_as_float(u.x << 16);
     x[4 * k + 1] = __uint_as_float(u.x & 0xffff0000u);
     x[4 * k + 2] = __uint_as_float(u.y << 16);
@@ -193,163 +231,409 @@ __device__ __forceinline__ void load_columns(const Kv8AttnArgs& a, int row0, int
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     const int u = __shfl_sync(0xffffffffu, up, (2 * t + e) * 4);
-    cq[e] = a.scale * kLog2e * __uint_as_float(static_cast<uint32_t>(127 - u) << 23);
+    cq[e] = scale * kLog2e * __uint_as_float(static_cast<uint32_t>(127 - u) << 23);
   }
 }
 
-// grid: (splits, kv heads * column groups, tiles). Four warps take a page each in turn.
-__global__ void __launch_bounds__(kWarps * 32) kv8_attn_kernel(const Kv8AttnArgs a) {
+// One item of work: a sequence (decode) or a tile. Its segments are `units` = KV heads x groups of
+// `cols` columns, of `pages` pages each.
+struct Item {
+  int seq, row0, nq, pos0, len, pages, groups, units;
+};
+template <int NT>
+__device__ __forceinline__ Item get_item(const Kv8AttnArgs& a, int s) {
+  Item it;
+  if (a.tiles) {
+    const int4 t = a.tiles[s];
+    it.seq = t.x, it.row0 = t.y, it.nq = max(t.z, 0), it.pos0 = t.w;
+    if (!kv8_tile_ok(a, t)) it.seq = it.row0 = it.nq = 0;
+  } else {
+    it.seq = it.row0 = s, it.nq = 1, it.pos0 = 0;
+  }
+  it.len = max(0, min(a.seq_lens[it.seq], a.max_blocks * kKv8Page));
+  if (!a.tiles) it.pos0 = it.len - 1;
+  const int G = a.n_q_heads / a.n_kv_heads;
+  it.groups = (it.nq * G + 8 * NT - 1) / (8 * NT);
+  it.units = a.n_kv_heads * it.groups;
+  it.pages = it.nq > 0 ? (max(0, min(it.len, it.pos0 + it.nq)) + kKv8Page - 1) / kKv8Page : 0;
+  return it;
+}
+
+// Place `at` of the laid-out pages: the item and the page within it (unit * pages + page). Every
+// lane of the warp calls it; a place past the end gives item == items.
+struct Place {
+  int item;
+  int64_t in_item;
+};
+template <int NT>
+__device__ __forceinline__ int64_t total_pages(const Kv8AttnArgs& a, int items, int lane) {
+  int64_t sum = 0;
+  for (int s = lane; s < items; s += 32) {
+    const Item it = get_item<NT>(a, s);
+    sum += static_cast<int64_t>(it.pages) * it.units;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return sum;
+}
+template <int NT>
+__device__ __forceinline__ Place find_place(const Kv8AttnArgs& a, int items, int64_t at, int lane) {
+  int64_t base = 0;
+  for (int s0 = 0; s0 < items; s0 += 32) {
+    int64_t n = 0;
+    if (s0 + lane < items) {
+      const Item it = get_item<NT>(a, s0 + lane);
+      n = static_cast<int64_t>(it.pages) * it.units;
+    }
+    int64_t sum = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t up = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += up;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, base + sum > at);
+    if (hit) {
+      const int l = __ffs(hit) - 1;
+      return {s0 + l, at - base - __shfl_sync(0xffffffffu, sum - n, l)};
+    }
+    base += __shfl_sync(0xffffffffu, sum, 31);
+  }
+  return {items, 0};
+}
+// Pages per CTA run; below 32 a run is not worth its joining.
+__device__ __forceinline__ int64_t run_pages(int64_t total, int ctas) {
+  const int64_t per = (total + ctas - 1) / ctas;
+  return per < 32 ? 32 : per;
+}
+
+__device__ __forceinline__ float base_or_zero(float x) { return x == -CUDART_INF_F ? 0.f : x; }
+__device__ __forceinline__ float factor(float x, float to) { return x == -CUDART_INF_F ? 1.f : ex2(x - to); }
+
+// The pieces that a CTA's run cuts out of the segments, in order. Loader and consumers walk the same.
+template <int NT>
+struct Walk {
+  int s;            // item
+  Item it;
+  int64_t left;     // pages left in the run
+  int unit, page;   // next piece
+  __device__ void start(const Kv8AttnArgs& a, int item, int64_t in_item, int64_t n) {
+    s = item;
+    left = n;
+    if (n <= 0) return;
+    it = get_item<NT>(a, s);
+    unit = static_cast<int>(in_item / it.pages);
+    page = static_cast<int>(in_item % it.pages);
+  }
+  // Pages of the current piece.
+  __device__ int count() const { return static_cast<int>(min(static_cast<int64_t>(it.pages - page), left)); }
+  __device__ void next(const Kv8AttnArgs& a) {
+    left -= count();
+    page = 0;
+    if (left > 0 && ++unit == it.units) {
+      unit = 0;
+      do it = get_item<NT>(a, ++s);
+      while (it.pages == 0);
+    }
+  }
+};
+
+template <int NT>
+__global__ void __launch_bounds__(kThreads, 2) kv8_attn_kernel(const Kv8AttnArgs a, const int whole) {
+  using S = Smem<NT>;
   extern __shared__ __align__(128) uint8_t smem[];
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kBarOff);
-  float* mo = reinterpret_cast<float*>(smem + kMergeOff);
-  float* ms = reinterpret_cast<float*>(smem + kStatOff);  // [warp][col][m, bo, l]
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kBar);
+  uint64_t* empty = full + S::kSlots;
+  uint64_t* q_full = empty + S::kSlots;
+  uint64_t* q_empty = q_full + 2;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = a.n_q_heads / a.n_kv_heads;
-  int seq, row0, nq, pos0;
-  if (a.tiles) {
-    const int4 t = a.tiles[blockIdx.z];
-    seq = t.x, row0 = t.y, nq = t.z, pos0 = t.w;
-  } else {
-    seq = row0 = blockIdx.z, nq = 1, pos0 = 0;
-  }
-  const int kvh = blockIdx.y;
-  const int len = min(a.seq_lens[seq], a.max_blocks * kKv8Page);
-  if (!a.tiles) pos0 = len - 1;
-  const int ncols = nq * G;
-  const int nblk = (max(len, 0) + kKv8Page - 1) / kKv8Page;
-  const int per = (nblk + a.splits - 1) / a.splits;
-  const int b0 = blockIdx.x * per, b1 = min(nblk, b0 + per);
-  const int n = max(0, b1 - b0);
-  const int* bt = a.block_tables + static_cast<int64_t>(seq) * a.bt_stride;
+  const int items = a.tiles ? a.num_tiles : a.num_seqs;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kSlots; ++i) mbar_init(&full[i], 1);
+    for (int i = 0; i < S::kSlots; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], kWarps);
+    }
     fence_mbar_init();
   }
   __syncthreads();
-  const uint8_t* base = a.arena + a.layer_offset + static_cast<int64_t>(kvh) * kKv8Head;
-  int issued = 0;  // pages of this warp issued since the kernel's start (warp w owns slots w, w + 4, ...)
-  int used = 0;
-  bool ok = true;
-  constexpr int kOwn = kSlots / kWarps;
-  for (int cb = 0; cb < ncols; cb += kCols) {
-    uint32_t qf[8][2];
-    float cq[2];
-    load_columns(a, row0, kvh, G, ncols, cb, lane, qf, cq);
-    ColState st;
-#pragma unroll
-    for (int c = 0; c < 8; ++c)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) st.o[c][e] = 0.f;
-    int lim[2];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      st.m[e] = st.bo[e] = -CUDART_INF_F;
-      st.l[e] = 0.f;
-      const int col = cb + (lane & 3) * 2 + e;
-      lim[e] = col < ncols ? min(len, pos0 + col / G + 1) : 0;
-    }
-    auto issue = [&](int i) {  // lane 0: page b0 + warp + i * kWarps into the warp's next slot
-      const int slot = (issued % kOwn) * kWarps + warp;
-      int page = bt[b0 + warp + i * kWarps];
-      if (page < 0 || page >= a.num_blocks) {
-        record_error(a.status, kErrBounds);
-        page = 0;
+  asm volatile("griddepcontrol.launch_dependents;");
+
+  Walk<NT> w;
+  int64_t run0 = 0, per = 0;
+  if (whole) {  // CTA = (KV head, item)
+    const Item it = get_item<NT>(a, blockIdx.y);
+    w.start(a, blockIdx.y, static_cast<int64_t>(blockIdx.x) * it.groups * it.pages,
+            static_cast<int64_t>(it.groups) * it.pages);
+  } else {
+    const int64_t total = total_pages<NT>(a, items, lane);
+    per = run_pages(total, gridDim.x);
+    run0 = blockIdx.x * per;
+    const Place p = find_place<NT>(a, items, run0, lane);
+    w.start(a, p.item, p.in_item, max(int64_t(0), min(per, total - run0)));
+  }
+
+  if (warp == kWarps) {
+    // -------------------------------------------------------------- loader
+    bool ok = true;
+    int n = 0;  // pages so far
+    for (int piece = 0; w.left > 0 && ok; ++piece, w.next(a)) {
+      const int kvh = w.unit / w.it.groups, cg = w.unit % w.it.groups;
+      const int cnt = w.count();
+      // queries: the group's columns c = row * G + head, bf16 rows of 256 bytes; a row's heads are contiguous
+      {
+        const int qb = piece & 1, c0 = cg * S::kCols, c1 = min(w.it.nq * G, c0 + S::kCols);
+        ok = mbar_wait(&q_empty[qb], ((piece >> 1) & 1) ^ 1, nullptr, a.status);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (lane == 0) mbar_expect_tx(&q_full[qb], (c1 - c0) * 256);
+        __syncwarp();
+        for (int c = c0 + lane; c < c1; c += 32)
+          bulk_load(smem + S::kQ + (qb * S::kCols + c - c0) * 256,
+                    a.q + static_cast<int64_t>(w.it.row0 + c / G) * a.q_stride +
+                        (static_cast<int64_t>(kvh) * G + c % G) * kKv8Dim,
+                    256, &q_full[qb]);
       }
-      mbar_expect_tx(&full[slot], kKv8Head);
-      bulk_load(smem + slot * kKv8Head, base + page * a.block_bytes, kKv8Head, &full[slot]);
-      ++issued;
-    };
-    const int mine = n > warp ? (n - warp + kWarps - 1) / kWarps : 0;
-    if (lane == 0)
-      for (int i = 0; i < min(mine, kOwn); ++i) issue(i);
-    for (int i = 0; i < mine; ++i) {
-      const int slot = (used % kOwn) * kWarps + warp;
-      ok = __all_sync(0xffffffffu, ok && mbar_wait(&full[slot], (used / kOwn) & 1, nullptr, a.status));
-      if (!ok) break;
-      page_step(smem + slot * kKv8Head, (b0 + warp + i * kWarps) * kKv8Page, len, lim, qf, cq, lane, st);
-      __syncwarp();
-      ++used;
-      if (lane == 0 && i + kOwn < mine) issue(i + kOwn);  // every lane has read the slot
+      const int* bt = a.block_tables + static_cast<int64_t>(w.it.seq) * a.bt_stride + w.page;
+      const uint8_t* base = a.arena + a.layer_offset + static_cast<int64_t>(kvh) * kKv8Head;
+      int ids = lane < cnt ? bt[lane] : 0;
+      for (int i0 = 0; i0 < cnt && ok; i0 += 32) {
+        int now = ids;
+        if (i0 + 32 + lane < cnt) ids = bt[i0 + 32 + lane];
+        if (i0 + lane < cnt && (now < 0 || now >= a.num_blocks)) {
+          record_error(a.status, kErrBounds);
+          now = 0;
+        }
+        const int m = min(32, cnt - i0);
+        for (int i = 0; i < m; ++i, ++n) {
+          const int slot = n % S::kSlots;
+          const int id = __shfl_sync(0xffffffffu, now, i);
+          if (lane == 0) {
+            ok = ok && mbar_wait(&empty[slot], ((n / S::kSlots) & 1) ^ 1, nullptr, a.status);
+            if (ok) {
+              mbar_expect_tx(&full[slot], kKv8Head);
+              bulk_load(smem + slot * kKv8Head, base + id * a.block_bytes, kKv8Head, &full[slot]);
+            }
+          }
+        }
+        ok = __all_sync(0xffffffffu, ok);
+      }
     }
+    return;
+  }
+
+  // ---------------------------------------------------------------- consumers
+  float* mo = reinterpret_cast<float*>(smem + S::kO);
+  float* ms = reinterpret_cast<float*>(smem + S::kStat);
+  const int g = lane >> 2, t2 = (lane & 3) * 2;
+  // rows of sequences without keys
+  for (int s = whole ? blockIdx.y : blockIdx.x; s < items; s += whole ? items : gridDim.x) {
+    const Item it = get_item<NT>(a, s);
+    if (it.pages > 0) continue;
+    const int h0 = whole ? blockIdx.x * G : 0, nh = whole ? G : a.n_q_heads;
+    for (int i = threadIdx.x; i < it.nq * nh * kKv8Dim; i += kWarps * 32)
+      a.out[static_cast<int64_t>(it.row0 + i / (nh * kKv8Dim)) * a.out_stride + h0 * kKv8Dim + i % (nh * kKv8Dim)] =
+          __float2bfloat16(0.f);
+  }
+  bool ok = true;
+  int n = 0;
+  for (int piece = 0; w.left > 0; ++piece, w.next(a)) {
+    const Item& it = w.it;
+    const int kvh = w.unit / it.groups, cb = w.unit % it.groups * S::kCols;
+    const int ncols = min(S::kCols, it.nq * G - cb);
+    const int cnt = w.count();
+    uint32_t qf[NT][8][2];
+    float cq[NT][2];
+    int lim[NT][2];
+    ColState st[NT];
+    const int qb = piece & 1;
+    ok = __all_sync(0xffffffffu, ok && mbar_wait(&q_full[qb], (piece >> 1) & 1, nullptr, a.status));
 #pragma unroll
-    for (int e = 0; e < 2; ++e)
+    for (int k = 0; k < NT; ++k) {
+      load_columns(smem + S::kQ + (qb * S::kCols + 8 * k) * 256, ncols - 8 * k, a.scale, lane, qf[k], cq[k]);
 #pragma unroll
-      for (int o = 4; o < 32; o <<= 1) st.l[e] += __shfl_xor_sync(0xffffffffu, st.l[e], o);
-    const int g = lane >> 2, t2 = (lane & 3) * 2;
+      for (int c = 0; c < 8; ++c)
 #pragma unroll
-    for (int c = 0; c < 8; ++c)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        mo[(warp * kCols + t2 + (e & 1)) * kKv8Dim + 16 * c + 2 * g + (e >> 1)] = st.o[c][e];
-    if (g == 0)
+        for (int e = 0; e < 4; ++e) st[k].o[c][e] = 0.f;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float* d = ms + (warp * kCols + t2 + e) * 3;
-        d[0] = st.m[e], d[1] = st.bo[e], d[2] = st.l[e];
-      }
-    __syncthreads();
-    for (int idx = threadIdx.x; idx < min(kCols, ncols - cb) * kKv8Dim; idx += kWarps * 32) {
-      const int col = idx / kKv8Dim, d = idx % kKv8Dim;
-      float M = -CUDART_INF_F, B = -CUDART_INF_F;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        M = fmaxf(M, ms[(w * kCols + col) * 3]);
-        B = fmaxf(B, ms[(w * kCols + col) * 3 + 1]);
-      }
-      float acc = 0.f, L = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float* x = ms + (w * kCols + col) * 3;
-        const float fm = x[0] == -CUDART_INF_F ? 1.f : ex2(x[0] - M), fb = x[1] == -CUDART_INF_F ? 1.f : ex2(x[1] - B);
-        L += x[2] * fm;
-        acc += mo[(w * kCols + col) * kKv8Dim + d] * fb;
-      }
-      const int gc = cb + col;
-      const int row = row0 + gc / G, head = kvh * G + gc % G;
-      if (a.splits == 1) {
-        const float o = L == 0.f ? 0.f : acc / L * ex2((B == -CUDART_INF_F ? 0.f : B) - (M == -CUDART_INF_F ? 0.f : M) - kPBias);
-        a.out[static_cast<int64_t>(row) * a.out_stride + head * kKv8Dim + d] = __float2bfloat16(o);
-      } else {
-        const int64_t part = (static_cast<int64_t>(row) * a.n_q_heads + head) * a.splits + blockIdx.x;
-        a.ws_o[part * kKv8Dim + d] = acc;
-        if (d == 0) {
-          float* x = a.ws_ml + part * 4;
-          x[0] = M, x[1] = B, x[2] = L;
-        }
+        st[k].m[e] = st[k].bo[e] = -CUDART_INF_F;
+        st[k].l[e] = 0.f;
+        const int col = 8 * k + t2 + e;
+        lim[k][e] = col < ncols ? min(it.len, it.pos0 + (cb + col) / G + 1) : 0;
       }
     }
-    __syncthreads();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&q_empty[qb]);
+    for (int i = (warp - n % kWarps + kWarps) % kWarps; i < cnt; i += kWarps) {
+      const int slot = (n + i) % S::kSlots;
+      ok = __all_sync(0xffffffffu, ok && mbar_wait(&full[slot], ((n + i) / S::kSlots) & 1, nullptr, a.status));
+      if (!ok) break;
+      page_step<NT>(smem + slot * kKv8Head, (w.page + i) * kKv8Page, it.len, lim, qf, cq, lane, st);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[slot]);
+    }
+    n += cnt;
+    // join the four warps' sums
+#pragma unroll
+    for (int k = 0; k < NT; ++k) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) st[k].l[e] += __shfl_xor_sync(0xffffffffu, st[k].l[e], o);
+      float* d = mo + (warp * S::kCols + 8 * k + t2) * kKv8Dim + 2 * g;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        *reinterpret_cast<float2*>(d + 16 * c) = make_float2(st[k].o[c][0], st[k].o[c][2]);
+        *reinterpret_cast<float2*>(d + kKv8Dim + 16 * c) = make_float2(st[k].o[c][1], st[k].o[c][3]);
+      }
+      if (g == 0)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float* x = ms + (warp * S::kCols + 8 * k + t2 + e) * 3;
+          x[0] = st[k].m[e], x[1] = st[k].bo[e], x[2] = st[k].l[e];
+        }
+    }
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    const bool entire = cnt == it.pages;
+    const int64_t part = (2 * static_cast<int64_t>(blockIdx.x) + (piece > 0)) * S::kCols;
+    for (int col = warp; col < ncols; col += kWarps) {
+      float M = -CUDART_INF_F, B = -CUDART_INF_F;
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) {
+        M = fmaxf(M, ms[(k * S::kCols + col) * 3]);
+        B = fmaxf(B, ms[(k * S::kCols + col) * 3 + 1]);
+      }
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      float L = 0.f;
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) {
+        const float* x = ms + (k * S::kCols + col) * 3;
+        L += x[2] * factor(x[0], M);
+        const float f = factor(x[1], B);
+        const float4 v = *reinterpret_cast<const float4*>(mo + (k * S::kCols + col) * kKv8Dim + 4 * lane);
+        acc.x += v.x * f;
+        acc.y += v.y * f;
+        acc.z += v.z * f;
+        acc.w += v.w * f;
+      }
+      if (entire) {
+        const int c = cb + col;
+        const float f = L == 0.f ? 0.f : ex2(base_or_zero(B) - base_or_zero(M) - kPBias) / L;
+        *reinterpret_cast<uint2*>(a.out + static_cast<int64_t>(it.row0 + c / G) * a.out_stride +
+                                  (kvh * G + c % G) * kKv8Dim + 4 * lane) =
+            make_uint2(pack_bf16x2(acc.x * f, acc.y * f), pack_bf16x2(acc.z * f, acc.w * f));
+      } else {
+        *reinterpret_cast<float4*>(a.ws_o + (part + col) * kKv8Dim + 4 * lane) = acc;
+        if (lane == 0) *reinterpret_cast<float4*>(a.ws_ml + (part + col) * 4) = make_float4(M, B, L, 0.f);
+      }
+    }
+    asm volatile("bar.sync 1, 128;" ::: "memory");
   }
 }
 
-__global__ void __launch_bounds__(kKv8Dim) kv8_combine_kernel(const Kv8AttnArgs a) {
-  const int head = blockIdx.x, row = blockIdx.y, d = threadIdx.x;
-  const int64_t base = (static_cast<int64_t>(row) * a.n_q_heads + head) * a.splits;
-  float M = -CUDART_INF_F, B = -CUDART_INF_F;
-  for (int s = 0; s < a.splits; ++s) {
-    M = fmaxf(M, a.ws_ml[(base + s) * 4]);
-    B = fmaxf(B, a.ws_ml[(base + s) * 4 + 1]);
+// Joins the segment that begins in CTA run c and ends in a later one (CTA c of this kernel). Its
+// first piece is c's last one, the others are the first pieces of the runs c + 1, c + 2, ...
+template <int NT>
+__global__ void __launch_bounds__(256) kv8_join_kernel(const Kv8AttnArgs a) {
+  constexpr int kCols = 8 * NT;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int G = a.n_q_heads / a.n_kv_heads;
+  const int items = a.tiles ? a.num_tiles : a.num_seqs;
+  // lengths and tiles are not the first kernel's to write: the search needs no wait
+  const int64_t total = total_pages<NT>(a, items, lane);
+  const int64_t per = run_pages(total, gridDim.x);
+  const int64_t last = (blockIdx.x + 1) * per - 1;  // the run's last page
+  if (last + 1 >= total) return;
+  const Place p = find_place<NT>(a, items, last, lane);
+  const Item it = get_item<NT>(a, p.item);
+  const int unit = static_cast<int>(p.in_item / it.pages);
+  const int64_t first = last - p.in_item % it.pages;  // the segment's first page
+  const int64_t end = first + it.pages;
+  if (first < last + 1 - per || end <= last + 1) return;  // begins in an earlier run, or ends here
+  const int pieces = static_cast<int>((end - 1) / per - blockIdx.x) + 1;
+  const int slot0 = 2 * static_cast<int>(blockIdx.x) + (first > last + 1 - per);
+  const int kvh = unit / it.groups, cb = unit % it.groups * kCols;
+  const int ncols = min(kCols, it.nq * G - cb);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  for (int col = warp; col < ncols; col += 8) {
+    // as in the first kernel, the bases first; lane i looks at piece i, i + 32, ...
+    float M = -CUDART_INF_F, B = -CUDART_INF_F;
+    auto slot = [&](int i) { return static_cast<int64_t>(i == 0 ? slot0 : 2 * (static_cast<int>(blockIdx.x) + i)) * kCols + col; };
+    for (int i = lane; i < pieces; i += 32) {
+      const float4 x = *reinterpret_cast<const float4*>(a.ws_ml + slot(i) * 4);
+      M = fmaxf(M, x.x);
+      B = fmaxf(B, x.y);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+      B = fmaxf(B, __shfl_xor_sync(0xffffffffu, B, o));
+    }
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float L = 0.f;
+    for (int i = 0; i < pieces; ++i) {
+      const float4 x = *reinterpret_cast<const float4*>(a.ws_ml + slot(i) * 4);
+      const float4 v = *reinterpret_cast<const float4*>(a.ws_o + slot(i) * kKv8Dim + 4 * lane);
+      L += x.z * factor(x.x, M);
+      const float f = factor(x.y, B);
+      acc.x += v.x * f;
+      acc.y += v.y * f;
+      acc.z += v.z * f;
+      acc.w += v.w * f;
+    }
+    const int c = cb + col;
+    const float f = L == 0.f ? 0.f : ex2(base_or_zero(B) - base_or_zero(M) - kPBias) / L;
+    *reinterpret_cast<uint2*>(a.out + static_cast<int64_t>(it.row0 + c / G) * a.out_stride +
+                              (kvh * G + c % G) * kKv8Dim + 4 * lane) =
+        make_uint2(pack_bf16x2(acc.x * f, acc.y * f), pack_bf16x2(acc.z * f, acc.w * f));
   }
-  float acc = 0.f, L = 0.f;
-  for (int s = 0; s < a.splits; ++s) {
-    const float* x = a.ws_ml + (base + s) * 4;
-    L += x[2] * (x[0] == -CUDART_INF_F ? 1.f : ex2(x[0] - M));
-    acc += a.ws_o[(base + s) * kKv8Dim + d] * (x[1] == -CUDART_INF_F ? 1.f : ex2(x[1] - B));
+}
+
+template <int NT>
+int launch(const Kv8AttnArgs& a, cudaStream_t stream) {
+  const int items = a.tiles ? a.num_tiles : a.num_seqs;
+  if (int e = ensure_smem_attr(reinterpret_cast<const void*>(kv8_attn_kernel<NT>), Smem<NT>::kBytes)) return e;
+  if (a.max_blocks <= kWholePages) {
+    kv8_attn_kernel<NT><<<dim3(a.n_kv_heads, items), kThreads, Smem<NT>::kBytes, stream>>>(a, 1);
+    return cudaGetLastError();
   }
-  const float o = L == 0.f ? 0.f : acc / L * ex2((B == -CUDART_INF_F ? 0.f : B) - (M == -CUDART_INF_F ? 0.f : M) - kPBias);
-  a.out[static_cast<int64_t>(row) * a.out_stride + head * kKv8Dim + d] = __float2bfloat16(o);
+  const int ctas = kv8_attention_ctas();
+  kv8_attn_kernel<NT><<<ctas, kThreads, Smem<NT>::kBytes, stream>>>(a, 0);
+  if (int e = cudaGetLastError()) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;  // its prologue runs while the first kernel ends
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kv8_join_kernel<NT>, a);
 }
 
 }  // namespace
 
+int kv8_attention_ctas() { return 2 * num_sms(); }
+
+int64_t kv8_attention_ws_floats(const Kv8AttnArgs& a) {
+  return a.max_blocks <= kWholePages ? 0 : int64_t(2) * kv8_attention_ctas() * 8 * kv8_attention_groups(a) * (kKv8Dim + 4);
+}
+
+// Columns of 8 that a CTA holds at once: two where a tile has more than 8 columns on average.
+int kv8_attention_groups(const Kv8AttnArgs& a) {
+  const int64_t cols = static_cast<int64_t>(a.n_q_heads / a.n_kv_heads) * (a.tiles ? (a.num_rows + a.num_tiles - 1) / a.num_tiles : 1);
+  return cols > 8 ? 2 : 1;
+}
+
 int kv8_attention(const Kv8AttnArgs& a, cudaStream_t stream) {
-  const int items = a.tiles ? a.num_tiles : a.num_seqs;
-  if (items <= 0) return 0;
-  if (int e = ensure_smem_attr(reinterpret_cast<const void*>(kv8_attn_kernel), kSmem)) return e;
-  kv8_attn_kernel<<<dim3(a.splits, a.n_kv_heads, items), kWarps * 32, kSmem, stream>>>(a);
-  if (a.splits > 1) kv8_combine_kernel<<<dim3(a.n_q_heads, a.num_rows), kKv8Dim, 0, stream>>>(a);
-  return cudaGetLastError();
+  if ((a.tiles ? a.num_tiles : a.num_seqs) <= 0) return 0;
+  return kv8_attention_groups(a) == 2 ? launch<2>(a, stream) : launch<1>(a, stream);
 }
 
 }  // namespace lakeb

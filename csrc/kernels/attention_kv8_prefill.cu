@@ -158,6 +158,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int4 tile = a.tiles[a.num_tiles - 1 - static_cast<int>(blockIdx.x)];
   const int seq = tile.x, qrow0 = tile.y, nq = tile.z, pos0 = tile.w;
   if (nq <= 0) return;
+  if (!kv8_tile_ok(a, tile)) return;
   if (smem_u32(smem) & 1023) {  // the swizzled tiles need it; the launch gives it
     if (threadIdx.x == 0) record_error(a.status, kErrBadArg);
     return;

@@ -15,6 +15,7 @@
 #include <cuda_fp16.h>
 
 #include "common.cuh"
+#include "lakeb_kernels.h"
 
 namespace lakeb {
 
@@ -40,6 +41,13 @@ __device__ __forceinline__ float kv8_inv_scale(int b) {
 // 2^(b - 127); NaN for b = 255 (b = 0 counts as 0: an arena that was never written reads as zeros).
 __device__ __forceinline__ float kv8_scale(int b) {
   return __uint_as_float(b == 255 ? 0x7fffffffu : static_cast<uint32_t>(b) << 23);
+}
+
+// A query tile names a sequence and rows of the call (otherwise it is reported and skipped).
+__device__ __forceinline__ bool kv8_tile_ok(const Kv8AttnArgs& a, const int4& t) {
+  const bool ok = t.z <= 0 || (t.x >= 0 && t.x < a.num_seqs && t.y >= 0 && t.y < a.num_rows && t.z <= a.num_rows - t.y && t.w >= 0);
+  if (!ok) record_error(a.status, kErrBounds);
+  return ok;
 }
 
 // Two fp32 -> two e4m3 codes (round to nearest even), lo in the low byte.

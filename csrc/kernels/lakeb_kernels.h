@@ -231,12 +231,17 @@ struct Kv8AttnArgs {
   float scale = 0.f;
   const int4* tiles = nullptr;  // (seq, first query row, number of queries, position of the first)
   int num_tiles = 0;
-  int splits = 1;
-  float* ws_o = nullptr;   // [num_rows, n_q_heads, splits, 128]
-  float* ws_ml = nullptr;  // [num_rows, n_q_heads, splits, 4]
+  // pieces of segments cut between CTAs (kv8_attention_ws_floats; ws_ml follows ws_o): per CTA two
+  // pieces of 8 x kv8_attention_groups columns, 128 sums and 4 statistics each
+  float* ws_o = nullptr;
+  float* ws_ml = nullptr;
   int* status = nullptr;
 };
+// Few query rows per sequence (any number is right; large tiles belong to kv8_prefill_tc).
 int kv8_attention(const Kv8AttnArgs& a, cudaStream_t stream);
+int kv8_attention_ctas();
+int kv8_attention_groups(const Kv8AttnArgs& a);
+int64_t kv8_attention_ws_floats(const Kv8AttnArgs& a);
 // Query tiles of <= 128 rows on the tcgen05 tensor cores.
 int kv8_prefill_tc(const Kv8AttnArgs& a, cudaStream_t stream);
 
