@@ -25,7 +25,9 @@
 // block table is wider than kWholePages, a CTA takes a whole segment and there is no second kernel.
 //
 // In a CTA one warp copies pages into a ring (bulk copies of 4128 bytes, page ids fetched 32 at a
-// time, queries of the next segment ahead) and four warps take the pages in turn.
+// time, queries of the next segment ahead) and the others take pairs of pages in turn: a page alone
+// is a chain of dependent products, exponentials and products of ~1400 cycles, two at once cost
+// little more than one.
 #include <math_constants.h>
 
 #include "common.cuh"
@@ -37,8 +39,6 @@
 namespace lakeb {
 namespace {
 
-constexpr int kWarps = 4;                     // consumers; warp 4 loads
-constexpr int kThreads = kWarps * 32 + 32;
 constexpr int kWholePages = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.f;  // a base trails the true maximum by at most this
@@ -49,12 +49,17 @@ constexpr float kPBias = 7.f;  // P = 2^(w - bo + 7): fp16 subnormals begin at 2
 template <int NT>
 struct Smem {
   static constexpr int kCols = 8 * NT;
-  static constexpr int kSlots = NT == 1 ? 20 : 16;  // pages; a multiple of kWarps
-  static constexpr int kQ = kSlots * kKv8Head;
+  static constexpr int kWarps = NT == 1 ? 5 : 4;  // consumers; one more warp loads
+  static constexpr int kThreads = kWarps * 32 + 32;
+  static constexpr int kSlots = NT == 1 ? 10 : 8;  // pairs of pages
+  static constexpr int kQ = kSlots * 2 * kKv8Head;
   static constexpr int kO = kQ + 2 * kCols * 256;
   static constexpr int kStat = kO + kWarps * kCols * kKv8Dim * 4;  // [warp][col][m, bo, l]
   static constexpr int kBar = kStat + kWarps * kCols * 3 * 4;
   static constexpr int kBytes = kBar + (2 * kSlots + 4) * 8;
+  // A slot belongs to one warp: pairs land out of order, and a warp that had not itself waited for
+  // the slot's last phase could take it for the one it waits for.
+  static_assert(kSlots % kWarps == 0, "");
   static_assert(kQ % 16 == 0 && kO % 16 == 0 && kBar % 8 == 0 && kBytes <= 113 * 1024, "");
 };
 
@@ -89,59 +94,68 @@ struct ColState {
   float m[2], bo[2], l[2];  // bases and this lane's part of the sum of p
 };
 
-// Adds one page (16 tokens from tok0) to the states. lim[n][e]: keys of column 8n+2t+e end before
-// it; len: tokens from len on are not the sequence's (their bytes may be anything).
+// Adds a pair of pages (32 tokens from tok0) to the states. lim[n][e]: keys of column 8n+2t+e end
+// before it; len: tokens from len on are not the sequence's (their bytes may be anything).
 template <int NT>
-__device__ __forceinline__ void page_step(const uint8_t* page, int tok0, int len, const int (&lim)[NT][2],
+__device__ __forceinline__ void pair_step(const uint8_t* pages, int tok0, int len, const int (&lim)[NT][2],
                                           const uint32_t (&qf)[NT][8][2], const float (&cq)[NT][2], int lane,
                                           ColState (&st)[NT]) {
   const int g = lane >> 2, j = lane >> 3, r8 = lane & 7;
   const int tok = (j & 1) * 8 + r8;
-  const uint32_t kb = smem_u32(page), vb = kb + kKv8Side;
-  float s[NT][4];
+  const uint32_t kb = smem_u32(pages), vb = kb + kKv8Side;
+  float s[2][NT][4];
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
-#pragma unroll
-  for (int c2 = 0; c2 < 4; ++c2) {
-    uint32_t m0, m1, m2, m3;
-    ldsm_x4(kb + kv8_chunk(tok, 2 * c2 + (j >> 1)), m0, m1, m2, m3);
-    const uint32_t a0 = f16x2_lo(m0), a1 = f16x2_lo(m1), a2 = f16x2_hi(m0), a3 = f16x2_hi(m1);
-    const uint32_t b0 = f16x2_lo(m2), b1 = f16x2_lo(m3), b2 = f16x2_hi(m2), b3 = f16x2_hi(m3);
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      mma_f16_16816(s[n], a0, a1, a2, a3, qf[n][2 * c2][0], qf[n][2 * c2][1]);
-      mma_f16_16816(s[n], b0, b1, b2, b3, qf[n][2 * c2 + 1][0], qf[n][2 * c2 + 1][1]);
-    }
-  }
-  const uint8_t* sk = page + kKv8Page * kKv8Dim;
-  const uint8_t* sv = sk + kKv8Side;
-  float w[NT][4];
-  bool grow = false;
-#pragma unroll
-  for (int hi = 0; hi < 2; ++hi) {
-    const int tk = g + 8 * hi;
-    const float ks = kv8_scale(sk[tk]);
-    const int b = sv[tk];
-    const float ev = b == 255 ? CUDART_NAN_F : static_cast<float>(b - 127);
+  for (int p = 0; p < 2; ++p)
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const bool see = tok0 + tk < lim[n][e];
-        float& z = s[n][2 * hi + e];
-        z = see ? z * (ks * cq[n][e]) : -CUDART_INF_F;
-        w[n][2 * hi + e] = see ? z + ev : -CUDART_INF_F;
-        grow |= z > st[n].m[e] + kSlack || w[n][2 * hi + e] > st[n].bo[e] + kSlack;
+      for (int e = 0; e < 4; ++e) s[p][n][e] = 0.f;
+#pragma unroll
+  for (int c2 = 0; c2 < 4; ++c2)
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      uint32_t m0, m1, m2, m3;
+      ldsm_x4(kb + p * kKv8Head + kv8_chunk(tok, 2 * c2 + (j >> 1)), m0, m1, m2, m3);
+      const uint32_t a0 = f16x2_lo(m0), a1 = f16x2_lo(m1), a2 = f16x2_hi(m0), a3 = f16x2_hi(m1);
+      const uint32_t b0 = f16x2_lo(m2), b1 = f16x2_lo(m3), b2 = f16x2_hi(m2), b3 = f16x2_hi(m3);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        mma_f16_16816(s[p][n], a0, a1, a2, a3, qf[n][2 * c2][0], qf[n][2 * c2][1]);
+        mma_f16_16816(s[p][n], b0, b1, b2, b3, qf[n][2 * c2 + 1][0], qf[n][2 * c2 + 1][1]);
       }
-  }
+    }
+  float ev[2][2];
+  bool grow = false;
+#pragma unroll
+  for (int p = 0; p < 2; ++p)
+#pragma unroll
+    for (int hi = 0; hi < 2; ++hi) {
+      const int tk = g + 8 * hi;
+      const uint8_t* sk = pages + p * kKv8Head + kKv8Page * kKv8Dim + tk;
+      const float ks = kv8_scale(*sk);
+      const int b = sk[kKv8Side];
+      ev[p][hi] = b == 255 ? CUDART_NAN_F : static_cast<float>(b - 127);
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float& z = s[p][n][2 * hi + e];
+          z = tok0 + 16 * p + tk < lim[n][e] ? z * (ks * cq[n][e]) : -CUDART_INF_F;
+          grow |= z > st[n].m[e] + kSlack || z + ev[p][hi] > st[n].bo[e] + kSlack;
+        }
+    }
+  // w = z + ev: -inf where the key is not seen, whatever its scale byte is
+  auto w = [&](int p, int n, int x) {
+    const float z = s[p][n][x];
+    return z == -CUDART_INF_F ? z : z + ev[p][x >> 1];
+  };
   if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float zm = fmaxf(s[n][e], s[n][2 + e]), wm = fmaxf(w[n][e], w[n][2 + e]);
+        float zm = fmaxf(fmaxf(s[0][n][e], s[0][n][2 + e]), fmaxf(s[1][n][e], s[1][n][2 + e]));
+        float wm = fmaxf(fmaxf(w(0, n, e), w(0, n, 2 + e)), fmaxf(w(1, n, e), w(1, n, 2 + e)));
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) {
           zm = fmaxf(zm, __shfl_xor_sync(0xffffffffu, zm, o));
@@ -161,42 +175,53 @@ __device__ __forceinline__ void page_step(const uint8_t* page, int tok0, int len
         }
       }
   }
-  uint32_t p0[NT], p1[NT];
+  uint32_t p0[2][NT], p1[2][NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    float P[4];
+    float mb[2], bb[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const float mb = st[n].m[e] == -CUDART_INF_F ? 0.f : st[n].m[e];
-      const float bb = st[n].bo[e] == -CUDART_INF_F ? 0.f : st[n].bo[e] - kPBias;
-      st[n].l[e] += ex2(s[n][e] - mb) + ex2(s[n][2 + e] - mb);
-      P[e] = ex2(w[n][e] - bb);
-      P[2 + e] = ex2(w[n][2 + e] - bb);
+      mb[e] = st[n].m[e] == -CUDART_INF_F ? 0.f : st[n].m[e];
+      bb[e] = st[n].bo[e] == -CUDART_INF_F ? 0.f : st[n].bo[e] - kPBias;
     }
-    p0[n] = movmatrix_t(pack_f16x2(P[0], P[1]));
-    p1[n] = movmatrix_t(pack_f16x2(P[2], P[3]));
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      float P[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        st[n].l[x & 1] += ex2(s[p][n][x] - mb[x & 1]);
+        P[x] = ex2(w(p, n, x) - bb[x & 1]);
+      }
+      p0[p][n] = movmatrix_t(pack_f16x2(P[0], P[1]));
+      p1[p][n] = movmatrix_t(pack_f16x2(P[2], P[3]));
+    }
   }
   const int t2 = (lane & 3) * 2;
-  uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
-  if (tok0 + kKv8Page > len) {  // codes past the sequence's end may be NaNs: P is 0 there, but 0 * NaN is not
-    keep0 = (tok0 + t2 < len ? 0x00ff00ffu : 0u) | (tok0 + t2 + 1 < len ? 0xff00ff00u : 0u);
-    keep1 = (tok0 + t2 + 8 < len ? 0x00ff00ffu : 0u) | (tok0 + t2 + 9 < len ? 0xff00ff00u : 0u);
-  }
+  const bool tail = tok0 + 2 * kKv8Page > len;
 #pragma unroll
-  for (int c2 = 0; c2 < 4; ++c2) {
-    uint32_t m0, m1, m2, m3;
-    ldsm_x4_t(vb + kv8_chunk(tok, 2 * c2 + (j >> 1)), m0, m1, m2, m3);
-    // a transposed register holds (token 2t: dims 2g, 2g+1), (token 2t+1: the same): pair the tokens
-    m0 = __byte_perm(m0, 0, 0x3120) & keep0;
-    m1 = __byte_perm(m1, 0, 0x3120) & keep1;
-    m2 = __byte_perm(m2, 0, 0x3120) & keep0;
-    m3 = __byte_perm(m3, 0, 0x3120) & keep1;
-    const uint32_t a0 = f16x2_lo(m0), a1 = f16x2_hi(m0), a2 = f16x2_lo(m1), a3 = f16x2_hi(m1);
-    const uint32_t b0 = f16x2_lo(m2), b1 = f16x2_hi(m2), b2 = f16x2_lo(m3), b3 = f16x2_hi(m3);
+  for (int p = 0; p < 2; ++p) {
+    uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
+    if (tail) {  // codes past the sequence's end may be NaNs: P is 0 there, but 0 * NaN is not
+      const int left = len - (tok0 + 16 * p + t2);
+      keep0 = (left > 0 ? 0x00ff00ffu : 0u) | (left > 1 ? 0xff00ff00u : 0u);
+      keep1 = (left > 8 ? 0x00ff00ffu : 0u) | (left > 9 ? 0xff00ff00u : 0u);
+    }
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      mma_f16_16816(st[n].o[2 * c2], a0, a1, a2, a3, p0[n], p1[n]);
-      mma_f16_16816(st[n].o[2 * c2 + 1], b0, b1, b2, b3, p0[n], p1[n]);
+    for (int c2 = 0; c2 < 4; ++c2) {
+      uint32_t m0, m1, m2, m3;
+      ldsm_x4_t(vb + p * kKv8Head + kv8_chunk(tok, 2 * c2 + (j >> 1)), m0, m1, m2, m3);
+      // a transposed register holds (token 2t: dims 2g, 2g+1), (token 2t+1: the same): pair the tokens
+      m0 = __byte_perm(m0, 0, 0x3120) & keep0;
+      m1 = __byte_perm(m1, 0, 0x3120) & keep1;
+      m2 = __byte_perm(m2, 0, 0x3120) & keep0;
+      m3 = __byte_perm(m3, 0, 0x3120) & keep1;
+      const uint32_t a0 = f16x2_lo(m0), a1 = f16x2_hi(m0), a2 = f16x2_lo(m1), a3 = f16x2_hi(m1);
+      const uint32_t b0 = f16x2_lo(m2), b1 = f16x2_hi(m2), b2 = f16x2_lo(m3), b3 = f16x2_hi(m3);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        mma_f16_16816(st[n].o[2 * c2], a0, a1, a2, a3, p0[p][n], p1[p][n]);
+        mma_f16_16816(st[n].o[2 * c2 + 1], b0, b1, b2, b3, p0[p][n], p1[p][n]);
+      }
     }
   }
 }
@@ -259,46 +284,56 @@ __device__ __forceinline__ Item get_item(const Kv8AttnArgs& a, int s) {
   return it;
 }
 
-// Place `at` of the laid-out pages: the item and the page within it (unit * pages + page). Every
-// lane of the warp calls it; a place past the end gives item == items.
+// A place in the laid-out pages: the item and the page within it (unit * pages + page).
 struct Place {
   int item;
-  int64_t in_item;
+  int in_item;
 };
 template <int NT>
-__device__ __forceinline__ int64_t total_pages(const Kv8AttnArgs& a, int items, int lane) {
+__device__ __forceinline__ int item_pages(const Kv8AttnArgs& a, int s) {
+  const Item it = get_item<NT>(a, s);
+  return it.pages * it.units;
+}
+// All pages (for every lane). The first 256 items' stay in `keep` for find_place.
+template <int NT>
+__device__ __forceinline__ int64_t total_pages(const Kv8AttnArgs& a, int items, int lane, int (&keep)[8]) {
   int64_t sum = 0;
-  for (int s = lane; s < items; s += 32) {
-    const Item it = get_item<NT>(a, s);
-    sum += static_cast<int64_t>(it.pages) * it.units;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    keep[k] = 32 * k + lane < items ? item_pages<NT>(a, 32 * k + lane) : 0;
+    sum += keep[k];
   }
+  for (int s = 256 + lane; s < items; s += 32) sum += item_pages<NT>(a, s);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   return sum;
 }
+// Place `at` (every lane of the warp calls it); past the end: item == items.
 template <int NT>
-__device__ __forceinline__ Place find_place(const Kv8AttnArgs& a, int items, int64_t at, int lane) {
-  int64_t base = 0;
-  for (int s0 = 0; s0 < items; s0 += 32) {
-    int64_t n = 0;
-    if (s0 + lane < items) {
-      const Item it = get_item<NT>(a, s0 + lane);
-      n = static_cast<int64_t>(it.pages) * it.units;
-    }
+__device__ __forceinline__ Place find_place(const Kv8AttnArgs& a, int items, int64_t at, int lane, const int (&keep)[8]) {
+  Place found = {items, 0};
+  auto look = [&](int s0, int n) {  // true: found in items s0 .. s0 + 31
     int64_t sum = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int64_t up = __shfl_up_sync(0xffffffffu, sum, o);
       if (lane >= o) sum += up;
     }
-    const unsigned hit = __ballot_sync(0xffffffffu, base + sum > at);
+    const unsigned hit = __ballot_sync(0xffffffffu, sum > at);
     if (hit) {
       const int l = __ffs(hit) - 1;
-      return {s0 + l, at - base - __shfl_sync(0xffffffffu, sum - n, l)};
+      found = {s0 + l, static_cast<int>(at - __shfl_sync(0xffffffffu, sum - n, l))};
+      return true;
     }
-    base += __shfl_sync(0xffffffffu, sum, 31);
-  }
-  return {items, 0};
+    at -= __shfl_sync(0xffffffffu, sum, 31);
+    return false;
+  };
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    if (32 * k < items && look(32 * k, keep[k])) return found;
+  for (int s0 = 256; s0 < items; s0 += 32)
+    if (look(s0, s0 + lane < items ? item_pages<NT>(a, s0 + lane) : 0)) return found;
+  return found;
 }
 // Pages per CTA run; below 32 a run is not worth its joining.
 __device__ __forceinline__ int64_t run_pages(int64_t total, int ctas) {
@@ -316,13 +351,13 @@ struct Walk {
   Item it;
   int64_t left;     // pages left in the run
   int unit, page;   // next piece
-  __device__ void start(const Kv8AttnArgs& a, int item, int64_t in_item, int64_t n) {
+  __device__ void start(const Kv8AttnArgs& a, int item, int in_item, int64_t n) {
     s = item;
     left = n;
     if (n <= 0) return;
     it = get_item<NT>(a, s);
-    unit = static_cast<int>(in_item / it.pages);
-    page = static_cast<int>(in_item % it.pages);
+    unit = in_item / it.pages;
+    page = in_item - unit * it.pages;
   }
   // Pages of the current piece.
   __device__ int count() const { return static_cast<int>(min(static_cast<int64_t>(it.pages - page), left)); }
@@ -338,8 +373,9 @@ struct Walk {
 };
 
 template <int NT>
-__global__ void __launch_bounds__(kThreads, 2) kv8_attn_kernel(const Kv8AttnArgs a, const int whole) {
+__global__ void __launch_bounds__(Smem<NT>::kThreads, 2) kv8_attn_kernel(const Kv8AttnArgs a, const int whole) {
   using S = Smem<NT>;
+  constexpr int kWarps = S::kWarps;
   extern __shared__ __align__(128) uint8_t smem[];
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kBar);
   uint64_t* empty = full + S::kSlots;
@@ -367,40 +403,37 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attn_kernel(const Kv8AttnArgs
   int64_t run0 = 0, per = 0;
   if (whole) {  // CTA = (KV head, item)
     const Item it = get_item<NT>(a, blockIdx.y);
-    w.start(a, blockIdx.y, static_cast<int64_t>(blockIdx.x) * it.groups * it.pages,
-            static_cast<int64_t>(it.groups) * it.pages);
+    w.start(a, blockIdx.y, blockIdx.x * it.groups * it.pages, it.groups * it.pages);
   } else {
-    const int64_t total = total_pages<NT>(a, items, lane);
+    int keep[8];
+    const int64_t total = total_pages<NT>(a, items, lane, keep);
     per = run_pages(total, gridDim.x);
     run0 = blockIdx.x * per;
-    const Place p = find_place<NT>(a, items, run0, lane);
+    const Place p = find_place<NT>(a, items, run0, lane, keep);
     w.start(a, p.item, p.in_item, max(int64_t(0), min(per, total - run0)));
   }
 
   if (warp == kWarps) {
     // -------------------------------------------------------------- loader
     bool ok = true;
-    int n = 0;  // pages so far
+    int n = 0;  // pairs so far
     for (int piece = 0; w.left > 0 && ok; ++piece, w.next(a)) {
       const int kvh = w.unit / w.it.groups, cg = w.unit % w.it.groups;
       const int cnt = w.count();
-      // queries: the group's columns c = row * G + head, bf16 rows of 256 bytes; a row's heads are contiguous
-      {
-        const int qb = piece & 1, c0 = cg * S::kCols, c1 = min(w.it.nq * G, c0 + S::kCols);
-        ok = mbar_wait(&q_empty[qb], ((piece >> 1) & 1) ^ 1, nullptr, a.status);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        if (lane == 0) mbar_expect_tx(&q_full[qb], (c1 - c0) * 256);
-        __syncwarp();
-        for (int c = c0 + lane; c < c1; c += 32)
-          bulk_load(smem + S::kQ + (qb * S::kCols + c - c0) * 256,
-                    a.q + static_cast<int64_t>(w.it.row0 + c / G) * a.q_stride +
-                        (static_cast<int64_t>(kvh) * G + c % G) * kKv8Dim,
-                    256, &q_full[qb]);
-      }
       const int* bt = a.block_tables + static_cast<int64_t>(w.it.seq) * a.bt_stride + w.page;
-      const uint8_t* base = a.arena + a.layer_offset + static_cast<int64_t>(kvh) * kKv8Head;
       int ids = lane < cnt ? bt[lane] : 0;
+      // queries: the group's columns c = row * G + head, bf16 rows of 256 bytes
+      const int qb = piece & 1, c0 = cg * S::kCols, c1 = min(w.it.nq * G, c0 + S::kCols);
+      ok = __all_sync(0xffffffffu, mbar_wait(&q_empty[qb], ((piece >> 1) & 1) ^ 1, nullptr, a.status));
+      if (!ok) break;
+      if (lane == 0) mbar_expect_tx(&q_full[qb], (c1 - c0) * 256);
+      __syncwarp();
+      if (c0 + lane < c1)
+        bulk_load(smem + S::kQ + (qb * S::kCols + lane) * 256,
+                  a.q + static_cast<int64_t>(w.it.row0 + (c0 + lane) / G) * a.q_stride +
+                      (static_cast<int64_t>(kvh) * G + (c0 + lane) % G) * kKv8Dim,
+                  256, &q_full[qb]);
+      const uint8_t* base = a.arena + a.layer_offset + static_cast<int64_t>(kvh) * kKv8Head;
       for (int i0 = 0; i0 < cnt && ok; i0 += 32) {
         int now = ids;
         if (i0 + 32 + lane < cnt) ids = bt[i0 + 32 + lane];
@@ -409,18 +442,16 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attn_kernel(const Kv8AttnArgs
           now = 0;
         }
         const int m = min(32, cnt - i0);
-        for (int i = 0; i < m; ++i, ++n) {
-          const int slot = n % S::kSlots;
-          const int id = __shfl_sync(0xffffffffu, now, i);
-          if (lane == 0) {
-            ok = ok && mbar_wait(&empty[slot], ((n / S::kSlots) & 1) ^ 1, nullptr, a.status);
-            if (ok) {
-              mbar_expect_tx(&full[slot], kKv8Head);
-              bulk_load(smem + slot * kKv8Head, base + id * a.block_bytes, kKv8Head, &full[slot]);
-            }
-          }
+        for (int i = 0; i < m; i += 2, ++n) {
+          const int slot = n % S::kSlots, two = min(2, m - i);
+          const int id = __shfl_sync(0xffffffffu, now, i + (lane & 1));  // (lane 31 reads within the 32: i <= 30)
+          ok = __all_sync(0xffffffffu, mbar_wait(&empty[slot], ((n / S::kSlots) & 1) ^ 1, nullptr, a.status));
+          if (!ok) break;
+          if (lane == 0) mbar_expect_tx(&full[slot], two * kKv8Head);
+          __syncwarp();
+          if (lane < two)
+            bulk_load(smem + (2 * slot + lane) * kKv8Head, base + id * a.block_bytes, kKv8Head, &full[slot]);
         }
-        ok = __all_sync(0xffffffffu, ok);
       }
     }
     return;
@@ -469,16 +500,22 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attn_kernel(const Kv8AttnArgs
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(&q_empty[qb]);
-    for (int i = (warp - n % kWarps + kWarps) % kWarps; i < cnt; i += kWarps) {
+    const int pairs = (cnt + 1) >> 1;
+    for (int i = (warp + kWarps - n % kWarps) % kWarps; i < pairs; i += kWarps) {
       const int slot = (n + i) % S::kSlots;
       ok = __all_sync(0xffffffffu, ok && mbar_wait(&full[slot], ((n + i) / S::kSlots) & 1, nullptr, a.status));
       if (!ok) break;
-      page_step<NT>(smem + slot * kKv8Head, (w.page + i) * kKv8Page, it.len, lim, qf, cq, lane, st);
+      // a piece's last pair may be one page: the rest of its slot is not the piece's
+      const int end = (w.page + cnt) * kKv8Page;
+      int lm[NT][2];
+#pragma unroll
+      for (int k = 0; k < NT; ++k) lm[k][0] = min(lim[k][0], end), lm[k][1] = min(lim[k][1], end);
+      pair_step<NT>(smem + 2 * slot * kKv8Head, (w.page + 2 * i) * kKv8Page, min(it.len, end), lm, qf, cq, lane, st);
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[slot]);
     }
-    n += cnt;
-    // join the four warps' sums
+    n += pairs;
+    // join the warps' sums
 #pragma unroll
     for (int k = 0; k < NT; ++k) {
 #pragma unroll
@@ -498,7 +535,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attn_kernel(const Kv8AttnArgs
           x[0] = st[k].m[e], x[1] = st[k].bo[e], x[2] = st[k].l[e];
         }
     }
-    asm volatile("bar.sync 1, 128;" ::: "memory");
+    asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory");
     const bool entire = cnt == it.pages;
     const int64_t part = (2 * static_cast<int64_t>(blockIdx.x) + (piece > 0)) * S::kCols;
     for (int col = warp; col < ncols; col += kWarps) {
@@ -532,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv8_attn_kernel(const Kv8AttnArgs
         if (lane == 0) *reinterpret_cast<float4*>(a.ws_ml + (part + col) * 4) = make_float4(M, B, L, 0.f);
       }
     }
-    asm volatile("bar.sync 1, 128;" ::: "memory");
+    asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory");
   }
 }
 
@@ -545,13 +582,14 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(const Kv8AttnArgs a) {
   const int G = a.n_q_heads / a.n_kv_heads;
   const int items = a.tiles ? a.num_tiles : a.num_seqs;
   // lengths and tiles are not the first kernel's to write: the search needs no wait
-  const int64_t total = total_pages<NT>(a, items, lane);
+  int keep[8];
+  const int64_t total = total_pages<NT>(a, items, lane, keep);
   const int64_t per = run_pages(total, gridDim.x);
   const int64_t last = (blockIdx.x + 1) * per - 1;  // the run's last page
   if (last + 1 >= total) return;
-  const Place p = find_place<NT>(a, items, last, lane);
+  const Place p = find_place<NT>(a, items, last, lane, keep);
   const Item it = get_item<NT>(a, p.item);
-  const int unit = static_cast<int>(p.in_item / it.pages);
+  const int unit = p.in_item / it.pages;
   const int64_t first = last - p.in_item % it.pages;  // the segment's first page
   const int64_t end = first + it.pages;
   if (first < last + 1 - per || end <= last + 1) return;  // begins in an earlier run, or ends here
@@ -599,11 +637,11 @@ int launch(const Kv8AttnArgs& a, cudaStream_t stream) {
   const int items = a.tiles ? a.num_tiles : a.num_seqs;
   if (int e = ensure_smem_attr(reinterpret_cast<const void*>(kv8_attn_kernel<NT>), Smem<NT>::kBytes)) return e;
   if (a.max_blocks <= kWholePages) {
-    kv8_attn_kernel<NT><<<dim3(a.n_kv_heads, items), kThreads, Smem<NT>::kBytes, stream>>>(a, 1);
+    kv8_attn_kernel<NT><<<dim3(a.n_kv_heads, items), Smem<NT>::kThreads, Smem<NT>::kBytes, stream>>>(a, 1);
     return cudaGetLastError();
   }
   const int ctas = kv8_attention_ctas();
-  kv8_attn_kernel<NT><<<ctas, kThreads, Smem<NT>::kBytes, stream>>>(a, 0);
+  kv8_attn_kernel<NT><<<ctas, Smem<NT>::kThreads, Smem<NT>::kBytes, stream>>>(a, 0);
   if (int e = cudaGetLastError()) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
