@@ -555,13 +555,20 @@ void kv8_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& slots
   LAKEB_CHECK_RC(lakeb::kv8_write(a, cur_stream()), "kv8_write");
 }
 
-void kv8_read(const at::Tensor& arena, int64_t layer, const at::Tensor& slots, at::Tensor& k_out, at::Tensor& v_out,
-              c10::optional<at::Tensor> status) {
-  lakeb::Kv8RowArgs a = kv8_row_args(k_out, v_out, slots, arena, layer, status);
-  a.k_out = bfm(k_out);
-  a.v_out = bfm(v_out);
+std::tuple<at::Tensor, at::Tensor> kv8_read(const at::Tensor& arena, int64_t layer, const at::Tensor& slots,
+                                            c10::optional<at::Tensor> k_out, c10::optional<at::Tensor> v_out,
+                                            c10::optional<at::Tensor> status) {
+  TORCH_CHECK(arena.is_cuda() && arena.dim() == 5, "an 8-bit KV arena is a uint8 CUDA tensor [blocks, layers, heads, 2, 2064]");
   const c10::cuda::CUDAGuard guard(arena.device());
+  auto rows = [&](const c10::optional<at::Tensor>& t) {
+    return t.has_value() ? *t : at::empty({slots.numel(), arena.size(2) * 128}, arena.options().dtype(at::kBFloat16));
+  };
+  at::Tensor k = rows(k_out), v = rows(v_out);
+  lakeb::Kv8RowArgs a = kv8_row_args(k, v, slots, arena, layer, status);
+  a.k_out = bfm(k);
+  a.v_out = bfm(v);
   LAKEB_CHECK_RC(lakeb::kv8_read(a, cur_stream()), "kv8_read");
+  return {k, v};
 }
 
 lakeb::Kv8AttnArgs kv8_attn_args(const at::Tensor& q, const at::Tensor& out, const at::Tensor& arena, int64_t layer,
@@ -570,7 +577,7 @@ lakeb::Kv8AttnArgs kv8_attn_args(const at::Tensor& q, const at::Tensor& out, con
   check_bf16_2d(q, "q");
   check_bf16_2d(out, "out");
   check_kv8_arena(arena, layer, n_kv_heads);
-  TORCH_CHECK(n_q_heads > 0 && n_q_heads % n_kv_heads == 0, "q heads (", n_q_heads, ") must be a multiple of kv heads (",
+  TORCH_CHECK(n_kv_heads > 0 && n_q_heads > 0 && n_q_heads % n_kv_heads == 0, "q heads (", n_q_heads, ") must be a multiple of kv heads (",
               n_kv_heads, ")");
   TORCH_CHECK(q.size(1) == n_q_heads * 128 && out.size(1) == n_q_heads * 128 && out.size(0) >= q.size(0),
               "q and out are [rows, n_q_heads * 128]");
@@ -605,8 +612,16 @@ lakeb::Kv8AttnArgs kv8_attn_args(const at::Tensor& q, const at::Tensor& out, con
   return p;
 }
 
+at::Tensor attn_out(const at::Tensor& q, const c10::optional<at::Tensor>& out, int64_t n_q_heads) {
+  if (out.has_value()) return *out;
+  TORCH_CHECK(q.is_cuda() && q.dim() == 2 && n_q_heads > 0, "q is a CUDA tensor [rows, n_q_heads * 128]");
+  const c10::cuda::CUDAGuard guard(q.device());
+  return at::empty({q.size(0), n_q_heads * 128}, q.options());
+}
+
 // Workspace (this call's own, so calls on several streams and captured graphs share none) and launch.
 void kv8_few_rows(lakeb::Kv8AttnArgs& p, const at::Tensor& q) {
+  if ((p.tiles ? p.num_tiles : p.num_seqs) == 0) return;
   at::Tensor ws;
   if (const int64_t n = lakeb::kv8_attention_ws_floats(p)) {
     ws = at::empty({n}, q.options().dtype(at::kFloat));
@@ -616,20 +631,23 @@ void kv8_few_rows(lakeb::Kv8AttnArgs& p, const at::Tensor& q) {
   LAKEB_CHECK_RC(lakeb::kv8_attention(p, cur_stream()), "kv8_attention");
 }
 
-void kv8_decode(const at::Tensor& q, at::Tensor& out, const at::Tensor& arena, int64_t layer,
-                const at::Tensor& block_tables, const at::Tensor& seq_lens, int64_t n_q_heads, int64_t n_kv_heads,
-                double scale, c10::optional<at::Tensor> status) {
+at::Tensor kv8_decode(const at::Tensor& q, c10::optional<at::Tensor> out_arg, const at::Tensor& arena, int64_t layer,
+                      const at::Tensor& block_tables, const at::Tensor& seq_lens, int64_t n_q_heads,
+                      int64_t n_kv_heads, double scale, c10::optional<at::Tensor> status) {
+  at::Tensor out = attn_out(q, out_arg, n_q_heads);
   lakeb::Kv8AttnArgs p =
       kv8_attn_args(q, out, arena, layer, block_tables, seq_lens, n_q_heads, n_kv_heads, scale, status);
   TORCH_CHECK(q.size(0) >= p.num_seqs, "one query row per sequence");
   const c10::cuda::CUDAGuard guard(arena.device());
   p.num_rows = p.num_seqs;
   kv8_few_rows(p, q);
+  return out;
 }
 
-void kv8_prefill(const at::Tensor& q, at::Tensor& out, const at::Tensor& arena, int64_t layer,
-                 const at::Tensor& block_tables, const at::Tensor& seq_lens, const at::Tensor& tiles, int64_t n_q_heads,
-                 int64_t n_kv_heads, double scale, c10::optional<at::Tensor> status) {
+at::Tensor kv8_prefill(const at::Tensor& q, c10::optional<at::Tensor> out_arg, const at::Tensor& arena, int64_t layer,
+                       const at::Tensor& block_tables, const at::Tensor& seq_lens, const at::Tensor& tiles,
+                       int64_t n_q_heads, int64_t n_kv_heads, double scale, c10::optional<at::Tensor> status) {
+  at::Tensor out = attn_out(q, out_arg, n_q_heads);
   lakeb::Kv8AttnArgs p =
       kv8_attn_args(q, out, arena, layer, block_tables, seq_lens, n_q_heads, n_kv_heads, scale, status);
   TORCH_CHECK(tiles.scalar_type() == at::kInt && tiles.dim() == 2 && tiles.size(1) == 4 && tiles.is_contiguous(),
@@ -638,42 +656,43 @@ void kv8_prefill(const at::Tensor& q, at::Tensor& out, const at::Tensor& arena, 
   check_same_device(tiles, arena, "tiles");
   p.tiles = reinterpret_cast<const int4*>(tiles.data_ptr<int>());
   p.num_tiles = static_cast<int>(tiles.size(0));
+  if (p.num_tiles == 0) return out;
   const c10::cuda::CUDAGuard guard(arena.device());
   if (p.num_rows > 8 * p.num_tiles) {
     LAKEB_CHECK_RC(lakeb::kv8_prefill_tc(p, cur_stream()), "kv8_prefill");
   } else {
     kv8_few_rows(p, q);
   }
+  return out;
 }
 
 // ------------------------------------------------------------------ step tables
-void step_tables(const at::Tensor& pages, const at::Tensor& rows, const at::Tensor& context_lens,
-                 const at::Tensor& new_lens, int64_t n_decode, int64_t block_size, int64_t tile,
-                 at::Tensor& block_tables, at::Tensor& seq_lens, at::Tensor& query_start, at::Tensor& positions,
-                 at::Tensor& slots, at::Tensor& tiles, at::Tensor& counts, c10::optional<at::Tensor> status) {
+std::vector<at::Tensor> step_tables(const at::Tensor& pages, const at::Tensor& rows, const at::Tensor& context_lens,
+                                    const at::Tensor& new_lens, int64_t max_tokens, int64_t max_tiles,
+                                    int64_t n_decode, int64_t block_size, int64_t tile,
+                                    c10::optional<at::Tensor> status) {
   TORCH_CHECK(pages.is_cuda() && pages.scalar_type() == at::kInt && pages.dim() == 2 &&
                   (pages.size(1) <= 1 || pages.stride(1) == 1),
               "pages int32 [request rows, max_blocks] with unit inner stride");
   const int64_t n = rows.numel();
   const std::pair<const at::Tensor*, const char*> ints[] = {
-      {&rows, "rows"},           {&context_lens, "context_lens"}, {&new_lens, "new_lens"},
-      {&block_tables, "block_tables"}, {&seq_lens, "seq_lens"},   {&query_start, "query_start"},
-      {&positions, "positions"}, {&tiles, "tiles"},               {&counts, "counts"}};
+      {&rows, "rows"}, {&context_lens, "context_lens"}, {&new_lens, "new_lens"}};
   for (const auto& [t, name] : ints) {
-    TORCH_CHECK(t->scalar_type() == at::kInt && t->is_contiguous(), name, " must be contiguous int32");
+    TORCH_CHECK(t->scalar_type() == at::kInt && t->dim() == 1 && t->is_contiguous(), name, " must be contiguous int32 [seqs]");
     check_same_device(*t, pages, name);
   }
-  TORCH_CHECK(slots.scalar_type() == at::kLong && slots.is_contiguous(), "slots must be contiguous int64");
-  check_same_device(slots, pages, "slots");
   TORCH_CHECK(context_lens.numel() == n && new_lens.numel() == n, "one context and one new length per sequence");
   TORCH_CHECK(n <= lakeb::kStepTableMaxSeqs, "at most ", lakeb::kStepTableMaxSeqs, " sequences, got ", n);
   TORCH_CHECK(n_decode >= 0 && n_decode <= n, "n_decode ", n_decode, " of ", n, " sequences");
-  TORCH_CHECK(block_size > 0 && tile > 0, "block_size and tile must be positive");
-  TORCH_CHECK(block_tables.dim() == 2 && block_tables.size(0) == n && block_tables.size(1) == pages.size(1) &&
-                  seq_lens.numel() == n && query_start.numel() == n + 1 && positions.numel() == slots.numel() &&
-                  tiles.dim() == 2 && tiles.size(1) == 4 && counts.numel() == 2,
-              "output sizes");
-  check_aligned(tiles, "tiles");
+  TORCH_CHECK(block_size > 0 && block_size < (1 << 30) && tile > 0 && tile < (1 << 30), "block_size and tile must be positive");
+  TORCH_CHECK(max_tokens >= 0 && max_tiles >= 0 && max_tokens < (int64_t(1) << 30) && max_tiles < (int64_t(1) << 28),
+              "max_tokens and max_tiles must not be negative (or past 2^30, 2^28)");
+  const c10::cuda::CUDAGuard guard(pages.device());
+  const auto i32 = pages.options();
+  std::vector<at::Tensor> out = {at::empty({n, pages.size(1)}, i32),  at::empty({n}, i32),
+                                 at::empty({n + 1}, i32),             at::empty({max_tokens}, i32),
+                                 at::empty({max_tokens}, i32.dtype(at::kLong)), at::empty({max_tiles, 4}, i32),
+                                 at::empty({2}, i32)};
   lakeb::StepTableArgs a;
   a.pages = pages.data_ptr<int>();
   a.pages_stride = pages.stride(0);
@@ -684,20 +703,20 @@ void step_tables(const at::Tensor& pages, const at::Tensor& rows, const at::Tens
   a.new_lens = new_lens.data_ptr<int>();
   a.num_seqs = static_cast<int>(n);
   a.num_decode = static_cast<int>(n_decode);
-  a.max_tokens = static_cast<int>(positions.numel());
-  a.max_tiles = static_cast<int>(tiles.size(0));
+  a.max_tokens = static_cast<int>(max_tokens);
+  a.max_tiles = static_cast<int>(max_tiles);
   a.block_size = static_cast<int>(block_size);
   a.tile = static_cast<int>(tile);
-  a.block_tables = block_tables.data_ptr<int>();
-  a.seq_lens = seq_lens.data_ptr<int>();
-  a.query_start = query_start.data_ptr<int>();
-  a.positions = positions.data_ptr<int>();
-  a.slots = slots.data_ptr<int64_t>();
-  a.tiles = reinterpret_cast<int4*>(tiles.data_ptr<int>());
-  a.counts = counts.data_ptr<int>();
+  a.block_tables = out[0].data_ptr<int>();
+  a.seq_lens = out[1].data_ptr<int>();
+  a.query_start = out[2].data_ptr<int>();
+  a.positions = out[3].data_ptr<int>();
+  a.slots = out[4].data_ptr<int64_t>();
+  a.tiles = reinterpret_cast<int4*>(out[5].data_ptr<int>());
+  a.counts = out[6].data_ptr<int>();
   a.status = status_ptr(status);
-  const c10::cuda::CUDAGuard guard(pages.device());
   LAKEB_CHECK_RC(lakeb::step_tables(a, cur_stream()), "step_tables");
+  return out;
 }
 
 void rmsnorm(const at::Tensor& x, const at::Tensor& w, at::Tensor& out, double eps) {
@@ -955,8 +974,8 @@ PYBIND11_MODULE(LAKEB_MODULE, m) {
         py::arg("scale"), py::arg("status") = py::none(), py::arg("tensor_core") = true);
   m.def("kv8_write", &kv8_write, py::arg("k"), py::arg("v"), py::arg("slots"), py::arg("arena"), py::arg("layer"),
         py::arg("status") = py::none());
-  m.def("kv8_read", &kv8_read, py::arg("arena"), py::arg("layer"), py::arg("slots"), py::arg("k_out"),
-        py::arg("v_out"), py::arg("status") = py::none());
+  m.def("kv8_read", &kv8_read, py::arg("arena"), py::arg("layer"), py::arg("slots"), py::arg("k_out") = py::none(),
+        py::arg("v_out") = py::none(), py::arg("status") = py::none());
   m.def("kv8_decode", &kv8_decode, py::arg("q"), py::arg("out"), py::arg("arena"), py::arg("layer"),
         py::arg("block_tables"), py::arg("seq_lens"), py::arg("n_q_heads"), py::arg("n_kv_heads"), py::arg("scale"),
         py::arg("status") = py::none());
@@ -964,8 +983,7 @@ PYBIND11_MODULE(LAKEB_MODULE, m) {
         py::arg("block_tables"), py::arg("seq_lens"), py::arg("tiles"), py::arg("n_q_heads"), py::arg("n_kv_heads"),
         py::arg("scale"), py::arg("status") = py::none());
   m.def("step_tables", &step_tables, py::arg("pages"), py::arg("rows"), py::arg("context_lens"), py::arg("new_lens"),
-        py::arg("n_decode"), py::arg("block_size"), py::arg("tile"), py::arg("block_tables"), py::arg("seq_lens"),
-        py::arg("query_start"), py::arg("positions"), py::arg("slots"), py::arg("tiles"), py::arg("counts"),
+        py::arg("max_tokens"), py::arg("max_tiles"), py::arg("n_decode"), py::arg("block_size"), py::arg("tile"),
         py::arg("status") = py::none());
   m.def("rmsnorm", &rmsnorm);
   m.def("embedding", &embedding, py::arg("ids"), py::arg("table"), py::arg("out"), py::arg("status") = py::none());

@@ -18,8 +18,8 @@
 // needs) in range whatever the tokens' scales are.
 //
 // Work is cut by pages, not by sequences: the pages of every (sequence, KV head, column group) are
-// laid end to end and each CTA takes an equal run of them, whatever the lengths are (two CTAs per
-// SM, all resident). A segment that lies within one CTA's run goes straight to the output; a CTA
+// laid end to end, a segment counting kSegCost pages more for its start and join, and each CTA takes
+// an equal run of them, whatever the lengths are (all CTAs resident). A segment that lies within one CTA's run goes straight to the output; a CTA
 // has at most two pieces of segments (its first and its last) that go to the workspace, and a
 // second kernel joins them in the order of the CTAs, so results do not depend on timing. When no
 // block table is wider than kWholePages, a CTA takes a whole segment and there is no second kernel.
@@ -44,14 +44,18 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.f;  // a base trails the true maximum by at most this
 constexpr float kPBias = 7.f;  // P = 2^(w - bo + 7): fp16 subnormals begin at 2^-21 of the base
 
-// Shared memory of a CTA with NT groups of 8 columns: ring of pages, two query buffers, the
-// consumers' sums for the join at a segment's end. Two CTAs fit an SM (113 KB each).
+constexpr int kSegCost = 6;    // pages that the start and the join of a segment cost as much as
+
+// Shared memory of a CTA with NT groups of 8 columns: ring of page pairs, two query buffers, the
+// consumers' sums for the join at a segment's end. One group: two CTAs per SM. More groups need more
+// registers: one CTA per SM (with two of 16 columns the sums spill at 168 registers).
 template <int NT>
 struct Smem {
   static constexpr int kCols = 8 * NT;
-  static constexpr int kWarps = NT == 1 ? 5 : 4;  // consumers; one more warp loads
+  static constexpr int kWarps = NT == 1 ? 5 : 7;  // consumers; one more warp loads
   static constexpr int kThreads = kWarps * 32 + 32;
-  static constexpr int kSlots = NT == 1 ? 10 : 8;  // pairs of pages
+  static constexpr int kPerSm = NT == 1 ? 2 : 1;
+  static constexpr int kSlots = NT == 1 ? 10 : 14;  // pairs of pages
   static constexpr int kQ = kSlots * 2 * kKv8Head;
   static constexpr int kO = kQ + 2 * kCols * 256;
   static constexpr int kStat = kO + kWarps * kCols * kKv8Dim * 4;  // [warp][col][m, bo, l]
@@ -60,7 +64,7 @@ struct Smem {
   // A slot belongs to one warp: pairs land out of order, and a warp that had not itself waited for
   // the slot's last phase could take it for the one it waits for.
   static_assert(kSlots % kWarps == 0, "");
-  static_assert(kQ % 16 == 0 && kO % 16 == 0 && kBar % 8 == 0 && kBytes <= 113 * 1024, "");
+  static_assert(kQ % 16 == 0 && kO % 16 == 0 && kBar % 8 == 0 && kBytes <= (NT == 1 ? 113 : 227) * 1024, "");
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -284,26 +288,27 @@ __device__ __forceinline__ Item get_item(const Kv8AttnArgs& a, int s) {
   return it;
 }
 
-// A place in the laid-out pages: the item and the page within it (unit * pages + page).
+// A place in the laid-out work, in pages: the item and the offset in it (each of its units is
+// kSegCost + pages long, the start's cost first).
 struct Place {
   int item;
   int in_item;
 };
 template <int NT>
-__device__ __forceinline__ int item_pages(const Kv8AttnArgs& a, int s) {
+__device__ __forceinline__ int item_cost(const Kv8AttnArgs& a, int s) {
   const Item it = get_item<NT>(a, s);
-  return it.pages * it.units;
+  return it.pages > 0 ? (it.pages + kSegCost) * it.units : 0;
 }
-// All pages (for every lane). The first 256 items' stay in `keep` for find_place.
+// The whole length (for every lane). The first 256 items' stay in `keep` for find_place.
 template <int NT>
-__device__ __forceinline__ int64_t total_pages(const Kv8AttnArgs& a, int items, int lane, int (&keep)[8]) {
+__device__ __forceinline__ int64_t total_cost(const Kv8AttnArgs& a, int items, int lane, int (&keep)[8]) {
   int64_t sum = 0;
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
-    keep[k] = 32 * k + lane < items ? item_pages<NT>(a, 32 * k + lane) : 0;
+    keep[k] = 32 * k + lane < items ? item_cost<NT>(a, 32 * k + lane) : 0;
     sum += keep[k];
   }
-  for (int s = 256 + lane; s < items; s += 32) sum += item_pages<NT>(a, s);
+  for (int s = 256 + lane; s < items; s += 32) sum += item_cost<NT>(a, s);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   return sum;
@@ -332,12 +337,13 @@ __device__ __forceinline__ Place find_place(const Kv8AttnArgs& a, int items, int
   for (int k = 0; k < 8; ++k)
     if (32 * k < items && look(32 * k, keep[k])) return found;
   for (int s0 = 256; s0 < items; s0 += 32)
-    if (look(s0, s0 + lane < items ? item_pages<NT>(a, s0 + lane) : 0)) return found;
+    if (look(s0, s0 + lane < items ? item_cost<NT>(a, s0 + lane) : 0)) return found;
   return found;
 }
-// Pages per CTA run; below 32 a run is not worth its joining.
-__device__ __forceinline__ int64_t run_pages(int64_t total, int ctas) {
-  const int64_t per = (total + ctas - 1) / ctas;
+// Length of a CTA's run; below 32 pages a run is not worth its joining.
+__device__ __forceinline__ int64_t run_length(int64_t total, int ctas) {
+  const int64_t per = total < (int64_t(1) << 31) ? static_cast<uint32_t>(total + ctas - 1) / static_cast<uint32_t>(ctas)
+                                                 : (total + ctas - 1) / ctas;
   return per < 32 ? 32 : per;
 }
 
@@ -349,31 +355,37 @@ template <int NT>
 struct Walk {
   int s;            // item
   Item it;
-  int64_t left;     // pages left in the run
-  int unit, page;   // next piece
+  int64_t left;     // of the run, from offset x of segment `unit` on
+  int unit, x;
   __device__ void start(const Kv8AttnArgs& a, int item, int in_item, int64_t n) {
     s = item;
     left = n;
     if (n <= 0) return;
     it = get_item<NT>(a, s);
-    unit = in_item / it.pages;
-    page = in_item - unit * it.pages;
+    unit = in_item / (it.pages + kSegCost);
+    x = in_item - unit * (it.pages + kSegCost);
+    if (count() == 0) left = 0;
   }
-  // Pages of the current piece.
-  __device__ int count() const { return static_cast<int>(min(static_cast<int64_t>(it.pages - page), left)); }
+  __device__ int end() const {  // offset in the segment at which the run leaves it
+    return static_cast<int>(min(static_cast<int64_t>(it.pages + kSegCost), x + left));
+  }
+  __device__ int page() const { return max(0, x - kSegCost); }
+  __device__ int count() const { return max(0, end() - kSegCost) - page(); }  // pages of the piece
   __device__ void next(const Kv8AttnArgs& a) {
-    left -= count();
-    page = 0;
-    if (left > 0 && ++unit == it.units) {
+    left -= end() - x;
+    if (left <= 0) return;
+    x = 0;
+    if (++unit == it.units) {
       unit = 0;
       do it = get_item<NT>(a, ++s);
       while (it.pages == 0);
     }
+    if (count() == 0) left = 0;  // the run ends in the segment's start cost: all its pages are the next one's
   }
 };
 
 template <int NT>
-__global__ void __launch_bounds__(Smem<NT>::kThreads, 2) kv8_attn_kernel(const Kv8AttnArgs a, const int whole) {
+__global__ void __launch_bounds__(Smem<NT>::kThreads, Smem<NT>::kPerSm) kv8_attn_kernel(const Kv8AttnArgs a, const int whole) {
   using S = Smem<NT>;
   constexpr int kWarps = S::kWarps;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -385,30 +397,22 @@ __global__ void __launch_bounds__(Smem<NT>::kThreads, 2) kv8_attn_kernel(const K
   const int G = a.n_q_heads / a.n_kv_heads;
   const int items = a.tiles ? a.num_tiles : a.num_seqs;
 
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < S::kSlots; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
-    }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&q_full[i], 1);
-      mbar_init(&q_empty[i], kWarps);
-    }
+  asm volatile("griddepcontrol.launch_dependents;");
+  if (threadIdx.x < 2 * S::kSlots + 4) {
+    mbar_init(full + threadIdx.x, threadIdx.x < 2 * S::kSlots + 2 ? 1 : kWarps);
     fence_mbar_init();
   }
   __syncthreads();
-  asm volatile("griddepcontrol.launch_dependents;");
 
   Walk<NT> w;
-  int64_t run0 = 0, per = 0;
   if (whole) {  // CTA = (KV head, item)
     const Item it = get_item<NT>(a, blockIdx.y);
-    w.start(a, blockIdx.y, blockIdx.x * it.groups * it.pages, it.groups * it.pages);
+    const int n = it.pages > 0 ? it.groups * (it.pages + kSegCost) : 0;
+    w.start(a, blockIdx.y, blockIdx.x * n, n);
   } else {
     int keep[8];
-    const int64_t total = total_pages<NT>(a, items, lane, keep);
-    per = run_pages(total, gridDim.x);
-    run0 = blockIdx.x * per;
+    const int64_t total = total_cost<NT>(a, items, lane, keep);
+    const int64_t per = run_length(total, gridDim.x), run0 = blockIdx.x * per;
     const Place p = find_place<NT>(a, items, run0, lane, keep);
     w.start(a, p.item, p.in_item, max(int64_t(0), min(per, total - run0)));
   }
@@ -420,7 +424,7 @@ __global__ void __launch_bounds__(Smem<NT>::kThreads, 2) kv8_attn_kernel(const K
     for (int piece = 0; w.left > 0 && ok; ++piece, w.next(a)) {
       const int kvh = w.unit / w.it.groups, cg = w.unit % w.it.groups;
       const int cnt = w.count();
-      const int* bt = a.block_tables + static_cast<int64_t>(w.it.seq) * a.bt_stride + w.page;
+      const int* bt = a.block_tables + static_cast<int64_t>(w.it.seq) * a.bt_stride + w.page();
       int ids = lane < cnt ? bt[lane] : 0;
       // queries: the group's columns c = row * G + head, bf16 rows of 256 bytes
       const int qb = piece & 1, c0 = cg * S::kCols, c1 = min(w.it.nq * G, c0 + S::kCols);
@@ -506,11 +510,11 @@ __global__ void __launch_bounds__(Smem<NT>::kThreads, 2) kv8_attn_kernel(const K
       ok = __all_sync(0xffffffffu, ok && mbar_wait(&full[slot], ((n + i) / S::kSlots) & 1, nullptr, a.status));
       if (!ok) break;
       // a piece's last pair may be one page: the rest of its slot is not the piece's
-      const int end = (w.page + cnt) * kKv8Page;
+      const int end = (w.page() + cnt) * kKv8Page;
       int lm[NT][2];
 #pragma unroll
       for (int k = 0; k < NT; ++k) lm[k][0] = min(lim[k][0], end), lm[k][1] = min(lim[k][1], end);
-      pair_step<NT>(smem + 2 * slot * kKv8Head, (w.page + 2 * i) * kKv8Page, min(it.len, end), lm, qf, cq, lane, st);
+      pair_step<NT>(smem + 2 * slot * kKv8Head, (w.page() + 2 * i) * kKv8Page, min(it.len, end), lm, qf, cq, lane, st);
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[slot]);
     }
@@ -573,7 +577,7 @@ __global__ void __launch_bounds__(Smem<NT>::kThreads, 2) kv8_attn_kernel(const K
   }
 }
 
-// Joins the segment that begins in CTA run c and ends in a later one (CTA c of this kernel). Its
+// Joins the segment whose pages begin in CTA run c and end in a later one (CTA c of this kernel). Its
 // first piece is c's last one, the others are the first pieces of the runs c + 1, c + 2, ...
 template <int NT>
 __global__ void __launch_bounds__(256) kv8_join_kernel(const Kv8AttnArgs a) {
@@ -583,18 +587,19 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(const Kv8AttnArgs a) {
   const int items = a.tiles ? a.num_tiles : a.num_seqs;
   // lengths and tiles are not the first kernel's to write: the search needs no wait
   int keep[8];
-  const int64_t total = total_pages<NT>(a, items, lane, keep);
-  const int64_t per = run_pages(total, gridDim.x);
-  const int64_t last = (blockIdx.x + 1) * per - 1;  // the run's last page
-  if (last + 1 >= total) return;
-  const Place p = find_place<NT>(a, items, last, lane, keep);
+  const int64_t total = total_cost<NT>(a, items, lane, keep);
+  const int64_t per = run_length(total, gridDim.x);
+  const int64_t run0 = blockIdx.x * per, run1 = run0 + per;
+  if (run1 >= total) return;
+  const Place p = find_place<NT>(a, items, run1 - 1, lane, keep);
   const Item it = get_item<NT>(a, p.item);
-  const int unit = p.in_item / it.pages;
-  const int64_t first = last - p.in_item % it.pages;  // the segment's first page
-  const int64_t end = first + it.pages;
-  if (first < last + 1 - per || end <= last + 1) return;  // begins in an earlier run, or ends here
-  const int pieces = static_cast<int>((end - 1) / per - blockIdx.x) + 1;
-  const int slot0 = 2 * static_cast<int>(blockIdx.x) + (first > last + 1 - per);
+  const int unit = p.in_item / (it.pages + kSegCost);
+  const int64_t seg0 = run1 - 1 - p.in_item % (it.pages + kSegCost);
+  const int64_t seg1 = seg0 + kSegCost + it.pages;
+  const int64_t first = seg0 + kSegCost;  // its first page
+  if (first < run0 || first >= run1 || seg1 <= run1) return;
+  const int pieces = static_cast<int>((seg1 - 1) / per - blockIdx.x) + 1;
+  const int slot0 = 2 * static_cast<int>(blockIdx.x) + (seg0 > run0);
   const int kvh = unit / it.groups, cb = unit % it.groups * kCols;
   const int ncols = min(kCols, it.nq * G - cb);
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -640,7 +645,7 @@ int launch(const Kv8AttnArgs& a, cudaStream_t stream) {
     kv8_attn_kernel<NT><<<dim3(a.n_kv_heads, items), Smem<NT>::kThreads, Smem<NT>::kBytes, stream>>>(a, 1);
     return cudaGetLastError();
   }
-  const int ctas = kv8_attention_ctas();
+  const int ctas = Smem<NT>::kPerSm * num_sms();
   kv8_attn_kernel<NT><<<ctas, Smem<NT>::kThreads, Smem<NT>::kBytes, stream>>>(a, 0);
   if (int e = cudaGetLastError()) return e;
   cudaLaunchConfig_t cfg = {};
@@ -657,21 +662,27 @@ int launch(const Kv8AttnArgs& a, cudaStream_t stream) {
 
 }  // namespace
 
-int kv8_attention_ctas() { return 2 * num_sms(); }
-
 int64_t kv8_attention_ws_floats(const Kv8AttnArgs& a) {
-  return a.max_blocks <= kWholePages ? 0 : int64_t(2) * kv8_attention_ctas() * 8 * kv8_attention_groups(a) * (kKv8Dim + 4);
+  const int nt = kv8_attention_groups(a);
+  return a.max_blocks <= kWholePages ? 0 : int64_t(2) * (nt == 1 ? 2 : 1) * num_sms() * 8 * nt * (kKv8Dim + 4);
 }
 
-// Columns of 8 that a CTA holds at once: two where a tile has more than 8 columns on average.
+// Groups of 8 columns that a CTA holds at once, by the columns of a tile on average: a pass over the
+// pages costs 16 MMAs of 16 cycles per page and group, so a group that stays empty costs as much as
+// a full one, and columns beyond the groups cost another pass.
 int kv8_attention_groups(const Kv8AttnArgs& a) {
-  const int64_t cols = static_cast<int64_t>(a.n_q_heads / a.n_kv_heads) * (a.tiles ? (a.num_rows + a.num_tiles - 1) / a.num_tiles : 1);
-  return cols > 8 ? 2 : 1;
+  const int64_t rows = a.tiles ? (a.num_rows + a.num_tiles - 1) / a.num_tiles : 1;
+  const int64_t groups = (rows * (a.n_q_heads / a.n_kv_heads) + 7) / 8;
+  return groups < 3 ? static_cast<int>(groups) : 3;
 }
 
 int kv8_attention(const Kv8AttnArgs& a, cudaStream_t stream) {
   if ((a.tiles ? a.num_tiles : a.num_seqs) <= 0) return 0;
-  return kv8_attention_groups(a) == 2 ? launch<2>(a, stream) : launch<1>(a, stream);
+  switch (kv8_attention_groups(a)) {
+    case 1: return launch<1>(a, stream);
+    case 2: return launch<2>(a, stream);
+    default: return launch<3>(a, stream);
+  }
 }
 
 }  // namespace lakeb

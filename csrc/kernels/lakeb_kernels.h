@@ -239,7 +239,6 @@ struct Kv8AttnArgs {
 };
 // Few query rows per sequence (any number is right; large tiles belong to kv8_prefill_tc).
 int kv8_attention(const Kv8AttnArgs& a, cudaStream_t stream);
-int kv8_attention_ctas();
 int kv8_attention_groups(const Kv8AttnArgs& a);
 int64_t kv8_attention_ws_floats(const Kv8AttnArgs& a);
 // Query tiles of <= 128 rows on the tcgen05 tensor cores.

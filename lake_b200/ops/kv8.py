@@ -56,16 +56,14 @@ def kv8_read(arena: torch.Tensor, layer: int, slots: torch.Tensor, k_out: torch.
              v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """The cached K and V of `slots` (int64 [T]) as dense bf16 rows [T, kv_heads * head_dim]; a
     negative slot gives a row of zeros (so does one past the arena, which is reported)."""
-    d = ref.arena_head_dim(arena)
-    shape = (slots.shape[0], arena.shape[2] * d)
-    if k_out is None:
-        k_out = torch.empty(shape, dtype=torch.bfloat16, device=arena.device)
-    if v_out is None:
-        v_out = torch.empty(shape, dtype=torch.bfloat16, device=arena.device)
     if arena.is_cuda:
-        native().kv8_read(arena, layer, slots, k_out, v_out, core.status_word(arena.device))
         core.LAUNCHES[0] += 1
-        return k_out, v_out
+        return native().kv8_read(arena, layer, slots, k_out, v_out, core.status_word(arena.device))
+    shape = (slots.shape[0], arena.shape[2] * ref.arena_head_dim(arena))
+    if k_out is None:
+        k_out = torch.empty(shape, dtype=torch.bfloat16)
+    if v_out is None:
+        v_out = torch.empty(shape, dtype=torch.bfloat16)
     x = ref.kv8_rows(arena, layer, slots)
     k_out.copy_(x[:, :, 0].reshape(shape).to(k_out.dtype))
     v_out.copy_(x[:, :, 1].reshape(shape).to(v_out.dtype))

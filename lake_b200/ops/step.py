@@ -37,20 +37,11 @@ def build_step_tables(pages: torch.Tensor, rows: torch.Tensor, context_lens: tor
     lengths. More tokens or tiles than max_tokens / max_tiles, a negative length, a request row
     outside `pages`, or a token whose page is missing (negative, or past the row's end) is reported
     (the status word on the GPU, ValueError on the CPU); on the GPU such a token gets slot -1."""
-    n, dev = rows.shape[0], pages.device
+    if pages.is_cuda:
+        core.LAUNCHES[0] += 1
+        return StepTables(*native().step_tables(pages, rows, context_lens, new_lens, max_tokens, max_tiles, n_decode,
+                                                block_size, tile, core.status_word(pages.device)))
     if max_tokens < 0 or max_tiles < 0:
         raise ValueError(f"max_tokens and max_tiles must not be negative, got {max_tokens} and {max_tiles}")
-    if not pages.is_cuda:
-        return StepTables(*ref.step_tables(pages, rows, context_lens, new_lens, max_tokens, max_tiles, n_decode,
-                                           block_size, tile))
-    out = StepTables(torch.empty(n, pages.shape[1], dtype=torch.int32, device=dev),
-                     torch.empty(n, dtype=torch.int32, device=dev),
-                     torch.empty(n + 1, dtype=torch.int32, device=dev),
-                     torch.empty(max_tokens, dtype=torch.int32, device=dev),
-                     torch.empty(max_tokens, dtype=torch.int64, device=dev),
-                     torch.empty(max_tiles, 4, dtype=torch.int32, device=dev),
-                     torch.empty(2, dtype=torch.int32, device=dev))
-    native().step_tables(pages, rows, context_lens, new_lens, n_decode, block_size, tile, *out,
-                         core.status_word(dev))
-    core.LAUNCHES[0] += 1
-    return out
+    return StepTables(*ref.step_tables(pages, rows, context_lens, new_lens, max_tokens, max_tiles, n_decode,
+                                       block_size, tile))
