@@ -25,9 +25,9 @@
 // block table is wider than kWholePages, a CTA takes a whole segment and there is no second kernel.
 //
 // In a CTA one warp copies pages into a ring (bulk copies of 4128 bytes, page ids fetched 32 at a
-// time, queries of the next segment ahead) and the others take pairs of pages in turn: a page alone
-// is a chain of dependent products, exponentials and products of ~1400 cycles, two at once cost
-// little more than one.
+// time, queries of the next segment ahead) and the others take pages in turn: with 8 columns two at
+// once, since a page alone is a chain of dependent products, exponentials and products of ~1400
+// cycles and two cost little more; with more columns the groups fill the chain's gaps.
 #include <math_constants.h>
 
 #include "common.cuh"
@@ -46,7 +46,7 @@ constexpr float kPBias = 7.f;  // P = 2^(w - bo + 7): fp16 subnormals begin at 2
 
 constexpr int kSegCost = 6;    // pages that the start and the join of a segment cost as much as
 
-// Shared memory of a CTA with NT groups of 8 columns: ring of page pairs, two query buffers, the
+// Shared memory of a CTA with NT groups of 8 columns: ring of pages, two query buffers, the
 // consumers' sums for the join at a segment's end. One group: two CTAs per SM. More groups need more
 // registers: one CTA per SM (with two of 16 columns the sums spill at 168 registers).
 template <int NT>
@@ -55,13 +55,14 @@ struct Smem {
   static constexpr int kWarps = NT == 1 ? 5 : 7;  // consumers; one more warp loads
   static constexpr int kThreads = kWarps * 32 + 32;
   static constexpr int kPerSm = NT == 1 ? 2 : 1;
-  static constexpr int kSlots = NT == 1 ? 10 : 14;  // pairs of pages
-  static constexpr int kQ = kSlots * 2 * kKv8Head;
+  static constexpr int kPages = NT == 1 ? 2 : 1;  // of a step
+  static constexpr int kSlots = NT == 1 ? 10 : 28;
+  static constexpr int kQ = kSlots * kPages * kKv8Head;
   static constexpr int kO = kQ + 2 * kCols * 256;
   static constexpr int kStat = kO + kWarps * kCols * kKv8Dim * 4;  // [warp][col][m, bo, l]
   static constexpr int kBar = kStat + kWarps * kCols * 3 * 4;
   static constexpr int kBytes = kBar + (2 * kSlots + 4) * 8;
-  // A slot belongs to one warp: pairs land out of order, and a warp that had not itself waited for
+  // A slot belongs to one warp: pages land out of order, and a warp that had not itself waited for
   // the slot's last phase could take it for the one it waits for.
   static_assert(kSlots % kWarps == 0, "");
   static_assert(kQ % 16 == 0 && kO % 16 == 0 && kBar % 8 == 0 && kBytes <= (NT == 1 ? 113 : 227) * 1024, "");
@@ -98,18 +99,18 @@ struct ColState {
   float m[2], bo[2], l[2];  // bases and this lane's part of the sum of p
 };
 
-// Adds a pair of pages (32 tokens from tok0) to the states. lim[n][e]: keys of column 8n+2t+e end
+// Adds NP pages (16 tokens each, from tok0) to the states. lim[n][e]: keys of column 8n+2t+e end
 // before it; len: tokens from len on are not the sequence's (their bytes may be anything).
-template <int NT>
-__device__ __forceinline__ void pair_step(const uint8_t* pages, int tok0, int len, const int (&lim)[NT][2],
+template <int NT, int NP>
+__device__ __forceinline__ void pages_step(const uint8_t* pages, int tok0, int len, const int (&lim)[NT][2],
                                           const uint32_t (&qf)[NT][8][2], const float (&cq)[NT][2], int lane,
                                           ColState (&st)[NT]) {
   const int g = lane >> 2, j = lane >> 3, r8 = lane & 7;
   const int tok = (j & 1) * 8 + r8;
   const uint32_t kb = smem_u32(pages), vb = kb + kKv8Side;
-  float s[2][NT][4];
+  float s[NP][NT][4];
 #pragma unroll
-  for (int p = 0; p < 2; ++p)
+  for (int p = 0; p < NP; ++p)
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -117,7 +118,7 @@ __device__ __forceinline__ void pair_step(const uint8_t* pages, int tok0, int le
 #pragma unroll
   for (int c2 = 0; c2 < 4; ++c2)
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
+    for (int p = 0; p < NP; ++p) {
       uint32_t m0, m1, m2, m3;
       ldsm_x4(kb + p * kKv8Head + kv8_chunk(tok, 2 * c2 + (j >> 1)), m0, m1, m2, m3);
       const uint32_t a0 = f16x2_lo(m0), a1 = f16x2_lo(m1), a2 = f16x2_hi(m0), a3 = f16x2_hi(m1);
@@ -128,10 +129,10 @@ __device__ __forceinline__ void pair_step(const uint8_t* pages, int tok0, int le
         mma_f16_16816(s[p][n], b0, b1, b2, b3, qf[n][2 * c2 + 1][0], qf[n][2 * c2 + 1][1]);
       }
     }
-  float ev[2][2];
+  float ev[NP][2];
   bool grow = false;
 #pragma unroll
-  for (int p = 0; p < 2; ++p)
+  for (int p = 0; p < NP; ++p)
 #pragma unroll
     for (int hi = 0; hi < 2; ++hi) {
       const int tk = g + 8 * hi;
@@ -158,8 +159,12 @@ __device__ __forceinline__ void pair_step(const uint8_t* pages, int tok0, int le
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float zm = fmaxf(fmaxf(s[0][n][e], s[0][n][2 + e]), fmaxf(s[1][n][e], s[1][n][2 + e]));
-        float wm = fmaxf(fmaxf(w(0, n, e), w(0, n, 2 + e)), fmaxf(w(1, n, e), w(1, n, 2 + e)));
+        float zm = -CUDART_INF_F, wm = -CUDART_INF_F;
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+          zm = fmaxf(zm, fmaxf(s[p][n][e], s[p][n][2 + e]));
+          wm = fmaxf(wm, fmaxf(w(p, n, e), w(p, n, 2 + e)));
+        }
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) {
           zm = fmaxf(zm, __shfl_xor_sync(0xffffffffu, zm, o));
@@ -179,7 +184,7 @@ __device__ __forceinline__ void pair_step(const uint8_t* pages, int tok0, int le
         }
       }
   }
-  uint32_t p0[2][NT], p1[2][NT];
+  uint32_t p0[NP][NT], p1[NP][NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     float mb[2], bb[2];
@@ -189,7 +194,7 @@ __device__ __forceinline__ void pair_step(const uint8_t* pages, int tok0, int le
       bb[e] = st[n].bo[e] == -CUDART_INF_F ? 0.f : st[n].bo[e] - kPBias;
     }
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
+    for (int p = 0; p < NP; ++p) {
       float P[4];
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
@@ -201,9 +206,9 @@ __device__ __forceinline__ void pair_step(const uint8_t* pages, int tok0, int le
     }
   }
   const int t2 = (lane & 3) * 2;
-  const bool tail = tok0 + 2 * kKv8Page > len;
+  const bool tail = tok0 + NP * kKv8Page > len;
 #pragma unroll
-  for (int p = 0; p < 2; ++p) {
+  for (int p = 0; p < NP; ++p) {
     uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
     if (tail) {  // codes past the sequence's end may be NaNs: P is 0 there, but 0 * NaN is not
       const int left = len - (tok0 + 16 * p + t2);
@@ -316,29 +321,33 @@ __device__ __forceinline__ int64_t total_cost(const Kv8AttnArgs& a, int items, i
 // Place `at` (every lane of the warp calls it); past the end: item == items.
 template <int NT>
 __device__ __forceinline__ Place find_place(const Kv8AttnArgs& a, int items, int64_t at, int lane, const int (&keep)[8]) {
-  Place found = {items, 0};
-  auto look = [&](int s0, int n) {  // true: found in items s0 .. s0 + 31
-    int64_t sum = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t up = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += up;
-    }
-    const unsigned hit = __ballot_sync(0xffffffffu, sum > at);
-    if (hit) {
-      const int l = __ffs(hit) - 1;
-      found = {s0 + l, static_cast<int>(at - __shfl_sync(0xffffffffu, sum - n, l))};
-      return true;
-    }
-    at -= __shfl_sync(0xffffffffu, sum, 31);
-    return false;
-  };
+  // the 32 items that hold it, by their sums; then the item, by a scan of them
+  int s0 = 0, mine = 0;
+  bool hit = false;
 #pragma unroll
   for (int k = 0; k < 8; ++k)
-    if (32 * k < items && look(32 * k, keep[k])) return found;
-  for (int s0 = 256; s0 < items; s0 += 32)
-    if (look(s0, s0 + lane < items ? item_cost<NT>(a, s0 + lane) : 0)) return found;
-  return found;
+    if (!hit) {
+      const unsigned sum = __reduce_add_sync(0xffffffffu, static_cast<unsigned>(keep[k]));
+      hit = at < sum;
+      if (hit) s0 = 32 * k, mine = keep[k];
+      else at -= sum;
+    }
+  for (int s = 256; s < items && !hit; s += 32) {
+    const int n = s + lane < items ? item_cost<NT>(a, s + lane) : 0;
+    const unsigned sum = __reduce_add_sync(0xffffffffu, static_cast<unsigned>(n));
+    hit = at < sum;
+    if (hit) s0 = s, mine = n;
+    else at -= sum;
+  }
+  if (!hit) return {items, 0};
+  int sum = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += up;
+  }
+  const int l = __ffs(__ballot_sync(0xffffffffu, sum > static_cast<int>(at))) - 1;
+  return {s0 + l, static_cast<int>(at) - __shfl_sync(0xffffffffu, sum - mine, l)};
 }
 // Length of a CTA's run; below 32 pages a run is not worth its joining.
 __device__ __forceinline__ int64_t run_length(int64_t total, int ctas) {
@@ -420,7 +429,7 @@ __global__ void __launch_bounds__(Smem<NT>::kThreads, Smem<NT>::kPerSm) kv8_attn
   if (warp == kWarps) {
     // -------------------------------------------------------------- loader
     bool ok = true;
-    int n = 0;  // pairs so far
+    int n = 0;  // steps so far
     for (int piece = 0; w.left > 0 && ok; ++piece, w.next(a)) {
       const int kvh = w.unit / w.it.groups, cg = w.unit % w.it.groups;
       const int cnt = w.count();
@@ -446,15 +455,15 @@ __global__ void __launch_bounds__(Smem<NT>::kThreads, Smem<NT>::kPerSm) kv8_attn
           now = 0;
         }
         const int m = min(32, cnt - i0);
-        for (int i = 0; i < m; i += 2, ++n) {
-          const int slot = n % S::kSlots, two = min(2, m - i);
-          const int id = __shfl_sync(0xffffffffu, now, i + (lane & 1));  // (lane 31 reads within the 32: i <= 30)
+        for (int i = 0; i < m; i += S::kPages, ++n) {
+          const int slot = n % S::kSlots, here = min(S::kPages, m - i);
+          const int id = __shfl_sync(0xffffffffu, now, i + lane % S::kPages);
           ok = __all_sync(0xffffffffu, mbar_wait(&empty[slot], ((n / S::kSlots) & 1) ^ 1, nullptr, a.status));
           if (!ok) break;
-          if (lane == 0) mbar_expect_tx(&full[slot], two * kKv8Head);
+          if (lane == 0) mbar_expect_tx(&full[slot], here * kKv8Head);
           __syncwarp();
-          if (lane < two)
-            bulk_load(smem + (2 * slot + lane) * kKv8Head, base + id * a.block_bytes, kKv8Head, &full[slot]);
+          if (lane < here)
+            bulk_load(smem + (S::kPages * slot + lane) * kKv8Head, base + id * a.block_bytes, kKv8Head, &full[slot]);
         }
       }
     }
@@ -504,21 +513,22 @@ __global__ void __launch_bounds__(Smem<NT>::kThreads, Smem<NT>::kPerSm) kv8_attn
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(&q_empty[qb]);
-    const int pairs = (cnt + 1) >> 1;
-    for (int i = (warp + kWarps - n % kWarps) % kWarps; i < pairs; i += kWarps) {
+    const int steps = (cnt + S::kPages - 1) / S::kPages;
+    for (int i = (warp + kWarps - n % kWarps) % kWarps; i < steps; i += kWarps) {
       const int slot = (n + i) % S::kSlots;
       ok = __all_sync(0xffffffffu, ok && mbar_wait(&full[slot], ((n + i) / S::kSlots) & 1, nullptr, a.status));
       if (!ok) break;
-      // a piece's last pair may be one page: the rest of its slot is not the piece's
+      // a piece's last step may have fewer pages: the rest of its slot is not the piece's
       const int end = (w.page() + cnt) * kKv8Page;
       int lm[NT][2];
 #pragma unroll
       for (int k = 0; k < NT; ++k) lm[k][0] = min(lim[k][0], end), lm[k][1] = min(lim[k][1], end);
-      pair_step<NT>(smem + 2 * slot * kKv8Head, (w.page() + 2 * i) * kKv8Page, min(it.len, end), lm, qf, cq, lane, st);
+      pages_step<NT, S::kPages>(smem + S::kPages * slot * kKv8Head, (w.page() + S::kPages * i) * kKv8Page,
+                                min(it.len, end), lm, qf, cq, lane, st);
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[slot]);
     }
-    n += pairs;
+    n += steps;
     // join the warps' sums
 #pragma unroll
     for (int k = 0; k < NT; ++k) {
@@ -603,38 +613,55 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(const Kv8AttnArgs a) {
   const int kvh = unit / it.groups, cb = unit % it.groups * kCols;
   const int ncols = min(kCols, it.nq * G - cb);
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  for (int col = warp; col < ncols; col += 8) {
-    // as in the first kernel, the bases first; lane i looks at piece i, i + 32, ...
-    float M = -CUDART_INF_F, B = -CUDART_INF_F;
-    auto slot = [&](int i) { return static_cast<int64_t>(i == 0 ? slot0 : 2 * (static_cast<int>(blockIdx.x) + i)) * kCols + col; };
-    for (int i = lane; i < pieces; i += 32) {
-      const float4 x = *reinterpret_cast<const float4*>(a.ws_ml + slot(i) * 4);
-      M = fmaxf(M, x.x);
-      B = fmaxf(B, x.y);
-    }
+  // A warp has the columns warp, warp + 8, ... all at once: one after the other, each would wait twice
+  // for memory.
+  float M[NT], B[NT], L[NT];
+  float4 acc[NT];
+  auto slot = [&](int i, int k) {
+    return static_cast<int64_t>(i == 0 ? slot0 : 2 * (static_cast<int>(blockIdx.x) + i)) * kCols + warp + 8 * k;
+  };
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-      B = fmaxf(B, __shfl_xor_sync(0xffffffffu, B, o));
-    }
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float L = 0.f;
-    for (int i = 0; i < pieces; ++i) {
-      const float4 x = *reinterpret_cast<const float4*>(a.ws_ml + slot(i) * 4);
-      const float4 v = *reinterpret_cast<const float4*>(a.ws_o + slot(i) * kKv8Dim + 4 * lane);
-      L += x.z * factor(x.x, M);
-      const float f = factor(x.y, B);
-      acc.x += v.x * f;
-      acc.y += v.y * f;
-      acc.z += v.z * f;
-      acc.w += v.w * f;
-    }
-    const int c = cb + col;
-    const float f = L == 0.f ? 0.f : ex2(base_or_zero(B) - base_or_zero(M) - kPBias) / L;
-    *reinterpret_cast<uint2*>(a.out + static_cast<int64_t>(it.row0 + c / G) * a.out_stride +
-                              (kvh * G + c % G) * kKv8Dim + 4 * lane) =
-        make_uint2(pack_bf16x2(acc.x * f, acc.y * f), pack_bf16x2(acc.z * f, acc.w * f));
+  for (int k = 0; k < NT; ++k) {
+    M[k] = B[k] = -CUDART_INF_F;
+    L[k] = 0.f;
+    acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
+  for (int i = 0; i < pieces; i += 2) {
+    float4 x[2][NT], v[2][NT];
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int k = 0; k < NT; ++k) {
+        const bool real = i + j < pieces && warp + 8 * k < ncols;
+        x[j][k] = real ? *reinterpret_cast<const float4*>(a.ws_ml + slot(i + j, k) * 4)
+                       : make_float4(-CUDART_INF_F, -CUDART_INF_F, 0.f, 0.f);
+        v[j][k] = real ? *reinterpret_cast<const float4*>(a.ws_o + slot(i + j, k) * kKv8Dim + 4 * lane)
+                       : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int k = 0; k < NT; ++k) {
+        const float m = fmaxf(M[k], x[j][k].x), b = fmaxf(B[k], x[j][k].y);
+        const float fl = factor(M[k], m), gl = factor(x[j][k].x, m), fo = factor(B[k], b), go = factor(x[j][k].y, b);
+        L[k] = L[k] * fl + x[j][k].z * gl;
+        acc[k].x = acc[k].x * fo + v[j][k].x * go;
+        acc[k].y = acc[k].y * fo + v[j][k].y * go;
+        acc[k].z = acc[k].z * fo + v[j][k].z * go;
+        acc[k].w = acc[k].w * fo + v[j][k].w * go;
+        M[k] = m;
+        B[k] = b;
+      }
+  }
+#pragma unroll
+  for (int k = 0; k < NT; ++k)
+    if (warp + 8 * k < ncols) {
+      const int c = cb + warp + 8 * k;
+      const float f = L[k] == 0.f ? 0.f : ex2(base_or_zero(B[k]) - base_or_zero(M[k]) - kPBias) / L[k];
+      *reinterpret_cast<uint2*>(a.out + static_cast<int64_t>(it.row0 + c / G) * a.out_stride +
+                                (kvh * G + c % G) * kKv8Dim + 4 * lane) =
+          make_uint2(pack_bf16x2(acc[k].x * f, acc[k].y * f), pack_bf16x2(acc[k].z * f, acc[k].w * f));
+    }
 }
 
 template <int NT>
