@@ -503,6 +503,26 @@ void paged_prefill(const at::Tensor& q, at::Tensor& out, const at::Tensor& arena
   }
 }
 
+// Several contiguous tensors in one allocation, each 16-byte aligned: an op with seven small outputs
+// would spend more host time on seven allocations than its kernel takes.
+struct Carve {
+  at::Tensor bytes;
+  int64_t used = 0;
+  static int64_t room(int64_t n, at::ScalarType t) {
+    return (n * static_cast<int64_t>(c10::elementSize(t)) + 15) / 16 * 16;
+  }
+  Carve(int64_t total, const at::Device& dev)
+      : bytes(at::empty({total}, at::TensorOptions().dtype(at::kByte).device(dev))) {}
+  at::Tensor take(at::IntArrayRef sizes, at::ScalarType t) {
+    at::Tensor r = at::detail::make_tensor<at::TensorImpl>(c10::Storage(bytes.storage()), bytes.key_set(),
+                                                           c10::scalarTypeToTypeMeta(t));
+    r.unsafeGetTensorImpl()->set_storage_offset(used / static_cast<int64_t>(c10::elementSize(t)));
+    r.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+    used += room(r.numel(), t);
+    return r;
+  }
+};
+
 // ------------------------------------------------------------------ 8-bit KV arena
 void check_same_device(const at::Tensor& t, const at::Tensor& ref, const char* name) {
   TORCH_CHECK(t.is_cuda() && t.device() == ref.device(), name, " must be on ", ref.device(), ", got ", t.device());
@@ -560,10 +580,17 @@ std::tuple<at::Tensor, at::Tensor> kv8_read(const at::Tensor& arena, int64_t lay
                                             c10::optional<at::Tensor> status) {
   TORCH_CHECK(arena.is_cuda() && arena.dim() == 5, "an 8-bit KV arena is a uint8 CUDA tensor [blocks, layers, heads, 2, 2064]");
   const c10::cuda::CUDAGuard guard(arena.device());
-  auto rows = [&](const c10::optional<at::Tensor>& t) {
-    return t.has_value() ? *t : at::empty({slots.numel(), arena.size(2) * 128}, arena.options().dtype(at::kBFloat16));
-  };
-  at::Tensor k = rows(k_out), v = rows(v_out);
+  const int64_t n = slots.numel(), w = arena.size(2) * 128;
+  at::Tensor k, v;
+  if (k_out.has_value()) k = *k_out;
+  if (v_out.has_value()) v = *v_out;
+  if (!k.defined() && !v.defined()) {
+    Carve c(2 * Carve::room(n * w, at::kBFloat16), arena.device());
+    k = c.take({n, w}, at::kBFloat16);
+    v = c.take({n, w}, at::kBFloat16);
+  } else if (!k.defined() || !v.defined()) {
+    (k.defined() ? v : k) = at::empty({n, w}, arena.options().dtype(at::kBFloat16));
+  }
   lakeb::Kv8RowArgs a = kv8_row_args(k, v, slots, arena, layer, status);
   a.k_out = bfm(k);
   a.v_out = bfm(v);
@@ -688,11 +715,20 @@ std::vector<at::Tensor> step_tables(const at::Tensor& pages, const at::Tensor& r
   TORCH_CHECK(max_tokens >= 0 && max_tiles >= 0 && max_tokens < (int64_t(1) << 30) && max_tiles < (int64_t(1) << 28),
               "max_tokens and max_tiles must not be negative (or past 2^30, 2^28)");
   const c10::cuda::CUDAGuard guard(pages.device());
-  const auto i32 = pages.options();
-  std::vector<at::Tensor> out = {at::empty({n, pages.size(1)}, i32),  at::empty({n}, i32),
-                                 at::empty({n + 1}, i32),             at::empty({max_tokens}, i32),
-                                 at::empty({max_tokens}, i32.dtype(at::kLong)), at::empty({max_tiles, 4}, i32),
-                                 at::empty({2}, i32)};
+  const int64_t w = pages.size(1);
+  const auto i32 = at::kInt;
+  Carve c(Carve::room(n * w, i32) + Carve::room(n, i32) + Carve::room(n + 1, i32) + Carve::room(max_tokens, i32) +
+              Carve::room(max_tokens, at::kLong) + Carve::room(4 * max_tiles, i32) + Carve::room(2, i32),
+          pages.device());
+  std::vector<at::Tensor> out;
+  out.reserve(7);
+  out.push_back(c.take({n, w}, i32));
+  out.push_back(c.take({n}, i32));
+  out.push_back(c.take({n + 1}, i32));
+  out.push_back(c.take({max_tokens}, i32));
+  out.push_back(c.take({max_tokens}, at::kLong));
+  out.push_back(c.take({max_tiles, 4}, i32));
+  out.push_back(c.take({2}, i32));
   lakeb::StepTableArgs a;
   a.pages = pages.data_ptr<int>();
   a.pages_stride = pages.stride(0);

@@ -4,9 +4,10 @@
 //  * kv8_read: the cached rows of a list of slots -> dense bf16 rows.
 //  * step_tables: positions, slots, query starts, block tables and query tiles from request lengths.
 //
-// The first two move bytes: 258 + 512 per (row, head), against which 256 conversions are nothing.
-// A warp takes one (row, head) at a time, half of it K and half V, 16 bytes of bf16 and 8 bytes
-// of codes per lane, so both sides of a head move as whole 128- and 256-byte rows.
+// The first two move bytes: 258 + 512 per (row, head), against which 256 conversions are nothing. A
+// warp takes one row and up to four heads at a time, half of it K and half V, 16 bytes of bf16 and 8
+// bytes of codes per lane and head: both sides of a head move as whole 128- and 256-byte rows, and
+// four independent loads per lane are in flight behind the one load of the slot.
 #include "common.cuh"
 #include "kv8.cuh"
 #include "lakeb_kernels.h"
@@ -16,22 +17,38 @@ namespace lakeb {
 namespace {
 
 constexpr int kRowWarps = 8;
+constexpr int kHeads = 4;  // of one warp's turn
+
+// Warp `u` of the launch: row and first head.
+__device__ __forceinline__ bool row_unit(const Kv8RowArgs& a, uint32_t u, int& row, int& head, int64_t& slot) {
+  const uint32_t groups = (a.heads + kHeads - 1) / kHeads;
+  row = static_cast<int>(u / groups);
+  head = static_cast<int>(u % groups) * kHeads;
+  if (row >= a.rows) return false;
+  slot = a.slots[row];
+  if (slot >= a.num_blocks * kKv8Page) {
+    if ((threadIdx.x & 31) == 0) record_error(a.status, kErrBounds);
+    slot = -1;
+  }
+  return true;
+}
 
 __global__ void __launch_bounds__(kRowWarps * 32) kv8_write_kernel(const Kv8RowArgs a) {
   const int lane = threadIdx.x & 31, side = lane >> 4, l = lane & 15;
-  const int64_t units = static_cast<int64_t>(a.rows) * a.heads;
-  for (int64_t u = static_cast<int64_t>(blockIdx.x) * kRowWarps + (threadIdx.x >> 5); u < units;
-       u += static_cast<int64_t>(gridDim.x) * kRowWarps) {
-    const int row = static_cast<int>(u / a.heads), head = static_cast<int>(u % a.heads);
-    const int64_t slot = a.slots[row];
-    if (slot < 0) continue;
-    if (slot >= a.num_blocks * kKv8Page) {
-      if (lane == 0) record_error(a.status, kErrBounds);
-      continue;
-    }
-    const __nv_bfloat16* src = (side ? a.v + row * a.v_stride : a.k + row * a.k_stride) + head * kKv8Dim + l * 8;
-    const uint4 x = *reinterpret_cast<const uint4*>(src);
-    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  int row, head;
+  int64_t slot;
+  if (!row_unit(a, blockIdx.x * kRowWarps + (threadIdx.x >> 5), row, head, slot) || slot < 0) return;
+  const __nv_bfloat16* src = (side ? a.v + row * a.v_stride : a.k + row * a.k_stride) + head * kKv8Dim + l * 8;
+  const int t = static_cast<int>(slot & (kKv8Page - 1));
+  uint8_t* dst = a.arena + (slot / kKv8Page) * a.block_bytes + a.layer_offset + head * kKv8Head + side * kKv8Side;
+  const int n = min(kHeads, a.heads - head);
+  uint4 x[kHeads];
+#pragma unroll
+  for (int h = 0; h < kHeads; ++h)
+    x[h] = h < n ? __ldcs(reinterpret_cast<const uint4*>(src + h * kKv8Dim)) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+  for (int h = 0; h < kHeads; ++h) {
+    const uint32_t w[4] = {x[h].x, x[h].y, x[h].z, x[h].w};
     uint32_t top = 0;  // |bf16| as integers, both halves of each word
 #pragma unroll
     for (int i = 0; i < 4; ++i) top = max(top, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
@@ -46,43 +63,47 @@ __global__ void __launch_bounds__(kRowWarps * 32) kv8_write_kernel(const Kv8RowA
       q[i] = e4m3x2(x0, x1) | e4m3x2(x2, x3) << 16;
     }
     if (b == 255) q[0] = q[1] = 0;
-    const int t = static_cast<int>(slot % kKv8Page);
-    uint8_t* dst = a.arena + (slot / kKv8Page) * a.block_bytes + a.layer_offset + head * kKv8Head + side * kKv8Side;
-    *reinterpret_cast<uint2*>(dst + kv8_chunk(t, l >> 1) + (l & 1) * 8) = make_uint2(q[0], q[1]);
-    if (l == 0) dst[kKv8Page * kKv8Dim + t] = static_cast<uint8_t>(b);
+    if (h < n) {
+      *reinterpret_cast<uint2*>(dst + h * kKv8Head + kv8_chunk(t, l >> 1) + (l & 1) * 8) = make_uint2(q[0], q[1]);
+      if (l == 0) dst[h * kKv8Head + kKv8Page * kKv8Dim + t] = static_cast<uint8_t>(b);
+    }
   }
 }
 
 __global__ void __launch_bounds__(kRowWarps * 32) kv8_read_kernel(const Kv8RowArgs a) {
   const int lane = threadIdx.x & 31, side = lane >> 4, l = lane & 15;
-  const int64_t units = static_cast<int64_t>(a.rows) * a.heads;
-  for (int64_t u = static_cast<int64_t>(blockIdx.x) * kRowWarps + (threadIdx.x >> 5); u < units;
-       u += static_cast<int64_t>(gridDim.x) * kRowWarps) {
-    const int row = static_cast<int>(u / a.heads), head = static_cast<int>(u % a.heads);
-    const int64_t slot = a.slots[row];
-    const bool ok = slot >= 0 && slot < a.num_blocks * kKv8Page;
-    if (slot >= 0 && !ok && lane == 0) record_error(a.status, kErrBounds);
-    uint4 out = make_uint4(0, 0, 0, 0);
-    if (ok) {
-      const int t = static_cast<int>(slot % kKv8Page);
-      const uint8_t* src =
-          a.arena + (slot / kKv8Page) * a.block_bytes + a.layer_offset + head * kKv8Head + side * kKv8Side;
-      const uint2 q = *reinterpret_cast<const uint2*>(src + kv8_chunk(t, l >> 1) + (l & 1) * 8);
-      const float f = kv8_scale(src[kKv8Page * kKv8Dim + t]);
-      auto two = [&](uint32_t h) {
-        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h));
-        return pack_bf16x2(v.x * f, v.y * f);
-      };
-      out = make_uint4(two(f16x2_lo(q.x)), two(f16x2_hi(q.x)), two(f16x2_lo(q.y)), two(f16x2_hi(q.y)));
-    }
-    __nv_bfloat16* dst = (side ? a.v_out + row * a.v_stride : a.k_out + row * a.k_stride) + head * kKv8Dim + l * 8;
-    *reinterpret_cast<uint4*>(dst) = out;
+  int row, head;
+  int64_t slot;
+  if (!row_unit(a, blockIdx.x * kRowWarps + (threadIdx.x >> 5), row, head, slot)) return;
+  const int n = min(kHeads, a.heads - head);
+  const int t = static_cast<int>(slot & (kKv8Page - 1));
+  const uint8_t* src =
+      a.arena + (max(slot, int64_t(0)) / kKv8Page) * a.block_bytes + a.layer_offset + head * kKv8Head + side * kKv8Side;
+  uint2 q[kHeads];
+  int b[kHeads];
+#pragma unroll
+  for (int h = 0; h < kHeads; ++h) {
+    const bool real = slot >= 0 && h < n;
+    q[h] = real ? *reinterpret_cast<const uint2*>(src + h * kKv8Head + kv8_chunk(t, l >> 1) + (l & 1) * 8)
+                : make_uint2(0, 0);
+    b[h] = real ? src[h * kKv8Head + kKv8Page * kKv8Dim + t] : 0;
+  }
+  __nv_bfloat16* dst = (side ? a.v_out + row * a.v_stride : a.k_out + row * a.k_stride) + head * kKv8Dim + l * 8;
+#pragma unroll
+  for (int h = 0; h < kHeads; ++h) {
+    const float f = kv8_scale(b[h]);
+    auto two = [&](uint32_t c) {
+      const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&c));
+      return pack_bf16x2(v.x * f, v.y * f);
+    };
+    if (h < n)
+      *reinterpret_cast<uint4*>(dst + h * kKv8Dim) =
+          make_uint4(two(f16x2_lo(q[h].x)), two(f16x2_hi(q[h].x)), two(f16x2_lo(q[h].y)), two(f16x2_hi(q[h].y)));
   }
 }
 
-int row_grid(const Kv8RowArgs& a) {
-  const int64_t ctas = (static_cast<int64_t>(a.rows) * a.heads + kRowWarps - 1) / kRowWarps;
-  return static_cast<int>(ctas < int64_t(num_sms()) * 16 ? ctas : int64_t(num_sms()) * 16);
+int64_t row_grid(const Kv8RowArgs& a) {
+  return (static_cast<int64_t>(a.rows) * ((a.heads + kHeads - 1) / kHeads) + kRowWarps - 1) / kRowWarps;
 }
 
 // ------------------------------------------------------------------ step tables
@@ -199,13 +220,15 @@ __global__ void __launch_bounds__(kTabThreads) step_tables_kernel(const StepTabl
 
 int kv8_write(const Kv8RowArgs& a, cudaStream_t stream) {
   if (a.rows <= 0) return 0;
-  kv8_write_kernel<<<row_grid(a), kRowWarps * 32, 0, stream>>>(a);
+  if (row_grid(a) * kRowWarps >= (int64_t(1) << 32) || row_grid(a) >= (int64_t(1) << 31)) return -1;
+  kv8_write_kernel<<<static_cast<unsigned>(row_grid(a)), kRowWarps * 32, 0, stream>>>(a);
   return cudaGetLastError();
 }
 
 int kv8_read(const Kv8RowArgs& a, cudaStream_t stream) {
   if (a.rows <= 0) return 0;
-  kv8_read_kernel<<<row_grid(a), kRowWarps * 32, 0, stream>>>(a);
+  if (row_grid(a) * kRowWarps >= (int64_t(1) << 32) || row_grid(a) >= (int64_t(1) << 31)) return -1;
+  kv8_read_kernel<<<static_cast<unsigned>(row_grid(a)), kRowWarps * 32, 0, stream>>>(a);
   return cudaGetLastError();
 }
 

@@ -39,7 +39,7 @@ def build_step_tables(pages: torch.Tensor, rows: torch.Tensor, context_lens: tor
     (the status word on the GPU, ValueError on the CPU); on the GPU such a token gets slot -1."""
     if pages.is_cuda:
         core.LAUNCHES[0] += 1
-        return StepTables(*native().step_tables(pages, rows, context_lens, new_lens, max_tokens, max_tiles, n_decode,
+        return StepTables._make(native().step_tables(pages, rows, context_lens, new_lens, max_tokens, max_tiles, n_decode,
                                                 block_size, tile, core.status_word(pages.device)))
     if max_tokens < 0 or max_tiles < 0:
         raise ValueError(f"max_tokens and max_tiles must not be negative, got {max_tokens} and {max_tiles}")
