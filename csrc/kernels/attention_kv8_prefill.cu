@@ -149,16 +149,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* v_empty = bars + 12;    // [2]
   uint64_t* s_full = bars + 14;     // [2 heads][2 buffers]
   uint64_t* p_full = bars + 18;     // [2 heads][2 buffers]
-  uint64_t* o_done = bars + 22;     // [2 heads]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 25);
+  uint64_t* o_done = bars + 22;     // [2 heads], a phase per step
+  uint64_t* o_last = bars + 24;     // [2 heads], the last step's PV
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 26);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 27);
   TileParams* params = reinterpret_cast<TileParams*>(smem + kParams);
 
   // heavy (late) query tiles first: the grid runs in reverse tile order
   const int4 tile = a.tiles[a.num_tiles - 1 - static_cast<int>(blockIdx.x)];
   const int seq = tile.x, qrow0 = tile.y, nq = tile.z, pos0 = tile.w;
   if (nq <= 0) return;
-  if (!kv8_tile_ok(a, tile)) return;
   if (smem_u32(smem) & 1023) {  // the swizzled tiles need it; the launch gives it
     if (threadIdx.x == 0) record_error(a.status, kErrBadArg);
     return;
@@ -184,6 +184,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&v_full[i], 128);
       mbar_init(&v_empty[i], 1);
       mbar_init(&o_done[i], 1);
+      mbar_init(&o_last[i], 1);
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(&s_full[i], 1);
@@ -264,6 +265,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int k = 0; k < 4; ++k) mma_ts(d, p + 8 * k, vd + k * 128, idesc_o, i > 0 || k > 0, lead);
         commit(&o_done[h], lead);
+        if (i == n_steps - 1) commit(&o_last[h], lead);
       };
       bool ok = mbar_wait(q_ready, 0, abort_flag, a.status) && mbar_wait(&k_full[0], 0, abort_flag, a.status);
       ok = __all_sync(0xffffffffu, ok);
@@ -276,28 +278,28 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto wait = [&](uint64_t* bar, int parity) {
         return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, a.status));
       };
-      // S(h, i) goes over P(h, i - 2): PV(h, i - 2) has to be done with it, not just issued (products of
-      // different shapes may overlap). It is issued behind the other head's next PV, so that the wait
-      // for o_done finds it done.
-      auto next_s = [&](int h, int i) {
-        if (i < 2 || i >= n_steps) return true;
-        if (h == 0 && (i & 1) == 0 && !wait(&k_full[(i >> 1) & 1], (i >> 2) & 1)) return false;
-        if (!wait(&o_done[h], i & 1)) return false;
-        tc_fence_after();
-        issue_s(h, i);
-        if (h == heads - 1 && ((i & 1) || i + 1 == n_steps)) commit(&k_empty[(i >> 1) & 1], lead);
-        return true;
-      };
+      // S(h, i + 2) goes over P(h, i): PV(h, i) has to be done with it, not just issued (products of
+      // different shapes may overlap). The other head's softmax runs meanwhile.
       for (int i = 0; i < n_steps && ok; ++i) {
-        const int j = i >> 1;
-        if ((i & 1) == 0) ok = wait(&v_full[j & 1], (j >> 1) & 1);
+        const int j = i >> 1, jn = j + 1;
+        const bool more = i + 2 < n_steps, last = (i & 1) || i + 1 == n_steps;
+        if ((i & 1) == 0) {
+          ok = wait(&v_full[j & 1], (j >> 1) & 1);
+          if (ok && more) ok = wait(&k_full[jn & 1], (jn >> 1) & 1);
+        }
         for (int h = 0; h < heads && ok; ++h) {
           ok = wait(&p_full[2 * h + (i & 1)], j & 1);
           if (!ok) break;
           tc_fence_after();
           issue_pv(h, i);
-          if (h == heads - 1 && ((i & 1) || i + 1 == n_steps)) commit(&v_empty[j & 1], lead);
-          ok = heads == 1 ? next_s(0, i + 2) : h == 0 ? next_s(1, i + 1) : next_s(0, i + 2);
+          if (h == heads - 1 && last) commit(&v_empty[j & 1], lead);
+          if (more) {
+            ok = wait(&o_done[h], i & 1);
+            if (!ok) break;
+            tc_fence_after();
+            issue_s(h, i + 2);
+            if (h == heads - 1 && ((i & 1) || i + 3 == n_steps)) commit(&k_empty[jn & 1], lead);
+          }
         }
       }
     }
@@ -476,10 +478,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_before();
         mbar_arrive(&p_full[2 * h + buf]);
       }
-      // This warp may have ended its last step before another one's arrival let PV(n_steps - 2) go: both
-      // phases in turn (one wait for the last could be met by the phase two before it).
-      ok = ok && (n_steps < 2 || mbar_wait(&o_done[h], n_steps & 1, abort_flag, a.status)) &&
-           mbar_wait(&o_done[h], (n_steps - 1) & 1, abort_flag, a.status);
+      // (o_done's last phases may pass before this warp looks, or be two behind: parity alone cannot tell)
+      ok = ok && mbar_wait(&o_last[h], 0, abort_flag, a.status);
       if (__all_sync(0xffffffffu, ok)) {
         tc_fence_after();
         const float inv = l == 0.f ? 0.f : exp2f(static_cast<float>(e0)) / l;
