@@ -671,6 +671,8 @@ at::Tensor kv8_decode(const at::Tensor& q, c10::optional<at::Tensor> out_arg, co
   return out;
 }
 
+constexpr int kFewRows = 32;
+
 at::Tensor kv8_prefill(const at::Tensor& q, c10::optional<at::Tensor> out_arg, const at::Tensor& arena, int64_t layer,
                        const at::Tensor& block_tables, const at::Tensor& seq_lens, const at::Tensor& tiles,
                        int64_t n_q_heads, int64_t n_kv_heads, double scale, c10::optional<at::Tensor> status) {
@@ -685,10 +687,18 @@ at::Tensor kv8_prefill(const at::Tensor& q, c10::optional<at::Tensor> out_arg, c
   p.num_tiles = static_cast<int>(tiles.size(0));
   if (p.num_tiles == 0) return out;
   const c10::cuda::CUDAGuard guard(arena.device());
-  if (p.num_rows > 8 * p.num_tiles) {
-    LAKEB_CHECK_RC(lakeb::kv8_prefill_tc(p, cur_stream()), "kv8_prefill");
-  } else {
+  // A tile of at most 32 rows costs less as columns of the few-row kernel (192 cycles of an SM per page
+  // and 24 columns, cut evenly over the GPU) than as 128 rows of the tcgen05 one (550 per page and two
+  // heads, one CTA for all its keys). The host does not see the tiles' rows: with several sequences
+  // both kernels run, each on its own, where their rows on average leave it open.
+  if (p.num_rows <= 8 * int64_t(p.num_tiles) || (p.num_seqs == 1 && p.num_rows <= kFewRows)) {
     kv8_few_rows(p, q);
+  } else {
+    if (p.num_seqs > 1) {
+      p.most_rows = p.few_rows = kFewRows;
+      kv8_few_rows(p, q);
+    }
+    LAKEB_CHECK_RC(lakeb::kv8_prefill_tc(p, cur_stream()), "kv8_prefill");
   }
   return out;
 }

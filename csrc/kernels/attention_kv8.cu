@@ -280,7 +280,7 @@ __device__ __forceinline__ Item get_item(const Kv8AttnArgs& a, int s) {
   if (a.tiles) {
     const int4 t = a.tiles[s];
     it.seq = t.x, it.row0 = t.y, it.nq = max(t.z, 0), it.pos0 = t.w;
-    if (!kv8_tile_ok(a, t)) it.seq = it.row0 = it.nq = 0;
+    if (it.nq > a.most_rows || !kv8_tile_ok(a, t)) it.seq = it.row0 = it.nq = 0;
   } else {
     it.seq = it.row0 = s, it.nq = 1, it.pos0 = 0;
   }
@@ -595,19 +595,28 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(const Kv8AttnArgs a) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = a.n_q_heads / a.n_kv_heads;
   const int items = a.tiles ? a.num_tiles : a.num_seqs;
+  asm volatile("griddepcontrol.launch_dependents;");
   // lengths and tiles are not the first kernel's to write: the search needs no wait
   int keep[8];
   const int64_t total = total_cost<NT>(a, items, lane, keep);
   const int64_t per = run_length(total, gridDim.x);
   const int64_t run0 = blockIdx.x * per, run1 = run0 + per;
-  if (run1 >= total) return;
+  // (every CTA waits for the first kernel, those with nothing to do as well: what is launched next
+  // follows this kernel's end alone)
+  if (run1 >= total) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
+  }
   const Place p = find_place<NT>(a, items, run1 - 1, lane, keep);
   const Item it = get_item<NT>(a, p.item);
   const int unit = p.in_item / (it.pages + kSegCost);
   const int64_t seg0 = run1 - 1 - p.in_item % (it.pages + kSegCost);
   const int64_t seg1 = seg0 + kSegCost + it.pages;
   const int64_t first = seg0 + kSegCost;  // its first page
-  if (first < run0 || first >= run1 || seg1 <= run1) return;
+  if (first < run0 || first >= run1 || seg1 <= run1) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
+  }
   const int pieces = static_cast<int>((seg1 - 1) / per - blockIdx.x) + 1;
   const int slot0 = 2 * static_cast<int>(blockIdx.x) + (seg0 > run0);
   const int kvh = unit / it.groups, cb = unit % it.groups * kCols;
@@ -698,7 +707,7 @@ int64_t kv8_attention_ws_floats(const Kv8AttnArgs& a) {
 // pages costs 16 MMAs of 16 cycles per page and group, so a group that stays empty costs as much as
 // a full one, and columns beyond the groups cost another pass.
 int kv8_attention_groups(const Kv8AttnArgs& a) {
-  const int64_t rows = a.tiles ? (a.num_rows + a.num_tiles - 1) / a.num_tiles : 1;
+  const int64_t rows = !a.tiles ? 1 : a.most_rows < a.num_rows ? a.most_rows : (a.num_rows + a.num_tiles - 1) / a.num_tiles;
   const int64_t groups = (rows * (a.n_q_heads / a.n_kv_heads) + 7) / 8;
   return groups < 3 ? static_cast<int>(groups) : 3;
 }

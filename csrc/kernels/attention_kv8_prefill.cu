@@ -6,17 +6,19 @@
 //   S_h   = Q_h K_i^T           tcgen05.mma fp16 (M=128, N=64, K=128), fp32 in tensor memory
 //   P_h   = 2^(S_h c + e_j - b) softmax warpgroup h: thread = query row; fp16 over S_h's columns
 //   O_h  += P_h V_i             tcgen05.mma, A = P_h from tensor memory, V_i MN-major in shared memory
-// A head has two S buffers of 64 columns: S(i+1) is there when the softmax of step i ends, so the
-// softmax warps never wait for a product, and PV(i) and S(i+2) run behind them. With one buffer of
-// 128 columns (tensor memory holds no more beside the two O) softmax and products of a head take
-// turns: 5.1k cycles per 128 keys and two heads, against 2.0k of products and 2.0k of exponentials.
+// A head has two S buffers of 64 columns: S(i+1) is there when the softmax of step i ends, and PV(i)
+// and S(i+2) run behind it. With one buffer of 128 columns (tensor memory holds no more beside the
+// two O) softmax and products of a head take turns, and 128 keys of two heads took 5.1k cycles; so
+// they take 4.4k, of which the products run 2.6k and the exponentials 2.0k. What binds is shared
+// memory (products' operands, conversion and copies move ~390 KB per tile, 3.0k cycles) and the
+// hand-offs that wait behind it. Measured: one 8192-token prompt of 32 query and 8 KV heads 0.64 ms,
+// 860 TFLOP/s; four of 2048 tokens 0.23 ms.
 //
 // 8-bit operands become fp16 ones in shared memory: bulk copies bring the K and the V sides of the
 // tile's eight pages (2064 bytes each, scales included) into a staging buffer each, a warpgroup for
 // each side turns codes into fp16 rows of the 128-byte swizzle (thread = key; e4m3 -> fp16 is
-// exact). The tensor cores' own fp8
-// products would need Q and P in 8 bits as well, or twice the products. A tile is scaled
-// against its own largest K scale and V scale: a row keeps code * 2^(e_row - e_tile), exact while
+// exact). The tensor cores' own fp8 products would need Q and P in 8 bits as well, or twice the
+// products. A tile is scaled against its own largest K scale and V scale: a row keeps code * 2^(e_row - e_tile), exact while
 // e_tile - e_row <= 15 (a code's last bit is 2^-9, fp16's 2^-24), and e_tile itself is one
 // multiplier of the tile's scores, or one addend of its exponents, not work per element. Where
 // rows of one tile differ by more than 2^15, the small rows' last bits are lost: an error of
@@ -28,8 +30,7 @@
 //
 // Warps: 0 = loads, 1 = tensor memory and MMA issue, 2-3 idle, 4-7 = converters of K, 8-11 = of V,
 // 12-15 and 16-19 = softmax of head A and B. Registers move from the first three warpgroups to the
-// softmax ones.
-// Every wait is bounded; a role whose wait ran out goes on through its loop without work, so that
+// softmax ones. Every wait is bounded; a role whose wait ran out goes on through its loop without work, so that
 // the converters' named barriers are always reached by all of their warps.
 #include <math_constants.h>
 
@@ -55,6 +56,7 @@ constexpr int kRed = kParams + 4 * 32;               // [2 tiles][K, V][4] conve
 constexpr int kSmem = kRed + 2 * 2 * 4 * 8;
 constexpr int kThreads = 640;
 constexpr int kStep = 64;                            // keys per softmax step
+constexpr int kRanked = 256;                         // tiles of a launch that are ordered by their keys
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.0f;
 constexpr float kPBias = 7.0f;
@@ -89,7 +91,9 @@ __device__ __forceinline__ uint32_t f16x2_exp2(int d) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// One lane of the warp (the same each time).
+// One lane of the warp, the same each time. The MMA warp runs its loop as a whole and this lane's
+// products take effect: descriptors stay in uniform registers, and products issue as fast as they
+// run (48 cycles for 128 x 64 x 16, 64 for 128 x 128 x 16; from a branch of one lane ~120).
 __device__ __forceinline__ uint32_t elect_one() {
   uint32_t r;
   asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(r));
@@ -155,12 +159,43 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 27);
   TileParams* params = reinterpret_cast<TileParams*>(smem + kParams);
 
-  // heavy (late) query tiles first: the grid runs in reverse tile order
-  const int4 tile = a.tiles[a.num_tiles - 1 - static_cast<int>(blockIdx.x)];
-  const int seq = tile.x, qrow0 = tile.y, nq = tile.z, pos0 = tile.w;
-  if (nq <= 0) return;
+  // Heavy query tiles first, or one of them would run on alone at the end. Of one sequence they are the
+  // late ones; of several, each CTA finds the tile of its rank by the keys that it sees.
   if (smem_u32(smem) & 1023) {  // the swizzled tiles need it; the launch gives it
     if (threadIdx.x == 0) record_error(a.status, kErrBadArg);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
+  }
+  int rank = a.num_tiles - 1 - static_cast<int>(blockIdx.x);
+  if (a.num_seqs > 1 && a.num_tiles <= kRanked) {
+    int* keys = reinterpret_cast<int*>(smem + kK);
+    const int t = threadIdx.x;
+    if (t < kRanked) {
+      int n = -1;
+      if (t < a.num_tiles) {
+        const int4 x = a.tiles[t];
+        n = x.z > a.few_rows && kv8_tile_ok(a, x) ? min(x.w + x.z, a.seq_lens[x.x]) : 0;
+      }
+      keys[t] = n;
+    }
+    __syncthreads();
+    if (t < a.num_tiles) {
+      const int mine = keys[t];
+      int before = 0;
+      for (int u = 0; u < a.num_tiles; u += 4) {
+        const int4 k = *reinterpret_cast<const int4*>(keys + u);
+        before += (k.x > mine || (k.x == mine && u < t)) + (k.y > mine || (k.y == mine && u + 1 < t)) +
+                  (k.z > mine || (k.z == mine && u + 2 < t)) + (k.w > mine || (k.w == mine && u + 3 < t));
+      }
+      if (before == static_cast<int>(blockIdx.x)) keys[kRanked] = t;
+    }
+    __syncthreads();
+    rank = keys[kRanked];
+  }
+  const int4 tile = a.tiles[rank];
+  const int seq = tile.x, qrow0 = tile.y, nq = tile.z, pos0 = tile.w;
+  if (nq <= a.few_rows || !kv8_tile_ok(a, tile)) {  // none, or kv8_attention's
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     return;
   }
   const int G = a.n_q_heads / a.n_kv_heads, pairs = (G + 1) / 2;
@@ -278,28 +313,28 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto wait = [&](uint64_t* bar, int parity) {
         return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, a.status));
       };
-      // S(h, i + 2) goes over P(h, i): PV(h, i) has to be done with it, not just issued (products of
-      // different shapes may overlap). The other head's softmax runs meanwhile.
+      // S(h, i) goes over P(h, i - 2): PV(h, i - 2) has to be done with it, not just issued (products of
+      // different shapes may overlap). It is issued behind the other head's next PV, so that the wait
+      // for o_done finds it done.
+      auto next_s = [&](int h, int i) {
+        if (i < 2 || i >= n_steps) return true;
+        if (h == 0 && (i & 1) == 0 && !wait(&k_full[(i >> 1) & 1], (i >> 2) & 1)) return false;
+        if (!wait(&o_done[h], i & 1)) return false;
+        tc_fence_after();
+        issue_s(h, i);
+        if (h == heads - 1 && ((i & 1) || i + 1 == n_steps)) commit(&k_empty[(i >> 1) & 1], lead);
+        return true;
+      };
       for (int i = 0; i < n_steps && ok; ++i) {
-        const int j = i >> 1, jn = j + 1;
-        const bool more = i + 2 < n_steps, last = (i & 1) || i + 1 == n_steps;
-        if ((i & 1) == 0) {
-          ok = wait(&v_full[j & 1], (j >> 1) & 1);
-          if (ok && more) ok = wait(&k_full[jn & 1], (jn >> 1) & 1);
-        }
+        const int j = i >> 1;
+        if ((i & 1) == 0) ok = wait(&v_full[j & 1], (j >> 1) & 1);
         for (int h = 0; h < heads && ok; ++h) {
           ok = wait(&p_full[2 * h + (i & 1)], j & 1);
           if (!ok) break;
           tc_fence_after();
           issue_pv(h, i);
-          if (h == heads - 1 && last) commit(&v_empty[j & 1], lead);
-          if (more) {
-            ok = wait(&o_done[h], i & 1);
-            if (!ok) break;
-            tc_fence_after();
-            issue_s(h, i + 2);
-            if (h == heads - 1 && ((i & 1) || i + 3 == n_steps)) commit(&k_empty[jn & 1], lead);
-          }
+          if (h == heads - 1 && ((i & 1) || i + 1 == n_steps)) commit(&v_empty[j & 1], lead);
+          ok = heads == 1 ? next_s(0, i + 2) : h == 0 ? next_s(1, i + 1) : next_s(0, i + 2);
         }
       }
     }
@@ -511,6 +546,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+  // after kv8_attention's kernels for the small tiles, which this one does not read from: the call is
+  // done when all are
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 }  // namespace
@@ -522,8 +560,17 @@ int kv8_prefill_tc(const Kv8AttnArgs& a, cudaStream_t stream) {
   if (!encode_bf16_map(&qmap, a.q, a.num_rows, cols, a.num_rows > 1 ? a.q_stride : cols, 128, 64)) return -5;
   if (int e = ensure_smem_attr(reinterpret_cast<const void*>(kv8_prefill_kernel), kSmem)) return e;
   const int G = a.n_q_heads / a.n_kv_heads;
-  kv8_prefill_kernel<<<dim3(a.num_tiles, a.n_kv_heads * ((G + 1) / 2)), kThreads, kSmem, stream>>>(qmap, a);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(a.num_tiles, a.n_kv_heads * ((G + 1) / 2));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = a.few_rows > 0 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kv8_prefill_kernel, qmap, a);
 }
 
 }  // namespace lakeb
