@@ -110,6 +110,18 @@ KVArenaView arena_view(const at::Tensor& arena, int64_t layer, bool host_ok = fa
   TORCH_CHECK(arena.is_cuda() || (host_ok && is_registered_host(arena)),
               "arena must be device memory (or, as a second K/V target, pinned host memory registered with "
               "register_host_arena)");
+  if (arena.scalar_type() == at::kByte) {  // 8-bit arena (kv8.cuh)
+    TORCH_CHECK(arena.dim() == 5 && arena.is_contiguous() && arena.size(3) == 2 && arena.size(4) == 2064,
+                "an 8-bit KV arena is a contiguous uint8 tensor [blocks, layers, kv_heads, 2, 2064] (head_dim 128)");
+    TORCH_CHECK(layer >= 0 && layer < arena.size(1), "layer ", layer, " of an arena of ", arena.size(1));
+    check_aligned(arena, "arena");
+    KVArenaView v;
+    v.base8 = arena.data_ptr<uint8_t>();
+    v.block_stride = arena.stride(0);
+    v.layer_offset = layer * arena.stride(1);
+    v.num_slots = arena.size(0) * 16;
+    return v;
+  }
   TORCH_CHECK(arena.scalar_type() == at::kBFloat16 && arena.dim() == 6 && arena.is_contiguous(),
               "arena must be a contiguous bf16 [blocks, layers, 2, kv_heads, block, 128] tensor");
   TORCH_CHECK(arena.size(5) == 128, "head_dim must be 128");
@@ -235,9 +247,11 @@ void linear_qkv(const at::Tensor& a, const at::Tensor& w, at::Tensor& q_out, con
   g.positions = positions.data_ptr<int>();
   g.slots = slots.data_ptr<int64_t>();
   g.kv = arena_view(arena, layer);
+  if (g.kv.base8) TORCH_CHECK(arena.size(2) == n_kv_heads, "kv heads mismatch: ", n_kv_heads, " for an arena of ", arena.size(2));
   g.n_q_heads = static_cast<int>(n_q_heads);
   g.n_kv_heads = static_cast<int>(n_kv_heads);
   if (peer_arena.has_value() && peer_slots.has_value()) {
+    TORCH_CHECK(peer_arena->scalar_type() == arena.scalar_type(), "peer arena of another type");
     g.peer_kv = arena_view(*peer_arena, layer, /*host_ok=*/true);
     TORCH_CHECK(peer_slots->scalar_type() == at::kLong, "peer_slots int64");
     g.peer_slots = peer_slots->data_ptr<int64_t>();

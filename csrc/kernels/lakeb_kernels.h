@@ -55,6 +55,7 @@ struct KVArenaView {
   int64_t head_stride = 0;        // elements between kv heads
   int block_size = 16;            // tokens per block
   int64_t num_slots = 0;          // blocks x block_size (index checks of the debug build)
+  uint8_t* base8 = nullptr;       // 8-bit arena (kv8.cuh) instead: block_stride and layer_offset in bytes
 };
 
 struct GemmArgs {

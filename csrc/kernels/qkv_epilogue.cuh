@@ -5,6 +5,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "kv8.cuh"
 #include "lakeb_kernels.h"
 
 namespace lakeb {
@@ -58,6 +59,72 @@ __device__ __forceinline__ __nv_bfloat16* kv_ptr(const KVArenaView& kv, int64_t 
          off * 128;
 }
 
+// K (roped, optionally normed before) or V of one head and row into an 8-bit arena: the row's scale
+// needs its largest element first, so the accumulators are read twice (a TMEM load costs less than
+// holding 128 results). The row is quantised from fp32; the codes go to token t of the page side `row`
+// of this arena and to the peer's (nullptr: neither).
+// Not inlined: the bf16 epilogue keeps its registers.
+__device__ __noinline__ void qkv_head_kv8(uint32_t tbase, bool is_k, uint8_t* row, uint8_t* peer_row, int t, int peer_t,
+                                          const float2* cs, const __nv_bfloat16* nw, float inv) {
+  auto piece = [&](int half, float (&o1)[32], float (&o2)[32]) {  // elements 32 * half.., 64 + 32 * half..
+    uint32_t r1[32], r2[32];
+    tmem_ld32(tbase + half * 32, r1);
+    tmem_ld32(tbase + 64 + half * 32, r2);
+    tmem_ld_wait();
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      float x1 = __uint_as_float(r1[j]), x2 = __uint_as_float(r2[j]);
+      if (is_k) {
+        if (nw) {
+          x1 *= inv * __bfloat162float(nw[half * 32 + j]);
+          x2 *= inv * __bfloat162float(nw[64 + half * 32 + j]);
+        }
+        const float2 c = cs[half * 32 + j];
+        const float a = x1 * c.x - x2 * c.y;
+        x2 = x2 * c.x + x1 * c.y;
+        x1 = a;
+      }
+      o1[j] = x1;
+      o2[j] = x2;
+    }
+  };
+  uint32_t top = 0;
+#pragma unroll 1
+  for (int half = 0; half < 2; ++half) {
+    float o1[32], o2[32];
+    piece(half, o1, o2);
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      top = max(top, max(__float_as_uint(o1[j]) & 0x7fffffffu, __float_as_uint(o2[j]) & 0x7fffffffu));
+  }
+  const int b = kv8_scale_byte(top);
+  const float f = kv8_inv_scale(b);
+#pragma unroll 1
+  for (int half = 0; half < 2; ++half) {
+    float o1[32], o2[32];
+    piece(half, o1, o2);
+    uint32_t q[2][8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      q[0][j] = e4m3x2(o1[4 * j] * f, o1[4 * j + 1] * f) | e4m3x2(o1[4 * j + 2] * f, o1[4 * j + 3] * f) << 16;
+      q[1][j] = e4m3x2(o2[4 * j] * f, o2[4 * j + 1] * f) | e4m3x2(o2[4 * j + 2] * f, o2[4 * j + 3] * f) << 16;
+      if (b == 255) q[0][j] = q[1][j] = 0;
+    }
+#pragma unroll
+    for (int d = 0; d < 2; ++d) {
+      uint8_t* side = d ? peer_row : row;
+      const int tok = d ? peer_t : t;
+      if (!side) continue;
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        *reinterpret_cast<uint4*>(side + kv8_chunk(tok, (c >> 1) * 4 + half * 2 + (c & 1))) =
+            make_uint4(q[c >> 1][4 * (c & 1)], q[c >> 1][4 * (c & 1) + 1], q[c >> 1][4 * (c & 1) + 2],
+                       q[c >> 1][4 * (c & 1) + 3]);
+      if (half == 0) side[kKv8Page * kKv8Dim + tok] = static_cast<uint8_t>(b);
+    }
+  }
+}
+
 // Head `head` of accumulator row `row` (this thread's TMEM lane; `tbase` addresses the head's
 // 128 fp32 columns). Every lane of the warp calls it (the TMEM loads are warp-aligned). With
 // `stage` (2 KB of this warp's shared memory) the peer-arena K/V stores are coalesced per warp.
@@ -72,12 +139,41 @@ __device__ __forceinline__ void qkv_head_epilogue(const GemmArgs& p, uint32_t tb
     pos = p.positions[row];
     if (!is_q) {
       slot = p.slots ? p.slots[row] : -1;
-      if (p.peer_kv.base && p.peer_slots) pslot = p.peer_slots[row];
+      if ((p.peer_kv.base || p.peer_kv.base8) && p.peer_slots) pslot = p.peer_slots[row];
       // debug build: a slot past the arena is reported and its store skipped
       if (slot >= 0 && !in_bounds(p.kv.num_slots <= 0 || slot < p.kv.num_slots, p.status)) slot = -1;
       if (pslot >= 0 && !in_bounds(p.peer_kv.num_slots <= 0 || pslot < p.peer_kv.num_slots, p.status))
         pslot = -1;
     }
+  }
+  if (p.kv.base8 && !is_q) {
+    // 8-bit arena: a slot past it is reported and skipped
+    if (slot >= p.kv.num_slots) record_error(p.status, kErrBounds), slot = -1;
+    if (p.peer_kv.base8 && pslot >= p.peer_kv.num_slots) record_error(p.status, kErrBounds), pslot = -1;
+    float inv = 1.f;
+    if (is_k && p.k_norm_w) {
+      float ss = 0.f;
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        uint32_t r[32];
+        tmem_ld32(tbase + c * 32, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 32; ++j) ss += __uint_as_float(r[j]) * __uint_as_float(r[j]);
+      }
+      inv = rsqrtf(ss * (1.f / 128.f) + p.qk_eps);
+    }
+    const int64_t in_page = (head - p.n_q_heads - (is_k ? 0 : p.n_kv_heads)) * kKv8Head + (is_k ? 0 : kKv8Side);
+    uint8_t* mine = slot < 0 ? nullptr
+                             : p.kv.base8 + (slot / kKv8Page) * p.kv.block_stride + p.kv.layer_offset + in_page;
+    uint8_t* theirs = pslot < 0 || !p.peer_kv.base8 ? nullptr
+                                                    : p.peer_kv.base8 + (pslot / kKv8Page) * p.peer_kv.block_stride +
+                                                          p.peer_kv.layer_offset + in_page;
+    // (a row outside the matrix has slot -1 and position 0: it stores nothing)
+    qkv_head_kv8(tbase, is_k, mine, theirs, static_cast<int>(slot & (kKv8Page - 1)),
+                 static_cast<int>(pslot & (kKv8Page - 1)), p.rope_cs + static_cast<int64_t>(pos) * 64,
+                 is_k ? p.k_norm_w : nullptr, inv);
+    return;
   }
   if (is_q || is_k) {
     const int kvh = head - p.n_q_heads;

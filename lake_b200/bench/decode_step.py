@@ -27,6 +27,7 @@ def main(argv=None):
     ap.add_argument("--steps", type=int, default=30)
     ap.add_argument("--warmup", type=int, default=5)
     ap.add_argument("--weights", choices=["bf16", "fp8"], default="bf16")
+    ap.add_argument("--kv", choices=["bf16", "fp8"], default="bf16", help="KV arena (fp8: 8 bits, EngineConfig.kv_dtype)")
     ap.add_argument("--profile", action="store_true")
     args = ap.parse_args(argv)
 
@@ -37,7 +38,8 @@ def main(argv=None):
     steps_total = args.warmup + (3 if args.profile else args.steps) + 2
     max_len = C + steps_total + 16
     eng = LLMEngine(args.model, device="cuda:0", max_running=B, max_batched_tokens=max(512, B),
-                    max_model_len=max_len, num_blocks=B * ((max_len + 15) // 16) + 64, weight_dtype=args.weights)
+                    max_model_len=max_len, num_blocks=B * ((max_len + 15) // 16) + 64, weight_dtype=args.weights,
+                    kv_dtype=args.kv)
     cfg = eng.cfg
     rng = random.Random(0)
     for i in range(B):
@@ -74,7 +76,7 @@ def main(argv=None):
         else:  # block-scaled fp8: e4m3 bytes + fp32 scales
             n = t.q.numel() + t.s.numel() * 4
         wbytes += (B * cfg.hidden * 2) if name == "embed_tokens" else n
-    kv_tok = cfg.n_layers * 2 * cfg.n_kv_heads * cfg.head_dim * 2
+    kv_tok = eng.arena[0].numel() * eng.arena.element_size() // 16  # pages of 16 tokens, either arena
     ctx_mid = C + args.warmup + args.steps // 2
     kvbytes = B * ctx_mid * kv_tok
     peaks = {}
@@ -84,7 +86,7 @@ def main(argv=None):
         peaks = json.load(open(p))
     hbm = float(peaks.get("hbm_gbs", 6650.0))
     roof_ms = (wbytes + kvbytes) / (hbm * 1e9) * 1e3
-    print(json.dumps({"bench": "decode_step", "model": args.model, "weights": args.weights, "batch": B,
+    print(json.dumps({"bench": "decode_step", "model": args.model, "weights": args.weights, "kv": args.kv, "batch": B,
                       "ctx": ctx_mid, "ms_median": round(ms, 3), "ms_min": round(times[0], 3),
                       "tok_s": round(B / ms * 1e3, 1), "weight_gb": round(wbytes / 1e9, 2),
                       "kv_gb": round(kvbytes / 1e9, 2), "roofline_ms": round(roof_ms, 3),

@@ -48,6 +48,10 @@ class EngineConfig:
     # group runs an engine with the same requests and makes the same scheduling decisions.
     tp: tuple | None = None
     weight_dtype: str = "bf16"  # "fp8": block-scaled e4m3 projection weights (W8A16 GEMMs)
+    # KV cache: "bf16" (the model's dtype on the CPU path), or "fp8": the 8-bit arena of
+    # ops.kv8_arena (e4m3 with a power-of-two scale per token and head), 258/512 of the bytes per
+    # cached token. Instances that exchange pages (PD, storage pool) use the same setting.
+    kv_dtype: str = "bf16"
     # Expert parallel (MoE): (rank, world, process group). Each rank serves its own requests and
     # steps in lockstep with the group (a step with no work still runs the expert exchange).
     ep: tuple | None = None
@@ -80,6 +84,11 @@ class StepOutput:
     finished: bool
 
 
+def kv8_arena_shape(cfg: ModelConfig, num_blocks: int, block_size: int = 16) -> tuple[int, ...]:
+    """8-bit arena [num_blocks, layers, kv_heads, 2, block_size * head_dim + block_size] (uint8)."""
+    return (num_blocks, cfg.n_layers, cfg.n_kv_heads, 2, block_size * cfg.head_dim + block_size)
+
+
 def alloc_arena(cfg: ModelConfig, num_blocks: int, device, dtype, block_size: int = 16) -> torch.Tensor:
     """Page-first KV arena [num_blocks, layers, 2, kv_heads, block_size, head_dim] (zero-filled)."""
     return torch.zeros(num_blocks, cfg.n_layers, 2, cfg.n_kv_heads, block_size, cfg.head_dim, dtype=dtype,
@@ -93,7 +102,9 @@ def _local_kv_cfg(cfg: ModelConfig, world: int) -> ModelConfig:
     return dataclasses.replace(cfg, n_kv_heads=cfg.n_kv_heads // world, n_q_heads=cfg.n_q_heads // world)
 
 
-def page_bytes(cfg: ModelConfig, block_size: int = 16, elem: int = 2) -> int:
+def page_bytes(cfg: ModelConfig, block_size: int = 16, elem: int = 2, kv8: bool = False) -> int:
+    if kv8:  # codes and one scale byte per token
+        return cfg.n_layers * 2 * cfg.n_kv_heads * block_size * (cfg.head_dim + 1)
     return cfg.n_layers * 2 * cfg.n_kv_heads * block_size * cfg.head_dim * elem
 
 
@@ -109,6 +120,15 @@ class LLMEngine:
             torch.cuda.set_device(self.device)
         maxb = (ec.max_model_len + ec.block_size - 1) // ec.block_size
         max_tokens = ec.max_batched_tokens + ec.max_running
+        if ec.kv_dtype not in ("bf16", "fp8"):
+            raise ValueError(f"kv_dtype is 'bf16' or 'fp8', got {ec.kv_dtype!r}")
+        kv8 = ec.kv_dtype == "fp8"
+        if kv8 and ec.block_size != 16:
+            raise ValueError(f"an 8-bit KV arena has pages of 16 tokens, got block_size={ec.block_size}")
+        if kv8 and ec.model_impl == "library":
+            raise ValueError("the library model reads a bf16 KV arena")
+        if kv8 and (cfg.head_dim % 16 or (self.device.type == "cuda" and cfg.head_dim != 128)):
+            raise ValueError(f"8-bit KV: head_dim 128 on the GPU, a multiple of 16 on the CPU, got {cfg.head_dim}")
         self.tp_world = 1
         weights = ec.weights
         if weights is None and isinstance(model, str) and not isinstance(model, ModelConfig):
@@ -171,11 +191,13 @@ class LLMEngine:
                 if ec.model_impl == "library":  # unfused intermediates + the decode batch's gathered K/V
                     act += max_tokens * cfg.intermediate * 8 + 2 * page_bytes(cfg, ec.block_size) // cfg.n_layers \
                         * ec.max_running * maxb
-                num_blocks = int((free - act) * ec.kv_mem_fraction) // page_bytes(cfg, ec.block_size)
+                num_blocks = int((free - act) * ec.kv_mem_fraction) // page_bytes(cfg, ec.block_size, kv8=kv8)
             else:
                 num_blocks = 256
         self.arena_path = None
         shape = (num_blocks, cfg.n_layers, 2, cfg.n_kv_heads, ec.block_size, cfg.head_dim)
+        if kv8:
+            shape, dtype = kv8_arena_shape(cfg, num_blocks, ec.block_size), torch.uint8
         cfg = self.cfg
         if ec.shared_arena and self.device.type == "cpu":
             from ..parallel.peer import alloc_shared_cpu_arena
@@ -328,8 +350,7 @@ class LLMEngine:
 
         dev = self.arena.device
         ops.page_copy(self.arena, self.runner.peer_arena, torch.tensor(src, device=dev),
-                      torch.tensor(dst, device=dev), page_bytes(self._arena_cfg, self.ec.block_size,
-                                                                self.arena.element_size()))
+                      torch.tensor(dst, device=dev), self.arena[0].numel() * self.arena.element_size())
 
     def has_unfinished(self) -> bool:
         return self.scheduler.has_work() or self.inflight is not None

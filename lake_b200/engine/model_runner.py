@@ -47,7 +47,7 @@ class ModelRunner:
         self.vocab_words = (model.cfg.vocab + 31) // 32
         cfg = model.cfg
         self.max_splits = 1
-        if self.cuda:
+        if self.cuda and not ops.is_kv8(arena):  # (8-bit decode attention brings its own workspace)
             self.max_splits = max(ops.decode_splits(n, cfg.n_kv_heads // row_multiple, max_blocks_per_seq)
                                   for n in range(1, max_seqs + 1))
         self.ws = model.new_workspace(max_tokens, max_samples, max_seqs, self.max_splits)

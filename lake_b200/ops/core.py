@@ -113,7 +113,8 @@ def linear_qkv(a: torch.Tensor, w_qkv: torch.Tensor, q_out: torch.Tensor, rope_c
                peer_slots: torch.Tensor | None = None, q_norm: torch.Tensor | None = None,
                k_norm: torch.Tensor | None = None, qk_eps: float = 1e-6) -> torch.Tensor:
     """QKV projection with RoPE (and, with q_norm/k_norm, per-head RMSNorm before RoPE as in
-    Qwen3). q -> q_out; K, V -> arena at `slots` (and peer_arena at peer_slots)."""
+    Qwen3). q -> q_out; K, V -> arena at `slots` (and peer_arena at peer_slots); an 8-bit arena
+    (ops.kv8_arena) takes them quantised from the fp32 sums."""
     if a.is_cuda:
         wq, ws = unpack(w_qkv)
         native().linear_qkv(a, wq, q_out, rope_cs, positions, slots, arena, layer, n_q_heads, n_kv_heads,

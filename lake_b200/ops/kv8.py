@@ -12,9 +12,11 @@ The scale belongs to the token, not to the page, so that a row's bytes depend on
 alone: pages are shared by the hash of their tokens, and a page must not differ by how its
 prompt was chunked or by a draft that was rejected.
 
-The bf16 arena's entry points take this arena too, told apart by its dtype:
-``paged_decode_attention``, ``paged_prefill_attention`` and, on the CPU, ``linear_qkv``.
-``kv8_write`` and ``kv8_read`` move dense rows in and out.
+The bf16 arena's entry points take this arena too, told apart by its dtype: ``linear_qkv``
+(its epilogue quantises K and V from the fp32 accumulators), ``paged_decode_attention`` and
+``paged_prefill_attention``; so do ``page_copy`` and the pool agents, which move whole pages.
+``kv8_write`` and ``kv8_read`` move dense rows in and out. An engine takes it with
+``LLMEngine(..., kv_dtype="fp8")``.
 """
 from __future__ import annotations
 

@@ -82,6 +82,7 @@ class RoleConfig:
     warmup_tokens_per_req: int = 1
     device: str = "cuda"
     num_blocks: int = 0
+    kv_dtype: str = "bf16"  # "fp8": 8-bit KV arena (engine.llm_engine.EngineConfig.kv_dtype)
 
     def __post_init__(self):
         if self.max_num_scheduled_tokens <= 0:
@@ -117,6 +118,7 @@ class RoleConfig:
             warmup_tokens_per_req=_env_int("LAKE_WARMUP_TOKENS_PER_REQ", 1),
             device=os.environ.get("LAKE_DEVICE", "cuda").strip() or "cuda",
             num_blocks=_env_int("LAKE_NUM_BLOCKS", 0),
+            kv_dtype=os.environ.get("LAKE_KV_DTYPE", "bf16").strip().lower() or "bf16",
         )
 
 

@@ -109,14 +109,15 @@ def main() -> None:
         serve_metrics(eng.metrics, metrics_addr)
     if cp_addr and factory is None:  # publish resident prefix blocks to the control plane's view
         from ..engine.llm_engine import page_bytes
+        from ..ops import is_kv8
         from .cp_reporter import ControlPlaneReporter
 
         e = eng.engine
         ch = grpc.insecure_channel(cp_addr)
         eng.on_finished = ControlPlaneReporter(
             proto.Stub(ch, "ControlPlaneService"), node_id,
-            cfg.served_model_name, page_bytes(e.cfg, e.ec.block_size, e.arena.element_size()), e.ec.block_size,
-            e.cfg.n_layers)
+            cfg.served_model_name, page_bytes(e.cfg, e.ec.block_size, e.arena.element_size(), kv8=is_kv8(e.arena)),
+            e.ec.block_size, e.cfg.n_layers)
     try:
         server.wait_for_termination()
     finally:

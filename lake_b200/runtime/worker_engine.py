@@ -75,7 +75,7 @@ def build_engine(cfg: RoleConfig, **kw):
                      long_prefill_threshold=cfg.long_prefill_token_threshold,
                      max_model_len=cfg.max_model_length or 8192, num_blocks=cfg.num_blocks,
                      use_cuda_graphs=device != "cpu",
-                     **{"overlap": cfg.enable_overlap,
+                     **{"overlap": cfg.enable_overlap, "kv_dtype": cfg.kv_dtype,
                         "spec_tokens": cfg.num_draft_tokens if cfg.enable_drafter else 0, **kw})
 
 

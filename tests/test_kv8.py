@@ -592,3 +592,184 @@ def test_offsets_past_32_bits(cuda_dev):
     b = ops.paged_prefill_attention(q, small, 0, near, sl, tiles, None, None, hq, 2, 0.1)
     assert torch.equal(a, b)
     ops.core.check_status(cuda_dev)
+
+
+# ------------------------------------------------------------------ QKV projection and engine
+@pytest.mark.gpu
+@pytest.mark.parametrize("t,norm", [(1, False), (70, False), (70, True), (600, False)])  # 600: two-SM kernel
+def test_linear_qkv_writes_the_8bit_arena(cuda_dev, t, norm):
+    """Cached rows are within a quantisation step of the fp32 rows, q is what the bf16 arena's call gives."""
+    g = torch.Generator(device=cuda_dev).manual_seed(21)
+    hid, hq, hkv = 512, 4, 2
+    a = torch.randn(t, hid, device=cuda_dev, generator=g).to(BF)
+    w = (torch.randn((hq + 2 * hkv) * 128, hid, device=cuda_dev, generator=g) / 20).to(BF)
+    cs = ref.rope_cache(4096, 500000.0, device=cuda_dev)
+    pos = torch.randint(0, 4000, (t,), device=cuda_dev, dtype=torch.int32, generator=g)
+    slots = torch.randperm(64 * 16, device=cuda_dev, generator=g)[:t]
+    if t > 5:
+        slots[5] = -1
+    nw = [(1 + 0.1 * torch.randn(128, device=cuda_dev, generator=g)).to(BF) for _ in range(2)] if norm else [None] * 2
+    arena = ops.kv8_arena(64, 3, hkv, device=cuda_dev)
+    peer = ops.kv8_arena(64, 3, hkv, device=cuda_dev)
+    dense = torch.zeros(64, 3, 2, hkv, 16, 128, dtype=BF, device=cuda_dev)
+    qa, qb = torch.empty(t, hq * 128, dtype=BF, device=cuda_dev), torch.empty(t, hq * 128, dtype=BF, device=cuda_dev)
+    peer_slots = torch.where(slots >= 0, (slots + 16) % 1024, slots)
+    ops.linear_qkv(a, w, qa, cs, pos, slots, arena, 1, hq, hkv, peer, peer_slots, *nw)
+    ops.linear_qkv(a, w, qb, cs, pos, slots, dense, 1, hq, hkv, None, None, *nw)
+    ops.core.check_status(cuda_dev)
+    assert torch.equal(qa, qb)
+    assert not arena[:, 0].any() and not arena[:, 2].any()
+    acc = a.double() @ w.double().t()
+    k, v = acc[:, hq * 128:(hq + hkv) * 128].view(t, hkv, 128), acc[:, (hq + hkv) * 128:].view(t, hkv, 128)
+    if norm:
+        k = k * torch.rsqrt(k.pow(2).mean(-1, keepdim=True) + 1e-6) * nw[1].double()
+    k = ref.apply_rope(k, pos, cs.double())
+    keep = slots >= 0
+    for side, got in zip((k, v), ops.kv8_read(arena, 1, slots)):
+        got, want = got.view(t, hkv, 128).double()[keep], side[keep]
+        top = want.abs().amax(-1, keepdim=True)
+        # half a step of e4m3: 2^-4 of the value, at least half its smallest, 2^-10 2^e with 2^e <= top / 224; the
+        # fp32 sums of 512 products move the value by less than 2^-12 of the row's largest and may move it over a step
+        assert bool(((got - want).abs() <= 2.0 ** -4 * want.abs() + 2.0 ** -10 * top / 224 + 2.0 ** -12 * top).all())
+    assert not ops.kv8_read(arena, 1, slots)[0][~keep].any()
+    for x, y in zip(ops.kv8_read(arena, 1, slots), ops.kv8_read(peer, 1, peer_slots)):
+        assert torch.equal(x, y)
+    with pytest.raises(RuntimeError, match="another type"):
+        ops.linear_qkv(a, w, qa, cs, pos, slots, arena, 1, hq, hkv, dense, slots)
+    with pytest.raises(RuntimeError, match="layer"):
+        ops.linear_qkv(a, w, qa, cs, pos, slots, arena, 3, hq, hkv)
+    far = slots.clone()
+    far[0] = 64 * 16
+    ops.linear_qkv(a, w, qa, cs, pos, far, arena, 1, hq, hkv)
+    with pytest.raises(ops.core.KernelError, match="out of bounds"):
+        ops.core.check_status(cuda_dev)
+
+
+def _engine(device, model, **kw):
+    from lake_b200.engine.llm_engine import LLMEngine
+
+    return LLMEngine(model, device=device, max_running=8, max_batched_tokens=256, max_model_len=512, num_blocks=128, **kw)
+
+
+def _prompts(n, vocab, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randint(0, vocab, (x,), generator=g).tolist() for x in n]
+
+
+def test_engine_8bit_kv_cpu():
+    """The CPU engine with an 8-bit cache: chunked prefill, decode and a reused prefix give what one
+    prefill of the same tokens gives, since a row's bytes do not depend on how its page was filled."""
+    prompts = _prompts([5, 40, 33, 100], 1024)
+    eng = _engine("cpu", "tiny", kv_dtype="fp8")
+    assert eng.arena.dtype == torch.uint8 and eng.arena.shape == (128, 2, 2, 2, 16 * 64 + 16)
+    out = eng.generate(prompts, max_new_tokens=6)
+    chunked = _engine("cpu", "tiny", kv_dtype="fp8", long_prefill_threshold=16)
+    assert chunked.generate(prompts, max_new_tokens=6) == out
+    assert eng.generate([prompts[3]], max_new_tokens=6) == [out[3]] and eng.pool.stats["hits"] > 0
+    from lake_b200.engine.llm_engine import page_bytes
+
+    assert page_bytes(eng.cfg, 16, kv8=True) == eng.arena[0].numel()
+
+
+def test_engine_8bit_kv_refusals():
+    for bad in (dict(kv_dtype="int4"), dict(kv_dtype="fp8", block_size=32), dict(kv_dtype="fp8", model_impl="library")):
+        with pytest.raises(ValueError):
+            _engine("cpu", "tiny", **bad)
+
+
+def test_worker_config_takes_kv_dtype(monkeypatch):
+    from lake_b200.runtime.config import RoleConfig
+    from lake_b200.runtime.worker_engine import build_engine
+
+    monkeypatch.setenv("LAKE_KV_DTYPE", "FP8")
+    cfg = RoleConfig.from_env()
+    cfg.model_backend, cfg.num_blocks, cfg.max_running_reqs, cfg.max_model_length = "mock", 64, 4, 256
+    assert cfg.kv_dtype == "fp8" and build_engine(cfg).arena.dtype == torch.uint8
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("model", ["tiny-gpu", "qwen"])
+def test_engine_8bit_kv_gpu(cuda_dev, model):
+    """The engine's steps over the 8-bit cache (mixed steps, graph decode, prefix reuse, drafts) against the
+    model run by the CPU oracle's ops on the same weights and the same cached values: logits of every
+    position agree within bf16 activations' rounding, and tokens where the oracle's are clear."""
+    over = {} if model == "tiny-gpu" else dict(qk_norm=True, n_q_heads=8, n_kv_heads=1)
+    prompts = _prompts([7, 130, 64, 200], 2048, 3)
+    eng = _engine(cuda_dev, "tiny-gpu", kv_dtype="fp8", model_overrides=over)
+    out = eng.generate(prompts, max_new_tokens=12)
+    eager = _engine(cuda_dev, "tiny-gpu", kv_dtype="fp8", model_overrides=over, use_cuda_graphs=False,
+                    long_prefill_threshold=32)
+    out2 = eager.generate(prompts, max_new_tokens=12)
+    ops.core.check_status(cuda_dev)
+    cpu = _engine("cpu", "tiny-gpu", kv_dtype="fp8", model_overrides=over)
+    for k, w in eng.model.w.items():
+        cpu.model.w[k].copy_(w.float().cpu())
+    # teacher-forced logits of the oracle for prompt + output: the engine's token is within the rounding of the
+    # largest logit (bf16 activations over two layers: 2^-8 a rounding, under 32 of them, of logits ~ |h| |w|)
+    for p, o in zip(prompts, out):
+        lg = _logits(cpu, p + o[:-1])[len(p) - 1:]
+        top = lg.amax(-1)
+        got = lg[torch.arange(len(o)), torch.tensor(o)]
+        assert bool((top - got <= 32 * 2.0 ** -8 * lg.std(-1)).all())
+    same_first = sum(a[0] == b[0] for a, b in zip(out, out2))
+    assert same_first >= 3 and all(len(o) == 12 for o in out2)
+    assert eng.generate([prompts[3]], max_new_tokens=3)[0][0] == out[3][0] and eng.pool.stats["hits"] > 0
+
+
+def _logits(eng, tokens):
+    from lake_b200.models.llama import ForwardBatch
+
+    t = len(tokens)
+    blocks = eng.reserve_blocks(t)
+    pos = torch.arange(t, dtype=torch.int32)
+    bt = torch.tensor([blocks], dtype=torch.int32)
+    b = ForwardBatch(input_ids=torch.tensor(tokens, dtype=torch.int32), positions=pos,
+                     slots=bt[0].long()[pos.long() // 16] * 16 + pos.long() % 16, block_tables=bt,
+                     seq_lens=torch.tensor([t], dtype=torch.int32), n_decode=0,
+                     prefill_tiles=ops.build_prefill_tiles([0, t], [0]),
+                     query_start=torch.tensor([0, t], dtype=torch.int32), sample_rows=pos.long(), want_logits=True)
+    ws = eng.model.new_workspace(t, t, 1)
+    lg = eng.model.forward(b, eng.arena, ws)
+    eng.release_blocks(blocks)
+    return lg
+
+
+@pytest.mark.gpu
+def test_one_step_from_the_tables_on(cuda_dev):
+    """A mixed step as they are used together: tables from lengths, rows written, decode rows and prompt
+    chunks attended, against 64-bit attention over what the cache holds."""
+    g = torch.Generator().manual_seed(31)
+    hq, hkv, nd = 8, 2, 3
+    ctx = [40, 0, 333, 100, 0, 7]
+    new = [1, 1, 1, 70, 140, 2]
+    lens = [a + b for a, b in zip(ctx, new)]
+    pages = torch.randperm(128, generator=g)[:8 * 16].view(8, 16).to(torch.int32)
+    pages = torch.cat([pages, torch.full((8, 9), -1, dtype=torch.int32)], 1)
+    pages[2, 16:22] = torch.arange(128, 134)
+    rows_of = torch.tensor([4, 0, 2, 5, 1, 7], dtype=torch.int32)
+    dev = [x.to(cuda_dev) for x in (pages, rows_of, torch.tensor(ctx, dtype=torch.int32), torch.tensor(new, dtype=torch.int32))]
+    arena = torch.randint(0, 256, (134, 2, hkv, 2, 2064), generator=g, dtype=torch.uint8).to(cuda_dev)
+    # what was cached before the step
+    old = ops.build_step_tables(dev[0], dev[1], torch.zeros_like(dev[2]), dev[2], sum(ctx), 8)
+    k, v = (torch.randn(sum(ctx), hkv * 128, generator=g).to(BF).to(cuda_dev) for _ in range(2))
+    ops.kv8_write(k, v, old.slots, arena, 1)
+    t = ops.build_step_tables(*dev, sum(new) + 5, 8, n_decode=nd)
+    qkv = torch.randn(sum(new) + 5, (hq + 2 * hkv) * 128, generator=g).to(BF).to(cuda_dev)
+    q, kn, vn = qkv[:, :hq * 128], qkv[:, hq * 128:(hq + hkv) * 128], qkv[:, (hq + hkv) * 128:]
+    ops.kv8_write(kn, vn, t.slots, arena, 1)
+    out = torch.full((sum(new) + 5, hq * 128), 9.0, dtype=BF, device=cuda_dev)
+    ops.paged_decode_attention(q[:nd], arena, 1, t.block_tables[:nd], t.seq_lens[:nd], hq, hkv, 0.09, out=out[:nd])
+    ops.paged_prefill_attention(q, arena, 1, t.block_tables, t.seq_lens, t.tiles, t.query_start, t.positions, hq, hkv,
+                                0.09, out=out)
+    ops.core.check_status(cuda_dev)
+    assert bool((out[sum(new):] == 9.0).all())
+    starts, o0 = t.query_start.tolist(), 0
+    for s, n in enumerate(lens):
+        j = torch.arange(n)
+        slots = pages[rows_of[s]].long()[j // PAGE] * PAGE + j % PAGE
+        kk, vv = (x.view(n, hkv, 128).double() for x in ops.kv8_read(arena, 1, slots.to(cuda_dev)))
+        a, b = starts[s], starts[s + 1]
+        lim = torch.arange(ctx[s], n, device=cuda_dev) + 1
+        o, w, size = attend64(q[a:b].double().view(b - a, hq, 128), kk, vv, lim, 0.09)
+        err = (out[a:b].double().view(b - a, hq, 128) - o).abs()
+        assert bool((err <= attention_tolerance(o, w, size, vv.abs().amax())).all()), s
