@@ -11,18 +11,23 @@
 // two O) softmax and products of a head take turns, and 128 keys of two heads took 5.1k cycles; so
 // they take 4.4k, of which the products run 2.6k and the exponentials 2.0k. What binds is shared
 // memory (products' operands, conversion and copies move ~390 KB per tile, 3.0k cycles) and the
-// hand-offs that wait behind it. Measured: one 8192-token prompt of 32 query and 8 KV heads 0.64 ms,
-// 860 TFLOP/s; four of 2048 tokens 0.23 ms.
+// hand-offs that wait behind it. Measured: one 8192-token prompt of 32 query and 8 KV heads 0.56 ms,
+// 980 TFLOP/s; four of 2048 tokens 0.21 ms. A CTA spends ~8 us around its main loop (queries 1.9 us
+// to arrive and 1.6 us to convert, output 2.3 us, start and end 2.5 us), so eight prompts of 500
+// tokens, seven steps a CTA on average, run at 255 TFLOP/s. CTAs that stay and take tile after tile
+// overlapped none of that and issued products more slowly (1152 rows behind 7040
+// tokens: 181 us against 163), so a tile is a CTA. The grid goes tile by tile, heaviest first,
+// all heads of a tile side by side: head by head, the last heads' heavy tiles started late (0.63 ms).
 //
 // 8-bit operands become fp16 ones in shared memory: bulk copies bring the K and the V sides of the
 // tile's eight pages (2064 bytes each, scales included) into a staging buffer each, a warpgroup for
 // each side turns codes into fp16 rows of the 128-byte swizzle (thread = key; e4m3 -> fp16 is
 // exact). The tensor cores' own fp8 products would need Q and P in 8 bits as well, or twice the
-// products. A tile is scaled against its own largest K scale and V scale: a row keeps code * 2^(e_row - e_tile), exact while
-// e_tile - e_row <= 15 (a code's last bit is 2^-9, fp16's 2^-24), and e_tile itself is one
-// multiplier of the tile's scores, or one addend of its exponents, not work per element. Where
-// rows of one tile differ by more than 2^15, the small rows' last bits are lost: an error of
-// 2^-24 of the largest element of the tile.
+// products. A tile is scaled against its own largest K scale and V scale: a row keeps
+// code * 2^(e_row - e_tile), exact while e_tile - e_row <= 15 (a code's last bit is 2^-9, fp16's
+// 2^-24), and e_tile itself is one multiplier of the tile's scores, or one addend of its exponents,
+// not work per element. Where rows of one tile differ by more than 2^15, the small rows' last bits
+// are lost: an error of 2^-24 of the largest element of the tile.
 //
 // Softmax statistics: w = score in log2 units + e_j, b = a base that follows the largest w of the
 // row lazily (it moves when w grows by more than 2^8), P = 2^(w - b + 7) <= 2^15. The row sum is
@@ -30,8 +35,8 @@
 //
 // Warps: 0 = loads, 1 = tensor memory and MMA issue, 2-3 idle, 4-7 = converters of K, 8-11 = of V,
 // 12-15 and 16-19 = softmax of head A and B. Registers move from the first three warpgroups to the
-// softmax ones. Every wait is bounded; a role whose wait ran out goes on through its loop without work, so that
-// the converters' named barriers are always reached by all of their warps.
+// softmax ones. Every wait is bounded; a role whose wait ran out goes on through its loop without
+// work, so that the converters' named barriers are always reached by all of their warps.
 #include <math_constants.h>
 
 #include "common.cuh"
@@ -89,6 +94,12 @@ __device__ __forceinline__ uint32_t f16x2_exp2(int d) {
   const __half h = __float2half_rn(d < -40 ? 0.f : __uint_as_float(static_cast<uint32_t>(127 + d) << 23));
   const __half2 r = __halves2half2(h, h);
   return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// A value that every lane holds, as the result of a vote: the compiler then knows it to be the same
+// in the whole warp (uniform registers and branches; the 8192-token prompt 640 -> 626 us).
+__device__ __forceinline__ int uniform(int v) {
+  return static_cast<int>(__ballot_sync(0xffffffffu, (v >> (threadIdx.x & 31)) & 1));
 }
 
 // One lane of the warp, the same each time. The MMA warp runs its loop as a whole and this lane's
@@ -166,7 +177,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("griddepcontrol.wait;" ::: "memory");
     return;
   }
-  int rank = a.num_tiles - 1 - static_cast<int>(blockIdx.x);
+  const int G = a.n_q_heads / a.n_kv_heads, pairs = (G + 1) / 2;
+  const int place = static_cast<int>(blockIdx.x) / (a.n_kv_heads * pairs);  // all heads of a tile side by side
+  const int head = static_cast<int>(blockIdx.x) % (a.n_kv_heads * pairs);
+  int rank = a.num_tiles - 1 - place;
   if (a.num_seqs > 1 && a.num_tiles <= kRanked) {
     int* keys = reinterpret_cast<int*>(smem + kK);
     const int t = threadIdx.x;
@@ -187,7 +201,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         before += (k.x > mine || (k.x == mine && u < t)) + (k.y > mine || (k.y == mine && u + 1 < t)) +
                   (k.z > mine || (k.z == mine && u + 2 < t)) + (k.w > mine || (k.w == mine && u + 3 < t));
       }
-      if (before == static_cast<int>(blockIdx.x)) keys[kRanked] = t;
+      if (before == place) keys[kRanked] = t;
     }
     __syncthreads();
     rank = keys[kRanked];
@@ -198,14 +212,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("griddepcontrol.wait;" ::: "memory");
     return;
   }
-  const int G = a.n_q_heads / a.n_kv_heads, pairs = (G + 1) / 2;
-  const int kvh = static_cast<int>(blockIdx.y) / pairs, pair = static_cast<int>(blockIdx.y) % pairs;
+  const int kvh = head / pairs, pair = head % pairs;
   const int qh0 = kvh * G + 2 * pair;
-  const int heads = min(2, G - 2 * pair);
+  const int heads = uniform(min(2, G - 2 * pair));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int len = min(a.seq_lens[seq], a.max_blocks * kKv8Page);
   const int max_pos = min(pos0 + nq - 1, len - 1);
-  const int n_steps = max_pos < 0 ? 0 : max_pos / kStep + 1;
+  const int n_steps = uniform(max_pos < 0 ? 0 : max_pos / kStep + 1);
   const int n_tiles = (n_steps + 1) / 2;
 
   if (threadIdx.x == 0) {
@@ -232,7 +245,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = uniform(*tmem_slot);
   const uint32_t t_s[2] = {tmem, tmem + 128};        // S of head A, B: two buffers of 64 columns (P over the first 32)
   const uint32_t t_o[2] = {tmem + 256, tmem + 384};  // O of head A, B
 
@@ -414,9 +427,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           x[c] = *at(c);
           const uint32_t w[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
 #pragma unroll
-          for (int i = 0; i < 4; ++i) top = max(top, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
+          for (int i = 0; i < 4; ++i) top = __vmaxu2(top, w[i] & 0x7fff7fffu);
         }
-        const int E = static_cast<int>(top >> 7);
+        const int E = static_cast<int>(max(top >> 16, top & 0xffffu) >> 7);
         const int up = E == 255 ? 0 : min(141 - E, 126);
         const float f = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
         cr = a.scale * kLog2e * __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
@@ -560,8 +573,10 @@ int kv8_prefill_tc(const Kv8AttnArgs& a, cudaStream_t stream) {
   if (!encode_bf16_map(&qmap, a.q, a.num_rows, cols, a.num_rows > 1 ? a.q_stride : cols, 128, 64)) return -5;
   if (int e = ensure_smem_attr(reinterpret_cast<const void*>(kv8_prefill_kernel), kSmem)) return e;
   const int G = a.n_q_heads / a.n_kv_heads;
+  const int64_t items = static_cast<int64_t>(a.num_tiles) * a.n_kv_heads * ((G + 1) / 2);
+  if (items > INT32_MAX) return -1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(a.num_tiles, a.n_kv_heads * ((G + 1) / 2));
+  cfg.gridDim = dim3(static_cast<unsigned>(items));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = kSmem;
   cfg.stream = stream;
