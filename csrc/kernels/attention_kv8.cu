@@ -46,6 +46,11 @@ constexpr float kPBias = 7.f;  // P = 2^(w - bo + 7): fp16 subnormals begin at 2
 
 constexpr int kSegCost = 6;    // pages that the start and the join of a segment cost as much as
 
+// Bytes of a column of Q and floats of a column of a warp's sums in shared memory: a quarter-warp's
+// accesses to several columns fall on different banks (16 sequences of 5 rows: 31.5 -> 28.7 us).
+constexpr int kQPitch = 256 + 32;
+constexpr int kOPitch = kKv8Dim + 4;
+
 // Shared memory of a CTA with NT groups of 8 columns: ring of pages, two query buffers, the
 // consumers' sums for the join at a segment's end. One group: two CTAs per SM. More groups need more
 // registers: one CTA per SM (with two of 16 columns the sums spill at 168 registers).
@@ -58,8 +63,8 @@ struct Smem {
   static constexpr int kPages = NT == 1 ? 2 : 1;  // of a step
   static constexpr int kSlots = NT == 1 ? 10 : 28;
   static constexpr int kQ = kSlots * kPages * kKv8Head;
-  static constexpr int kO = kQ + 2 * kCols * 256;
-  static constexpr int kStat = kO + kWarps * kCols * kKv8Dim * 4;  // [warp][col][m, bo, l]
+  static constexpr int kO = kQ + 2 * kCols * kQPitch;
+  static constexpr int kStat = kO + kWarps * kCols * kOPitch * 4;  // [warp][col][m, bo, l]
   static constexpr int kBar = kStat + kWarps * kCols * 3 * 4;
   static constexpr int kBytes = kBar + (2 * kSlots + 4) * 8;
   // A slot belongs to one warp: pages land out of order, and a warp that had not itself waited for
@@ -244,7 +249,7 @@ __device__ __forceinline__ void load_columns(const uint8_t* q, int real, float s
   float top = 0.f;
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
-    const uint2 u = g < real ? *reinterpret_cast<const uint2*>(q + g * 256 + k * 32 + t * 8) : make_uint2(0, 0);
+    const uint2 u = g < real ? *reinterpret_cast<const uint2*>(q + g * kQPitch + k * 32 + t * 8) : make_uint2(0, 0);
     x[4 * k] = __uint_as_float(u.x << 16);
     x[4 * k + 1] = __uint_as_float(u.x & 0xffff0000u);
     x[4 * k + 2] = __uint_as_float(u.y << 16);
@@ -310,8 +315,11 @@ __device__ __forceinline__ int64_t total_cost(const Kv8AttnArgs& a, int items, i
   int64_t sum = 0;
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
-    keep[k] = 32 * k + lane < items ? item_cost<NT>(a, 32 * k + lane) : 0;
-    sum += keep[k];
+    keep[k] = 0;
+    if (32 * k < items) {  // (a branch for the whole warp: code that is not run is not fetched either)
+      if (32 * k + lane < items) keep[k] = item_cost<NT>(a, 32 * k + lane);
+      sum += keep[k];
+    }
   }
   for (int s = 256 + lane; s < items; s += 32) sum += item_cost<NT>(a, s);
 #pragma unroll
@@ -442,7 +450,7 @@ __global__ void __launch_bounds__(Smem<NT>::kThreads, Smem<NT>::kPerSm) kv8_attn
       if (lane == 0) mbar_expect_tx(&q_full[qb], (c1 - c0) * 256);
       __syncwarp();
       if (c0 + lane < c1)
-        bulk_load(smem + S::kQ + (qb * S::kCols + lane) * 256,
+        bulk_load(smem + S::kQ + (qb * S::kCols + lane) * kQPitch,
                   a.q + static_cast<int64_t>(w.it.row0 + (c0 + lane) / G) * a.q_stride +
                       (static_cast<int64_t>(kvh) * G + (c0 + lane) % G) * kKv8Dim,
                   256, &q_full[qb]);
@@ -498,7 +506,7 @@ __global__ void __launch_bounds__(Smem<NT>::kThreads, Smem<NT>::kPerSm) kv8_attn
     ok = __all_sync(0xffffffffu, ok && mbar_wait(&q_full[qb], (piece >> 1) & 1, nullptr, a.status));
 #pragma unroll
     for (int k = 0; k < NT; ++k) {
-      load_columns(smem + S::kQ + (qb * S::kCols + 8 * k) * 256, ncols - 8 * k, a.scale, lane, qf[k], cq[k]);
+      load_columns(smem + S::kQ + (qb * S::kCols + 8 * k) * kQPitch, ncols - 8 * k, a.scale, lane, qf[k], cq[k]);
 #pragma unroll
       for (int c = 0; c < 8; ++c)
 #pragma unroll
@@ -536,11 +544,11 @@ __global__ void __launch_bounds__(Smem<NT>::kThreads, Smem<NT>::kPerSm) kv8_attn
       for (int e = 0; e < 2; ++e)
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) st[k].l[e] += __shfl_xor_sync(0xffffffffu, st[k].l[e], o);
-      float* d = mo + (warp * S::kCols + 8 * k + t2) * kKv8Dim + 2 * g;
+      float* d = mo + (warp * S::kCols + 8 * k + t2) * kOPitch + 2 * g;
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
         *reinterpret_cast<float2*>(d + 16 * c) = make_float2(st[k].o[c][0], st[k].o[c][2]);
-        *reinterpret_cast<float2*>(d + kKv8Dim + 16 * c) = make_float2(st[k].o[c][1], st[k].o[c][3]);
+        *reinterpret_cast<float2*>(d + kOPitch + 16 * c) = make_float2(st[k].o[c][1], st[k].o[c][3]);
       }
       if (g == 0)
 #pragma unroll
@@ -566,7 +574,7 @@ __global__ void __launch_bounds__(Smem<NT>::kThreads, Smem<NT>::kPerSm) kv8_attn
         const float* x = ms + (k * S::kCols + col) * 3;
         L += x[2] * factor(x[0], M);
         const float f = factor(x[1], B);
-        const float4 v = *reinterpret_cast<const float4*>(mo + (k * S::kCols + col) * kKv8Dim + 4 * lane);
+        const float4 v = *reinterpret_cast<const float4*>(mo + (k * S::kCols + col) * kOPitch + 4 * lane);
         acc.x += v.x * f;
         acc.y += v.y * f;
         acc.z += v.z * f;
