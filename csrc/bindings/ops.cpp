@@ -547,7 +547,7 @@ void check_kv8_arena(const at::Tensor& arena, int64_t layer, int64_t n_kv_heads)
               "an 8-bit KV arena is a contiguous uint8 CUDA tensor [blocks, layers, kv_heads, 2, 2064]");
   TORCH_CHECK(arena.size(3) == 2 && arena.size(4) == 2064,
               "8-bit KV arena: head_dim must be 128 and pages 16 tokens (last sizes 2, 2064)");
-  TORCH_CHECK(arena.size(2) == n_kv_heads, "kv heads mismatch: ", n_kv_heads, " for an arena of ", arena.size(2));
+  TORCH_CHECK(arena.size(2) == n_kv_heads && n_kv_heads > 0, "kv heads mismatch: ", n_kv_heads, " for an arena of ", arena.size(2));
   TORCH_CHECK(layer >= 0 && layer < arena.size(1), "layer ", layer, " of an arena of ", arena.size(1));
   check_aligned(arena, "arena");
 }
@@ -631,6 +631,8 @@ lakeb::Kv8AttnArgs kv8_attn_args(const at::Tensor& q, const at::Tensor& out, con
   check_same_device(out, arena, "out");
   check_same_device(block_tables, arena, "block_tables");
   check_same_device(seq_lens, arena, "seq_lens");
+  TORCH_CHECK(block_tables.size(1) < (int64_t(1) << 26), "block tables of at most 2^26 pages, got ", block_tables.size(1));
+  TORCH_CHECK(q.numel() == 0 || out.data_ptr() != q.data_ptr(), "out must not be q");
   lakeb::Kv8AttnArgs p;
   p.q = bf(q);
   p.q_stride = q.stride(0);
@@ -738,6 +740,8 @@ std::vector<at::Tensor> step_tables(const at::Tensor& pages, const at::Tensor& r
   TORCH_CHECK(block_size > 0 && block_size < (1 << 30) && tile > 0 && tile < (1 << 30), "block_size and tile must be positive");
   TORCH_CHECK(max_tokens >= 0 && max_tiles >= 0 && max_tokens < (int64_t(1) << 30) && max_tiles < (int64_t(1) << 28),
               "max_tokens and max_tiles must not be negative (or past 2^30, 2^28)");
+  TORCH_CHECK((n + 1) * (max_tokens + 2) < (int64_t(1) << 31), "max_tokens times sequences must stay below 2^31, got ", max_tokens,
+              " and ", n);
   const c10::cuda::CUDAGuard guard(pages.device());
   const int64_t w = pages.size(1);
   const auto i32 = at::kInt;

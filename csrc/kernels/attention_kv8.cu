@@ -285,7 +285,7 @@ __device__ __forceinline__ Item get_item(const Kv8AttnArgs& a, int s) {
   if (a.tiles) {
     const int4 t = a.tiles[s];
     it.seq = t.x, it.row0 = t.y, it.nq = max(t.z, 0), it.pos0 = t.w;
-    if (it.nq > a.most_rows || !kv8_tile_ok(a, t)) it.seq = it.row0 = it.nq = 0;
+    if (!kv8_tile_ok(a, t) || it.nq > a.most_rows) it.seq = it.row0 = it.nq = 0;
   } else {
     it.seq = it.row0 = s, it.nq = 1, it.pos0 = 0;
   }
@@ -422,10 +422,11 @@ __global__ void __launch_bounds__(Smem<NT>::kThreads, Smem<NT>::kPerSm) kv8_attn
   __syncthreads();
 
   Walk<NT> w;
-  if (whole) {  // CTA = (KV head, item)
-    const Item it = get_item<NT>(a, blockIdx.y);
+  const int own = static_cast<int>(blockIdx.x) / a.n_kv_heads, own_head = static_cast<int>(blockIdx.x) % a.n_kv_heads;
+  if (whole) {  // CTA = (item, KV head)
+    const Item it = get_item<NT>(a, own);
     const int n = it.pages > 0 ? it.groups * (it.pages + kSegCost) : 0;
-    w.start(a, blockIdx.y, blockIdx.x * n, n);
+    w.start(a, own, own_head * n, n);
   } else {
     int keep[8];
     const int64_t total = total_cost<NT>(a, items, lane, keep);
@@ -483,10 +484,10 @@ __global__ void __launch_bounds__(Smem<NT>::kThreads, Smem<NT>::kPerSm) kv8_attn
   float* ms = reinterpret_cast<float*>(smem + S::kStat);
   const int g = lane >> 2, t2 = (lane & 3) * 2;
   // rows of sequences without keys
-  for (int s = whole ? blockIdx.y : blockIdx.x; s < items; s += whole ? items : gridDim.x) {
+  for (int s = whole ? own : blockIdx.x; s < items; s += whole ? items : gridDim.x) {
     const Item it = get_item<NT>(a, s);
     if (it.pages > 0) continue;
-    const int h0 = whole ? blockIdx.x * G : 0, nh = whole ? G : a.n_q_heads;
+    const int h0 = whole ? own_head * G : 0, nh = whole ? G : a.n_q_heads;
     for (int i = threadIdx.x; i < it.nq * nh * kKv8Dim; i += kWarps * 32)
       a.out[static_cast<int64_t>(it.row0 + i / (nh * kKv8Dim)) * a.out_stride + h0 * kKv8Dim + i % (nh * kKv8Dim)] =
           __float2bfloat16(0.f);
@@ -686,7 +687,9 @@ int launch(const Kv8AttnArgs& a, cudaStream_t stream) {
   const int items = a.tiles ? a.num_tiles : a.num_seqs;
   if (int e = ensure_smem_attr(reinterpret_cast<const void*>(kv8_attn_kernel<NT>), Smem<NT>::kBytes)) return e;
   if (a.max_blocks <= kWholePages) {
-    kv8_attn_kernel<NT><<<dim3(a.n_kv_heads, items), Smem<NT>::kThreads, Smem<NT>::kBytes, stream>>>(a, 1);
+    const int64_t ctas = static_cast<int64_t>(items) * a.n_kv_heads;
+    if (ctas > INT32_MAX) return -1;
+    kv8_attn_kernel<NT><<<static_cast<unsigned>(ctas), Smem<NT>::kThreads, Smem<NT>::kBytes, stream>>>(a, 1);
     return cudaGetLastError();
   }
   const int ctas = Smem<NT>::kPerSm * num_sms();
@@ -722,6 +725,10 @@ int kv8_attention_groups(const Kv8AttnArgs& a) {
 
 int kv8_attention(const Kv8AttnArgs& a, cudaStream_t stream) {
   if ((a.tiles ? a.num_tiles : a.num_seqs) <= 0) return 0;
+  const int64_t rows = !a.tiles ? 1 : a.most_rows < kKv8TileRows ? a.most_rows : kKv8TileRows;
+  const int64_t cols = 8 * kv8_attention_groups(a);
+  const int64_t units = a.n_kv_heads * ((rows * (a.n_q_heads / a.n_kv_heads) + cols - 1) / cols);
+  if (units > INT32_MAX / 32 || (int64_t(a.max_blocks) + kSegCost) * units > INT32_MAX / 32) return -1;
   switch (kv8_attention_groups(a)) {
     case 1: return launch<1>(a, stream);
     case 2: return launch<2>(a, stream);

@@ -43,9 +43,11 @@ __device__ __forceinline__ float kv8_scale(int b) {
   return __uint_as_float(b == 255 ? 0x7fffffffu : static_cast<uint32_t>(b) << 23);
 }
 
-// A query tile names a sequence and rows of the call (otherwise it is reported and skipped).
+// A query tile names a sequence and up to kKv8TileRows rows of the call (otherwise it is reported and
+// skipped).
 __device__ __forceinline__ bool kv8_tile_ok(const Kv8AttnArgs& a, const int4& t) {
-  const bool ok = t.z <= 0 || (t.x >= 0 && t.x < a.num_seqs && t.y >= 0 && t.y < a.num_rows && t.z <= a.num_rows - t.y && t.w >= 0);
+  const bool ok = t.z <= 0 || (t.x >= 0 && t.x < a.num_seqs && t.y >= 0 && t.y < a.num_rows && t.z <= kKv8TileRows &&
+                               t.z <= a.num_rows - t.y && t.w >= 0 && t.w < (1 << 30));
   if (!ok) record_error(a.status, kErrBounds);
   return ok;
 }

@@ -123,7 +123,8 @@ __global__ void __launch_bounds__(kTabThreads) step_tables_kernel(const StepTabl
   for (int s0 = 0; s0 < a.num_seqs; s0 += kTabThreads) {
     const int s = s0 + tid;
     const int raw = s < a.num_seqs ? a.new_lens[s] : 0;
-    const int n = max(raw, 0), t = s >= a.num_decode ? (n + a.tile - 1) / a.tile : 0;
+    // a length that no table has room for is reported with the totals: cut off here, sums stay in 32 bits
+    const int n = min(max(raw, 0), a.max_tokens + 1), t = s >= a.num_decode ? (n + a.tile - 1) / a.tile : 0;
     if (raw < 0 && lead) record_error(a.status, kErrBadArg);
     int cn = n, ct = t;
 #pragma unroll
@@ -167,16 +168,18 @@ __global__ void __launch_bounds__(kTabThreads) step_tables_kernel(const StepTabl
     record_error(a.status, kErrBounds);
     return -1;
   };
+  // (a context past 2^30 tokens is reported with its pages: cut off, so that lengths stay in 32 bits)
+  auto context = [&](int s) { return min(a.context_lens[s], 1 << 30); };
   for (int s = gid; s <= a.num_seqs; s += stride) {
     a.query_start[s] = start[s];
-    if (s < a.num_seqs) a.seq_lens[s] = a.context_lens[s] + (start[s + 1] - start[s]);
+    if (s < a.num_seqs) a.seq_lens[s] = context(s) + (start[s + 1] - start[s]);
   }
   for (int i = gid; i < a.max_tokens; i += stride) {
     int pos = 0;
     int64_t slot = -1;
     if (i < total) {
       const int s = find(start, i), r = row_of(s);
-      pos = a.context_lens[s] + i - start[s];
+      pos = context(s) + (i - start[s]);
       const int p = pos / a.block_size;
       if (r >= 0 && pos >= 0 && p < a.max_blocks) {
         const int page = a.pages[static_cast<int64_t>(r) * a.pages_stride + p];
@@ -191,15 +194,16 @@ __global__ void __launch_bounds__(kTabThreads) step_tables_kernel(const StepTabl
     int4 t = make_int4(0, 0, 0, 0);
     if (i < tiles) {
       const int s = find(first, i), at = (i - first[s]) * a.tile;
-      t = make_int4(s, start[s] + at, min(a.tile, start[s + 1] - start[s] - at), a.context_lens[s] + at);
+      t = make_int4(s, start[s] + at, min(a.tile, start[s + 1] - start[s] - at), context(s) + at);
     }
     a.tiles[i] = t;
   }
   // block tables: a CTA per sequence, entries past the sequence's pages 0
   for (int s = blockIdx.x; s < a.num_seqs; s += gridDim.x) {
-    const int len = a.context_lens[s] + (start[s + 1] - start[s]);
-    const int nb = min((len + a.block_size - 1) / a.block_size, a.max_blocks);
+    const int ctx = context(s), len = ctx + (start[s + 1] - start[s]);
+    const int need = len > 0 ? (len - 1) / a.block_size + 1 : 0, nb = min(need, a.max_blocks);
     const int r = row_of(s);
+    if (tid == 0 && (ctx < 0 || need > a.max_blocks)) record_error(a.status, kErrBounds);
     const int* src = a.pages + static_cast<int64_t>(max(r, 0)) * a.pages_stride;
     int* dst = a.block_tables + static_cast<int64_t>(s) * a.max_blocks;
     for (int p = tid; p < a.max_blocks; p += kTabThreads) {

@@ -240,7 +240,9 @@ struct Kv8AttnArgs {
   float* ws_ml = nullptr;
   int* status = nullptr;
 };
-// Few query rows per sequence (any number is right; large tiles belong to kv8_prefill_tc).
+constexpr int kKv8TileRows = 128;  // of a query tile at most
+// Few query rows per sequence (any number is right; large tiles belong to kv8_prefill_tc). -1 where
+// the pages of 32 items times their KV heads and column groups could pass 32 bits.
 int kv8_attention(const Kv8AttnArgs& a, cudaStream_t stream);
 int kv8_attention_groups(const Kv8AttnArgs& a);
 int64_t kv8_attention_ws_floats(const Kv8AttnArgs& a);

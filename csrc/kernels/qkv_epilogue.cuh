@@ -68,6 +68,7 @@ __device__ __noinline__ void qkv_head_kv8(uint32_t tbase, bool is_k, uint8_t* ro
                                           const float2* cs, const __nv_bfloat16* nw, float inv) {
   auto piece = [&](int half, float (&o1)[32], float (&o2)[32]) {  // elements 32 * half.., 64 + 32 * half..
     uint32_t r1[32], r2[32];
+    __syncwarp();  // the stores before are each lane's own
     tmem_ld32(tbase + half * 32, r1);
     tmem_ld32(tbase + 64 + half * 32, r2);
     tmem_ld_wait();

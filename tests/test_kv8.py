@@ -531,6 +531,85 @@ def test_prefill_refusals(cuda_dev):
     assert none.shape == (0, 1024)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [2, 200])  # both kernels
+def test_prefill_bad_tiles_are_reported_and_skipped(cuda_dev, rows):
+    g = torch.Generator().manual_seed(14)
+    arena, bt, _ = build([rows, 30], 8, 2, 1, 0, g, cuda_dev)
+    n = rows + 2
+    q = torch.randn(n, 1024, generator=g).to(BF).to(cuda_dev)
+    sl = torch.tensor([rows, 30], dtype=torch.int32, device=cuda_dev)
+    tiles = ops.build_prefill_tiles([0, rows, n], [0, 28], device=cuda_dev)
+    args = (bt, sl)
+    good = ops.paged_prefill_attention(q, arena, 0, *args, tiles, None, None, 8, 2, 0.1)
+    ops.core.check_status(cuda_dev)
+    for bad in ([2, 0, 1, 0], [-1, 0, 1, 0], [0, n, 1, 0], [0, -1, 1, 0], [0, n - 1, 2, 0], [0, 0, 129, 0],
+                [0, 0, 2 ** 31 - 1, 0], [0, 0, 1, -1], [0, 0, 1, 2 ** 31 - 1]):
+        t2 = torch.cat([tiles, torch.tensor([bad], dtype=torch.int32, device=cuda_dev)])
+        out = ops.paged_prefill_attention(q, arena, 0, *args, t2, None, None, 8, 2, 0.1)
+        with pytest.raises(ops.core.KernelError, match="out of bounds"):
+            ops.core.check_status(cuda_dev)
+        assert torch.equal(out, good), bad
+
+
+@pytest.mark.gpu
+def test_calls_that_are_refused_for_their_size_or_memory(cuda_dev):
+    arena = ops.kv8_arena(1, 1, 1, device=cuda_dev)
+    sl = torch.ones(1, dtype=torch.int32, device=cuda_dev)
+    q = torch.zeros(1, 1024, dtype=BF, device=cuda_dev)
+    tiles = torch.tensor([[0, 0, 1, 0]], dtype=torch.int32, device=cuda_dev)
+    wide = torch.zeros(1, 600_000, dtype=torch.int32, device=cuda_dev)  # 32 such tiles could pass 32 bits of pages
+    with pytest.raises(RuntimeError):
+        ops.paged_prefill_attention(q, arena, 0, wide, sl, tiles, None, None, 8, 1, 0.1)
+    ops.paged_prefill_attention(q, arena, 0, wide[:, :500_000], sl, tiles, None, None, 8, 1, 0.1)
+    ops.paged_decode_attention(q, arena, 0, wide, sl, 8, 1, 0.1)
+    for f in (lambda: ops.paged_prefill_attention(q, arena, 0, wide[:, :4], sl, tiles, None, None, 8, 1, 0.1, out=q),
+              lambda: ops.paged_decode_attention(q, arena, 0, wide[:, :4], sl, 8, 1, 0.1, out=q)):
+        with pytest.raises(RuntimeError, match="out must not be q"):
+            f()
+    ops.core.check_status(cuda_dev)
+    empty = ops.kv8_arena(2, 1, 0, device=cuda_dev)  # no heads
+    for n in (1, 3):
+        none, at = torch.zeros(n, 0, dtype=BF, device=cuda_dev), torch.arange(n, device=cuda_dev)
+        with pytest.raises(RuntimeError):
+            ops.kv8_write(none, none, at, empty, 0)
+        with pytest.raises(RuntimeError):
+            ops.kv8_read(empty, 0, at)
+
+
+@pytest.mark.gpu
+def test_decode_more_sequences_than_a_grid_axis(cuda_dev):
+    n = 70_000
+    g = torch.Generator().manual_seed(15)
+    arena, bt, _ = build([16], 4, 1, 1, 0, g, cuda_dev)
+    q = torch.randn(16, 512, generator=g).to(BF).to(cuda_dev)
+    lens = torch.arange(1, 17, dtype=torch.int32, device=cuda_dev)
+    few = ops.paged_decode_attention(q, arena, 0, bt.expand(16, -1), lens, 4, 1, 0.1)
+    pick = torch.randint(0, 16, (n,), generator=g).to(cuda_dev)
+    many = ops.paged_decode_attention(q[pick], arena, 0, bt.expand(n, -1), lens[pick], 4, 1, 0.1)
+    ops.core.check_status(cuda_dev)
+    assert torch.equal(many, few[pick])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,new,hq,hkv", [([256], [256], 2, 1), ([1500], [640], 8, 2), ([3000, 40], [640, 20], 8, 2),
+                                             ([700] * 6, [129] * 6, 10, 2), ([2500] * 3, [3, 9, 5], 8, 2)])
+def test_prefill_repeats_bit_for_bit(cuda_dev, lens, new, hq, hkv):
+    """Back to back, without a wait between the calls: a hand-off that is early by one phase shows here."""
+    g = torch.Generator().manual_seed(16)
+    arena, bt, _ = build(lens, hq, hkv, 1, 0, g, cuda_dev)
+    starts = [0]
+    for n in new:
+        starts.append(starts[-1] + n)
+    q = (torch.randn(starts[-1], hq * 128, generator=g) * 1.5).to(BF).to(cuda_dev)
+    sl = torch.tensor(lens, dtype=torch.int32, device=cuda_dev)
+    tiles = ops.build_prefill_tiles(starts, [n - m for n, m in zip(lens, new)], device=cuda_dev)
+    outs = [ops.paged_prefill_attention(q, arena, 0, bt, sl, tiles, None, None, hq, hkv, 0.09) for _ in range(16)]
+    ops.core.check_status(cuda_dev)
+    for o in outs[1:]:
+        assert torch.equal(o, outs[0])
+
+
 # ------------------------------------------------------------------ streams, graphs, sizes
 @pytest.mark.gpu
 def test_two_streams_and_a_replayed_graph(cuda_dev):

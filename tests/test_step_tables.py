@@ -97,6 +97,19 @@ def test_reports_gpu(cuda_dev):
             ops.core.check_status(cuda_dev)
         if "pages" in bad:  # the other sequences are as they should be
             assert torch.equal(got.slots[1:], ok.slots[1:])
+    # lengths that no row of pages holds, of sequences without new tokens as well
+    for c, n in ((-1, 0), (129, 0), (2 ** 31 - 1, 0), (2 ** 31 - 1, 1), (5, 2 ** 31 - 1), (2 ** 30, 2 ** 30)):
+        c2, n2 = ctx.clone(), new.clone()
+        c2[0], n2[0] = c, n
+        ops.build_step_tables(**(good | dict(context_lens=c2, new_lens=n2)))
+        with pytest.raises(ops.core.KernelError):
+            ops.core.check_status(cuda_dev)
+    many = torch.full((3,), 2 ** 31 - 1, dtype=torch.int32, device=cuda_dev)  # sums past 32 bits
+    ops.build_step_tables(**(good | dict(new_lens=many)))
+    with pytest.raises(ops.core.KernelError):
+        ops.core.check_status(cuda_dev)
+    with pytest.raises(RuntimeError):
+        ops.build_step_tables(**(good | dict(max_tokens=2 ** 29)))
     for bad in (dict(rows=rows.long()), dict(n_decode=4), dict(context_lens=ctx[:1]), dict(new_lens=new.cpu()),
                 dict(block_size=0), dict(pages=pages.long())):
         with pytest.raises(RuntimeError):
