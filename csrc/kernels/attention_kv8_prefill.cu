@@ -12,12 +12,13 @@
 // they take 4.4k, of which the products run 2.6k and the exponentials 2.0k. What binds is shared
 // memory (products' operands, conversion and copies move ~390 KB per tile, 3.0k cycles) and the
 // hand-offs that wait behind it. Measured: one 8192-token prompt of 32 query and 8 KV heads 0.56 ms,
-// 980 TFLOP/s; four of 2048 tokens 0.21 ms. A CTA spends ~8 us around its main loop (queries 1.9 us
-// to arrive and 1.6 us to convert, output 2.3 us, start and end 2.5 us), so eight prompts of 500
-// tokens, seven steps a CTA on average, run at 255 TFLOP/s. CTAs that stay and take tile after tile
-// overlapped none of that and issued products more slowly (1152 rows behind 7040
-// tokens: 181 us against 163), so a tile is a CTA. The grid goes tile by tile, heaviest first,
-// all heads of a tile side by side: head by head, the last heads' heavy tiles started late (0.63 ms).
+// 985 TFLOP/s; four of 2048 tokens 0.205 ms, 670 TFLOP/s. A CTA spends ~7 us around its main loop
+// (1.9 us until its queries arrive, 1.6 to convert them, about as long for the output, the rest start
+// and end), so eight prompts of 500 tokens, four tiles of keys a CTA at most, run at 275 TFLOP/s. CTAs
+// that stay and take tile after tile overlapped little of that and issued products more slowly (1152
+// rows behind 7040 tokens: 181 us against 161), so a tile is a CTA. The grid goes tile by tile,
+// heaviest first, all heads of a tile side by side: head by head, the last heads' heavy tiles started
+// late (0.63 ms).
 //
 // 8-bit operands become fp16 ones in shared memory: bulk copies bring the K and the V sides of the
 // tile's eight pages (2064 bytes each, scales included) into a staging buffer each, a warpgroup for
@@ -35,7 +36,7 @@
 //
 // Warps: 0 = loads, 1 = tensor memory and MMA issue, 2-3 idle, 4-7 = converters of K, 8-11 = of V,
 // 12-15 and 16-19 = softmax of head A and B. Registers move from the first three warpgroups to the
-// softmax ones. Every wait is bounded; a role whose wait ran out goes on through its loop without
+// softmax ones (80, 80, 80, 120 and 120 of 96 each: the split with the fewest spills). Every wait is bounded; a role whose wait ran out goes on through its loop without
 // work, so that the converters' named barriers are always reached by all of their warps.
 #include <math_constants.h>
 
@@ -250,7 +251,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t t_o[2] = {tmem + 256, tmem + 384};  // O of head A, B
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     if (warp == 0 && n_tiles > 0) {
       // ------------------------------------------------------------ loads
       if (lane == 0) {
@@ -352,7 +353,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else if (warp < 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     // ------------------------------- converters of K (kv = 0) and of V (kv = 1): thread = key of the tile
     const int kv = (warp - 4) >> 2, row = (threadIdx.x - 128) & 127, t = row & 15;
     const uint8_t* side = smem + kRaw + (kv * 8 + (row >> 4)) * kKv8Side;
@@ -407,7 +408,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 120;");
     // -------------------------------------------------------------- softmax + epilogue: thread = query row
     const int h = (warp - 12) >> 2;
     const int r = (warp & 3) * 32 + lane;  // query row in the tile = TMEM lane
@@ -531,20 +532,32 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (__all_sync(0xffffffffu, ok)) {
         tc_fence_after();
         const float inv = l == 0.f ? 0.f : exp2f(static_cast<float>(e0)) / l;
-        __nv_bfloat16* orow = a.out + static_cast<int64_t>(qrow0 + r) * a.out_stride + (qh0 + h) * 128;
-#pragma unroll
+        // Rows go through this head's Q, which no product reads any more, so that the warp stores whole
+        // rows two at a time (a row per lane, 16 bytes at a time: eight prompts of 500 tokens 62.5 us
+        // instead of 59). Chunk c of row r lies at chunk c ^ (r & 7): both ways are free of bank conflicts.
+        uint8_t* stage = smem + kQ + h * kOperand + (warp & 3) * 32 * 256;
+#pragma unroll 1
         for (int q = 0; q < 4; ++q) {
           uint32_t ov[32];
           tmem_ld32(t_o[h] + lane_off + q * 32, ov);
           tmem_ld_wait();
-          if (r < nq) {
-            uint4* dst = reinterpret_cast<uint4*>(orow + q * 32);
-            auto two = [&](int k) {
-              return pack_bf16x2(__uint_as_float(ov[k]) * inv, __uint_as_float(ov[k + 1]) * inv);
-            };
+          auto two = [&](int k) {
+            return pack_bf16x2(__uint_as_float(ov[k]) * inv, __uint_as_float(ov[k + 1]) * inv);
+          };
 #pragma unroll
-            for (int v = 0; v < 4; ++v) dst[v] = make_uint4(two(8 * v), two(8 * v + 2), two(8 * v + 4), two(8 * v + 6));
-          }
+          for (int v = 0; v < 4; ++v)
+            *reinterpret_cast<uint4*>(stage + lane * 256 + (((4 * q + v) ^ (lane & 7)) << 4)) =
+                make_uint4(two(8 * v), two(8 * v + 2), two(8 * v + 4), two(8 * v + 6));
+        }
+        __syncwarp();
+        const int l = lane & 15, row0 = (warp & 3) * 32;
+        __nv_bfloat16* o0 = a.out + static_cast<int64_t>(qrow0 + row0) * a.out_stride + (qh0 + h) * 128 + l * 8;
+#pragma unroll 2
+        for (int i = 0; i < 16; ++i) {
+          const int x = 2 * i + (lane >> 4);
+          if (row0 + x < nq)
+            *reinterpret_cast<uint4*>(o0 + x * a.out_stride) =
+                *reinterpret_cast<const uint4*>(stage + x * 256 + ((l ^ (x & 7)) << 4));
         }
       }
       tc_fence_before();

@@ -2,14 +2,15 @@
 library counterpart (cuBLAS via torch.matmul, SDPA), timed with CUDA events
 after warm-up, L2 flushed between iterations.
 
-    python -m lake_b200.bench.kernels [--only gemm,decode,prefill,norm,moe]
+    python -m lake_b200.bench.kernels [--only gemm,decode,prefill,kv8,norm,moe]
     python -m lake_b200.bench.kernels --profile CASE   # 3 launches of one kernel, for an ncu capture
 
 Profile cases (inputs larger than the 126 MB L2, a few GB on the device at most):
 tp2_rs / tp2_norm / tp2_swiglu_ag / tp4_* (the fused tensor-parallel kernels of one MLP hop at
 4096 tokens, driven from GPU 0), gemm_gate_up (M=4096 K=4096 N=28672), gemm_w8a8_gate_up (the same shape with block-scaled fp8
 weights, W8A8), decode (256 seqs x 2304 ctx, 1 layer),
-prefill_tc (4 x 2048), moe_decode (8 experts, 128 tokens top-2, grouped GEMM),
+prefill_tc (4 x 2048), kv8_decode / kv8_prefill / kv8_write (the 8-bit KV arena: 256 seqs x 2304 ctx,
+4 x 2048, 16384 rows of 8 heads), moe_decode (8 experts, 128 tokens top-2, grouped GEMM),
 gemm_decode_qkv (M=80 QKV + RoPE + KV write, stream-K; 50 MB of weights: ncu flushes
 the caches between passes, so its DRAM figures still count the weight stream).
 """
@@ -148,6 +149,46 @@ def bench_prefill(t: Timer, out: list):
             ms_ref = t(lambda: torch.nn.functional.scaled_dot_product_attention(qd, kd, kd, is_causal=True))
             row.update(sdpa_ms=ms_ref, sdpa_tflops=fl / ms_ref / 1e9, vs_sdpa=ms_ref / ms)
         out.append(row)
+
+
+def _kv8_case(nseq: int, ctx: int, hq: int = 32, hkv: int = 8):
+    """An 8-bit arena of nseq sequences (shuffled pages, random rows), its tables, and K and V rows."""
+    nb = (ctx + 15) // 16
+    arena = ops.kv8_arena(nseq * nb + 1, 1, hkv)
+    bt = torch.randperm(nseq * nb, device="cuda").view(nseq, nb).to(torch.int32)
+    sl = torch.full((nseq,), ctx, dtype=torch.int32, device="cuda")
+    n = nseq * nb * 16
+    k, v = (torch.randn(n, hkv * 128, device="cuda").to(BF) for _ in range(2))
+    slots = torch.randperm(n, device="cuda")
+    ops.kv8_write(k, v, slots, arena, 0)
+    return arena, bt, sl, k, v, slots
+
+
+def bench_kv8(t: Timer, out: list):
+    """The 8-bit KV arena: rows in and out, decode and prefill attention (Llama-3-8B heads, 32q/8kv)."""
+    hq, hkv = 32, 8
+    for rows in (256, 8192):
+        arena, bt, sl, k, v, slots = _kv8_case(1, 16384)
+        k, v, slots = k[:rows], v[:rows], slots[:rows]
+        byt = rows * hkv * (258 + 512)
+        ms = t(lambda: ops.kv8_write(k, v, slots, arena, 0))
+        ms_read = t(lambda: ops.kv8_read(arena, 0, slots, k, v))
+        out.append(dict(kernel="kv8_write/read", rows=rows, ms=ms, gbs=byt / ms / 1e6, read_ms=ms_read,
+                        read_gbs=byt / ms_read / 1e6))
+    for nseq, ctx in [(256, 2304), (64, 4096), (8, 8192), (1, 8192)]:
+        arena, bt, sl, *_ = _kv8_case(nseq, ctx)
+        q = torch.randn(nseq, hq * 128, device="cuda").to(BF)
+        o = torch.empty_like(q)
+        ms = t(lambda: ops.paged_decode_attention(q, arena, 0, bt, sl, hq, hkv, 0.088, out=o))
+        out.append(dict(kernel="paged_decode kv8", nseq=nseq, ctx=ctx, ms=ms, gbs=nseq * ctx * hkv * 258 / ms / 1e6))
+    for nseq, prefix, new in [(4, 0, 2048), (1, 0, 8192), (4, 4096, 2048), (16, 2000, 5)]:
+        arena, bt, sl, *_ = _kv8_case(nseq, prefix + new)
+        tiles = ops.build_prefill_tiles([i * new for i in range(nseq + 1)], [prefix] * nseq, device="cuda")
+        q = torch.randn(nseq * new, hq * 128, device="cuda").to(BF)
+        o = torch.empty_like(q)
+        ms = t(lambda: ops.paged_prefill_attention(q, arena, 0, bt, sl, tiles, None, None, hq, hkv, 0.088, out=o))
+        fl = 4 * nseq * (new * prefix + new * (new + 1) // 2) * hq * 128
+        out.append(dict(kernel="paged_prefill kv8", nseq=nseq, prefix=prefix, new=new, ms=ms, tflops=fl / ms / 1e9))
 
 
 def prefill_timeline(t: Timer, out: list):
@@ -384,6 +425,17 @@ def profile(case: str) -> None:
         qs_t = torch.tensor(qs, dtype=torch.int32, device="cuda")
         fn = lambda: ops.paged_prefill_attention(q, arena, 0, bt, sl, tiles, qs_t, None, hq, hkv, 0.088,  # noqa
                                                  out=o)
+    elif case in ("kv8_decode", "kv8_prefill", "kv8_write"):
+        nseq, ctx, hq, hkv = {"kv8_decode": (256, 2304), "kv8_prefill": (4, 2048), "kv8_write": (1, 16384)}[case] + (32, 8)
+        arena, bt, sl, k, v, slots = _kv8_case(nseq, ctx, hq, hkv)
+        rows = nseq if case == "kv8_decode" else nseq * ctx
+        q = torch.randn(rows, hq * 128, device="cuda").to(BF)
+        o = torch.empty_like(q)
+        tiles = ops.build_prefill_tiles([i * ctx for i in range(nseq + 1)], [0] * nseq, device="cuda")
+        fn = {"kv8_decode": lambda: ops.paged_decode_attention(q, arena, 0, bt, sl, hq, hkv, 0.088, out=o),
+              "kv8_prefill": lambda: ops.paged_prefill_attention(q, arena, 0, bt, sl, tiles, None, None, hq, hkv, 0.088,
+                                                                 out=o),
+              "kv8_write": lambda: ops.kv8_write(k, v, slots, arena, 0)}[case]
     elif case == "gemm_decode_qkv":
         # decode-size QKV projection (80 tokens, 4096 -> 6144) with RoPE + paged KV write: stream-K
         m, hq, hkv, hidden = 80, 32, 8, 4096
@@ -434,7 +486,7 @@ def main(argv=None):
     res: list = []
     for name in args.only.split(","):
         {"gemm": bench_gemm, "gemm_fp8": bench_gemm_fp8, "decode": bench_decode, "prefill": bench_prefill, "norm": bench_norm,
-         "moe": bench_moe, "pd_qkv": bench_pd_qkv, "prefill_timeline": prefill_timeline,
+         "moe": bench_moe, "kv8": bench_kv8, "pd_qkv": bench_pd_qkv, "prefill_timeline": prefill_timeline,
          "tp": bench_tp_kernels}[name](t, res)
     for r in res:
         print(json.dumps({k: (round(v, 4) if isinstance(v, float) else v) for k, v in r.items()}))
