@@ -11,6 +11,7 @@
 #include <vector>
 
 #include "../kernels/lakeb_kernels.h"
+#include "../kernels/tma_host.h"
 
 namespace {
 
@@ -703,15 +704,17 @@ at::Tensor kv8_prefill(const at::Tensor& q, c10::optional<at::Tensor> out_arg, c
   p.num_tiles = static_cast<int>(tiles.size(0));
   if (p.num_tiles == 0) return out;
   const c10::cuda::CUDAGuard guard(arena.device());
-  // A tile of at most 32 rows costs less as columns of the few-row kernel (192 cycles of an SM per page
-  // and 24 columns, cut evenly over the GPU) than as 128 rows of the tcgen05 one (550 per page and two
-  // heads, one CTA for all its keys). The host does not see the tiles' rows: with several sequences
-  // both kernels run, each on its own, where their rows on average leave it open.
+  // A tile of at most 32 rows takes less time as columns of the few-row kernel, which cuts its pages evenly
+  // over the GPU, than in a CTA per KV head of the tcgen05 one: one of 17 rows behind 6001 keys, 64 query
+  // and 8 KV heads, 43 us and 115; two of 32 behind 3000 take 71 us there and two of 33 68 us here. The
+  // host does not see the tiles' rows: where their sum leaves it open that some of several sequences are
+  // few, both kernels run and find from the lengths which tiles are whose (kv8_tile_is_few).
   if (p.num_rows <= 8 * int64_t(p.num_tiles) || (p.num_seqs == 1 && p.num_rows <= kFewRows)) {
     kv8_few_rows(p, q);
   } else {
-    if (p.num_seqs > 1) {
-      p.most_rows = p.few_rows = kFewRows;
+    if (p.num_seqs > 1 && p.num_rows + lakeb::kKv8TileRows - kFewRows <= lakeb::kKv8TileRows * int64_t(p.num_tiles)) {
+      p.few_rows = kFewRows;
+      p.sms = lakeb::num_sms();
       kv8_few_rows(p, q);
     }
     LAKEB_CHECK_RC(lakeb::kv8_prefill_tc(p, cur_stream()), "kv8_prefill");

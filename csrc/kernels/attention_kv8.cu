@@ -274,18 +274,31 @@ __device__ __forceinline__ void load_columns(const uint8_t* q, int real, float s
   }
 }
 
+// The larger tiles' work (every lane calls it).
+__device__ __forceinline__ int64_t warp_work(const Kv8AttnArgs& a, int lane) {
+  if (a.few_rows == 0) return 0;
+  const Kv8Packing pk = kv8_packing(a.n_q_heads / a.n_kv_heads);
+  int sum = 0;
+  for (int s = lane; s < min(a.num_tiles, kKv8Ranked); s += 32) {
+    const int4 t = a.tiles[s];
+    if (t.z > a.few_rows && kv8_tile_ok(a, t)) sum += kv8_tile_work(a, pk, t, kv8_tile_keys(a, t));
+  }
+  return static_cast<int64_t>(__reduce_add_sync(0xffffffffu, sum)) * a.n_kv_heads;
+}
+
 // One item of work: a sequence (decode) or a tile. Its segments are `units` = KV heads x groups of
 // `cols` columns, of `pages` pages each.
 struct Item {
   int seq, row0, nq, pos0, len, pages, groups, units;
 };
 template <int NT>
-__device__ __forceinline__ Item get_item(const Kv8AttnArgs& a, int s) {
+__device__ __forceinline__ Item get_item(const Kv8AttnArgs& a, int s, int64_t work) {
   Item it;
   if (a.tiles) {
     const int4 t = a.tiles[s];
     it.seq = t.x, it.row0 = t.y, it.nq = max(t.z, 0), it.pos0 = t.w;
-    if (!kv8_tile_ok(a, t) || it.nq > a.most_rows) it.seq = it.row0 = it.nq = 0;
+    if (!kv8_tile_ok(a, t) || (a.few_rows > 0 && t.z > 0 && !kv8_tile_is_few(a, t, kv8_tile_keys(a, t), work)))
+      it.seq = it.row0 = it.nq = 0;
   } else {
     it.seq = it.row0 = s, it.nq = 1, it.pos0 = 0;
   }
@@ -305,30 +318,31 @@ struct Place {
   int in_item;
 };
 template <int NT>
-__device__ __forceinline__ int item_cost(const Kv8AttnArgs& a, int s) {
-  const Item it = get_item<NT>(a, s);
+__device__ __forceinline__ int item_cost(const Kv8AttnArgs& a, int s, int64_t work) {
+  const Item it = get_item<NT>(a, s, work);
   return it.pages > 0 ? (it.pages + kSegCost) * it.units : 0;
 }
 // The whole length (for every lane). The first 256 items' stay in `keep` for find_place.
 template <int NT>
-__device__ __forceinline__ int64_t total_cost(const Kv8AttnArgs& a, int items, int lane, int (&keep)[8]) {
+__device__ __forceinline__ int64_t total_cost(const Kv8AttnArgs& a, int items, int64_t work, int lane, int (&keep)[8]) {
   int64_t sum = 0;
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
     keep[k] = 0;
     if (32 * k < items) {  // (a branch for the whole warp: code that is not run is not fetched either)
-      if (32 * k + lane < items) keep[k] = item_cost<NT>(a, 32 * k + lane);
+      if (32 * k + lane < items) keep[k] = item_cost<NT>(a, 32 * k + lane, work);
       sum += keep[k];
     }
   }
-  for (int s = 256 + lane; s < items; s += 32) sum += item_cost<NT>(a, s);
+  for (int s = 256 + lane; s < items; s += 32) sum += item_cost<NT>(a, s, work);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   return sum;
 }
 // Place `at` (every lane of the warp calls it); past the end: item == items.
 template <int NT>
-__device__ __forceinline__ Place find_place(const Kv8AttnArgs& a, int items, int64_t at, int lane, const int (&keep)[8]) {
+__device__ __forceinline__ Place find_place(const Kv8AttnArgs& a, int items, int64_t work, int64_t at, int lane,
+                                            const int (&keep)[8]) {
   // the 32 items that hold it, by their sums; then the item, by a scan of them
   int s0 = 0, mine = 0;
   bool hit = false;
@@ -341,7 +355,7 @@ __device__ __forceinline__ Place find_place(const Kv8AttnArgs& a, int items, int
       else at -= sum;
     }
   for (int s = 256; s < items && !hit; s += 32) {
-    const int n = s + lane < items ? item_cost<NT>(a, s + lane) : 0;
+    const int n = s + lane < items ? item_cost<NT>(a, s + lane, work) : 0;
     const unsigned sum = __reduce_add_sync(0xffffffffu, static_cast<unsigned>(n));
     hit = at < sum;
     if (hit) s0 = s, mine = n;
@@ -374,11 +388,12 @@ struct Walk {
   Item it;
   int64_t left;     // of the run, from offset x of segment `unit` on
   int unit, x;
+  int64_t work;
   __device__ void start(const Kv8AttnArgs& a, int item, int in_item, int64_t n) {
     s = item;
     left = n;
     if (n <= 0) return;
-    it = get_item<NT>(a, s);
+    it = get_item<NT>(a, s, work);
     unit = in_item / (it.pages + kSegCost);
     x = in_item - unit * (it.pages + kSegCost);
     if (count() == 0) left = 0;
@@ -394,7 +409,7 @@ struct Walk {
     x = 0;
     if (++unit == it.units) {
       unit = 0;
-      do it = get_item<NT>(a, ++s);
+      do it = get_item<NT>(a, ++s, work);
       while (it.pages == 0);
     }
     if (count() == 0) left = 0;  // the run ends in the segment's start cost: all its pages are the next one's
@@ -422,16 +437,18 @@ __global__ void __launch_bounds__(Smem<NT>::kThreads, Smem<NT>::kPerSm) kv8_attn
   __syncthreads();
 
   Walk<NT> w;
+  const int64_t work = warp_work(a, lane);
+  w.work = work;
   const int own = static_cast<int>(blockIdx.x) / a.n_kv_heads, own_head = static_cast<int>(blockIdx.x) % a.n_kv_heads;
   if (whole) {  // CTA = (item, KV head)
-    const Item it = get_item<NT>(a, own);
+    const Item it = get_item<NT>(a, own, work);
     const int n = it.pages > 0 ? it.groups * (it.pages + kSegCost) : 0;
     w.start(a, own, own_head * n, n);
   } else {
     int keep[8];
-    const int64_t total = total_cost<NT>(a, items, lane, keep);
+    const int64_t total = total_cost<NT>(a, items, work, lane, keep);
     const int64_t per = run_length(total, gridDim.x), run0 = blockIdx.x * per;
-    const Place p = find_place<NT>(a, items, run0, lane, keep);
+    const Place p = find_place<NT>(a, items, work, run0, lane, keep);
     w.start(a, p.item, p.in_item, max(int64_t(0), min(per, total - run0)));
   }
 
@@ -485,7 +502,7 @@ __global__ void __launch_bounds__(Smem<NT>::kThreads, Smem<NT>::kPerSm) kv8_attn
   const int g = lane >> 2, t2 = (lane & 3) * 2;
   // rows of sequences without keys
   for (int s = whole ? own : blockIdx.x; s < items; s += whole ? items : gridDim.x) {
-    const Item it = get_item<NT>(a, s);
+    const Item it = get_item<NT>(a, s, work);
     if (it.pages > 0) continue;
     const int h0 = whole ? own_head * G : 0, nh = whole ? G : a.n_q_heads;
     for (int i = threadIdx.x; i < it.nq * nh * kKv8Dim; i += kWarps * 32)
@@ -607,7 +624,8 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(const Kv8AttnArgs a) {
   asm volatile("griddepcontrol.launch_dependents;");
   // lengths and tiles are not the first kernel's to write: the search needs no wait
   int keep[8];
-  const int64_t total = total_cost<NT>(a, items, lane, keep);
+  const int64_t work = warp_work(a, lane);
+  const int64_t total = total_cost<NT>(a, items, work, lane, keep);
   const int64_t per = run_length(total, gridDim.x);
   const int64_t run0 = blockIdx.x * per, run1 = run0 + per;
   // (every CTA waits for the first kernel, those with nothing to do as well: what is launched next
@@ -616,8 +634,8 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(const Kv8AttnArgs a) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     return;
   }
-  const Place p = find_place<NT>(a, items, run1 - 1, lane, keep);
-  const Item it = get_item<NT>(a, p.item);
+  const Place p = find_place<NT>(a, items, work, run1 - 1, lane, keep);
+  const Item it = get_item<NT>(a, p.item, work);
   const int unit = p.in_item / (it.pages + kSegCost);
   const int64_t seg0 = run1 - 1 - p.in_item % (it.pages + kSegCost);
   const int64_t seg1 = seg0 + kSegCost + it.pages;
@@ -718,14 +736,14 @@ int64_t kv8_attention_ws_floats(const Kv8AttnArgs& a) {
 // pages costs 16 MMAs of 16 cycles per page and group, so a group that stays empty costs as much as
 // a full one, and columns beyond the groups cost another pass.
 int kv8_attention_groups(const Kv8AttnArgs& a) {
-  const int64_t rows = !a.tiles ? 1 : a.most_rows < a.num_rows ? a.most_rows : (a.num_rows + a.num_tiles - 1) / a.num_tiles;
+  const int64_t rows = !a.tiles ? 1 : a.few_rows > 0 ? a.few_rows : (a.num_rows + a.num_tiles - 1) / a.num_tiles;
   const int64_t groups = (rows * (a.n_q_heads / a.n_kv_heads) + 7) / 8;
   return groups < 3 ? static_cast<int>(groups) : 3;
 }
 
 int kv8_attention(const Kv8AttnArgs& a, cudaStream_t stream) {
   if ((a.tiles ? a.num_tiles : a.num_seqs) <= 0) return 0;
-  const int64_t rows = !a.tiles ? 1 : a.most_rows < kKv8TileRows ? a.most_rows : kKv8TileRows;
+  const int64_t rows = !a.tiles ? 1 : a.few_rows > 0 ? a.few_rows : kKv8TileRows;
   const int64_t cols = 8 * kv8_attention_groups(a);
   const int64_t units = a.n_kv_heads * ((rows * (a.n_q_heads / a.n_kv_heads) + cols - 1) / cols);
   if (units > INT32_MAX / 32 || (int64_t(a.max_blocks) + kSegCost) * units > INT32_MAX / 32) return -1;

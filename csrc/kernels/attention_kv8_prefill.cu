@@ -1,22 +1,22 @@
 // Causal prefill attention over the 8-bit KV arena on tcgen05 tensor cores (sm_100a).
 //
-// A CTA owns up to 128 query rows of two query heads A and B of one KV head (the last head of an
-// odd group runs alone), so each K/V tile of 128 keys that it brings in and converts serves both.
-// Per step of 64 keys:
+// A CTA owns two products A and B of 128 rows, which are query rows and heads of one KV head
+// (kv8_packing), so each K/V tile of 128 keys that it brings in and converts serves both; where a tile's
+// rows or an odd group's heads end in A, it runs alone. Per step of 64 keys and h = A, B:
 //   S_h   = Q_h K_i^T           tcgen05.mma fp16 (M=128, N=64, K=128), fp32 in tensor memory
-//   P_h   = 2^(S_h c + e_j - b) softmax warpgroup h: thread = query row; fp16 over S_h's columns
+//   P_h   = 2^(S_h c + e_j - b) softmax warpgroup h: thread = row; fp16 over S_h's columns
 //   O_h  += P_h V_i             tcgen05.mma, A = P_h from tensor memory, V_i MN-major in shared memory
-// A head has two S buffers of 64 columns: S(i+1) is there when the softmax of step i ends, and PV(i)
+// A product has two S buffers of 64 columns: S(i+1) is there when the softmax of step i ends, and PV(i)
 // and S(i+2) run behind it. With one buffer of 128 columns (tensor memory holds no more beside the
-// two O) softmax and products of a head take turns, and 128 keys of two heads took 5.1k cycles; so
-// they take 4.4k, of which the products run 2.6k and the exponentials 2.0k. What binds is shared
+// two O) softmax and tensor cores take turns, and 128 keys of both took 5.1k cycles; so they take
+// 4.4k, of which the products run 2.6k and the exponentials 2.0k. What binds is shared
 // memory (products' operands, conversion and copies move ~390 KB per tile, 3.0k cycles) and the
 // hand-offs that wait behind it. Measured: one 8192-token prompt of 32 query and 8 KV heads 0.56 ms,
-// 985 TFLOP/s; four of 2048 tokens 0.205 ms, 670 TFLOP/s. A CTA spends ~7 us around its main loop
+// 980 TFLOP/s; four of 2048 tokens 0.20 ms, 690 TFLOP/s. A CTA spends ~7 us around its main loop
 // (1.9 us until its queries arrive, 1.6 to convert them, about as long for the output, the rest start
-// and end), so eight prompts of 500 tokens, four tiles of keys a CTA at most, run at 275 TFLOP/s. CTAs
+// and end), so eight prompts of 500 tokens, four tiles of keys a CTA at most, run at 270 TFLOP/s. CTAs
 // that stay and take tile after tile overlapped little of that and issued products more slowly (1152
-// rows behind 7040 tokens: 181 us against 161), so a tile is a CTA. The grid goes tile by tile,
+// rows behind 7040 tokens: 181 us against 165), so a CTA has one tile. The grid goes tile by tile,
 // heaviest first, all heads of a tile side by side: head by head, the last heads' heavy tiles started
 // late (0.63 ms).
 //
@@ -35,7 +35,7 @@
 // kept in fp32 over sum_j 2^(e_0 - e_j) rowsum(P_j), so O / sum needs 2^(e_0) at the end.
 //
 // Warps: 0 = loads, 1 = tensor memory and MMA issue, 2-3 idle, 4-7 = converters of K, 8-11 = of V,
-// 12-15 and 16-19 = softmax of head A and B. Registers move from the first three warpgroups to the
+// 12-15 and 16-19 = softmax of A and B. Registers move from the first three warpgroups to the
 // softmax ones (80, 80, 80, 120 and 120 of 96 each: the split with the fewest spills). Every wait is bounded; a role whose wait ran out goes on through its loop without
 // work, so that the converters' named barriers are always reached by all of their warps.
 #include <math_constants.h>
@@ -62,7 +62,6 @@ constexpr int kRed = kParams + 4 * 32;               // [2 tiles][K, V][4] conve
 constexpr int kSmem = kRed + 2 * 2 * 4 * 8;
 constexpr int kThreads = 640;
 constexpr int kStep = 64;                            // keys per softmax step
-constexpr int kRanked = 256;                         // tiles of a launch that are ordered by their keys
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.0f;
 constexpr float kPBias = 7.0f;
@@ -75,6 +74,12 @@ struct TileParams {
   int any_nan, pad;
 };
 static_assert(sizeof(TileParams) == 32, "");
+
+// Product A's first row in q and head, the rows from there to the tile's end, its first row's position,
+// and how far B's are from A's.
+struct Rows {
+  int row, head, left, pos, row_b, head_b;
+};
 
 // fp16 x fp16 -> fp32, both K-major; with bmn B is MN-major.
 __host__ __device__ constexpr uint32_t idesc_f16(int M, int N, bool bmn) {
@@ -151,6 +156,14 @@ __device__ __forceinline__ void zero_row(uint8_t* dst, int row) {
     *reinterpret_cast<uint4*>(dst + (c >> 3) * kHalf + row * 128 + (((c ^ row) & 7) << 4)) = make_uint4(0, 0, 0, 0);
 }
 
+__device__ __forceinline__ void tma_load_3d(void* dst, const void* tmap, uint64_t* bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
+}
+
 __global__ void __launch_bounds__(kThreads, 1)
     kv8_prefill_kernel(const __grid_constant__ CUtensorMap qmap, const Kv8AttnArgs a) {
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -169,6 +182,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* o_last = bars + 24;     // [2 heads], the last step's PV
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 26);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 27);
+  // This CTA's rows for the softmax warps, which read them again at the end rather than hold them.
+  volatile Rows* rows = reinterpret_cast<volatile Rows*>(bars + 28);
   TileParams* params = reinterpret_cast<TileParams*>(smem + kParams);
 
   // Heavy query tiles first, or one of them would run on alone at the end. Of one sequence they are the
@@ -178,44 +193,60 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("griddepcontrol.wait;" ::: "memory");
     return;
   }
-  const int G = a.n_q_heads / a.n_kv_heads, pairs = (G + 1) / 2;
-  const int place = static_cast<int>(blockIdx.x) / (a.n_kv_heads * pairs);  // all heads of a tile side by side
-  const int head = static_cast<int>(blockIdx.x) % (a.n_kv_heads * pairs);
+  const int G = a.n_q_heads / a.n_kv_heads;
+  const Kv8Packing pk = kv8_packing(G);
+  const int place = static_cast<int>(blockIdx.x) / (a.n_kv_heads * pk.units);  // all heads of a tile side by side
+  const int at = static_cast<int>(blockIdx.x) % (a.n_kv_heads * pk.units);
   int rank = a.num_tiles - 1 - place;
-  if (a.num_seqs > 1 && a.num_tiles <= kRanked) {
+  int64_t work = 0;
+  if (a.num_seqs > 1) {
     int* keys = reinterpret_cast<int*>(smem + kK);
+    int* sums = keys + kKv8Ranked;  // of each warp's tiles; then the rank's tile
     const int t = threadIdx.x;
-    if (t < kRanked) {
-      int n = -1;
+    int4 x = make_int4(0, 0, 0, 0);
+    int n = 0;
+    if (t < kKv8Ranked) {
+      if (t < a.num_tiles) x = a.tiles[t];
+      const bool ok = x.z > 0 && kv8_tile_ok(a, x);
+      if (ok) n = kv8_tile_keys(a, x);
+      const int sum = __reduce_add_sync(0xffffffffu, ok ? kv8_tile_work(a, pk, x, n) : 0);
+      if ((t & 31) == 0) sums[t >> 5] = sum;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kKv8Ranked / 32; ++w) work += sums[w];
+    work *= a.n_kv_heads;
+    if (a.num_tiles <= kKv8Ranked) {
+      if (n > 0 && kv8_tile_is_few(a, x, n, work)) n = 0;
+      if (t < kKv8Ranked) keys[t] = t < a.num_tiles ? n : -1;
+      __syncthreads();
       if (t < a.num_tiles) {
-        const int4 x = a.tiles[t];
-        n = x.z > a.few_rows && kv8_tile_ok(a, x) ? min(x.w + x.z, a.seq_lens[x.x]) : 0;
+        int before = 0;
+        for (int u = 0; u < a.num_tiles; u += 4) {
+          const int4 k = *reinterpret_cast<const int4*>(keys + u);
+          before += (k.x > n || (k.x == n && u < t)) + (k.y > n || (k.y == n && u + 1 < t)) +
+                    (k.z > n || (k.z == n && u + 2 < t)) + (k.w > n || (k.w == n && u + 3 < t));
+        }
+        if (before == place) sums[kKv8Ranked / 32] = t;
       }
-      keys[t] = n;
+      __syncthreads();
+      rank = sums[kKv8Ranked / 32];
     }
-    __syncthreads();
-    if (t < a.num_tiles) {
-      const int mine = keys[t];
-      int before = 0;
-      for (int u = 0; u < a.num_tiles; u += 4) {
-        const int4 k = *reinterpret_cast<const int4*>(keys + u);
-        before += (k.x > mine || (k.x == mine && u < t)) + (k.y > mine || (k.y == mine && u + 1 < t)) +
-                  (k.z > mine || (k.z == mine && u + 2 < t)) + (k.w > mine || (k.w == mine && u + 3 < t));
-      }
-      if (before == place) keys[kRanked] = t;
-    }
-    __syncthreads();
-    rank = keys[kRanked];
   }
   const int4 tile = a.tiles[rank];
-  const int seq = tile.x, qrow0 = tile.y, nq = tile.z, pos0 = tile.w;
-  if (nq <= a.few_rows || !kv8_tile_ok(a, tile)) {  // none, or kv8_attention's
+  const int seq = tile.x, pos0 = tile.w;
+  // this CTA's rows of the tile: the last rows, with the most keys, first
+  const int sub = pk.pack > 1 ? pk.subs - 1 - at % pk.subs : 0, row_a = sub * 2 * pk.rows;
+  const int nq = pk.pack > 1 ? min(tile.z, row_a + 2 * pk.rows) : tile.z;  // rows of the tile up to this CTA's last
+  if (nq <= row_a || !kv8_tile_ok(a, tile) || (a.few_rows > 0 && kv8_tile_is_few(a, tile, kv8_tile_keys(a, tile), work))) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     return;
   }
-  const int kvh = head / pairs, pair = head % pairs;
-  const int qh0 = kvh * G + 2 * pair;
-  const int heads = uniform(min(2, G - 2 * pair));
+  const int unit = at % pk.units;
+  const int head_a = at / pk.units * G + (pk.pack > 1 ? unit / pk.subs * pk.pack : 2 * unit);
+  const int row_b = pk.pack > 1 ? pk.rows : 0, head_b = pk.pack > 1 ? 0 : 1;  // product B begins so much later
+  const int heads = uniform(pk.pack > 1 ? (nq > row_a + pk.rows ? 2 : 1) : min(2, G - 2 * unit));  // products
+  const int kvh = at / pk.units;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int len = min(a.seq_lens[seq], a.max_blocks * kKv8Page);
   const int max_pos = min(pos0 + nq - 1, len - 1);
@@ -240,6 +271,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&p_full[i], 128);
     }
     *abort_flag = 0;
+    rows->row = tile.y + row_a;
+    rows->head = head_a;
+    rows->left = nq - row_a;
+    rows->pos = pos0 + row_a;
+    rows->row_b = row_b;
+    rows->head_b = head_b;
     fence_mbar_init();
   }
   if (warp == 1) tmem_alloc(tmem_slot, 512);
@@ -258,7 +295,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_expect_tx(q_full, heads * kOperand);
         for (int h = 0; h < heads; ++h)
           for (int half = 0; half < 2; ++half)
-            tma_load_2d(smem + kQ + h * kOperand + half * kHalf, &qmap, q_full, (qh0 + h) * 128 + half * 64, qrow0);
+            tma_load_3d(smem + kQ + h * kOperand + half * kHalf, &qmap, q_full, half * 64, head_a + h * head_b,
+                        tile.y + row_a + h * row_b);
       }
       const int* bt = a.block_tables + static_cast<int64_t>(seq) * a.bt_stride;
       const int nblk = (len + kKv8Page - 1) / kKv8Page;
@@ -411,10 +449,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 120;");
     // -------------------------------------------------------------- softmax + epilogue: thread = query row
     const int h = (warp - 12) >> 2;
-    const int r = (warp & 3) * 32 + lane;  // query row in the tile = TMEM lane
+    const int r = (warp & 3) * 32 + lane;  // row of the product = TMEM lane: a query row and head
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     if (h < heads && n_steps > 0) {
-      const int kmax = min(pos0 + r, len - 1);  // last key this row may see
+      const int kmax = min(rows->pos + h * rows->row_b + (r >> pk.shift), len - 1);  // last key this row may see
       bool ok = __all_sync(0xffffffffu, mbar_wait(q_full, 0, abort_flag, a.status));
       // Q: bf16 -> fp16 in place, times a power of two that brings the row's largest element to [2^14, 2^15)
       float cr;
@@ -551,18 +589,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
         const int l = lane & 15, row0 = (warp & 3) * 32;
-        __nv_bfloat16* o0 = a.out + static_cast<int64_t>(qrow0 + row0) * a.out_stride + (qh0 + h) * 128 + l * 8;
+        const int first = h * rows->row_b, left = rows->left, shift = kv8_packing(a.n_q_heads / a.n_kv_heads).shift;
+        __nv_bfloat16* o0 = a.out + rows->row * a.out_stride + (rows->head + h * rows->head_b) * 128 + l * 8;
 #pragma unroll 2
         for (int i = 0; i < 16; ++i) {
-          const int x = 2 * i + (lane >> 4);
-          if (row0 + x < nq)
-            *reinterpret_cast<uint4*>(o0 + x * a.out_stride) =
+          const int x = 2 * i + (lane >> 4), row = first + ((row0 + x) >> shift);
+          if (row < left)
+            *reinterpret_cast<uint4*>(o0 + row * a.out_stride + ((row0 + x) & ((1 << shift) - 1)) * 128) =
                 *reinterpret_cast<const uint4*>(stage + x * 256 + ((l ^ (x & 7)) << 4));
         }
       }
       tc_fence_before();
-    } else if (h < heads && r < nq) {  // an empty context
-      uint4* dst = reinterpret_cast<uint4*>(a.out + static_cast<int64_t>(qrow0 + r) * a.out_stride + (qh0 + h) * 128);
+    } else if (h < heads && h * rows->row_b + (r >> pk.shift) < rows->left) {  // an empty context
+      uint4* dst = reinterpret_cast<uint4*>(a.out + (rows->row + h * rows->row_b + (r >> pk.shift)) * a.out_stride +
+                                            (rows->head + h * rows->head_b + (r & (pk.pack - 1))) * 128);
 #pragma unroll
       for (int v = 0; v < 16; ++v) dst[v] = make_uint4(0, 0, 0, 0);
     }
@@ -582,11 +622,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 int kv8_prefill_tc(const Kv8AttnArgs& a, cudaStream_t stream) {
   if (a.num_tiles <= 0) return 0;
   CUtensorMap qmap;
-  const int64_t cols = static_cast<int64_t>(a.n_q_heads) * 128;
-  if (!encode_bf16_map(&qmap, a.q, a.num_rows, cols, a.num_rows > 1 ? a.q_stride : cols, 128, 64)) return -5;
+  const Kv8Packing pk = kv8_packing(a.n_q_heads / a.n_kv_heads);
+  if (!encode_heads_map(&qmap, a.q, a.num_rows, a.n_q_heads, a.num_rows > 1 ? a.q_stride : int64_t(a.n_q_heads) * 128, pk.rows,
+                        pk.pack))
+    return -5;
   if (int e = ensure_smem_attr(reinterpret_cast<const void*>(kv8_prefill_kernel), kSmem)) return e;
-  const int G = a.n_q_heads / a.n_kv_heads;
-  const int64_t items = static_cast<int64_t>(a.num_tiles) * a.n_kv_heads * ((G + 1) / 2);
+  const int64_t items = static_cast<int64_t>(a.num_tiles) * a.n_kv_heads * pk.units;
   if (items > INT32_MAX) return -1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(items));

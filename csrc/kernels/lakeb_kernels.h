@@ -232,8 +232,10 @@ struct Kv8AttnArgs {
   float scale = 0.f;
   const int4* tiles = nullptr;  // (seq, first query row, number of queries, position of the first)
   int num_tiles = 0;
-  int most_rows = 1 << 30;  // kv8_attention leaves out tiles of more rows,
-  int few_rows = 0;         // kv8_prefill_tc those of at most so many (it may follow kv8_attention then)
+  // Both kernels run when few_rows > 0 (kv8_attention first): tiles of more rows belong to
+  // kv8_prefill_tc, the others to either (kv8_tile_is_few).
+  int few_rows = 0;
+  int sms = 0;
   // pieces of segments cut between CTAs (kv8_attention_ws_floats; ws_ml follows ws_o): per CTA two
   // pieces of 8 x kv8_attention_groups columns, 128 sums and 4 statistics each
   float* ws_o = nullptr;

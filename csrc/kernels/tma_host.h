@@ -15,6 +15,12 @@ bool make_bf16_map(CUtensorMap* out, const void* ptr, int64_t rows, int64_t cols
 bool encode_bf16_map(CUtensorMap* out, const void* ptr, int64_t rows, int64_t cols, int64_t ld, int box_rows,
                      int box_cols = 64);
 
+// Map of bf16 rows of `heads` x 128 elements (`ld` elements apart) as [rows, heads, 128], boxes of box_rows
+// x box_heads x 64 elements in that order: a box is box_rows * box_heads rows of 128 bytes with the
+// 128-byte swizzle, zero fill outside the bounds.
+bool encode_heads_map(CUtensorMap* out, const void* ptr, int64_t rows, int64_t heads, int64_t ld, int box_rows,
+                      int box_heads);
+
 // Byte-element 2-D map without swizzle (fp8 operands staged for conversion).
 bool make_u8_map(CUtensorMap* out, const void* ptr, int64_t rows, int64_t cols, int64_t ld, int box_rows,
                  int box_cols);

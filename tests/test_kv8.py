@@ -469,7 +469,10 @@ def test_prefill_heads(cuda_dev, hq, hkv):
 @pytest.mark.parametrize("lens,new", [([1], [1]), ([16], [16]), ([17], [1]), ([127], [127]), ([128], [128]),
                                       ([129], [129]), ([300], [172]), ([700, 5, 90], [300, 5, 1]),
                                       ([40, 0, 60], [5, 0, 5]), ([513], [257]), ([1030, 2, 2], [6, 2, 1]),
-                                      ([1500], [640]), ([200] * 12, [5] * 12), ([256, 2000], [256, 3])])
+                                      ([1500], [640]), ([200] * 12, [5] * 12), ([256, 2000], [256, 3]),
+                                      # few rows beside many: of so many keys that they go by themselves, or not
+                                      ([300, 5000], [300, 20]), ([40, 2000, 1900], [20, 640, 513]),
+                                      ([60] * 300 + [900, 0], [40] * 300 + [7, 0])])
 def test_prefill_lengths(cuda_dev, lens, new):
     check_prefill(cuda_dev, lens, new, 8, 2, 200 + lens[0], pad_tiles=2)
 
@@ -593,7 +596,8 @@ def test_decode_more_sequences_than_a_grid_axis(cuda_dev):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("lens,new,hq,hkv", [([256], [256], 2, 1), ([1500], [640], 8, 2), ([3000, 40], [640, 20], 8, 2),
-                                             ([700] * 6, [129] * 6, 10, 2), ([2500] * 3, [3, 9, 5], 8, 2)])
+                                             ([700] * 6, [129] * 6, 10, 2), ([2500] * 3, [3, 9, 5], 8, 2),
+                                             ([300, 5000], [300, 20], 16, 2), ([40, 900, 900], [20, 640, 513], 16, 2)])
 def test_prefill_repeats_bit_for_bit(cuda_dev, lens, new, hq, hkv):
     """Back to back, without a wait between the calls: a hand-off that is early by one phase shows here."""
     g = torch.Generator().manual_seed(16)
