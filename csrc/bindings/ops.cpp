@@ -633,6 +633,8 @@ lakeb::Kv8AttnArgs kv8_attn_args(const at::Tensor& q, const at::Tensor& out, con
   check_same_device(block_tables, arena, "block_tables");
   check_same_device(seq_lens, arena, "seq_lens");
   TORCH_CHECK(block_tables.size(1) < (int64_t(1) << 26), "block tables of at most 2^26 pages, got ", block_tables.size(1));
+  // (a row's largest score is found before the scores are scaled)
+  TORCH_CHECK(std::isfinite(static_cast<float>(scale)) && scale >= 0, "scale must be finite and not negative, got ", scale);
   TORCH_CHECK(q.numel() == 0 || out.data_ptr() != q.data_ptr(), "out must not be q");
   lakeb::Kv8AttnArgs p;
   p.q = bf(q);

@@ -500,7 +500,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (buf == 0) {
           if (j == 0) e0 = tp.ev;
           ev = static_cast<float>(tp.ev);
-          c = cr * __uint_as_float(static_cast<uint32_t>(127 + tp.ek) << 23);
+          // (not 0, where a row of zeros or small keys would make it that: masked scores are -infinity)
+          c = fmaxf(cr * __uint_as_float(static_cast<uint32_t>(127 + tp.ek) << 23), 0x1p-126f);
           unscale = ex2(static_cast<float>(e0 - tp.ev));
         }
         const int k0 = i * kStep;

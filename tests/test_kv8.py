@@ -535,6 +535,37 @@ def test_prefill_refusals(cuda_dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", [3, 150])  # both kernels
+def test_scores_too_small_for_their_factor(cuda_dev, rows):
+    """Queries of zeros beside keys near fp32's smallest, and a scale of 0: every seen key weighs the same."""
+    g = torch.Generator().manual_seed(17)
+    n, hq, hkv = 150, 8, 2
+    arena, bt, _ = build([n], hq, hkv, 1, 0, g, cuda_dev)
+    j = torch.arange(n, device=cuda_dev)
+    slots = bt[0].long()[j // PAGE] * PAGE + j % PAGE
+    k = (torch.randn(n, hkv * 128, generator=g) * 1e-36).to(BF).to(cuda_dev)
+    v = torch.randn(n, hkv * 128, generator=g).to(BF).to(cuda_dev)
+    ops.kv8_write(k, v, slots, arena, 0)
+    sl = torch.tensor([n], dtype=torch.int32, device=cuda_dev)
+    tiles = ops.build_prefill_tiles([0, rows], [n - rows], device=cuda_dev)
+    cached = ops.kv8_read(arena, 0, slots)[1].double().view(n, hkv, 128)
+    lim = torch.arange(n - rows + 1, n + 1, device=cuda_dev)
+    want = cached.cumsum(0)[lim - 1] / lim[:, None, None]
+    # the weights are 2^0 up to an exponential's error and fp16's rounding (2^-11), the output is a bf16 number
+    tol = want.abs() * 2 ** -8 + 4 * 2 ** -11 * cached.abs().amax()
+    for q, scale in ((torch.zeros(rows, hq * 128), 0.09), (torch.randn(rows, hq * 128, generator=g), 0.0)):
+        out = ops.paged_prefill_attention(q.to(BF).to(cuda_dev), arena, 0, bt, sl, tiles, None, None, hq, hkv, scale)
+        ops.core.check_status(cuda_dev)
+        err = (out.double().view(rows, hkv, hq // hkv, 128) - want[:, :, None]).abs()
+        assert bool((err <= tol[:, :, None]).all())
+    for scale in (-0.1, float("nan"), float("inf")):
+        with pytest.raises(RuntimeError, match="scale"):
+            ops.paged_prefill_attention(q.to(BF).to(cuda_dev), arena, 0, bt, sl, tiles, None, None, hq, hkv, scale)
+        with pytest.raises(RuntimeError, match="scale"):
+            ops.paged_decode_attention(q[:1].to(BF).to(cuda_dev), arena, 0, bt, sl, hq, hkv, scale)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows", [2, 200])  # both kernels
 def test_prefill_bad_tiles_are_reported_and_skipped(cuda_dev, rows):
     g = torch.Generator().manual_seed(14)
