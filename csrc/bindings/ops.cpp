@@ -248,6 +248,7 @@ void linear_qkv(const at::Tensor& a, const at::Tensor& w, at::Tensor& q_out, con
   g.positions = positions.data_ptr<int>();
   g.slots = slots.data_ptr<int64_t>();
   g.kv = arena_view(arena, layer);
+  if (g.kv.base8) check_aligned(rope_cs, "rope_cs");
   if (g.kv.base8) TORCH_CHECK(arena.size(2) == n_kv_heads, "kv heads mismatch: ", n_kv_heads, " for an arena of ", arena.size(2));
   g.n_q_heads = static_cast<int>(n_q_heads);
   g.n_kv_heads = static_cast<int>(n_kv_heads);

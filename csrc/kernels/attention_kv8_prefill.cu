@@ -36,8 +36,9 @@
 //
 // Warps: 0 = loads, 1 = tensor memory and MMA issue, 2-3 idle, 4-7 = converters of K, 8-11 = of V,
 // 12-15 and 16-19 = softmax of A and B. Registers move from the first three warpgroups to the
-// softmax ones (80, 80, 80, 120 and 120 of 96 each: the split with the fewest spills). Every wait is bounded; a role whose wait ran out goes on through its loop without
-// work, so that the converters' named barriers are always reached by all of their warps.
+// softmax ones (80, 80, 80, 120 and 120 of 96 each: the split with the fewest spills). Every wait is
+// bounded; a role whose wait ran out goes on through its loop without work, so that the converters'
+// named barriers are always reached by all of their warps.
 #include <math_constants.h>
 
 #include "common.cuh"
@@ -624,9 +625,8 @@ int kv8_prefill_tc(const Kv8AttnArgs& a, cudaStream_t stream) {
   if (a.num_tiles <= 0) return 0;
   CUtensorMap qmap;
   const Kv8Packing pk = kv8_packing(a.n_q_heads / a.n_kv_heads);
-  if (!encode_heads_map(&qmap, a.q, a.num_rows, a.n_q_heads, a.num_rows > 1 ? a.q_stride : int64_t(a.n_q_heads) * 128, pk.rows,
-                        pk.pack))
-    return -5;
+  const int64_t stride = a.num_rows > 1 ? a.q_stride : int64_t(a.n_q_heads) * 128;
+  if (!encode_heads_map(&qmap, a.q, a.num_rows, a.n_q_heads, stride, pk.rows, pk.pack)) return -5;
   if (int e = ensure_smem_attr(reinterpret_cast<const void*>(kv8_prefill_kernel), kSmem)) return e;
   const int64_t items = static_cast<int64_t>(a.num_tiles) * a.n_kv_heads * pk.units;
   if (items > INT32_MAX) return -1;

@@ -7,7 +7,11 @@
 // The first two move bytes: 258 + 512 per (row, head), against which 256 conversions are nothing. A
 // warp takes one row and up to four heads at a time, half of it K and half V, 16 bytes of bf16 and 8
 // bytes of codes per lane and head: both sides of a head move as whole 128- and 256-byte rows, and
-// four independent loads per lane are in flight behind the one load of the slot.
+// four independent loads per lane are in flight behind the one load of the slot. Measured: 16384 rows of
+// 8 heads in 22.8 us (4.4 TB/s read and written, 0.68 of the copy rate; codes are written in 128-byte
+// rows), 24 prefixes of 33 to 4097 tokens read in 23.7 us (0.86); a few rows are a launch of 3.3 us.
+// step_tables is one launch and three dependent loads: 3.9 us for 256 decode rows, 5.3 us for a step of
+// 8448 rows.
 #include "common.cuh"
 #include "kv8.cuh"
 #include "lakeb_kernels.h"
