@@ -280,9 +280,10 @@ __device__ __forceinline__ void load_columns(const uint8_t* q, int real, float s
   }
 }
 
-// The larger tiles' work (every lane calls it).
+// The larger tiles' work where both kernels run (every lane calls it).
+template <bool kMixed>
 __device__ __forceinline__ int64_t warp_work(const Kv8AttnArgs& a, int lane) {
-  if (a.few_rows == 0) return 0;
+  if (!kMixed) return 0;
   const Kv8Packing pk = kv8_packing(a.n_q_heads / a.n_kv_heads);
   int sum = 0;
   for (int s = lane; s < min(a.num_tiles, kKv8Ranked); s += 32) {
@@ -297,13 +298,13 @@ __device__ __forceinline__ int64_t warp_work(const Kv8AttnArgs& a, int lane) {
 struct Item {
   int seq, row0, nq, pos0, len, pages, groups, units;
 };
-template <int NT>
+template <int NT, bool kMixed>
 __device__ __forceinline__ Item get_item(const Kv8AttnArgs& a, int s, int64_t work) {
   Item it;
   if (a.tiles) {
     const int4 t = a.tiles[s];
     it.seq = t.x, it.row0 = t.y, it.nq = max(t.z, 0), it.pos0 = t.w;
-    if (!kv8_tile_ok(a, t) || (a.few_rows > 0 && t.z > 0 && !kv8_tile_is_few(a, t, kv8_tile_keys(a, t), work)))
+    if (!kv8_tile_ok(a, t) || (kMixed && t.z > 0 && !kv8_tile_is_few(a, t, kv8_tile_keys(a, t), work)))
       it.seq = it.row0 = it.nq = 0;
   } else {
     it.seq = it.row0 = s, it.nq = 1, it.pos0 = 0;
@@ -323,30 +324,30 @@ struct Place {
   int item;
   int in_item;
 };
-template <int NT>
+template <int NT, bool kMixed>
 __device__ __forceinline__ int item_cost(const Kv8AttnArgs& a, int s, int64_t work) {
-  const Item it = get_item<NT>(a, s, work);
+  const Item it = get_item<NT, kMixed>(a, s, work);
   return it.pages > 0 ? (it.pages + kSegCost) * it.units : 0;
 }
 // The whole length (for every lane). The first 256 items' stay in `keep` for find_place.
-template <int NT>
+template <int NT, bool kMixed>
 __device__ __forceinline__ int64_t total_cost(const Kv8AttnArgs& a, int items, int64_t work, int lane, int (&keep)[8]) {
   int64_t sum = 0;
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
     keep[k] = 0;
     if (32 * k < items) {  // (a branch for the whole warp: code that is not run is not fetched either)
-      if (32 * k + lane < items) keep[k] = item_cost<NT>(a, 32 * k + lane, work);
+      if (32 * k + lane < items) keep[k] = item_cost<NT, kMixed>(a, 32 * k + lane, work);
       sum += keep[k];
     }
   }
-  for (int s = 256 + lane; s < items; s += 32) sum += item_cost<NT>(a, s, work);
+  for (int s = 256 + lane; s < items; s += 32) sum += item_cost<NT, kMixed>(a, s, work);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   return sum;
 }
 // Place `at` (every lane of the warp calls it); past the end: item == items.
-template <int NT>
+template <int NT, bool kMixed>
 __device__ __forceinline__ Place find_place(const Kv8AttnArgs& a, int items, int64_t work, int64_t at, int lane,
                                             const int (&keep)[8]) {
   // the 32 items that hold it, by their sums; then the item, by a scan of them
@@ -361,7 +362,7 @@ __device__ __forceinline__ Place find_place(const Kv8AttnArgs& a, int items, int
       else at -= sum;
     }
   for (int s = 256; s < items && !hit; s += 32) {
-    const int n = s + lane < items ? item_cost<NT>(a, s + lane, work) : 0;
+    const int n = s + lane < items ? item_cost<NT, kMixed>(a, s + lane, work) : 0;
     const unsigned sum = __reduce_add_sync(0xffffffffu, static_cast<unsigned>(n));
     hit = at < sum;
     if (hit) s0 = s, mine = n;
@@ -388,7 +389,7 @@ __device__ __forceinline__ float base_or_zero(float x) { return x == -CUDART_INF
 __device__ __forceinline__ float factor(float x, float to) { return x == -CUDART_INF_F ? 1.f : ex2(x - to); }
 
 // The pieces that a CTA's run cuts out of the segments, in order. Loader and consumers walk the same.
-template <int NT>
+template <int NT, bool kMixed>
 struct Walk {
   int s;            // item
   Item it;
@@ -399,7 +400,7 @@ struct Walk {
     s = item;
     left = n;
     if (n <= 0) return;
-    it = get_item<NT>(a, s, work);
+    it = get_item<NT, kMixed>(a, s, work);
     unit = in_item / (it.pages + kSegCost);
     x = in_item - unit * (it.pages + kSegCost);
     if (count() == 0) left = 0;
@@ -415,14 +416,14 @@ struct Walk {
     x = 0;
     if (++unit == it.units) {
       unit = 0;
-      do it = get_item<NT>(a, ++s, work);
+      do it = get_item<NT, kMixed>(a, ++s, work);
       while (it.pages == 0);
     }
     if (count() == 0) left = 0;  // the run ends in the segment's start cost: all its pages are the next one's
   }
 };
 
-template <int NT>
+template <int NT, bool kMixed>
 __global__ void __launch_bounds__(Smem<NT>::kThreads, Smem<NT>::kPerSm) kv8_attn_kernel(const Kv8AttnArgs a, const int whole) {
   using S = Smem<NT>;
   constexpr int kWarps = S::kWarps;
@@ -435,26 +436,26 @@ __global__ void __launch_bounds__(Smem<NT>::kThreads, Smem<NT>::kPerSm) kv8_attn
   const int G = a.n_q_heads / a.n_kv_heads;
   const int items = a.tiles ? a.num_tiles : a.num_seqs;
 
-  asm volatile("griddepcontrol.launch_dependents;");
   if (threadIdx.x < 2 * S::kSlots + 4) {
     mbar_init(full + threadIdx.x, threadIdx.x < 2 * S::kSlots + 2 ? 1 : kWarps);
     fence_mbar_init();
   }
   __syncthreads();
+  after_previous();
 
-  Walk<NT> w;
-  const int64_t work = warp_work(a, lane);
+  Walk<NT, kMixed> w;
+  const int64_t work = warp_work<kMixed>(a, lane);
   w.work = work;
   const int own = static_cast<int>(blockIdx.x) / a.n_kv_heads, own_head = static_cast<int>(blockIdx.x) % a.n_kv_heads;
   if (whole) {  // CTA = (item, KV head)
-    const Item it = get_item<NT>(a, own, work);
+    const Item it = get_item<NT, kMixed>(a, own, work);
     const int n = it.pages > 0 ? it.groups * (it.pages + kSegCost) : 0;
     w.start(a, own, own_head * n, n);
   } else {
     int keep[8];
-    const int64_t total = total_cost<NT>(a, items, work, lane, keep);
+    const int64_t total = total_cost<NT, kMixed>(a, items, work, lane, keep);
     const int64_t per = run_length(total, gridDim.x), run0 = blockIdx.x * per;
-    const Place p = find_place<NT>(a, items, work, run0, lane, keep);
+    const Place p = find_place<NT, kMixed>(a, items, work, run0, lane, keep);
     w.start(a, p.item, p.in_item, max(int64_t(0), min(per, total - run0)));
   }
 
@@ -508,7 +509,7 @@ __global__ void __launch_bounds__(Smem<NT>::kThreads, Smem<NT>::kPerSm) kv8_attn
   const int g = lane >> 2, t2 = (lane & 3) * 2;
   // rows of sequences without keys
   for (int s = whole ? own : blockIdx.x; s < items; s += whole ? items : gridDim.x) {
-    const Item it = get_item<NT>(a, s, work);
+    const Item it = get_item<NT, kMixed>(a, s, work);
     if (it.pages > 0) continue;
     const int h0 = whole ? own_head * G : 0, nh = whole ? G : a.n_q_heads;
     for (int i = threadIdx.x; i < it.nq * nh * kKv8Dim; i += kWarps * 32)
@@ -621,7 +622,7 @@ __global__ void __launch_bounds__(Smem<NT>::kThreads, Smem<NT>::kPerSm) kv8_attn
 
 // Joins the segment whose pages begin in CTA run c and end in a later one (CTA c of this kernel). Its
 // first piece is c's last one, the others are the first pieces of the runs c + 1, c + 2, ...
-template <int NT>
+template <int NT, bool kMixed>
 __global__ void __launch_bounds__(256) kv8_join_kernel(const Kv8AttnArgs a) {
   constexpr int kCols = 8 * NT;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -630,8 +631,8 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(const Kv8AttnArgs a) {
   asm volatile("griddepcontrol.launch_dependents;");
   // lengths and tiles are not the first kernel's to write: the search needs no wait
   int keep[8];
-  const int64_t work = warp_work(a, lane);
-  const int64_t total = total_cost<NT>(a, items, work, lane, keep);
+  const int64_t work = warp_work<kMixed>(a, lane);
+  const int64_t total = total_cost<NT, kMixed>(a, items, work, lane, keep);
   const int64_t per = run_length(total, gridDim.x);
   const int64_t run0 = blockIdx.x * per, run1 = run0 + per;
   // (every CTA waits for the first kernel, those with nothing to do as well: what is launched next
@@ -640,8 +641,8 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(const Kv8AttnArgs a) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     return;
   }
-  const Place p = find_place<NT>(a, items, work, run1 - 1, lane, keep);
-  const Item it = get_item<NT>(a, p.item, work);
+  const Place p = find_place<NT, kMixed>(a, items, work, run1 - 1, lane, keep);
+  const Item it = get_item<NT, kMixed>(a, p.item, work);
   const int unit = p.in_item / (it.pages + kSegCost);
   const int64_t seg0 = run1 - 1 - p.in_item % (it.pages + kSegCost);
   const int64_t seg1 = seg0 + kSegCost + it.pages;
@@ -706,29 +707,19 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(const Kv8AttnArgs a) {
     }
 }
 
-template <int NT>
+template <int NT, bool kMixed>
 int launch(const Kv8AttnArgs& a, cudaStream_t stream) {
   const int items = a.tiles ? a.num_tiles : a.num_seqs;
-  if (int e = ensure_smem_attr(reinterpret_cast<const void*>(kv8_attn_kernel<NT>), Smem<NT>::kBytes)) return e;
+  if (int e = ensure_smem_attr(reinterpret_cast<const void*>(kv8_attn_kernel<NT, kMixed>), Smem<NT>::kBytes)) return e;
   if (a.max_blocks <= kWholePages) {
     const int64_t ctas = static_cast<int64_t>(items) * a.n_kv_heads;
     if (ctas > INT32_MAX) return -1;
-    kv8_attn_kernel<NT><<<static_cast<unsigned>(ctas), Smem<NT>::kThreads, Smem<NT>::kBytes, stream>>>(a, 1);
-    return cudaGetLastError();
+    return launch_ahead(kv8_attn_kernel<NT, kMixed>, static_cast<unsigned>(ctas), Smem<NT>::kThreads, Smem<NT>::kBytes,
+                        stream, a, 1);
   }
   const int ctas = Smem<NT>::kPerSm * num_sms();
-  kv8_attn_kernel<NT><<<ctas, Smem<NT>::kThreads, Smem<NT>::kBytes, stream>>>(a, 0);
-  if (int e = cudaGetLastError()) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas);
-  cfg.blockDim = dim3(256);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr;  // its prologue runs while the first kernel ends
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kv8_join_kernel<NT>, a);
+  if (int e = launch_ahead(kv8_attn_kernel<NT, kMixed>, ctas, Smem<NT>::kThreads, Smem<NT>::kBytes, stream, a, 0)) return e;
+  return launch_ahead(kv8_join_kernel<NT, kMixed>, ctas, 256, 0, stream, a);  // its search runs while the first ends
 }
 
 }  // namespace
@@ -753,10 +744,13 @@ int kv8_attention(const Kv8AttnArgs& a, cudaStream_t stream) {
   const int64_t cols = 8 * kv8_attention_groups(a);
   const int64_t units = a.n_kv_heads * ((rows * (a.n_q_heads / a.n_kv_heads) + cols - 1) / cols);
   if (units > INT32_MAX / 32 || (int64_t(a.max_blocks) + kSegCost) * units > INT32_MAX / 32) return -1;
+  // Launches that share the tiles with kv8_prefill (their tiles fill three groups) have kernels of their
+  // own: the others are short, and slower by the code that they would have to fetch (one sequence of
+  // 8192 tokens 20 us instead of 18).
   switch (kv8_attention_groups(a)) {
-    case 1: return launch<1>(a, stream);
-    case 2: return launch<2>(a, stream);
-    default: return launch<3>(a, stream);
+    case 1: return launch<1, false>(a, stream);
+    case 2: return launch<2, false>(a, stream);
+    default: return a.few_rows > 0 ? launch<3, true>(a, stream) : launch<3, false>(a, stream);
   }
 }
 

@@ -187,6 +187,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile Rows* rows = reinterpret_cast<volatile Rows*>(bars + 28);
   TileParams* params = reinterpret_cast<TileParams*>(smem + kParams);
 
+  // (behind kv8_attention it waits at its end: what that read was there before it began)
+  if (a.few_rows == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
   // Heavy query tiles first, or one of them would run on alone at the end. Of one sequence they are the
   // late ones; of several, each CTA finds the tile of its rank by the keys that it sees.
   if (smem_u32(smem) & 1023) {  // the swizzled tiles need it; the launch gives it
@@ -630,17 +632,7 @@ int kv8_prefill_tc(const Kv8AttnArgs& a, cudaStream_t stream) {
   if (int e = ensure_smem_attr(reinterpret_cast<const void*>(kv8_prefill_kernel), kSmem)) return e;
   const int64_t items = static_cast<int64_t>(a.num_tiles) * a.n_kv_heads * pk.units;
   if (items > INT32_MAX) return -1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(items));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = kSmem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = a.few_rows > 0 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kv8_prefill_kernel, qmap, a);
+  return launch_ahead(kv8_prefill_kernel, static_cast<unsigned>(items), kThreads, kSmem, stream, qmap, a);
 }
 
 }  // namespace lakeb

@@ -97,6 +97,28 @@ __device__ __forceinline__ bool kv8_tile_is_few(const Kv8AttnArgs& a, const int4
   return static_cast<int64_t>(own) * (a.sms - units) > work;
 }
 
+// The kernels of this cache are launched ahead of the end of the one before (launch_ahead), so that their
+// start does not add to a chain of short ones. Each calls after_previous before it reads anything but its
+// arguments: then all that ran before is done, and the kernel after this one may come ahead too.
+__device__ __forceinline__ void after_previous() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;");
+}
+template <class Kernel, class... Args>
+int launch_ahead(Kernel kernel, unsigned grid, int threads, int smem, cudaStream_t stream, const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // Two fp32 -> two e4m3 codes (round to nearest even), lo in the low byte.
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
   uint16_t r;

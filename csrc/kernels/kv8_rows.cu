@@ -38,6 +38,7 @@ __device__ __forceinline__ bool row_unit(const Kv8RowArgs& a, uint32_t u, int& r
 }
 
 __global__ void __launch_bounds__(kRowWarps * 32) kv8_write_kernel(const Kv8RowArgs a) {
+  after_previous();
   const int lane = threadIdx.x & 31, side = lane >> 4, l = lane & 15;
   int row, head;
   int64_t slot;
@@ -75,6 +76,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) kv8_write_kernel(const Kv8RowA
 }
 
 __global__ void __launch_bounds__(kRowWarps * 32) kv8_read_kernel(const Kv8RowArgs a) {
+  after_previous();
   const int lane = threadIdx.x & 31, side = lane >> 4, l = lane & 15;
   int row, head;
   int64_t slot;
@@ -124,6 +126,7 @@ __global__ void __launch_bounds__(kTabThreads) step_tables_kernel(const StepTabl
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const bool lead = blockIdx.x == 0;
   int base_n = 0, base_t = 0;
+  after_previous();
   for (int s0 = 0; s0 < a.num_seqs; s0 += kTabThreads) {
     const int s = s0 + tid;
     const int raw = s < a.num_seqs ? a.new_lens[s] : 0;
@@ -229,15 +232,13 @@ __global__ void __launch_bounds__(kTabThreads) step_tables_kernel(const StepTabl
 int kv8_write(const Kv8RowArgs& a, cudaStream_t stream) {
   if (a.rows <= 0) return 0;
   if (row_grid(a) * kRowWarps >= (int64_t(1) << 32) || row_grid(a) >= (int64_t(1) << 31)) return -1;
-  kv8_write_kernel<<<static_cast<unsigned>(row_grid(a)), kRowWarps * 32, 0, stream>>>(a);
-  return cudaGetLastError();
+  return launch_ahead(kv8_write_kernel, static_cast<unsigned>(row_grid(a)), kRowWarps * 32, 0, stream, a);
 }
 
 int kv8_read(const Kv8RowArgs& a, cudaStream_t stream) {
   if (a.rows <= 0) return 0;
   if (row_grid(a) * kRowWarps >= (int64_t(1) << 32) || row_grid(a) >= (int64_t(1) << 31)) return -1;
-  kv8_read_kernel<<<static_cast<unsigned>(row_grid(a)), kRowWarps * 32, 0, stream>>>(a);
-  return cudaGetLastError();
+  return launch_ahead(kv8_read_kernel, static_cast<unsigned>(row_grid(a)), kRowWarps * 32, 0, stream, a);
 }
 
 int step_tables(const StepTableArgs& a, cudaStream_t stream) {
@@ -247,8 +248,7 @@ int step_tables(const StepTableArgs& a, cudaStream_t stream) {
   if (a.num_seqs > grid) grid = a.num_seqs;
   if (grid > 2 * num_sms()) grid = 2 * num_sms();
   if (grid < 1) grid = 1;
-  step_tables_kernel<<<grid, kTabThreads, smem, stream>>>(a);
-  return cudaGetLastError();
+  return launch_ahead(step_tables_kernel, grid, kTabThreads, smem, stream, a);
 }
 
 }  // namespace lakeb

@@ -681,6 +681,76 @@ def test_two_streams_and_a_replayed_graph(cuda_dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("lens,new,hq,hkv", [([700, 90, 1500], None, 8, 2), ([200, 90, 16], None, 8, 2),
+                                             ([700, 90, 1500], [5, 2, 3], 8, 2), ([700, 90, 5000], [300, 20, 30], 16, 2),
+                                             ([400, 90, 250], [300, 20, 30], 16, 2)])
+@pytest.mark.parametrize("graph", [False, True])
+def test_attention_right_behind_its_writers(cuda_dev, lens, new, hq, hkv, graph):
+    """Keys, queries, lengths and pages written by the kernels just before, on this stream and on one that
+    joins it, without a wait between the rounds; the outputs and the buffers are used again at once."""
+    g = torch.Generator().manual_seed(18)
+    rounds, total = 6, sum(lens)
+    arena, bt, _ = build(lens, hq, hkv, 1, 0, g, cuda_dev)
+    slots = torch.cat([bt[i].long()[torch.arange(n, device=cuda_dev) // PAGE] * PAGE + torch.arange(n, device=cuda_dev) % PAGE
+                       for i, n in enumerate(lens)])
+    starts = [0]
+    for n in new or [1] * len(lens):
+        starts.append(starts[-1] + n)
+    k, v, q = (torch.randn(rounds, n, w * 128, generator=g).to(BF).to(cuda_dev)
+               for n, w in ((total, hkv), (total, hkv), (starts[-1], hq)))
+    full = torch.tensor(lens, dtype=torch.int32, device=cuda_dev)
+    sls = [full - (i % 2) * 3 for i in range(rounds)]
+    tiles = ops.build_prefill_tiles(starts, [a - b for a, b in zip(lens, new or lens)], device=cuda_dev)
+    qb, slb, btb, tb = torch.zeros_like(q[0]), torch.zeros_like(full), torch.zeros_like(bt), torch.zeros_like(tiles)
+    side = torch.cuda.Stream()
+
+    def attend():
+        if new is None:
+            return ops.paged_decode_attention(qb, arena, 0, btb, slb, hq, hkv, 0.1)
+        return ops.paged_prefill_attention(qb, arena, 0, btb, slb, tb, None, None, hq, hkv, 0.1)
+
+    def one(i, split):
+        main = torch.cuda.current_stream()
+        if split:
+            side.wait_stream(main)
+        with torch.cuda.stream(side if split else main):
+            ops.kv8_write(k[i], v[i], slots, arena, 0)
+        tb.copy_(tiles)
+        btb.copy_(bt)
+        qb.copy_(q[i])
+        if split and i % 2:
+            main.wait_stream(side)
+        slb.copy_(sls[i])
+        if split:
+            main.wait_stream(side)
+        out = attend()
+        qb.zero_()
+        slb.zero_()
+        return out
+
+    want = []
+    for i in range(rounds):
+        ops.kv8_write(k[i], v[i], slots, arena, 0)
+        for b, x in ((tb, tiles), (btb, bt), (qb, q[i]), (slb, sls[i])):
+            b.copy_(x)
+        torch.cuda.synchronize()
+        want.append(attend())
+        torch.cuda.synchronize()
+    if graph:
+        run = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(run):
+            got = [one(i, split) for split in (False, True) for i in range(rounds)]
+        for _ in range(3):
+            run.replay()
+    else:
+        got = [one(i, split) for split in (False, True) for i in range(rounds)]
+    torch.cuda.synchronize()
+    ops.core.check_status(cuda_dev)
+    for i, o in enumerate(got):
+        assert torch.equal(o, want[i % rounds]), i
+
+
+@pytest.mark.gpu
 def test_offsets_past_32_bits(cuda_dev):
     """Pages beyond 4 GiB of the arena are written, read and attended to."""
     blocks = (1 << 32) // (4128 * 2) + 64
