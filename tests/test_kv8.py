@@ -343,7 +343,7 @@ def check_decode(dev, lens, hq, hkv, seed, layers=2, layer=1, spread=0.3, qscale
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("hq,hkv", [(1, 1), (4, 4), (4, 2), (8, 2), (6, 2), (16, 2), (7, 1), (24, 2), (40, 1)])
+@pytest.mark.parametrize("hq,hkv", [(1, 1), (4, 4), (4, 2), (8, 2), (6, 2), (16, 2), (7, 1), (24, 2), (40, 1), (128, 1)])
 def test_decode_heads(cuda_dev, hq, hkv):
     check_decode(cuda_dev, [1, 33, 200], hq, hkv, 10 + hq)
 
@@ -460,7 +460,8 @@ def check_prefill(dev, lens, new, hq, hkv, seed, layers=2, layer=1, tile=128, sp
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("hq,hkv", [(1, 1), (4, 4), (4, 2), (8, 2), (6, 2), (16, 2), (5, 1), (24, 2), (40, 1)])
+@pytest.mark.parametrize("hq,hkv", [(1, 1), (4, 4), (4, 2), (8, 2), (6, 2), (16, 2), (5, 1), (24, 2), (40, 1), (64, 1),
+                                    (96, 1), (128, 1), (256, 1)])
 def test_prefill_heads(cuda_dev, hq, hkv):
     check_prefill(cuda_dev, [140, 33], [140, 7], hq, hkv, 20 + hq)
 
@@ -640,6 +641,12 @@ def test_prefill_repeats_bit_for_bit(cuda_dev, lens, new, hq, hkv):
     sl = torch.tensor(lens, dtype=torch.int32, device=cuda_dev)
     tiles = ops.build_prefill_tiles(starts, [n - m for n, m in zip(lens, new)], device=cuda_dev)
     outs = [ops.paged_prefill_attention(q, arena, 0, bt, sl, tiles, None, None, hq, hkv, 0.09) for _ in range(16)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for i in range(12):  # two at once
+        with torch.cuda.stream(streams[i % 2]):
+            outs.append(ops.paged_prefill_attention(q, arena, 0, bt, sl, tiles, None, None, hq, hkv, 0.09))
+    torch.cuda.synchronize()
     ops.core.check_status(cuda_dev)
     for o in outs[1:]:
         assert torch.equal(o, outs[0])
