@@ -14,7 +14,7 @@
 // hand-offs that wait behind it. Measured: one 8192-token prompt of 32 query and 8 KV heads 0.56 ms,
 // 980 TFLOP/s; four of 2048 tokens 0.20 ms, 690 TFLOP/s. A CTA spends ~7 us around its main loop
 // (1.9 us until its queries arrive, 1.6 to convert them, about as long for the output, the rest start
-// and end), so eight prompts of 500 tokens, four tiles of keys a CTA at most, run at 270 TFLOP/s. CTAs
+// and end), so eight prompts of 500 tokens, four tiles of keys a CTA at most, run at 255 TFLOP/s. CTAs
 // that stay and take tile after tile overlapped little of that and issued products more slowly (1152
 // rows behind 7040 tokens: 181 us against 165), so a CTA has one tile. The grid goes tile by tile,
 // heaviest first, all heads of a tile side by side: head by head, the last heads' heavy tiles started
@@ -32,7 +32,8 @@
 //
 // Softmax statistics: w = score in log2 units + e_j, b = a base that follows the largest w of the
 // row lazily (it moves when w grows by more than 2^8), P = 2^(w - b + 7) <= 2^15. The row sum is
-// kept in fp32 over sum_j 2^(e_0 - e_j) rowsum(P_j), so O / sum needs 2^(e_0) at the end.
+// kept in fp32 over sum_j 2^-e_j rowsum(P_j): e_j is -90 to 120 (448 * 2^120 is bf16's largest), so
+// that it lies between 2^-121 and 2^125 for up to 2^20 keys.
 //
 // Warps: 0 = loads, 1 = tensor memory and MMA issue, 2-3 idle, 4-7 = converters of K, 8-11 = of V,
 // 12-15 and 16-19 = softmax of A and B. Registers move from the first three warpgroups to the
@@ -409,8 +410,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = ok && mbar_wait(&raw_full[kv], j & 1, abort_flag, a.status);
       const bool real = ok && j * kTile + row < len;
       const int b = real ? side[kKv8Page * kKv8Dim + t] : 0;
-      // rows of zeros (b <= 1) and NaN rows (255) say nothing about the tile's scale
-      const int top = __reduce_max_sync(0xffffffffu, b > 1 && b < 255 ? b - 127 : kNone);
+      // NaN rows (255) say nothing about the tile's scale, nor, of V, rows of zeros (1, which as K's smallest
+      // scale may have codes)
+      const int top = __reduce_max_sync(0xffffffffu, b > kv && b < 255 ? b - 127 : kNone);
       const uint32_t nan = __ballot_sync(0xffffffffu, b == 255);
       if (lane == 0) red[warp & 3] = make_int2(top, static_cast<int>(nan));
       asm volatile("bar.sync %0, 128;" ::"r"(1 + kv) : "memory");
@@ -420,7 +422,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (row == 0) p.ek = e;
       } else {
         // V's reference may fall by 15 per tile (what fp16 holds exactly) and to 2^-80 of the largest
-        // so far, so that the sum's factor 2^(e_0 - e_j) stays within fp32
+        // so far; from 2^-90 on the sum's factor 2^-e_j stays within fp32
         e = e == kNone ? (ev_last == kNone ? -30 : ev_last) : max(e, -90);
         if (ev_last != kNone) e = max(e, max(ev_last - 15, ev_top - 80));
         ev_last = e;
@@ -485,7 +487,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (ok) mbar_arrive(q_ready);
       float bo = -CUDART_INF_F;  // base of w, at most kSlack below the largest w so far
       float l = 0.f, c = 0.f, ev = 0.f, unscale = 0.f;
-      int e0 = 0;
       for (int i = 0; i < n_steps; ++i) {
         const int j = i >> 1, buf = i & 1;
         const TileParams& tp = params[j & 3];
@@ -501,11 +502,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_ld32(t_mine, *reinterpret_cast<uint32_t(*)[32]>(sv));
         tmem_ld32(t_mine + 32, *reinterpret_cast<uint32_t(*)[32]>(sv + 32));
         if (buf == 0) {
-          if (j == 0) e0 = tp.ev;
           ev = static_cast<float>(tp.ev);
           // (not 0, where a row of zeros or small keys would make it that: masked scores are -infinity)
           c = fmaxf(cr * __uint_as_float(static_cast<uint32_t>(127 + tp.ek) << 23), 0x1p-126f);
-          unscale = ex2(static_cast<float>(e0 - tp.ev));
+          unscale = ex2(-ev);
         }
         const int k0 = i * kStep;
         const bool nan = tp.any_nan != 0;
@@ -546,14 +546,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         rs[0] = add2(rs[0], rs[1]);
         // O and l still hold sums against the old base. tcgen05.ld/st are warp-collective: the whole
         // warp rescales when any of its rows needs it (rows that do not keep alpha = 1).
-        float alpha = 1.f;
         if (__any_sync(0xffffffffu, grow && i > 0)) {
           if (!__all_sync(0xffffffffu, mbar_wait(&o_done[h], (i - 1) & 1, abort_flag, a.status))) {
             ok = false;
             break;
           }
           tc_fence_after();
-          alpha = (grow && old != -CUDART_INF_F) ? ex2(old - bo) : 1.f;
+          // (in two halves: a base may move by more than fp32's range, which O then outgrows and l does not)
+          const float half = (grow && old != -CUDART_INF_F) ? ex2(0.5f * (old - bo)) : 1.f;
+          const float alpha = half * half;
+          l = l * half * half;
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             uint32_t ov[32];
@@ -564,7 +566,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_st32(t_o[h] + lane_off + q * 32, ov);
           }
         }
-        l = fmaf(l, alpha, (rs[0].x + rs[0].y) * unscale);
+        l = fmaf(rs[0].x + rs[0].y, unscale, l);
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(&p_full[2 * h + buf]);
@@ -573,7 +575,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = ok && mbar_wait(&o_last[h], 0, abort_flag, a.status);
       if (__all_sync(0xffffffffu, ok)) {
         tc_fence_after();
-        const float inv = l == 0.f ? 0.f : exp2f(static_cast<float>(e0)) / l;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
         // Rows go through this head's Q, which no product reads any more, so that the warp stores whole
         // rows two at a time (a row per lane, 16 bytes at a time: eight prompts of 500 tokens 62.5 us
         // instead of 59). Chunk c of row r lies at chunk c ^ (r & 7): both ways are free of bank conflicts.

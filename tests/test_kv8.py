@@ -536,6 +536,43 @@ def test_prefill_refusals(cuda_dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", [3, 200])  # both kernels
+@pytest.mark.parametrize("case", ["values grow", "values fall", "keys near the smallest"])
+def test_far_apart_magnitudes(cuda_dev, rows, case):
+    """V rows 2^160 apart in one sequence, and K rows of e4m3's smallest scale under queries that make up for it."""
+    g = torch.Generator().manual_seed(19)
+    n, hq, hkv, scale = 500, 8, 2, 0.09
+    arena, bt, _ = build([n], hq, hkv, 1, 0, g, cuda_dev)
+    j = torch.arange(n)
+    slots = bt[0].cpu().long()[j // PAGE] * PAGE + j % PAGE
+    k, v = torch.randn(n, hkv, 128, generator=g), torch.randn(n, hkv, 128, generator=g)
+    q = torch.randn(rows, hq, 128, generator=g)
+    if case == "values grow":
+        v[:300] *= 2.0 ** -70
+        v[300:] *= 2.0 ** 90
+    elif case == "values fall":
+        v[:300] *= 2.0 ** 90
+        v[300:] *= 2.0 ** -70
+    else:
+        k *= 2.0 ** -122
+        q *= 2.0 ** 121
+    k, v, q = k.to(BF), v.to(BF), q.to(BF)
+    ops.kv8_write(k.view(n, -1).to(cuda_dev), v.view(n, -1).to(cuda_dev), slots.to(cuda_dev), arena, 0)
+    sl = torch.tensor([n], dtype=torch.int32, device=cuda_dev)
+    tiles = ops.build_prefill_tiles([0, rows], [n - rows], device=cuda_dev)
+    out = ops.paged_prefill_attention(q.view(rows, -1).to(cuda_dev), arena, 0, bt, sl, tiles, None, None, hq, hkv, scale)
+    ops.core.check_status(cuda_dev)
+    k64, v64 = quantize64(k).to(cuda_dev), quantize64(v).to(cuda_dev)
+    lim = torch.arange(n - rows + 1, n + 1, device=cuda_dev)
+    o, w, size = attend64(q.double().to(cuda_dev), k64, v64, lim, scale)
+    # a row's own largest value: those that it does not see do not count for its error
+    big = torch.stack([v64[:int(x)].abs().amax() for x in lim])
+    tol = torch.stack([attention_tolerance(o[i:i + 1], w[i:i + 1], size[i:i + 1], big[i])[0] for i in range(rows)])
+    err = (out.double().view(rows, hq, 128) - o).abs()
+    assert bool((err <= tol).all()), float((err / tol).amax())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows", [3, 150])  # both kernels
 def test_scores_too_small_for_their_factor(cuda_dev, rows):
     """Queries of zeros beside keys near fp32's smallest, and a scale of 0: every seen key weighs the same."""
