@@ -692,6 +692,7 @@ at::Tensor kv8_decode(const at::Tensor& q, c10::optional<at::Tensor> out_arg, co
 }
 
 constexpr int kFewRows = 32;
+constexpr int kFewPages = 64;
 
 at::Tensor kv8_prefill(const at::Tensor& q, c10::optional<at::Tensor> out_arg, const at::Tensor& arena, int64_t layer,
                        const at::Tensor& block_tables, const at::Tensor& seq_lens, const at::Tensor& tiles,
@@ -707,17 +708,21 @@ at::Tensor kv8_prefill(const at::Tensor& q, c10::optional<at::Tensor> out_arg, c
   p.num_tiles = static_cast<int>(tiles.size(0));
   if (p.num_tiles == 0) return out;
   const c10::cuda::CUDAGuard guard(arena.device());
-  // A tile of at most 32 rows takes less time as columns of the few-row kernel, which cuts its pages evenly
-  // over the GPU, than in a CTA per KV head of the tcgen05 one: one of 17 rows behind 6001 keys, 64 query
-  // and 8 KV heads, 43 us and 115; two of 32 behind 3000 take 71 us there and two of 33 68 us here. The
-  // host does not see the tiles' rows: where their sum leaves it open that some of several sequences are
-  // few, both kernels run and find from the lengths which tiles are whose (kv8_tile_is_few).
+  // A tile of few rows behind many keys takes less time as columns of the few-row kernel, which cuts its
+  // pages evenly over the GPU (17 rows behind 6001 keys, 64 query and 8 KV heads: 43 us), than in a CTA per
+  // KV head of the tcgen05 one, which takes ~2 us per 128 keys. The host does not see the tiles' rows: where
+  // their sum leaves it open that some of several sequences are few (up to 32), both kernels run and find
+  // from the lengths which tiles are whose (kv8_tile_is_few); up to 64 pages the few-row kernel would gain
+  // less than its launches take (five chunks of 78 to 191 rows 13 us in one kernel, 22 in both).
   if (p.num_rows <= 8 * int64_t(p.num_tiles) || (p.num_seqs == 1 && p.num_rows <= kFewRows)) {
     kv8_few_rows(p, q);
   } else {
-    if (p.num_seqs > 1 && p.num_rows + lakeb::kKv8TileRows - kFewRows <= lakeb::kKv8TileRows * int64_t(p.num_tiles)) {
+    p.sms = lakeb::num_sms();
+    // (two products of every tile and KV head in (G + 1) / 2 CTAs; see kv8_packing)
+    if (p.num_tiles * n_kv_heads * ((n_q_heads / n_kv_heads + 1) / 2) * 2 <= p.sms) p.products = 1;
+    if (p.num_seqs > 1 && p.max_blocks > kFewPages &&
+        p.num_rows + lakeb::kKv8TileRows - kFewRows <= lakeb::kKv8TileRows * int64_t(p.num_tiles)) {
       p.few_rows = kFewRows;
-      p.sms = lakeb::num_sms();
       kv8_few_rows(p, q);
     }
     LAKEB_CHECK_RC(lakeb::kv8_prefill_tc(p, cur_stream()), "kv8_prefill");

@@ -22,7 +22,7 @@
 // an equal run of them, whatever the lengths are (all CTAs resident). A segment that lies within one
 // CTA's run goes straight to the output; a CTA has at most two pieces of segments (its first and its
 // last) that go to the workspace, and a second kernel joins them in the order of the CTAs, so results
-// do not depend on timing. When no block table is wider than kWholePages, a CTA takes a whole segment
+// do not depend on timing. When no block table is wider than kWholePages, a CTA takes whole segments
 // and there is no second kernel.
 //
 // In a CTA one warp copies pages into a ring (bulk copies of 4128 bytes, page ids fetched 32 at a
@@ -280,15 +280,15 @@ __device__ __forceinline__ void load_columns(const uint8_t* q, int real, float s
   }
 }
 
-// The larger tiles' work where both kernels run (every lane calls it).
+// The tiles' work where both kernels run (every lane calls it).
 template <bool kMixed>
 __device__ __forceinline__ int64_t warp_work(const Kv8AttnArgs& a, int lane) {
   if (!kMixed) return 0;
-  const Kv8Packing pk = kv8_packing(a.n_q_heads / a.n_kv_heads);
+  const Kv8Packing pk = kv8_packing(a.n_q_heads / a.n_kv_heads, a.products);
   int sum = 0;
   for (int s = lane; s < min(a.num_tiles, kKv8Ranked); s += 32) {
     const int4 t = a.tiles[s];
-    if (t.z > a.few_rows && kv8_tile_ok(a, t)) sum += kv8_tile_work(a, pk, t, kv8_tile_keys(a, t));
+    if (t.z > 0 && kv8_tile_ok(a, t)) sum += kv8_tile_work(a, pk, t, kv8_tile_keys(a, t));
   }
   return static_cast<int64_t>(__reduce_add_sync(0xffffffffu, sum)) * a.n_kv_heads;
 }
@@ -423,6 +423,8 @@ struct Walk {
   }
 };
 
+__device__ __forceinline__ int whole_ctas(const Kv8AttnArgs& a, int whole) { return a.n_kv_heads * max(whole, 1); }
+
 template <int NT, bool kMixed>
 __global__ void __launch_bounds__(Smem<NT>::kThreads, Smem<NT>::kPerSm) kv8_attn_kernel(const Kv8AttnArgs a, const int whole) {
   using S = Smem<NT>;
@@ -446,11 +448,14 @@ __global__ void __launch_bounds__(Smem<NT>::kThreads, Smem<NT>::kPerSm) kv8_attn
   Walk<NT, kMixed> w;
   const int64_t work = warp_work<kMixed>(a, lane);
   w.work = work;
-  const int own = static_cast<int>(blockIdx.x) / a.n_kv_heads, own_head = static_cast<int>(blockIdx.x) % a.n_kv_heads;
-  if (whole) {  // CTA = (item, KV head)
+  // whole: CTA = (item, KV head, part of its column groups); `whole` parts
+  const int own = static_cast<int>(blockIdx.x) / whole_ctas(a, whole), own_part = static_cast<int>(blockIdx.x) % max(whole, 1);
+  const int own_head = static_cast<int>(blockIdx.x) % whole_ctas(a, whole) / max(whole, 1);
+  if (whole) {
     const Item it = get_item<NT, kMixed>(a, own, work);
-    const int n = it.pages > 0 ? it.groups * (it.pages + kSegCost) : 0;
-    w.start(a, own, own_head * n, n);
+    const int each = (it.groups + whole - 1) / whole, g0 = min(own_part * each, it.groups), g1 = min(g0 + each, it.groups);
+    const int cost = it.pages > 0 ? it.pages + kSegCost : 0;
+    w.start(a, own, (own_head * it.groups + g0) * cost, (g1 - g0) * cost);
   } else {
     int keep[8];
     const int64_t total = total_cost<NT, kMixed>(a, items, work, lane, keep);
@@ -508,7 +513,7 @@ __global__ void __launch_bounds__(Smem<NT>::kThreads, Smem<NT>::kPerSm) kv8_attn
   float* ms = reinterpret_cast<float*>(smem + S::kStat);
   const int g = lane >> 2, t2 = (lane & 3) * 2;
   // rows of sequences without keys
-  for (int s = whole ? own : blockIdx.x; s < items; s += whole ? items : gridDim.x) {
+  for (int s = whole ? (own_part ? items : own) : blockIdx.x; s < items; s += whole ? items : gridDim.x) {
     const Item it = get_item<NT, kMixed>(a, s, work);
     if (it.pages > 0) continue;
     const int h0 = whole ? own_head * G : 0, nh = whole ? G : a.n_q_heads;
@@ -707,15 +712,20 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(const Kv8AttnArgs a) {
     }
 }
 
+// Whether a CTA takes whole segments: few pages.
+bool takes_whole(const Kv8AttnArgs& a) { return a.max_blocks <= kWholePages; }
+
 template <int NT, bool kMixed>
 int launch(const Kv8AttnArgs& a, cudaStream_t stream) {
   const int items = a.tiles ? a.num_tiles : a.num_seqs;
   if (int e = ensure_smem_attr(reinterpret_cast<const void*>(kv8_attn_kernel<NT, kMixed>), Smem<NT>::kBytes)) return e;
-  if (a.max_blocks <= kWholePages) {
-    const int64_t ctas = static_cast<int64_t>(items) * a.n_kv_heads;
+  if (takes_whole(a)) {
+    // each column group of an average tile has a CTA
+    const int64_t cols = (a.tiles ? (a.num_rows + a.num_tiles - 1) / a.num_tiles : 1) * int64_t(a.n_q_heads / a.n_kv_heads);
+    const int64_t parts = (cols + 8 * NT - 1) / (8 * NT), ctas = parts * items * a.n_kv_heads;
     if (ctas > INT32_MAX) return -1;
     return launch_ahead(kv8_attn_kernel<NT, kMixed>, static_cast<unsigned>(ctas), Smem<NT>::kThreads, Smem<NT>::kBytes,
-                        stream, a, 1);
+                        stream, a, static_cast<int>(parts));
   }
   const int ctas = Smem<NT>::kPerSm * num_sms();
   if (int e = launch_ahead(kv8_attn_kernel<NT, kMixed>, ctas, Smem<NT>::kThreads, Smem<NT>::kBytes, stream, a, 0)) return e;
@@ -726,7 +736,7 @@ int launch(const Kv8AttnArgs& a, cudaStream_t stream) {
 
 int64_t kv8_attention_ws_floats(const Kv8AttnArgs& a) {
   const int nt = kv8_attention_groups(a);
-  return a.max_blocks <= kWholePages ? 0 : int64_t(2) * (nt == 1 ? 2 : 1) * num_sms() * 8 * nt * (kKv8Dim + 4);
+  return takes_whole(a) ? 0 : int64_t(2) * (nt == 1 ? 2 : 1) * num_sms() * 8 * nt * (kKv8Dim + 4);
 }
 
 // Groups of 8 columns that a CTA holds at once, by the columns of a tile on average: a pass over the

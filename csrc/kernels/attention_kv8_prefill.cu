@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     return;
   }
   const int G = a.n_q_heads / a.n_kv_heads;
-  const Kv8Packing pk = kv8_packing(G);
+  const Kv8Packing pk = kv8_packing(G, a.products);
   const int place = static_cast<int>(blockIdx.x) / (a.n_kv_heads * pk.units);  // all heads of a tile side by side
   const int at = static_cast<int>(blockIdx.x) % (a.n_kv_heads * pk.units);
   int rank = a.num_tiles - 1 - place;
@@ -240,16 +240,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int4 tile = a.tiles[rank];
   const int seq = tile.x, pos0 = tile.w;
   // this CTA's rows of the tile: the last rows, with the most keys, first
-  const int sub = pk.pack > 1 ? pk.subs - 1 - at % pk.subs : 0, row_a = sub * 2 * pk.rows;
-  const int nq = pk.pack > 1 ? min(tile.z, row_a + 2 * pk.rows) : tile.z;  // rows of the tile up to this CTA's last
+  const int sub = pk.pack > 1 ? pk.subs - 1 - at % pk.subs : 0, row_a = sub * a.products * pk.rows;
+  const int nq = pk.pack > 1 ? min(tile.z, row_a + a.products * pk.rows) : tile.z;  // rows of the tile up to this CTA's last
   if (nq <= row_a || !kv8_tile_ok(a, tile) || (a.few_rows > 0 && kv8_tile_is_few(a, tile, kv8_tile_keys(a, tile), work))) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     return;
   }
   const int unit = at % pk.units;
-  const int head_a = at / pk.units * G + (pk.pack > 1 ? unit / pk.subs * pk.pack : 2 * unit);
+  const int head_a = at / pk.units * G + (pk.pack > 1 ? unit / pk.subs * pk.pack : a.products * unit);
   const int row_b = pk.pack > 1 ? pk.rows : 0, head_b = pk.pack > 1 ? 0 : 1;  // product B begins so much later
-  const int heads = uniform(pk.pack > 1 ? (nq > row_a + pk.rows ? 2 : 1) : min(2, G - 2 * unit));  // products
+  const int heads = uniform(pk.pack > 1 ? (nq > row_a + pk.rows ? 2 : 1) : min(a.products, G - a.products * unit));
   const int kvh = at / pk.units;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int len = min(a.seq_lens[seq], a.max_blocks * kKv8Page);
@@ -595,7 +595,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
         const int l = lane & 15, row0 = (warp & 3) * 32;
-        const int first = h * rows->row_b, left = rows->left, shift = kv8_packing(a.n_q_heads / a.n_kv_heads).shift;
+        const int first = h * rows->row_b, left = rows->left, shift = kv8_packing(a.n_q_heads / a.n_kv_heads, 2).shift;
         __nv_bfloat16* o0 = a.out + rows->row * a.out_stride + (rows->head + h * rows->head_b) * 128 + l * 8;
 #pragma unroll 2
         for (int i = 0; i < 16; ++i) {
@@ -628,7 +628,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 int kv8_prefill_tc(const Kv8AttnArgs& a, cudaStream_t stream) {
   if (a.num_tiles <= 0) return 0;
   CUtensorMap qmap;
-  const Kv8Packing pk = kv8_packing(a.n_q_heads / a.n_kv_heads);
+  const Kv8Packing pk = kv8_packing(a.n_q_heads / a.n_kv_heads, a.products);
   const int64_t stride = a.num_rows > 1 ? a.q_stride : int64_t(a.n_q_heads) * 128;
   if (!encode_heads_map(&qmap, a.q, a.num_rows, a.n_q_heads, stride, pk.rows, pk.pack)) return -5;
   if (int e = ensure_smem_attr(reinterpret_cast<const void*>(kv8_prefill_kernel), kSmem)) return e;

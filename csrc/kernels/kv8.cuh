@@ -55,46 +55,46 @@ __device__ __forceinline__ bool kv8_tile_ok(const Kv8AttnArgs& a, const int4& t)
 // kv8_prefill: how the 128 rows of a CTA's two products are filled from a tile's query rows and the G query heads
 // of a KV head: with `pack` heads of a row side by side, pack the largest power of two in G, so that a
 // tile of few rows fills them too and a CTA's keys end close behind its rows. The two products then
-// take consecutive blocks of rows; with an odd G they take all the tile's rows of two heads.
+// take consecutive blocks of rows; with an odd G they take all the tile's rows of two heads. A launch
+// that leaves more than half of the SMs idle has one product in a CTA, and twice the CTAs.
 struct Kv8Packing {
   int pack, shift, rows;  // heads of a row, log2; rows of a product
   int subs;               // CTAs that share a tile's rows
   int units;              // CTAs of a tile and KV head
 };
-__host__ __device__ __forceinline__ Kv8Packing kv8_packing(int G) {
+__host__ __device__ __forceinline__ Kv8Packing kv8_packing(int G, int products) {
   Kv8Packing p;
   p.shift = 0;
   while (p.shift < 7 && !(G >> p.shift & 1)) ++p.shift;
   p.pack = 1 << p.shift;
   p.rows = kKv8TileRows >> p.shift;
-  p.subs = p.pack > 1 ? p.pack / 2 : 1;
-  p.units = p.pack > 1 ? G / 2 : (G + 1) / 2;
+  p.subs = p.pack > 1 ? p.pack / products : 1;
+  p.units = p.pack > 1 ? G / products : (G + products - 1) / products;
   return p;
 }
-
 // Which kernel a tile belongs to when both run (few_rows > 0; both find the same). In units of 128 keys of
-// a kv8_prefill CTA (2.3 us; its start and end cost three): the larger tiles' CTAs take `work` of them,
-// work / sms of time. A tile of few rows takes `own` of time in kv8_prefill, beside the others, and in
-// kv8_attention the whole GPU for about own * units / sms, units being its KV heads times groups of 24
-// columns. So it belongs to kv8_attention when own > work / sms + own * units / sms.
-// Measured, 64 query and 8 KV heads: chunks of 42 to 1500 rows take 104 us, with one of 17 rows behind 6001
-// keys 129 us in kv8_prefill, 144 in both.
-constexpr int kKv8Ranked = 256;  // tiles that are looked at for `work`
+// a kv8_prefill CTA (2.3 us; its start and end cost three), a tile of few rows takes `own` of time in
+// kv8_prefill, beside the others, whose CTAs take their work / sms. In kv8_attention it takes the whole GPU
+// for own * groups / sms, groups of 24 columns, and four for start and join. So tiles of few rows go there
+// that are longer than all of that together.
+// Measured, 64 query and 8 KV heads: chunks of 42 to 1500 rows take 106 us, with one of 17 rows behind 6001
+// keys 131 us in kv8_prefill, 144 in both; two of 32 rows behind 3000 keys 56 us in kv8_prefill, 72 in
+// kv8_attention.
+constexpr int kKv8Ranked = 256;  // tiles that are looked at
 constexpr int kKv8CtaCost = 3;
 __device__ __forceinline__ int kv8_tile_keys(const Kv8AttnArgs& a, const int4& t) {
   return max(0, min(min(t.w + t.z, a.seq_lens[t.x]), a.max_blocks * kKv8Page));
 }
-// A tile's part of `work` per KV head (cut off where a sum of kKv8Ranked could pass 32 bits).
+// A tile's work per KV head (cut off where a sum of kKv8Ranked could pass 32 bits).
 __device__ __forceinline__ int kv8_tile_work(const Kv8AttnArgs& a, const Kv8Packing& pk, const int4& t, int keys) {
-  if (t.z <= a.few_rows) return 0;
-  const int ctas = pk.pack > 1 ? pk.units / pk.subs * ((t.z + 2 * pk.rows - 1) / (2 * pk.rows)) : pk.units;
-  return min(((keys + 127) >> 7) + kKv8CtaCost, (1 << 22) / ctas) * ctas;
+  int n = pk.units;
+  if (t.z <= a.few_rows) n = (t.z * (a.n_q_heads / a.n_kv_heads) + 23) / 24;
+  else if (pk.pack > 1) n = pk.units / pk.subs * ((t.z + a.products * pk.rows - 1) / (a.products * pk.rows));
+  return min(((keys + 127) >> 7) + kKv8CtaCost, (1 << 22) / n) * n;
 }
 __device__ __forceinline__ bool kv8_tile_is_few(const Kv8AttnArgs& a, const int4& t, int keys, int64_t work) {
-  if (t.z > a.few_rows) return false;
   const int own = ((keys + 127) >> 7) + kKv8CtaCost;
-  const int units = a.n_kv_heads * ((t.z * (a.n_q_heads / a.n_kv_heads) + 23) / 24);
-  return static_cast<int64_t>(own) * (a.sms - units) > work;
+  return t.z <= a.few_rows && static_cast<int64_t>(own - 4) * a.sms > work;
 }
 
 // The kernels of this cache are launched ahead of the end of the one before (launch_ahead), so that their

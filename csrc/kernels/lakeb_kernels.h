@@ -236,6 +236,7 @@ struct Kv8AttnArgs {
   // kv8_prefill_tc, the others to either (kv8_tile_is_few).
   int few_rows = 0;
   int sms = 0;
+  int products = 2;  // of a kv8_prefill CTA: 1 or 2 (kv8_packing)
   // pieces of segments cut between CTAs (kv8_attention_ws_floats; ws_ml follows ws_o): per CTA two
   // pieces of 8 x kv8_attention_groups columns, 128 sums and 4 statistics each
   float* ws_o = nullptr;

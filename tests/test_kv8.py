@@ -467,6 +467,14 @@ def test_prefill_heads(cuda_dev, hq, hkv):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv", [(32, 8), (64, 8), (40, 8), (24, 8), (16, 16), (128, 2)])
+def test_prefill_more_tiles_than_half_the_gpu(cuda_dev, hq, hkv):
+    """(the launches above have one product in a CTA, these two)"""
+    check_prefill(cuda_dev, [700, 900, 300], [640, 515, 300], hq, hkv, 60 + hq)
+    check_prefill(cuda_dev, [1300], [1201], hq, hkv, 61 + hq)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("lens,new", [([1], [1]), ([16], [16]), ([17], [1]), ([127], [127]), ([128], [128]),
                                       ([129], [129]), ([300], [172]), ([700, 5, 90], [300, 5, 1]),
                                       ([40, 0, 60], [5, 0, 5]), ([513], [257]), ([1030, 2, 2], [6, 2, 1]),
