@@ -34,6 +34,8 @@
 // of the copy rate): memory. One of 8192 tokens 17 us: start (4.5 us to the first page) and join (2 us of
 // waiting, 4 of loads). 16 of 5 rows behind 300 to 2000 tokens 28.5 us: MMAs at 16 cycles, 48 a page for
 // three groups, in 11 us of steps, the rest start, sums of the warps and join.
+#include <algorithm>
+
 #include <math_constants.h>
 
 #include "common.cuh"
@@ -722,7 +724,7 @@ int launch(const Kv8AttnArgs& a, cudaStream_t stream) {
   if (takes_whole(a)) {
     // each column group of an average tile has a CTA
     const int64_t cols = (a.tiles ? (a.num_rows + a.num_tiles - 1) / a.num_tiles : 1) * int64_t(a.n_q_heads / a.n_kv_heads);
-    const int64_t parts = (cols + 8 * NT - 1) / (8 * NT), ctas = parts * items * a.n_kv_heads;
+    const int64_t parts = std::max<int64_t>(1, (cols + 8 * NT - 1) / (8 * NT)), ctas = parts * items * a.n_kv_heads;
     if (ctas > INT32_MAX) return -1;
     return launch_ahead(kv8_attn_kernel<NT, kMixed>, static_cast<unsigned>(ctas), Smem<NT>::kThreads, Smem<NT>::kBytes,
                         stream, a, static_cast<int>(parts));
@@ -745,7 +747,7 @@ int64_t kv8_attention_ws_floats(const Kv8AttnArgs& a) {
 int kv8_attention_groups(const Kv8AttnArgs& a) {
   const int64_t rows = !a.tiles ? 1 : a.few_rows > 0 ? a.few_rows : (a.num_rows + a.num_tiles - 1) / a.num_tiles;
   const int64_t groups = (rows * (a.n_q_heads / a.n_kv_heads) + 7) / 8;
-  return groups < 3 ? static_cast<int>(groups) : 3;
+  return groups < 1 ? 1 : groups < 3 ? static_cast<int>(groups) : 3;  // (no rows: empty tiles alone)
 }
 
 int kv8_attention(const Kv8AttnArgs& a, cudaStream_t stream) {

@@ -541,6 +541,10 @@ def test_prefill_refusals(cuda_dev):
         ops.core.check_status(cuda_dev)
     none = ops.paged_prefill_attention(q[:0], arena, 0, bt, sl, tiles[:0], None, None, 8, 2, 0.1)
     assert none.shape == (0, 1024)
+    for table in (bt, bt[:, :1].expand(1, 80).contiguous()):  # no rows, tiles that are all padding
+        none = ops.paged_prefill_attention(q[:0], arena, 0, table, sl, torch.zeros_like(tiles), None, None, 8, 2, 0.1)
+        assert none.shape == (0, 1024)
+    ops.core.check_status(cuda_dev)
 
 
 @pytest.mark.gpu
