@@ -22,8 +22,9 @@
 // an equal run of them, whatever the lengths are (all CTAs resident). A segment that lies within one
 // CTA's run goes straight to the output; a CTA has at most two pieces of segments (its first and its
 // last) that go to the workspace, and a second kernel joins them in the order of the CTAs, so results
-// do not depend on timing. When no block table is wider than kWholePages, a CTA takes whole segments
-// and there is no second kernel.
+// do not depend on timing. A few segments of few pages are not cut (four sequences of 200 tokens: 7.1 us
+// instead of 12.5), and when no block table is wider than kWholePages, none is and there is no second
+// kernel (5.7 us).
 //
 // In a CTA one warp copies pages into a ring (bulk copies of 4128 bytes, page ids fetched 32 at a
 // time, queries of the next segment ahead) and the others take pages in turn: with 8 columns two at
@@ -48,6 +49,7 @@ namespace lakeb {
 namespace {
 
 constexpr int kWholePages = 64;
+constexpr int kApartPages = 48;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.f;  // a base trails the true maximum by at most this
 constexpr float kPBias = 7.f;  // P = 2^(w - bo + 7): fp16 subnormals begin at 2^-21 of the base
@@ -331,23 +333,43 @@ __device__ __forceinline__ int item_cost(const Kv8AttnArgs& a, int s, int64_t wo
   const Item it = get_item<NT, kMixed>(a, s, work);
   return it.pages > 0 ? (it.pages + kSegCost) * it.units : 0;
 }
-// The whole length (for every lane). The first 256 items' stay in `keep` for find_place.
+// The whole length, the number of segments and the pages of the longest one (for every lane; more than 256
+// items: as if it were too long for `apart`). The first 256 items' lengths and segments stay in `keep` and
+// `units`, for find_place.
+struct Total {
+  int64_t cost;
+  int segments, longest;
+};
 template <int NT, bool kMixed>
-__device__ __forceinline__ int64_t total_cost(const Kv8AttnArgs& a, int items, int64_t work, int lane, int (&keep)[8]) {
+__device__ __forceinline__ Total total_cost(const Kv8AttnArgs& a, int items, int64_t work, int lane, int (&keep)[8],
+                                            int (&units)[8]) {
   int64_t sum = 0;
+  int segments = 0, longest = items > 256 ? INT32_MAX : 0;
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
-    keep[k] = 0;
+    keep[k] = units[k] = 0;
     if (32 * k < items) {  // (a branch for the whole warp: code that is not run is not fetched either)
-      if (32 * k + lane < items) keep[k] = item_cost<NT, kMixed>(a, 32 * k + lane, work);
+      if (32 * k + lane < items) {
+        const Item it = get_item<NT, kMixed>(a, 32 * k + lane, work);
+        if (it.pages > 0) {
+          units[k] = it.units;
+          keep[k] = (it.pages + kSegCost) * it.units;
+          longest = max(longest, it.pages);
+        }
+      }
       sum += keep[k];
+      segments += units[k];
     }
   }
   for (int s = 256 + lane; s < items; s += 32) sum += item_cost<NT, kMixed>(a, s, work);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  return sum;
+  return {sum, static_cast<int>(__reduce_add_sync(0xffffffffu, static_cast<unsigned>(segments))),
+          __reduce_max_sync(0xffffffffu, longest)};
 }
+// A few short segments are not cut: each has a CTA, and there is nothing to join. (Four or sixteen of 63
+// pages a head take 1 us less when they are.)
+__device__ __forceinline__ bool apart(const Total& t, int ctas) { return t.longest <= kApartPages && t.segments <= ctas; }
 // Place `at` (every lane of the warp calls it); past the end: item == items.
 template <int NT, bool kMixed>
 __device__ __forceinline__ Place find_place(const Kv8AttnArgs& a, int items, int64_t work, int64_t at, int lane,
@@ -459,11 +481,17 @@ __global__ void __launch_bounds__(Smem<NT>::kThreads, Smem<NT>::kPerSm) kv8_attn
     const int cost = it.pages > 0 ? it.pages + kSegCost : 0;
     w.start(a, own, (own_head * it.groups + g0) * cost, (g1 - g0) * cost);
   } else {
-    int keep[8];
-    const int64_t total = total_cost<NT, kMixed>(a, items, work, lane, keep);
-    const int64_t per = run_length(total, gridDim.x), run0 = blockIdx.x * per;
-    const Place p = find_place<NT, kMixed>(a, items, work, run0, lane, keep);
-    w.start(a, p.item, p.in_item, max(int64_t(0), min(per, total - run0)));
+    int keep[8], units[8];
+    const Total total = total_cost<NT, kMixed>(a, items, work, lane, keep, units);
+    if (apart(total, gridDim.x)) {
+      const Place p = find_place<NT, kMixed>(a, items, work, blockIdx.x, lane, units);
+      const int n = p.item < items ? get_item<NT, kMixed>(a, p.item, work).pages + kSegCost : 0;
+      w.start(a, p.item, p.in_item * n, n);
+    } else {
+      const int64_t per = run_length(total.cost, gridDim.x), run0 = blockIdx.x * per;
+      const Place p = find_place<NT, kMixed>(a, items, work, run0, lane, keep);
+      w.start(a, p.item, p.in_item, max(int64_t(0), min(per, total.cost - run0)));
+    }
   }
 
   if (warp == kWarps) {
@@ -637,14 +665,14 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(const Kv8AttnArgs a) {
   const int items = a.tiles ? a.num_tiles : a.num_seqs;
   asm volatile("griddepcontrol.launch_dependents;");
   // lengths and tiles are not the first kernel's to write: the search needs no wait
-  int keep[8];
+  int keep[8], units[8];
   const int64_t work = warp_work<kMixed>(a, lane);
-  const int64_t total = total_cost<NT, kMixed>(a, items, work, lane, keep);
-  const int64_t per = run_length(total, gridDim.x);
+  const Total t = total_cost<NT, kMixed>(a, items, work, lane, keep, units);
+  const int64_t total = t.cost, per = run_length(total, gridDim.x);
   const int64_t run0 = blockIdx.x * per, run1 = run0 + per;
   // (every CTA waits for the first kernel, those with nothing to do as well: what is launched next
   // follows this kernel's end alone)
-  if (run1 >= total) {
+  if (run1 >= total || apart(t, gridDim.x)) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     return;
   }

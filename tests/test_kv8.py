@@ -356,6 +356,14 @@ def test_decode_lengths(cuda_dev, lens):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("lens,hq,hkv", [([200, 16, 0, 700], 8, 2), ([5], 16, 1), ([0, 0], 8, 2), ([768] * 12, 8, 2),
+                                         ([30] * 148, 4, 2), ([30] * 149, 4, 2), ([17] * 300, 2, 1), ([769, 20], 8, 2)])
+def test_decode_few_pages_in_a_wide_table(cuda_dev, lens, hq, hkv):
+    """Segments that are not cut although the table is wide, and the first that are."""
+    check_decode(cuda_dev, lens, hq, hkv, 70 + len(lens), extra_cols=80)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("spread,qscale", [(3.0, 1.0), (0.3, 40.0), (8.0, 0.01), (0.0, 1e-20)])
 def test_decode_values(cuda_dev, spread, qscale):
     """Rows whose scales differ by many octaves, sharp and flat softmax, tiny queries."""
