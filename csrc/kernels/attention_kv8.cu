@@ -304,21 +304,23 @@ struct Item {
 };
 template <int NT, bool kMixed>
 __device__ __forceinline__ Item get_item(const Kv8AttnArgs& a, int s, int64_t work) {
-  Item it;
+  Item it = {};
   if (a.tiles) {
     const int4 t = a.tiles[s];
-    it.seq = t.x, it.row0 = t.y, it.nq = max(t.z, 0), it.pos0 = t.w;
-    if (!kv8_tile_ok(a, t) || (kMixed && t.z > 0 && !kv8_tile_is_few(a, t, kv8_tile_keys(a, t), work)))
-      it.seq = it.row0 = it.nq = 0;
+    // A tile without rows names nothing (its sequence may be any number), a refused one no sequence of this
+    // call, and a call may have no sequences at all: no length is read for them.
+    if (t.z <= 0 || !kv8_tile_ok(a, t)) return it;
+    if (kMixed && !kv8_tile_is_few(a, t, kv8_tile_keys(a, t), work)) return it;
+    it.seq = t.x, it.row0 = t.y, it.nq = t.z, it.pos0 = t.w;
   } else {
-    it.seq = it.row0 = s, it.nq = 1, it.pos0 = 0;
+    it.seq = it.row0 = s, it.nq = 1;
   }
   it.len = max(0, min(a.seq_lens[it.seq], a.max_blocks * kKv8Page));
   if (!a.tiles) it.pos0 = it.len - 1;
   const int G = a.n_q_heads / a.n_kv_heads;
   it.groups = (it.nq * G + 8 * NT - 1) / (8 * NT);
   it.units = a.n_kv_heads * it.groups;
-  it.pages = it.nq > 0 ? (max(0, min(it.len, it.pos0 + it.nq)) + kKv8Page - 1) / kKv8Page : 0;
+  it.pages = (max(0, min(it.len, it.pos0 + it.nq)) + kKv8Page - 1) / kKv8Page;
   return it;
 }
 

@@ -644,6 +644,64 @@ def test_prefill_bad_tiles_are_reported_and_skipped(cuda_dev, rows):
         assert torch.equal(out, good), bad
 
 
+def check_rows(out, q, cached, lens, new, hkv, scale):
+    """Rows of `out` (packed prefill rows, the last `new` of each sequence) against 64-bit attention; what a row
+    does not see counts neither for its result nor for its error."""
+    dev, hq, at = out.device, q.shape[1] // 128, 0
+    for s, (n, m) in enumerate(zip(lens, new)):
+        k, v = (x.to(dev) for x in cached[s])
+        lim = torch.arange(n - m + 1, n + 1, device=dev)
+        o, w, size = attend64(q[at:at + m].double().view(m, hq, 128), k, v, lim, scale)
+        top = v.abs().amax((1, 2)).cummax(0).values[lim - 1][:, None, None] if m else torch.zeros(0, 1, 1, device=dev)
+        err = (out[at:at + m].double().view(m, hq, 128) - o).abs()
+        tol = attention_tolerance(o, w, size, top)
+        assert bool((err <= tol).all()), (s, float((err / tol).nan_to_num(nan=float("inf")).amax()))
+        at += m
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cols", [5, 80])  # whole segments, and segments that are cut
+@pytest.mark.parametrize("lens,new", [([40, 30], [3, 2]), ([200, 30], [200, 30]), ([300, 5000], [300, 20])])
+def test_padding_tiles_name_no_sequence(cuda_dev, cols, lens, new):
+    """Tiles of no rows may hold anything else."""
+    g = torch.Generator().manual_seed(22)
+    arena, bt, cached = build(lens, 8, 2, 1, 0, g, cuda_dev, extra_cols=cols)
+    starts = [0, new[0], sum(new)]
+    q = torch.randn(starts[-1], 1024, generator=g).to(BF).to(cuda_dev)
+    sl = torch.tensor(lens, dtype=torch.int32, device=cuda_dev)
+    tiles = ops.build_prefill_tiles(starts, [a - b for a, b in zip(lens, new)], device=cuda_dev)
+    odd = torch.tensor([[x, y, z, w] for x, y, w in ((-1, -1, -1), (2, 0, 0), (2 ** 31 - 1, 2 ** 31 - 1, 2 ** 31 - 1),
+                                                     (-2 ** 31, 5, 7), (10 ** 6, 0, 3)) for z in (0, -1, -2 ** 31)],
+                       dtype=torch.int32, device=cuda_dev)
+    for t2 in (torch.cat([tiles, odd]), torch.cat([odd, tiles])):
+        out = ops.paged_prefill_attention(q, arena, 0, bt, sl, t2, None, None, 8, 2, 0.1)
+        ops.core.check_status(cuda_dev)
+        check_rows(out, q, cached, lens, new, 2, 0.1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("maxb", [5, 80])
+@pytest.mark.parametrize("n", [0, 3, 600])
+def test_a_step_of_no_sequences(cuda_dev, maxb, n):
+    """The tables of no sequences are padding alone; attention over them touches nothing."""
+    i32 = dict(dtype=torch.int32, device=cuda_dev)
+    t = ops.build_step_tables(torch.zeros(4, maxb, **i32), *(torch.zeros(0, **i32) for _ in range(3)), n, 3)
+    arena = ops.kv8_arena(2, 1, 2, device=cuda_dev)
+    q = torch.ones(n, 1024, dtype=BF, device=cuda_dev)
+    out = torch.full_like(q, 4.0)
+    ops.paged_prefill_attention(q, arena, 0, t.block_tables, t.seq_lens, t.tiles, t.query_start, t.positions, 8, 2, 0.1,
+                                out=out)
+    ops.paged_decode_attention(q, arena, 0, t.block_tables, t.seq_lens, 8, 2, 0.1, out=out)
+    ops.core.check_status(cuda_dev)
+    assert bool((out == 4.0).all())
+    if n:  # a tile with rows names a sequence that is not there
+        t.tiles[0, 2] = 1
+        ops.paged_prefill_attention(q, arena, 0, t.block_tables, t.seq_lens, t.tiles, None, None, 8, 2, 0.1, out=out)
+        with pytest.raises(ops.core.KernelError, match="out of bounds"):
+            ops.core.check_status(cuda_dev)
+        assert bool((out == 4.0).all())
+
+
 @pytest.mark.gpu
 def test_calls_that_are_refused_for_their_size_or_memory(cuda_dev):
     arena = ops.kv8_arena(1, 1, 1, device=cuda_dev)
