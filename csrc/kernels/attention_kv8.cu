@@ -413,6 +413,12 @@ __device__ __forceinline__ int64_t run_length(int64_t total, int ctas) {
 
 __device__ __forceinline__ float base_or_zero(float x) { return x == -CUDART_INF_F ? 0.f : x; }
 __device__ __forceinline__ float factor(float x, float to) { return x == -CUDART_INF_F ? 1.f : ex2(x - to); }
+// Sums of a column as the output: acc * 2^(B - M - kPBias) / L. The power goes in as two halves, since it
+// alone may be below fp32's smallest (values near bf16's own: V scales of 2^-119 and less).
+__device__ __forceinline__ uint2 column_out(const float4& acc, float M, float B, float L) {
+  const float h = ex2(0.5f * (base_or_zero(B) - base_or_zero(M) - kPBias)), f = L == 0.f ? 0.f : h / L;
+  return make_uint2(pack_bf16x2(acc.x * f * h, acc.y * f * h), pack_bf16x2(acc.z * f * h, acc.w * f * h));
+}
 
 // The pieces that a CTA's run cuts out of the segments, in order. Loader and consumers walk the same.
 template <int NT, bool kMixed>
@@ -644,10 +650,8 @@ __global__ void __launch_bounds__(Smem<NT>::kThreads, Smem<NT>::kPerSm) kv8_attn
       }
       if (entire) {
         const int c = cb + col;
-        const float f = L == 0.f ? 0.f : ex2(base_or_zero(B) - base_or_zero(M) - kPBias) / L;
         *reinterpret_cast<uint2*>(a.out + static_cast<int64_t>(it.row0 + c / G) * a.out_stride +
-                                  (kvh * G + c % G) * kKv8Dim + 4 * lane) =
-            make_uint2(pack_bf16x2(acc.x * f, acc.y * f), pack_bf16x2(acc.z * f, acc.w * f));
+                                  (kvh * G + c % G) * kKv8Dim + 4 * lane) = column_out(acc, M, B, L);
       } else {
         *reinterpret_cast<float4*>(a.ws_o + (part + col) * kKv8Dim + 4 * lane) = acc;
         if (lane == 0) *reinterpret_cast<float4*>(a.ws_ml + (part + col) * 4) = make_float4(M, B, L, 0.f);
@@ -737,10 +741,8 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(const Kv8AttnArgs a) {
   for (int k = 0; k < NT; ++k)
     if (warp + 8 * k < ncols) {
       const int c = cb + warp + 8 * k;
-      const float f = L[k] == 0.f ? 0.f : ex2(base_or_zero(B[k]) - base_or_zero(M[k]) - kPBias) / L[k];
       *reinterpret_cast<uint2*>(a.out + static_cast<int64_t>(it.row0 + c / G) * a.out_stride +
-                                (kvh * G + c % G) * kKv8Dim + 4 * lane) =
-          make_uint2(pack_bf16x2(acc[k].x * f, acc[k].y * f), pack_bf16x2(acc[k].z * f, acc[k].w * f));
+                                (kvh * G + c % G) * kKv8Dim + 4 * lane) = column_out(acc[k], M[k], B[k], L[k]);
     }
 }
 

@@ -592,6 +592,76 @@ def test_far_apart_magnitudes(cuda_dev, rows, case):
     assert bool((err <= tol).all()), float((err / tol).amax())
 
 
+def check_contributions(out, q, k, v, lim, scale):
+    """`out` [n, hq, 128] against 64-bit attention, held to what a row's own keys add to it:
+    the final rounding, P's and the scores' as in attention_tolerance, with |v| weighted and the scores' size that
+    of the keys whose weight is at least 2^-40 (the others are below every bound here);
+    P below fp16's normal range: half of its smallest step, 2^-25, where the largest P |v| has a P of at least
+    2^-1 and both |v| are codes of at most 448 against one of at least 224: 2^-23 of the largest p |v| for each key."""
+    g = q.shape[1] // k.shape[1]
+    k, v = k.repeat_interleave(g, 1), v.repeat_interleave(g, 1)
+    for i in range(q.shape[0]):
+        n = int(lim[i])
+        z = torch.einsum("hd,lhd->hl", q[i], k[:n]) * scale
+        p = torch.softmax(z, -1)
+        size = (torch.einsum("hd,lhd->hl", q[i].abs(), k[:n].abs()) * scale).masked_fill(p < 2.0 ** -40, 0.0).amax(-1)
+        o, w = (torch.einsum("hl,lhd->hd", p, x) for x in (v[:n], v[:n].abs()))
+        top = (p * v[:n].abs().amax(-1).t()).amax(-1)[:, None]
+        tol = 2.0 ** -8 * o.abs() + (2.0 ** -11 + 2.0 ** -14 * (1 + size[:, None])) * w + n * 2.0 ** -23 * top
+        err = (out[i].double() - o).abs()
+        assert bool((err <= tol).all()), (i, n, float((err / tol).nan_to_num(nan=float("inf")).amax()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,n", [(5, 400), (5, 1300)])  # (the second is cut between CTAs)
+@pytest.mark.parametrize("case", ["mixed", "zero rows", "falling", "rising", "tiny", "huge", "never written"])
+def test_scales_over_the_whole_range(cuda_dev, rows, n, case):
+    """Rows of one call over all of e4m3's and the scale's range, in any order: each counts by its own value."""
+    g = torch.Generator().manual_seed(24)
+    hq, hkv, scale = 8, 2, 0.09
+    arena, bt, _ = build([n], hq, hkv, 1, 0, g, cuda_dev, garbage=False)
+    j = torch.arange(n)
+    slots = bt[0].cpu().long()[j // PAGE] * PAGE + j % PAGE
+    k, v = torch.randn(n, hkv, 128, generator=g), torch.randn(n, hkv, 128, generator=g)
+    q = torch.randn(rows, hq, 128, generator=g)
+    at = torch.arange(n).float()
+    if case == "mixed":  # neighbours far apart; keys' large ones score low or high
+        v *= torch.exp2(torch.randint(-124, 118, (n, hkv, 1), generator=g).float())
+        k *= torch.exp2(torch.randint(-60, 6, (n, hkv, 1), generator=g).float())
+    elif case == "zero rows":  # of K and of V, alone and over a whole tile of keys
+        zk, zv = (torch.rand(n, hkv, 1, generator=g) < 0.3 for _ in range(2))
+        zv[128:256] = True
+        zk[256:384] = True
+        k, v = torch.where(zk, 0.0, k), torch.where(zv, 0.0, v)
+    elif case == "falling":
+        v *= torch.exp2(110 - at * (220 / n))[:, None, None]
+    elif case == "rising":
+        v *= torch.exp2(-110 + at * (220 / n))[:, None, None]
+    elif case == "tiny":
+        v *= 2.0 ** -122
+    elif case == "huge":
+        v *= 2.0 ** 124
+    k, v, q = k.to(BF), v.to(BF), q.to(BF)
+    k64, v64 = quantize64(k), quantize64(v)
+    if case == "never written":  # pages as they were allocated: zeros
+        arena[:, 0] = 0
+        keep = (j // PAGE) % 3 != 1
+        k64[~keep], v64[~keep] = 0.0, 0.0
+    else:
+        keep = j >= 0
+    ops.kv8_write(k[keep].view(-1, hkv * 128).to(cuda_dev), v[keep].view(-1, hkv * 128).to(cuda_dev),
+                  slots[keep].to(cuda_dev), arena, 0)
+    sl = torch.tensor([n], dtype=torch.int32, device=cuda_dev)
+    tiles = ops.build_prefill_tiles([0, rows], [n - rows], device=cuda_dev)
+    out = ops.paged_prefill_attention(q.view(rows, -1).to(cuda_dev), arena, 0, bt, sl, tiles, None, None, hq, hkv, scale)
+    one = ops.paged_decode_attention(q[-1:].view(1, -1).to(cuda_dev), arena, 0, bt, sl, hq, hkv, scale)
+    ops.core.check_status(cuda_dev)
+    lim = torch.arange(n - rows + 1, n + 1)
+    args = q.double().to(cuda_dev), k64.to(cuda_dev), v64.to(cuda_dev)
+    check_contributions(out.view(rows, hq, 128), *args, lim, scale)
+    check_contributions(one.view(1, hq, 128), args[0][-1:], *args[1:], lim[-1:], scale)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows", [3, 150])  # both kernels
 def test_scores_too_small_for_their_factor(cuda_dev, rows):
