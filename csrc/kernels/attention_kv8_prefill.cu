@@ -4,15 +4,15 @@
 // (kv8_packing), so each K/V tile of 128 keys that it brings in and converts serves both; where a tile's
 // rows or an odd group's heads end in A, it runs alone. Per step of 64 keys and h = A, B:
 //   S_h   = Q_h K_i^T           tcgen05.mma fp16 (M=128, N=64, K=128), fp32 in tensor memory
-//   P_h   = 2^(S_h c + e_j - b) softmax warpgroup h: thread = row; fp16 over S_h's columns
+//   P_h   = 2^(S_h c + e - b)   softmax warpgroup h: thread = row; fp16 over S_h's columns
 //   O_h  += P_h V_i             tcgen05.mma, A = P_h from tensor memory, V_i MN-major in shared memory
 // A product has two S buffers of 64 columns: S(i+1) is there when the softmax of step i ends, and PV(i)
 // and S(i+2) run behind it. With one buffer of 128 columns (tensor memory holds no more beside the
 // two O) softmax and tensor cores take turns, and 128 keys of both took 5.1k cycles; so they take
 // 4.4k, of which the products run 2.6k and the exponentials 2.0k. What binds is shared
 // memory (products' operands, conversion and copies move ~390 KB per tile, 3.0k cycles) and the
-// hand-offs that wait behind it. Measured: one 8192-token prompt of 32 query and 8 KV heads 0.56 ms,
-// 980 TFLOP/s; four of 2048 tokens 0.20 ms, 690 TFLOP/s. A CTA spends ~7 us around its main loop
+// hand-offs that wait behind it. Measured: one 8192-token prompt of 32 query and 8 KV heads 0.57 ms,
+// 960 TFLOP/s; four of 2048 tokens 0.21 ms, 645 TFLOP/s. A CTA spends ~7 us around its main loop
 // (1.9 us until its queries arrive, 1.6 to convert them, about as long for the output, the rest start
 // and end), so eight prompts of 500 tokens, four tiles of keys a CTA at most, run at 255 TFLOP/s. CTAs
 // that stay and take tile after tile overlapped little of that and issued products more slowly (1152
@@ -24,16 +24,20 @@
 // tile's eight pages (2064 bytes each, scales included) into a staging buffer each, a warpgroup for
 // each side turns codes into fp16 rows of the 128-byte swizzle (thread = key; e4m3 -> fp16 is
 // exact). The tensor cores' own fp8 products would need Q and P in 8 bits as well, or twice the
-// products. A tile is scaled against its own largest K scale and V scale: a row keeps
-// code * 2^(e_row - e_tile), exact while e_tile - e_row <= 15 (a code's last bit is 2^-9, fp16's
-// 2^-24), and e_tile itself is one multiplier of the tile's scores, or one addend of its exponents,
-// not work per element. Where rows of one tile differ by more than 2^15, the small rows' last bits
-// are lost: an error of 2^-24 of the largest element of the tile.
+// products. Where the K scales of a tile's keys lie within 2^15 of each other, its rows are kept against
+// the largest: code * 2^(e_row - e_K), exact (a code's last bit is 2^-9, fp16's 2^-24), and e_K is one
+// multiplier of the tile's scores. Where the V scales lie within 2^8, the same: e_V is one addend of the
+// tile's exponents. (The largest scale may be that of a key that a row does not see, or sees with no weight:
+// its P are up to 2^8 smaller for it, of the 2^21 between P's base and fp16's subnormals.) A tile of a wider
+// range keeps its codes as they are, and each key's scale enters its own scores and exponents, as in
+// kv8_attention: then what a row does not see has no part in it whatever it holds. Tokens' scales lie within a
+// few octaves of each other as a rule; a prompt of 8192 tokens whose every tile is wider takes 2.0 ms, 3.5 times as long.
 //
-// Softmax statistics: w = score in log2 units + e_j, b = a base that follows the largest w of the
-// row lazily (it moves when w grows by more than 2^8), P = 2^(w - b + 7) <= 2^15. The row sum is
-// kept in fp32 over sum_j 2^-e_j rowsum(P_j): e_j is -90 to 120 (448 * 2^120 is bf16's largest), so
-// that it lies between 2^-121 and 2^125 for up to 2^20 keys.
+// Softmax statistics, for each row: z = score in log2 units, w = z + e (e of V, the key's or the tile's). bo
+// follows the largest w and m the largest z, lazily: O is kept against 2^(bo - 7), with P = 2^(w - bo + 7)
+// <= 2^15, and the sum l of 2^z against 2^m. Of a tile with one e, l gets the sum of P times 2^(bo - 7 - e - m);
+// where that factor is past 2^82, P may be below fp32's range and 2^(z - m) not: such a step takes the
+// exponentials of both.
 //
 // Warps: 0 = loads, 1 = tensor memory and MMA issue, 2-3 idle, 4-7 = converters of K, 8-11 = of V,
 // 12-15 and 16-19 = softmax of A and B. Registers move from the first three warpgroups to the
@@ -60,20 +64,25 @@ constexpr int kV = kK + 2 * kOperand; // fp16 V, 2 stages
 constexpr int kRaw = kV + 2 * kOperand;              // staging: the K and the V sides of 8 pages
 constexpr int kBars = kRaw + 8 * kKv8Head;           // 229,632
 constexpr int kParams = kBars + 256;                 // [4] TileParams
-constexpr int kRed = kParams + 4 * 32;               // [2 tiles][K, V][4] converter warps' maxima and flags
-constexpr int kSmem = kRed + 2 * 2 * 4 * 8;
+constexpr int kScales = kParams + 4 * 32;            // [4][K, V][128] scale bytes of the keys as they were converted
+constexpr int kRed = kScales + 4 * 2 * kTile;        // [2 tiles][K, V][4] converter warps' extremes and flags
+constexpr int kSmem = kRed + 2 * 2 * 4 * 16;
+static_assert(kSmem <= 227 * 1024, "");
 constexpr int kThreads = 640;
 constexpr int kStep = 64;                            // keys per softmax step
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.0f;
 constexpr float kPBias = 7.0f;
+constexpr float kSumSlack = 40.0f;                   // m trails the largest z by at most this (l <= 2^60 for 2^20 keys)
+constexpr float kSumFactor = 82.0f;
+constexpr int kSpanK = 15, kSpanV = 8;               // octaves between a tile's scales that one factor serves
 
-// e_tile of K and V, and the keys whose V row is NaN (their codes are 0: the softmax makes the
-// scores of rows that see them NaN, so that rows that do not stay clean).
+// e of K and V (of a tile within kSpanK, kSpanV), and the keys whose V row is NaN (their codes are 0: the softmax
+// makes the scores of rows that see them NaN, so that rows that do not stay clean).
 struct TileParams {
   int ek, ev;
   uint32_t nan[4];
-  int any_nan, pad;
+  int wide_k, wide_v;  // wide_v: bit 0; bit 1: there are NaN keys
 };
 static_assert(sizeof(TileParams) == 32, "");
 
@@ -151,6 +160,16 @@ __device__ __forceinline__ void convert_row(const uint8_t* side, int t, uint8_t*
     *reinterpret_cast<uint4*>(d + (((k + 1) ^ sw) << 4)) = make_uint4(
         hmul2(f16x2_lo(q.z), f), hmul2(f16x2_hi(q.z), f), hmul2(f16x2_lo(q.w), f), hmul2(f16x2_hi(q.w), f));
   }
+}
+// Whether a row of codes has any that is not 0.
+__device__ __forceinline__ bool any_code(const uint8_t* side, int t) {
+  uint32_t any = 0;
+#pragma unroll 1
+  for (int c = 0; c < 8; ++c) {
+    const uint4 q = *reinterpret_cast<const uint4*>(side + t * kKv8Dim + c * 16);
+    any |= (q.x | q.y | q.z | q.w) & 0x7f7f7f7fu;
+  }
+  return any != 0;
 }
 __device__ __forceinline__ void zero_row(uint8_t* dst, int row) {
 #pragma unroll
@@ -399,50 +418,48 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------------------------- converters of K (kv = 0) and of V (kv = 1): thread = key of the tile
     const int kv = (warp - 4) >> 2, row = (threadIdx.x - 128) & 127, t = row & 15;
     const uint8_t* side = smem + kRaw + (kv * 8 + (row >> 4)) * kKv8Side;
-    constexpr int kNone = -1000;
-    int ev_last = kNone, ev_top = kNone;
+    int e = kv ? -126 : 0;
     bool ok = true;
     for (int j = 0; j < n_tiles; ++j) {
       const int s = j & 1;
-      int2* red = reinterpret_cast<int2*>(smem + kRed) + (s * 2 + kv) * 4;  // largest scale, NaN keys of each warp
+      int4* red = reinterpret_cast<int4*>(smem + kRed) + (s * 2 + kv) * 4;  // each warp's extremes, NaN keys
       // tile j - 4's was read before PV(j - 4) and S(j - 3), which the waits of tile j - 1 waited for
       TileParams& p = params[j & 3];
       ok = ok && mbar_wait(&raw_full[kv], j & 1, abort_flag, a.status);
       const bool real = ok && j * kTile + row < len;
       const int b = real ? side[kKv8Page * kKv8Dim + t] : 0;
-      // NaN rows (255) say nothing about the tile's scale, nor, of V, rows of zeros (1, which as K's smallest
-      // scale may have codes)
-      const int top = __reduce_max_sync(0xffffffffu, b > kv && b < 255 ? b - 127 : kNone);
+      // rows of NaNs (255) and of zeros (the smallest scale, as rows that are not zeros may have) say nothing
+      const bool counts = b > 0 && b < 255 && (b > 1 || any_code(side, t));
+      const int top = __reduce_max_sync(0xffffffffu, counts ? b : 0), low = __reduce_min_sync(0xffffffffu, counts ? b : 255);
       const uint32_t nan = __ballot_sync(0xffffffffu, b == 255);
-      if (lane == 0) red[warp & 3] = make_int2(top, static_cast<int>(nan));
+      if (lane == 0) red[warp & 3] = make_int4(top, low, static_cast<int>(nan), 0);
       asm volatile("bar.sync %0, 128;" ::"r"(1 + kv) : "memory");
-      int e = max(max(red[0].x, red[1].x), max(red[2].x, red[3].x));
-      if (kv == 0) {
-        if (e == kNone) e = 0;
-        if (row == 0) p.ek = e;
-      } else {
-        // V's reference may fall by 15 per tile (what fp16 holds exactly) and to 2^-80 of the largest
-        // so far; from 2^-90 on the sum's factor 2^-e_j stays within fp32
-        e = e == kNone ? (ev_last == kNone ? -30 : ev_last) : max(e, -90);
-        if (ev_last != kNone) e = max(e, max(ev_last - 15, ev_top - 80));
-        ev_last = e;
-        ev_top = max(ev_top, e);
-        if (row == 0) {
+      const int hi = max(max(red[0].x, red[1].x), max(red[2].x, red[3].x));
+      const int lo = min(min(red[0].y, red[1].y), min(red[2].y, red[3].y));
+      const bool wide = hi - lo > (kv ? kSpanV : kSpanK);
+      if (hi > 0) e = hi - 127;  // (a tile without any keeps the last one's)
+      smem[kScales + ((j & 3) * 2 + kv) * kTile + row] = static_cast<uint8_t>(wide ? b : e + 127);
+      if (row == 0) {
+        if (kv == 0) {
+          p.ek = e;
+          p.wide_k = wide;
+        } else {
+          int any = 0;
           p.ev = e;
-          p.any_nan = 0;
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
-            p.nan[w] = static_cast<uint32_t>(red[w].y);
-            p.any_nan |= red[w].y;
+            p.nan[w] = static_cast<uint32_t>(red[w].z);
+            any |= red[w].z;
           }
+          p.wide_v = (wide ? 1 : 0) | (any ? 2 : 0);
         }
       }
       ok = ok && mbar_wait(kv ? &v_empty[s] : &k_empty[s], ((j >> 1) & 1) ^ 1, abort_flag, a.status);
       if (ok) {
         uint8_t* dst = smem + (kv ? kV : kK) + s * kOperand;
-        // a NaN row of K gives NaN scores; one of V becomes zeros, its NaNs come through P
-        if (real && !(kv && b == 255))
-          convert_row(side, t, dst, row, b == 255 ? 0x7fff7fffu : f16x2_exp2(min(b - 127 - e, 0)));
+        // a NaN row of K gives NaN scores; one of V becomes zeros, its NaNs come through P. (b = 0: never written)
+        if (b > 0 && !(kv && b == 255))
+          convert_row(side, t, dst, row, b == 255 ? 0x7fff7fffu : f16x2_exp2(wide ? 0 : min(b - 127 - e, 0)));
         else
           zero_row(dst, row);
         fence_proxy_async_smem();
@@ -486,7 +503,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       fence_proxy_async_smem();
       if (ok) mbar_arrive(q_ready);
       float bo = -CUDART_INF_F;  // base of w, at most kSlack below the largest w so far
-      float l = 0.f, c = 0.f, ev = 0.f, unscale = 0.f;
+      float m = -CUDART_INF_F;   // base of l
+      float l = 0.f, c = 0.f, ev = 0.f;
+      int flags = 0;  // of the tile: bit 0: by each key's own scales; bit 1: NaN keys
       for (int i = 0; i < n_steps; ++i) {
         const int j = i >> 1, buf = i & 1;
         const TileParams& tp = params[j & 3];
@@ -503,12 +522,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_ld32(t_mine + 32, *reinterpret_cast<uint32_t(*)[32]>(sv + 32));
         if (buf == 0) {
           ev = static_cast<float>(tp.ev);
+          flags = tp.wide_k | tp.wide_v;
           // (not 0, where a row of zeros or small keys would make it that: masked scores are -infinity)
           c = fmaxf(cr * __uint_as_float(static_cast<uint32_t>(127 + tp.ek) << 23), 0x1p-126f);
-          unscale = ex2(-ev);
         }
         const int k0 = i * kStep;
-        const bool nan = tp.any_nan != 0;
+        const bool nan = (flags & 2) != 0, wide = (flags & 1) != 0;
         tmem_ld_wait();
         if (k0 + kStep - 1 > kmax) {  // the diagonal or the sequence end: keys past this row's last
 #pragma unroll
@@ -528,23 +547,53 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int k = 8; k < 64; k += 8)
 #pragma unroll
           for (int q = 0; q < 4; ++q) mv[q] = max3f(mv[q], __uint_as_float(sv[k + q]), __uint_as_float(sv[k + 4 + q]));
-        const float mx = fmaf(fmaxf(max3f(mv[0], mv[1], mv[2]), mv[3]), c, ev);
-        const bool grow = mx > bo + kSlack;
+        const float zx = fmaxf(max3f(mv[0], mv[1], mv[2]), mv[3]) * c, mx = zx + ev;
         const float old = bo;
-        if (grow) bo = mx;
-        const float add = bo == -CUDART_INF_F ? 0.f : ev - bo + kPBias;
-        float2 rs[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        const float2 cv = make_float2(c, c), av = make_float2(add, add);
+        const float bn = mx > bo + kSlack ? mx : bo, mn = zx > m + kSumSlack ? zx : m;
+        const float up = bn == -CUDART_INF_F ? 0.f : bn - kPBias - ev - mn;
+        if (!__any_sync(0xffffffffu, wide || up > kSumFactor)) {
+          bo = bn;
+          if (mn > m) l *= ex2(m - mn), m = mn;
+          const float add = bo == -CUDART_INF_F ? 0.f : ev - bo + kPBias;
+          float2 rs[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+          const float2 cv = make_float2(c, c), av = make_float2(add, add);
 #pragma unroll
-        for (int k = 0; k < 32; ++k) {  // key pair k -> packed column k (written over consumed scores)
-          const float2 z = fma2(make_float2(__uint_as_float(sv[2 * k]), __uint_as_float(sv[2 * k + 1])), cv, av);
-          const float2 p = make_float2(ex2(z.x), ex2(z.y));
-          rs[k & 1] = add2(rs[k & 1], p);
-          sv[k] = pack_f16x2(p.x, p.y);
+          for (int k = 0; k < 32; ++k) {  // key pair k -> packed column k (written over consumed scores)
+            const float2 z = fma2(make_float2(__uint_as_float(sv[2 * k]), __uint_as_float(sv[2 * k + 1])), cv, av);
+            const float2 p = make_float2(ex2(z.x), ex2(z.y));
+            rs[k & 1] = add2(rs[k & 1], p);
+            sv[k] = pack_f16x2(p.x, p.y);
+          }
+          rs[0] = add2(rs[0], rs[1]);
+          l = fmaf(rs[0].x + rs[0].y, ex2(up), l);
+        } else {
+          // each key by its own scales (read a few at a time: all at once, they would push scores out of the registers)
+          const uint8_t* kb = smem + kScales + (j & 3) * 2 * kTile + buf * kStep;
+          const uint8_t* vb = kb + kTile;
+          float zt = -CUDART_INF_F, wt = -CUDART_INF_F;
+#pragma unroll
+          for (int k = 0; k < 64; ++k) {
+            const float x = __uint_as_float(sv[k]);  // (-infinity: not seen, and the factor may be 0)
+            const float z = x == -CUDART_INF_F ? x : x * (cr * kv8_scale(kb[k]));
+            if ((k & 7) == 7) asm volatile("" ::: "memory");
+            sv[k] = __float_as_uint(z);
+            zt = fmaxf(zt, z);
+            wt = fmaxf(wt, z + static_cast<float>(vb[k] - 127));
+          }
+          if (wt > bo + kSlack) bo = wt;
+          if (zt > m + kSumSlack) l *= ex2(m - zt), m = zt;
+          const float zb = m == -CUDART_INF_F ? 0.f : m, wb = (bo == -CUDART_INF_F ? 0.f : bo - kPBias) + 127.f;
+#pragma unroll
+          for (int k = 0; k < 32; ++k) {
+            if ((k & 3) == 0) asm volatile("" ::: "memory");
+            const float z0 = __uint_as_float(sv[2 * k]), z1 = __uint_as_float(sv[2 * k + 1]);
+            l += ex2(z0 - zb) + ex2(z1 - zb);
+            sv[k] = pack_f16x2(ex2(z0 + (static_cast<float>(vb[2 * k]) - wb)), ex2(z1 + (static_cast<float>(vb[2 * k + 1]) - wb)));
+          }
         }
+        const bool grow = bo > old;
         tmem_st32(t_mine, *reinterpret_cast<uint32_t(*)[32]>(sv));
-        rs[0] = add2(rs[0], rs[1]);
-        // O and l still hold sums against the old base. tcgen05.ld/st are warp-collective: the whole
+        // O still holds sums against the old base. tcgen05.ld/st are warp-collective: the whole
         // warp rescales when any of its rows needs it (rows that do not keep alpha = 1).
         if (__any_sync(0xffffffffu, grow && i > 0)) {
           if (!__all_sync(0xffffffffu, mbar_wait(&o_done[h], (i - 1) & 1, abort_flag, a.status))) {
@@ -552,10 +601,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             break;
           }
           tc_fence_after();
-          // (in two halves: a base may move by more than fp32's range, which O then outgrows and l does not)
-          const float half = (grow && old != -CUDART_INF_F) ? ex2(0.5f * (old - bo)) : 1.f;
-          const float alpha = half * half;
-          l = l * half * half;
+          const float alpha = (grow && old != -CUDART_INF_F) ? ex2(old - bo) : 1.f;
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             uint32_t ov[32];
@@ -566,7 +612,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_st32(t_o[h] + lane_off + q * 32, ov);
           }
         }
-        l = fmaf(rs[0].x + rs[0].y, unscale, l);
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(&p_full[2 * h + buf]);
@@ -575,7 +620,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = ok && mbar_wait(&o_last[h], 0, abort_flag, a.status);
       if (__all_sync(0xffffffffu, ok)) {
         tc_fence_after();
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+        // O * 2^(bo - 7 - m) / l, the power in two halves: alone it may be past what fp32 holds
+        const float half = bo == -CUDART_INF_F ? 1.f : ex2(0.5f * (bo - kPBias - m));
+        const float inv = l == 0.f ? 0.f : half / l;
         // Rows go through this head's Q, which no product reads any more, so that the warp stores whole
         // rows two at a time (a row per lane, 16 bytes at a time: eight prompts of 500 tokens 62.5 us
         // instead of 59). Chunk c of row r lies at chunk c ^ (r & 7): both ways are free of bank conflicts.
@@ -586,7 +633,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_ld32(t_o[h] + lane_off + q * 32, ov);
           tmem_ld_wait();
           auto two = [&](int k) {
-            return pack_bf16x2(__uint_as_float(ov[k]) * inv, __uint_as_float(ov[k + 1]) * inv);
+            return pack_bf16x2(__uint_as_float(ov[k]) * inv * half, __uint_as_float(ov[k + 1]) * inv * half);
           };
 #pragma unroll
           for (int v = 0; v < 4; ++v)

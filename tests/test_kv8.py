@@ -607,13 +607,46 @@ def check_contributions(out, q, k, v, lim, scale):
         size = (torch.einsum("hd,lhd->hl", q[i].abs(), k[:n].abs()) * scale).masked_fill(p < 2.0 ** -40, 0.0).amax(-1)
         o, w = (torch.einsum("hl,lhd->hd", p, x) for x in (v[:n], v[:n].abs()))
         top = (p * v[:n].abs().amax(-1).t()).amax(-1)[:, None]
-        tol = 2.0 ** -8 * o.abs() + (2.0 ** -11 + 2.0 ** -14 * (1 + size[:, None])) * w + n * 2.0 ** -23 * top
+        tol = 2.0 ** -8 * o.abs() + (2.0 ** -11 + 2.0 ** -14 * (1 + size[:, None])) * w + n * 2.0 ** -23 * top + 2.0 ** -134
         err = (out[i].double() - o).abs()
         assert bool((err <= tol).all()), (i, n, float((err / tol).nan_to_num(nan=float("inf")).amax()))
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("rows,n", [(5, 400), (5, 1300)])  # (the second is cut between CTAs)
+@pytest.mark.parametrize("rows", [4, 230])  # both kernels
+@pytest.mark.parametrize("octaves", [7, 9, 14, 17, 26, 60, 110])
+@pytest.mark.parametrize("side", ["k", "v"])
+def test_a_large_key_counts_for_the_rows_that_see_it(cuda_dev, rows, octaves, side):
+    """One key of the chunk is 2^octaves times the others: rows before it come out as if it were not there, to
+    the accuracy of their own keys, and rows that see it with hardly any weight as well."""
+    g = torch.Generator().manual_seed(23)
+    n, hq, hkv, scale = 300, 8, 2, 0.09
+    arena, bt, _ = build([n], hq, hkv, 1, 0, g, cuda_dev)
+    j = torch.arange(n)
+    slots = bt[0].cpu().long()[j // PAGE] * PAGE + j % PAGE
+    k, v = torch.randn(n, hkv, 128, generator=g), torch.randn(n, hkv, 128, generator=g)
+    q = torch.randn(rows, hq, 128, generator=g)
+    q[..., 0] = 3.0
+    for at, head in ((n - 2, 0), (n - rows // 2, 1)):
+        if side == "k":  # a score far below the others for the rows that see it
+            k[at, head] = 0.0
+            k[at, head, 0] = -(2.0 ** octaves)
+        else:  # a weight that the value does not make up for: 2^-160, octaves < 160
+            k[at, head] = 0.0
+            k[at, head, 0] = -420.0
+            v[at, head] *= 2.0 ** octaves
+    k, v, q = k.to(BF), v.to(BF), q.to(BF)
+    ops.kv8_write(k.view(n, -1).to(cuda_dev), v.view(n, -1).to(cuda_dev), slots.to(cuda_dev), arena, 0)
+    sl = torch.tensor([n], dtype=torch.int32, device=cuda_dev)
+    tiles = ops.build_prefill_tiles([0, rows], [n - rows], device=cuda_dev)
+    out = ops.paged_prefill_attention(q.view(rows, -1).to(cuda_dev), arena, 0, bt, sl, tiles, None, None, hq, hkv, scale)
+    ops.core.check_status(cuda_dev)
+    check_contributions(out.view(rows, hq, 128), q.double().to(cuda_dev), quantize64(k).to(cuda_dev),
+                        quantize64(v).to(cuda_dev), torch.arange(n - rows + 1, n + 1), scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,n", [(5, 400), (5, 1300), (400, 400)])  # few rows (whole; cut between CTAs), many
 @pytest.mark.parametrize("case", ["mixed", "zero rows", "falling", "rising", "tiny", "huge", "never written"])
 def test_scales_over_the_whole_range(cuda_dev, rows, n, case):
     """Rows of one call over all of e4m3's and the scale's range, in any order: each counts by its own value."""
