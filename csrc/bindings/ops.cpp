@@ -255,7 +255,11 @@ void linear_qkv(const at::Tensor& a, const at::Tensor& w, at::Tensor& q_out, con
   if (peer_arena.has_value() && peer_slots.has_value()) {
     TORCH_CHECK(peer_arena->scalar_type() == arena.scalar_type(), "peer arena of another type");
     g.peer_kv = arena_view(*peer_arena, layer, /*host_ok=*/true);
-    TORCH_CHECK(peer_slots->scalar_type() == at::kLong, "peer_slots int64");
+    if (g.peer_kv.base8)
+      TORCH_CHECK(peer_arena->size(2) == n_kv_heads, "kv heads mismatch: ", n_kv_heads, " for a peer arena of ",
+                  peer_arena->size(2));
+    TORCH_CHECK(peer_slots->scalar_type() == at::kLong && peer_slots->numel() >= a.size(0) && peer_slots->is_contiguous(),
+                "peer_slots int64, one for each row");
     g.peer_slots = peer_slots->data_ptr<int64_t>();
   }
   g.status = status_ptr(status);

@@ -1054,6 +1054,23 @@ def test_linear_qkv_writes_the_8bit_arena(cuda_dev, t, norm):
         ops.core.check_status(cuda_dev)
 
 
+@pytest.mark.gpu
+def test_linear_qkv_refuses_a_peer_arena_of_other_heads(cuda_dev):
+    """(its rows would land in the next layer, or past the arena's end)"""
+    a = torch.zeros(3, 256, dtype=BF, device=cuda_dev)
+    w = torch.zeros(8 * 128, 256, dtype=BF, device=cuda_dev)
+    q = torch.empty(3, 512, dtype=BF, device=cuda_dev)
+    pos, slots = torch.zeros(3, dtype=torch.int32, device=cuda_dev), torch.arange(3, device=cuda_dev)
+    cs = ref.rope_cache(16, 10000.0, device=cuda_dev)
+    arena = ops.kv8_arena(1, 1, 2, device=cuda_dev)
+    for peer, at in ((ops.kv8_arena(1, 1, 1, device=cuda_dev), slots), (ops.kv8_arena(1, 1, 4, device=cuda_dev), slots),
+                     (ops.kv8_arena(1, 1, 2, device=cuda_dev), slots[:2]), (arena, slots.int())):
+        with pytest.raises(RuntimeError):
+            ops.linear_qkv(a, w, q, cs, pos, slots, arena, 0, 4, 2, peer, at)
+    ops.linear_qkv(a, w, q, cs, pos, slots, arena, 0, 4, 2, ops.kv8_arena(1, 1, 2, device=cuda_dev), slots)
+    ops.core.check_status(cuda_dev)
+
+
 def _engine(device, model, **kw):
     from lake_b200.engine.llm_engine import LLMEngine
 
