@@ -315,7 +315,7 @@ __device__ __forceinline__ Item get_item(const Kv8AttnArgs& a, int s, int64_t wo
   } else {
     it.seq = it.row0 = s, it.nq = 1;
   }
-  it.len = max(0, min(a.seq_lens[it.seq], a.max_blocks * kKv8Page));
+  it.len = kv8_seq_len(a, it.seq);
   if (!a.tiles) it.pos0 = it.len - 1;
   const int G = a.n_q_heads / a.n_kv_heads;
   it.groups = (it.nq * G + 8 * NT - 1) / (8 * NT);

@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int heads = uniform(pk.pack > 1 ? (nq > row_a + pk.rows ? 2 : 1) : min(a.products, G - a.products * unit));
   const int kvh = at / pk.units;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int len = min(a.seq_lens[seq], a.max_blocks * kKv8Page);
+  const int len = kv8_seq_len(a, seq);
   const int max_pos = min(pos0 + nq - 1, len - 1);
   const int n_steps = uniform(max_pos < 0 ? 0 : max_pos / kStep + 1);
   const int n_tiles = (n_steps + 1) / 2;

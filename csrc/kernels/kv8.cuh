@@ -52,6 +52,13 @@ __device__ __forceinline__ bool kv8_tile_ok(const Kv8AttnArgs& a, const int4& t)
   return ok;
 }
 
+// A sequence's length in the pages that its block table holds; one past them, or negative, is reported and cut off.
+__device__ __forceinline__ int kv8_seq_len(const Kv8AttnArgs& a, int seq) {
+  const int len = a.seq_lens[seq], most = a.max_blocks * kKv8Page;
+  if (len < 0 || len > most) record_error(a.status, kErrBounds);
+  return max(0, min(len, most));
+}
+
 // kv8_prefill: how the 128 rows of a CTA's two products are filled from a tile's query rows and the G query heads
 // of a KV head: with `pack` heads of a row side by side, pack the largest power of two in G, so that a
 // tile of few rows fills them too and a CTA's keys end close behind its rows. The two products then

@@ -176,7 +176,9 @@ def paged_decode_attention(q: torch.Tensor, arena: torch.Tensor, layer: int, blo
     """One query row per sequence; row s attends to keys [0, seq_lens[s]) (none: a row of zeros).
 
     With an 8-bit arena (ops.kv8_arena) the sequences' pages are cut over the whole GPU by their
-    lengths, so `splits`, `ws_o` and `ws_ml` have no effect there."""
+    lengths, so `splits`, `ws_o` and `ws_ml` have no effect there. A length that is negative or past
+    what its block table holds is reported in the status word there, and the keys that the table holds
+    are attended to."""
     if q.is_cuda and ref.is_kv8(arena):
         LAUNCHES[0] += 2 if block_tables.shape[1] > KV8_WHOLE_PAGES else 1
         return native().kv8_decode(q, out, arena, layer, block_tables, seq_lens, n_q_heads, n_kv_heads, scale,
@@ -227,7 +229,7 @@ def paged_prefill_attention(q: torch.Tensor, arena: torch.Tensor, layer: int, bl
                             positions: torch.Tensor, n_q_heads: int, n_kv_heads: int, scale: float,
                             out: torch.Tensor | None = None, tensor_core: bool = True) -> torch.Tensor:
     """Causal attention of packed query rows against each sequence's paged context (bf16 arena, or
-    the 8-bit one of ops.kv8_arena).
+    the 8-bit one of ops.kv8_arena, which reports lengths as paged_decode_attention does).
 
     tensor_core=True runs the tcgen05 kernel (tiles of up to PREFILL_TILE rows);
     False runs the warp-MMA kernel (tiles of up to 64 rows)."""

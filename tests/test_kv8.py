@@ -806,6 +806,41 @@ def test_a_step_of_no_sequences(cuda_dev, maxb, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [304, 1600])  # whole segments, and segments that may be cut
+@pytest.mark.parametrize("new", [[1, 1], [5, 2], [140, 130], [300, 20]])  # decode, few rows, many, both
+def test_lengths_past_the_block_table_are_reported(cuda_dev, new, n):
+    """What the table holds is attended to, the other sequence is as ever, and the caller hears of it."""
+    g = torch.Generator().manual_seed(25)
+    hq, hkv = 8, 2
+    arena, bt, cached = build([n, 150], hq, hkv, 1, 0, g, cuda_dev)
+    cap = bt.shape[1] * PAGE
+    assert cap == n
+    q = torch.randn(sum(new), hq * 128, generator=g).to(BF).to(cuda_dev)
+    tiles = ops.build_prefill_tiles([0, new[0], sum(new)], [n - new[0], 150 - new[1]], device=cuda_dev)
+
+    def call(lens):
+        sl = torch.tensor(lens, dtype=torch.int32, device=cuda_dev)
+        if new == [1, 1]:
+            return ops.paged_decode_attention(q, arena, 0, bt, sl, hq, hkv, 0.1)
+        return ops.paged_prefill_attention(q, arena, 0, bt, sl, tiles, None, None, hq, hkv, 0.1)
+
+    good = call([cap, 150])
+    ops.core.check_status(cuda_dev)
+    check_rows(good, q, cached, [n, 150], new, hkv, 0.1)
+    for bad in (cap + 1, 2 ** 31 - 1):
+        out = call([bad, 150])
+        with pytest.raises(ops.core.KernelError, match="out of bounds"):
+            ops.core.check_status(cuda_dev)
+        assert torch.equal(out, good)
+    for bad in (-1, -2 ** 31):
+        out = call([cap, bad])
+        with pytest.raises(ops.core.KernelError, match="out of bounds"):
+            ops.core.check_status(cuda_dev)
+        assert not out[new[0]:].any() and torch.equal(out[:new[0]], call([cap, 0])[:new[0]])
+        ops.core.check_status(cuda_dev)
+
+
+@pytest.mark.gpu
 def test_calls_that_are_refused_for_their_size_or_memory(cuda_dev):
     arena = ops.kv8_arena(1, 1, 1, device=cuda_dev)
     sl = torch.ones(1, dtype=torch.int32, device=cuda_dev)
