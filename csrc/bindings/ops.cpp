@@ -670,6 +670,9 @@ at::Tensor attn_out(const at::Tensor& q, const c10::optional<at::Tensor>& out, i
   return at::empty({q.size(0), n_q_heads * 128}, q.options());
 }
 
+// Kernels of this thread's last kv8_decode or kv8_prefill, for the caller's launch count.
+thread_local int g_kv8_launches = 0;
+
 // Workspace (this call's own, so calls on several streams and captured graphs share none) and launch.
 void kv8_few_rows(lakeb::Kv8AttnArgs& p, const at::Tensor& q) {
   if ((p.tiles ? p.num_tiles : p.num_seqs) == 0) return;
@@ -680,11 +683,13 @@ void kv8_few_rows(lakeb::Kv8AttnArgs& p, const at::Tensor& q) {
     p.ws_ml = p.ws_o + n / 132 * 128;
   }
   LAKEB_CHECK_RC(lakeb::kv8_attention(p, cur_stream()), "kv8_attention");
+  g_kv8_launches += lakeb::kv8_attention_launches(p);
 }
 
 at::Tensor kv8_decode(const at::Tensor& q, c10::optional<at::Tensor> out_arg, const at::Tensor& arena, int64_t layer,
                       const at::Tensor& block_tables, const at::Tensor& seq_lens, int64_t n_q_heads,
                       int64_t n_kv_heads, double scale, c10::optional<at::Tensor> status) {
+  g_kv8_launches = 0;
   at::Tensor out = attn_out(q, out_arg, n_q_heads);
   lakeb::Kv8AttnArgs p =
       kv8_attn_args(q, out, arena, layer, block_tables, seq_lens, n_q_heads, n_kv_heads, scale, status);
@@ -696,11 +701,11 @@ at::Tensor kv8_decode(const at::Tensor& q, c10::optional<at::Tensor> out_arg, co
 }
 
 constexpr int kFewRows = 32;
-constexpr int kFewPages = 64;
 
 at::Tensor kv8_prefill(const at::Tensor& q, c10::optional<at::Tensor> out_arg, const at::Tensor& arena, int64_t layer,
                        const at::Tensor& block_tables, const at::Tensor& seq_lens, const at::Tensor& tiles,
                        int64_t n_q_heads, int64_t n_kv_heads, double scale, c10::optional<at::Tensor> status) {
+  g_kv8_launches = 0;
   at::Tensor out = attn_out(q, out_arg, n_q_heads);
   lakeb::Kv8AttnArgs p =
       kv8_attn_args(q, out, arena, layer, block_tables, seq_lens, n_q_heads, n_kv_heads, scale, status);
@@ -724,12 +729,13 @@ at::Tensor kv8_prefill(const at::Tensor& q, c10::optional<at::Tensor> out_arg, c
     p.sms = lakeb::num_sms();
     // (two products of every tile and KV head in (G + 1) / 2 CTAs; see kv8_packing)
     if (p.num_tiles * n_kv_heads * ((n_q_heads / n_kv_heads + 1) / 2) * 2 <= p.sms) p.products = 1;
-    if (p.num_seqs > 1 && p.max_blocks > kFewPages &&
+    if (p.num_seqs > 1 && p.max_blocks > lakeb::kKv8WholePages &&
         p.num_rows + lakeb::kKv8TileRows - kFewRows <= lakeb::kKv8TileRows * int64_t(p.num_tiles)) {
       p.few_rows = kFewRows;
       kv8_few_rows(p, q);
     }
     LAKEB_CHECK_RC(lakeb::kv8_prefill_tc(p, cur_stream()), "kv8_prefill");
+    ++g_kv8_launches;
   }
   return out;
 }
@@ -1061,6 +1067,7 @@ PYBIND11_MODULE(LAKEB_MODULE, m) {
   m.def("kv8_prefill", &kv8_prefill, py::arg("q"), py::arg("out"), py::arg("arena"), py::arg("layer"),
         py::arg("block_tables"), py::arg("seq_lens"), py::arg("tiles"), py::arg("n_q_heads"), py::arg("n_kv_heads"),
         py::arg("scale"), py::arg("status") = py::none());
+  m.def("kv8_launches", [] { return g_kv8_launches; });
   m.def("step_tables", &step_tables, py::arg("pages"), py::arg("rows"), py::arg("context_lens"), py::arg("new_lens"),
         py::arg("max_tokens"), py::arg("max_tiles"), py::arg("n_decode"), py::arg("block_size"), py::arg("tile"),
         py::arg("status") = py::none());

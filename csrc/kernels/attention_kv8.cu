@@ -23,7 +23,7 @@
 // CTA's run goes straight to the output; a CTA has at most two pieces of segments (its first and its
 // last) that go to the workspace, and a second kernel joins them in the order of the CTAs, so results
 // do not depend on timing. A few segments of few pages are not cut (four sequences of 200 tokens: 7.1 us
-// instead of 12.5), and when no block table is wider than kWholePages, none is and there is no second
+// instead of 12.5), and when no block table is wider than kKv8WholePages, none is and there is no second
 // kernel (5.7 us).
 //
 // In a CTA one warp copies pages into a ring (bulk copies of 4128 bytes, page ids fetched 32 at a
@@ -48,7 +48,6 @@
 namespace lakeb {
 namespace {
 
-constexpr int kWholePages = 64;
 constexpr int kApartPages = 48;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.f;  // a base trails the true maximum by at most this
@@ -747,7 +746,7 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(const Kv8AttnArgs a) {
 }
 
 // Whether a CTA takes whole segments: few pages.
-bool takes_whole(const Kv8AttnArgs& a) { return a.max_blocks <= kWholePages; }
+bool takes_whole(const Kv8AttnArgs& a) { return a.max_blocks <= kKv8WholePages; }
 
 template <int NT, bool kMixed>
 int launch(const Kv8AttnArgs& a, cudaStream_t stream) {
@@ -771,6 +770,10 @@ int launch(const Kv8AttnArgs& a, cudaStream_t stream) {
 int64_t kv8_attention_ws_floats(const Kv8AttnArgs& a) {
   const int nt = kv8_attention_groups(a);
   return takes_whole(a) ? 0 : int64_t(2) * (nt == 1 ? 2 : 1) * num_sms() * 8 * nt * (kKv8Dim + 4);
+}
+
+int kv8_attention_launches(const Kv8AttnArgs& a) {
+  return (a.tiles ? a.num_tiles : a.num_seqs) <= 0 ? 0 : takes_whole(a) ? 1 : 2;
 }
 
 // Groups of 8 columns that a CTA holds at once, by the columns of a tile on average: a pass over the

@@ -244,11 +244,15 @@ struct Kv8AttnArgs {
   int* status = nullptr;
 };
 constexpr int kKv8TileRows = 128;  // of a query tile at most
+// Block tables up to this width: segments are never cut between CTAs (no second kernel), and no launch
+// shares its tiles between kv8_attention and kv8_prefill_tc.
+constexpr int kKv8WholePages = 64;
 // Few query rows per sequence (any number is right; large tiles belong to kv8_prefill_tc). -1 where
 // the pages of 32 items times their KV heads and column groups could pass 32 bits.
 int kv8_attention(const Kv8AttnArgs& a, cudaStream_t stream);
 int kv8_attention_groups(const Kv8AttnArgs& a);
 int64_t kv8_attention_ws_floats(const Kv8AttnArgs& a);
+int kv8_attention_launches(const Kv8AttnArgs& a);
 // Query tiles of <= 128 rows on the tcgen05 tensor cores.
 int kv8_prefill_tc(const Kv8AttnArgs& a, cudaStream_t stream);
 

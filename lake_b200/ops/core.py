@@ -180,9 +180,10 @@ def paged_decode_attention(q: torch.Tensor, arena: torch.Tensor, layer: int, blo
     what its block table holds is reported in the status word there, and the keys that the table holds
     are attended to."""
     if q.is_cuda and ref.is_kv8(arena):
-        LAUNCHES[0] += 2 if block_tables.shape[1] > KV8_WHOLE_PAGES else 1
-        return native().kv8_decode(q, out, arena, layer, block_tables, seq_lens, n_q_heads, n_kv_heads, scale,
-                                   status_word(q.device))
+        out = native().kv8_decode(q, out, arena, layer, block_tables, seq_lens, n_q_heads, n_kv_heads, scale,
+                                  status_word(q.device))
+        LAUNCHES[0] += native().kv8_launches()
+        return out
     n = seq_lens.shape[0]
     if out is None:
         out = torch.empty(q.shape[0], n_q_heads * ref.arena_head_dim(arena), dtype=q.dtype, device=q.device)
@@ -204,7 +205,6 @@ def paged_decode_attention(q: torch.Tensor, arena: torch.Tensor, layer: int, blo
     return out
 
 
-KV8_WHOLE_PAGES = 64  # block tables up to this width: 8-bit decode attention is one launch, else two
 PREFILL_TILE = 128  # query rows per tile of the tensor-core prefill kernel
 
 
@@ -234,9 +234,10 @@ def paged_prefill_attention(q: torch.Tensor, arena: torch.Tensor, layer: int, bl
     tensor_core=True runs the tcgen05 kernel (tiles of up to PREFILL_TILE rows);
     False runs the warp-MMA kernel (tiles of up to 64 rows)."""
     if q.is_cuda and ref.is_kv8(arena):
-        LAUNCHES[0] += 1
-        return native().kv8_prefill(q, out, arena, layer, block_tables, seq_lens, tiles, n_q_heads, n_kv_heads, scale,
-                                    status_word(q.device))
+        out = native().kv8_prefill(q, out, arena, layer, block_tables, seq_lens, tiles, n_q_heads, n_kv_heads, scale,
+                                   status_word(q.device))
+        LAUNCHES[0] += native().kv8_launches()
+        return out
     if out is None:
         out = torch.empty(q.shape[0], n_q_heads * ref.arena_head_dim(arena), dtype=q.dtype, device=q.device)
     if q.is_cuda:

@@ -47,7 +47,7 @@ def kv8_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, arena: torc
     skipped."""
     if arena.is_cuda:
         native().kv8_write(k, v, slots, arena, layer, core.status_word(arena.device))
-        core.LAUNCHES[0] += 1
+        core.LAUNCHES[0] += slots.numel() > 0
         return
     d = ref.arena_head_dim(arena)
     h = arena.shape[2]
@@ -59,8 +59,9 @@ def kv8_read(arena: torch.Tensor, layer: int, slots: torch.Tensor, k_out: torch.
     """The cached K and V of `slots` (int64 [T]) as dense bf16 rows [T, kv_heads * head_dim]; a
     negative slot gives a row of zeros (so does one past the arena, which is reported)."""
     if arena.is_cuda:
-        core.LAUNCHES[0] += 1
-        return native().kv8_read(arena, layer, slots, k_out, v_out, core.status_word(arena.device))
+        got = native().kv8_read(arena, layer, slots, k_out, v_out, core.status_word(arena.device))
+        core.LAUNCHES[0] += slots.numel() > 0
+        return got
     shape = (slots.shape[0], arena.shape[2] * ref.arena_head_dim(arena))
     if k_out is None:
         k_out = torch.empty(shape, dtype=torch.bfloat16)

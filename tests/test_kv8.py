@@ -1011,6 +1011,52 @@ def test_attention_right_behind_its_writers(cuda_dev, lens, new, hq, hkv, graph)
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("cols", [0, 100])  # block tables of few pages and of many
+def test_launches_are_counted(cuda_dev, cols):
+    """The count that the benchmarks report grows by the kernels that a call really launches (those in its graph)."""
+    rt = pytest.importorskip("cuda.bindings.runtime")
+    g = torch.Generator().manual_seed(26)
+    lens = [300, 900, 40]
+    arena, bt, _ = build(lens, 8, 2, 1, 0, g, cuda_dev, extra_cols=cols)
+    sl = torch.tensor(lens, dtype=torch.int32, device=cuda_dev)
+    q = torch.randn(700, 1024, generator=g).to(BF).to(cuda_dev)
+    rows = torch.randn(5, 256, generator=g).to(BF).to(cuda_dev)
+    slots, at = torch.arange(5, device=cuda_dev), torch.arange(3, dtype=torch.int32, device=cuda_dev)
+    zero, out = torch.zeros_like(at), torch.empty_like(q)
+
+    def prefill(new):
+        starts = [sum(new[:i]) for i in range(4)]
+        tiles = ops.build_prefill_tiles(starts, [a - b for a, b in zip(lens, new)], device=cuda_dev)
+        return lambda: ops.paged_prefill_attention(q[:starts[-1]], arena, 0, bt, sl, tiles, None, None, 8, 2, 0.1, out=out)
+
+    calls = [prefill(x) for x in ([5, 3, 1], [20, 640, 30], [300, 300, 40], [0, 0, 0])]
+    calls += [lambda: ops.paged_decode_attention(q[:3], arena, 0, bt, sl, 8, 2, 0.1, out=out),
+              lambda: ops.paged_decode_attention(q[:0], arena, 0, bt, sl[:0], 8, 2, 0.1, out=out),
+              lambda: ops.kv8_write(rows, rows, slots, arena, 0),
+              lambda: ops.kv8_write(rows[:0], rows[:0], slots[:0], arena, 0), lambda: ops.kv8_read(arena, 0, slots),
+              lambda: ops.kv8_read(arena, 0, slots[:0]),
+              lambda: ops.build_step_tables(bt, at, zero, sl, 2000, 32)]
+    counts = []
+    for call in calls:
+        call()  # (what a first call sets up is none of its launches)
+        graph = torch.cuda.CUDAGraph(keep_graph=True)
+        with torch.cuda.graph(graph):
+            before = ops.core.LAUNCHES[0]
+            call()
+            counted = ops.core.LAUNCHES[0] - before
+        raw = rt.cudaGraph_t(graph.raw_cuda_graph())
+        err, _, n = rt.cudaGraphGetNodes(raw)
+        assert int(err) == 0
+        err, nodes, n = rt.cudaGraphGetNodes(raw, n) if n else (0, [], 0)
+        kinds = [rt.cudaGraphNodeGetType(x)[1] for x in nodes[:n]]
+        launched = sum(k == rt.cudaGraphNodeType.cudaGraphNodeTypeKernel for k in kinds)
+        counts.append((counted, launched))
+    assert all(a == b for a, b in counts), counts
+    assert max(b for _, b in counts) == (3 if cols else 1)
+    ops.core.check_status(cuda_dev)
+
+
+@pytest.mark.gpu
 def test_offsets_past_32_bits(cuda_dev):
     """Pages beyond 4 GiB of the arena are written, read and attended to."""
     blocks = (1 << 32) // (4128 * 2) + 64
