@@ -618,6 +618,18 @@ std::tuple<at::Tensor, at::Tensor> kv8_read(const at::Tensor& arena, int64_t lay
   return {k, v};
 }
 
+// Whether rows of a and b may share memory (2-D, unit inner stride): side by side in one buffer they do not.
+bool rows_overlap(const at::Tensor& a, const at::Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  const int64_t w = a.element_size(), sa = a.size(0) > 1 ? a.stride(0) : b.stride(0), sb = b.size(0) > 1 ? b.stride(0) : sa;
+  const int64_t a0 = reinterpret_cast<int64_t>(a.data_ptr()) / w, b0 = reinterpret_cast<int64_t>(b.data_ptr()) / w;
+  const int64_t a1 = a0 + (a.size(0) - 1) * a.stride(0) + a.size(1), b1 = b0 + (b.size(0) - 1) * b.stride(0) + b.size(1);
+  if (a1 <= b0 || b1 <= a0) return false;
+  if (sa != sb || sa <= 0) return true;
+  const int64_t d = ((b0 - a0) % sa + sa) % sa;  // b's first column, from a's
+  return d < a.size(1) || sa - d < b.size(1);
+}
+
 lakeb::Kv8AttnArgs kv8_attn_args(const at::Tensor& q, const at::Tensor& out, const at::Tensor& arena, int64_t layer,
                                  const at::Tensor& block_tables, const at::Tensor& seq_lens, int64_t n_q_heads,
                                  int64_t n_kv_heads, double scale, const c10::optional<at::Tensor>& status) {
@@ -641,6 +653,8 @@ lakeb::Kv8AttnArgs kv8_attn_args(const at::Tensor& q, const at::Tensor& out, con
   // (a row's largest score is found before the scores are scaled)
   TORCH_CHECK(std::isfinite(static_cast<float>(scale)) && scale >= 0, "scale must be finite and not negative, got ", scale);
   TORCH_CHECK(q.numel() == 0 || out.data_ptr() != q.data_ptr(), "out must not be q");
+  TORCH_CHECK(!rows_overlap(q, out), "out must not share memory with q");
+  TORCH_CHECK(out.size(0) <= 1 || out.stride(0) >= out.size(1), "rows of out must not overlap");
   lakeb::Kv8AttnArgs p;
   p.q = bf(q);
   p.q_stride = q.stride(0);

@@ -866,6 +866,36 @@ def test_calls_that_are_refused_for_their_size_or_memory(cuda_dev):
 
 
 @pytest.mark.gpu
+def test_out_beside_q_but_not_over_it(cuda_dev):
+    """q and out in one buffer: side by side they are as good as apart, over each other they are refused."""
+    g = torch.Generator().manual_seed(27)
+    lens, hq, hkv = [40, 300, 7], 8, 2
+    arena, bt, cached = build(lens, hq, hkv, 1, 0, g, cuda_dev)
+    sl = torch.tensor(lens, dtype=torch.int32, device=cuda_dev)
+    w = hq * 128
+    buf = torch.randn(8, 2 * w, generator=g).to(BF).to(cuda_dev)
+    flat, keep = buf.view(-1), buf.clone()
+    tiles = ops.build_prefill_tiles([0, 1, 2, 3], [n - 1 for n in lens], device=cuda_dev)
+
+    def calls(q, out):
+        yield lambda: ops.paged_decode_attention(q, arena, 0, bt, sl, hq, hkv, 0.1, out=out)
+        yield lambda: ops.paged_prefill_attention(q, arena, 0, bt, sl, tiles, None, None, hq, hkv, 0.1, out=out)
+
+    q = buf[:3, :w]
+    for out in (buf[:3, w:], buf[3:6, :w], buf[4:7, w:], flat[7 * w:10 * w].view(3, w)):
+        for call in calls(q, out):
+            check_rows(call(), q, cached, lens, [1, 1, 1], hkv, 0.1)
+            buf.copy_(keep)
+    for out in (buf[1:4, :w], buf[2:5, :w], buf[:3, 8:8 + w], buf[:3, w - 8:2 * w - 8], flat[8:8 + 3 * w].view(3, w),
+                flat[w:4 * w].view(3, w), flat[:w].expand(3, w), flat[6 * w:7 * w].expand(3, w)):
+        for call in calls(q, out):
+            with pytest.raises(RuntimeError, match="out must not|must not overlap"):
+                call()
+    assert torch.equal(buf, keep)
+    ops.core.check_status(cuda_dev)
+
+
+@pytest.mark.gpu
 def test_decode_more_sequences_than_a_grid_axis(cuda_dev):
     n = 70_000
     g = torch.Generator().manual_seed(15)
