@@ -636,6 +636,7 @@ lakeb::Kv8AttnArgs kv8_attn_args(const at::Tensor& q, const at::Tensor& out, con
   check_bf16_2d(q, "q");
   check_bf16_2d(out, "out");
   check_kv8_arena(arena, layer, n_kv_heads);
+  TORCH_CHECK(arena.size(0) > 0, "an arena of no pages");  // (a page id outside the arena is read as page 0)
   TORCH_CHECK(n_kv_heads > 0 && n_q_heads > 0 && n_q_heads % n_kv_heads == 0, "q heads (", n_q_heads, ") must be a multiple of kv heads (",
               n_kv_heads, ")");
   TORCH_CHECK(q.size(1) == n_q_heads * 128 && out.size(1) == n_q_heads * 128 && out.size(0) >= q.size(0),

@@ -896,6 +896,41 @@ def test_out_beside_q_but_not_over_it(cuda_dev):
 
 
 @pytest.mark.gpu
+def test_an_arena_of_no_pages(cuda_dev):
+    """Attention refuses it (there is no page to read in place of one that is not there); rows are reported."""
+    arena = ops.kv8_arena(0, 1, 1, device=cuda_dev)
+    i32 = dict(dtype=torch.int32, device=cuda_dev)
+    q, bt, sl = torch.zeros(1, 128, dtype=BF, device=cuda_dev), torch.zeros(1, 2, **i32), torch.ones(1, **i32)
+    with pytest.raises(RuntimeError, match="no pages"):
+        ops.paged_decode_attention(q, arena, 0, bt, sl, 1, 1, 0.1)
+    with pytest.raises(RuntimeError, match="no pages"):
+        ops.paged_prefill_attention(q, arena, 0, bt, sl, torch.tensor([[0, 0, 1, 0]], **i32), None, None, 1, 1, 0.1)
+    ops.core.check_status(cuda_dev)
+    at = torch.zeros(1, dtype=torch.int64, device=cuda_dev)
+    for call in (lambda: ops.kv8_write(q, q, at, arena, 0), lambda: ops.kv8_read(arena, 0, at)):
+        call()
+        with pytest.raises(ops.core.KernelError, match="out of bounds"):
+            ops.core.check_status(cuda_dev)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [3, 200])  # both kernels
+def test_one_query_row_broadcast_to_all(cuda_dev, rows):
+    """q may be a view whose rows are one row."""
+    g = torch.Generator().manual_seed(28)
+    arena, bt, cached = build([250], 8, 2, 1, 0, g, cuda_dev)
+    q = torch.randn(1, 1024, generator=g).to(BF).to(cuda_dev).expand(rows, -1)
+    sl = torch.tensor([250], dtype=torch.int32, device=cuda_dev)
+    tiles = ops.build_prefill_tiles([0, rows], [250 - rows], device=cuda_dev)
+    out = ops.paged_prefill_attention(q, arena, 0, bt, sl, tiles, None, None, 8, 2, 0.1)
+    check_rows(out, q, cached, [250], [rows], 2, 0.1)
+    out = ops.paged_decode_attention(q[:3], arena, 0, bt.expand(3, -1), sl.expand(3).contiguous(), 8, 2, 0.1)
+    for i in range(3):
+        check_rows(out[i:i + 1], q[:1], cached, [250], [1], 2, 0.1)
+    ops.core.check_status(cuda_dev)
+
+
+@pytest.mark.gpu
 def test_decode_more_sequences_than_a_grid_axis(cuda_dev):
     n = 70_000
     g = torch.Generator().manual_seed(15)
