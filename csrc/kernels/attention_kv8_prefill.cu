@@ -11,8 +11,8 @@
 // two O) softmax and tensor cores take turns, and 128 keys of both took 5.1k cycles; so they take
 // 4.4k, of which the products run 2.6k and the exponentials 2.0k. What binds is shared
 // memory (products' operands, conversion and copies move ~390 KB per tile, 3.0k cycles) and the
-// hand-offs that wait behind it. Measured: one 8192-token prompt of 32 query and 8 KV heads 0.57 ms,
-// 960 TFLOP/s; four of 2048 tokens 0.21 ms, 645 TFLOP/s. A CTA spends ~7 us around its main loop
+// hand-offs that wait behind it. Measured, single calls: one 8192-token prompt of 32 query and 8 KV heads
+// 0.57 to 0.64 ms by its data, 860 to 960 TFLOP/s; four of 2048 tokens 0.21 ms, 660 TFLOP/s. A CTA spends ~7 us around its main loop
 // (1.9 us until its queries arrive, 1.6 to convert them, about as long for the output, the rest start
 // and end), so eight prompts of 500 tokens, four tiles of keys a CTA at most, run at 255 TFLOP/s. CTAs
 // that stay and take tile after tile overlapped little of that and issued products more slowly (1152
@@ -31,12 +31,13 @@
 // its P are up to 2^8 smaller for it, of the 2^21 between P's base and fp16's subnormals.) A tile of a wider
 // range keeps its codes as they are, and each key's scale enters its own scores and exponents, as in
 // kv8_attention: then what a row does not see has no part in it whatever it holds. Tokens' scales lie within a
-// few octaves of each other as a rule; a prompt of 8192 tokens whose every tile is wider takes 2.0 ms, 3.5 times as long.
+// few octaves of each other as a rule; a prompt of 8192 tokens whose every tile is wider takes 2.7 ms, 4.7 times as
+// long (its steps are a function of their own: within the loop they cost the others registers, 2 % of the time).
 //
 // Softmax statistics, for each row: z = score in log2 units, w = z + e (e of V, the key's or the tile's). bo
 // follows the largest w and m the largest z, lazily: O is kept against 2^(bo - 7), with P = 2^(w - bo + 7)
 // <= 2^15, and the sum l of 2^z against 2^m. Of a tile with one e, l gets the sum of P times 2^(bo - 7 - e - m);
-// where that factor is past 2^82, P may be below fp32's range and 2^(z - m) not: such a step takes the
+// where that factor is past 2^82, P may be below fp32's range and 2^(z - m) not: such a tile's steps take the
 // exponentials of both.
 //
 // Warps: 0 = loads, 1 = tensor memory and MMA issue, 2-3 idle, 4-7 = converters of K, 8-11 = of V,
@@ -66,7 +67,7 @@ constexpr int kBars = kRaw + 8 * kKv8Head;           // 229,632
 constexpr int kParams = kBars + 256;                 // [4] TileParams
 constexpr int kScales = kParams + 4 * 32;            // [4][K, V][128] scale bytes of the keys as they were converted
 constexpr int kRed = kScales + 4 * 2 * kTile;        // [2 tiles][K, V][4] converter warps' extremes and flags
-constexpr int kSmem = kRed + 2 * 2 * 4 * 16;
+constexpr int kSmem = kRed + 2 * 2 * 4 * 8;
 static_assert(kSmem <= 227 * 1024, "");
 constexpr int kThreads = 640;
 constexpr int kStep = 64;                            // keys per softmax step
@@ -183,6 +184,53 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const void* tmap, uint64_
           smem_u32(dst)),
       "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
       : "memory");
+}
+
+// A softmax step of 64 keys where each has scales of its own (kb: the keys' K scales, their V scales one kTile
+// behind; keys past `last` are not seen): P over S in tensor memory, the row's bases and l brought up to date,
+// the step's part of l added to `sum`.
+__device__ __noinline__ void slow_step(uint32_t t_s, const uint8_t* kb, const uint32_t* nan, float cr, int last, float& bo, float& m,
+                               float& l, float& sum) {
+  const uint8_t* vb = kb + kTile;
+  uint32_t x[32], p[32];
+  auto scores = [&](int q) {
+    tmem_ld32(t_s + 32 * q, x);
+    tmem_ld_wait();
+#pragma unroll
+    for (int k = 0; k < 32; ++k) {
+      float z = __uint_as_float(x[k]) * (cr * kv8_scale(kb[32 * q + k]));
+      if ((nan[q] >> k) & 1u) z = CUDART_NAN_F;
+      x[k] = __float_as_uint(32 * q + k > last ? -CUDART_INF_F : z);
+      if ((k & 3) == 3) asm volatile("" ::: "memory");  // (few scales at a time: they are registers)
+    }
+  };
+  float zt = -CUDART_INF_F, wt = -CUDART_INF_F;
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    scores(q);
+#pragma unroll
+    for (int k = 0; k < 32; ++k) {
+      zt = fmaxf(zt, __uint_as_float(x[k]));
+      wt = fmaxf(wt, __uint_as_float(x[k]) + static_cast<float>(vb[32 * q + k] - 127));
+      if ((k & 3) == 3) asm volatile("" ::: "memory");
+    }
+  }
+  if (wt > bo + kSlack) bo = wt;
+  if (zt > m + kSumSlack) l *= ex2(m - zt), m = zt;
+  const float zb = m == -CUDART_INF_F ? 0.f : m, wb = (bo == -CUDART_INF_F ? 0.f : bo - kPBias) + 127.f;
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    scores(q);
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const float z0 = __uint_as_float(x[2 * k]), z1 = __uint_as_float(x[2 * k + 1]);
+      const float e0 = static_cast<float>(vb[32 * q + 2 * k]), e1 = static_cast<float>(vb[32 * q + 2 * k + 1]);
+      sum += ex2(z0 - zb) + ex2(z1 - zb);
+      p[16 * q + k] = pack_f16x2(ex2(z0 + (e0 - wb)), ex2(z1 + (e1 - wb)));
+      if ((k & 3) == 3) asm volatile("" ::: "memory");
+    }
+  }
+  tmem_st32(t_s, p);
 }
 
 __global__ void __launch_bounds__(kThreads, 1)
@@ -422,20 +470,25 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     for (int j = 0; j < n_tiles; ++j) {
       const int s = j & 1;
-      int4* red = reinterpret_cast<int4*>(smem + kRed) + (s * 2 + kv) * 4;  // each warp's extremes, NaN keys
+      uint4* red = reinterpret_cast<uint4*>(smem + kRed) + (s * 2 + kv) * 2;  // each warp's extremes and NaN keys
       // tile j - 4's was read before PV(j - 4) and S(j - 3), which the waits of tile j - 1 waited for
       TileParams& p = params[j & 3];
       ok = ok && mbar_wait(&raw_full[kv], j & 1, abort_flag, a.status);
       const bool real = ok && j * kTile + row < len;
       const int b = real ? side[kKv8Page * kKv8Dim + t] : 0;
       // rows of NaNs (255) and of zeros (the smallest scale, as rows that are not zeros may have) say nothing
-      const bool counts = b > 0 && b < 255 && (b > 1 || any_code(side, t));
-      const int top = __reduce_max_sync(0xffffffffu, counts ? b : 0), low = __reduce_min_sync(0xffffffffu, counts ? b : 255);
-      const uint32_t nan = __ballot_sync(0xffffffffu, b == 255);
-      if (lane == 0) red[warp & 3] = make_int4(top, low, static_cast<int>(nan), 0);
+      bool counts = true;
+      uint32_t nan = 0;
+      if (__any_sync(0xffffffffu, b <= 1 || b == 255)) {
+        nan = __ballot_sync(0xffffffffu, b == 255);
+        counts = b > 0 && b < 255 && (b > 1 || any_code(side, t));
+      }
+      const uint32_t top = __reduce_max_sync(0xffffffffu, counts ? b : 0u), low = __reduce_max_sync(0xffffffffu, counts ? 255u - b : 0u);
+      if (lane == 0) reinterpret_cast<uint2*>(red)[warp & 3] = make_uint2(top << 16 | low, nan);
       asm volatile("bar.sync %0, 128;" ::"r"(1 + kv) : "memory");
-      const int hi = max(max(red[0].x, red[1].x), max(red[2].x, red[3].x));
-      const int lo = min(min(red[0].y, red[1].y), min(red[2].y, red[3].y));
+      const uint4 r0 = red[0], r1 = red[1];
+      const uint32_t both = __vmaxu2(__vmaxu2(r0.x, r0.z), __vmaxu2(r1.x, r1.z));
+      const int hi = both >> 16, lo = 255 - static_cast<int>(both & 0xffffu);
       const bool wide = hi - lo > (kv ? kSpanV : kSpanK);
       if (hi > 0) e = hi - 127;  // (a tile without any keeps the last one's)
       smem[kScales + ((j & 3) * 2 + kv) * kTile + row] = static_cast<uint8_t>(wide ? b : e + 127);
@@ -444,13 +497,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           p.ek = e;
           p.wide_k = wide;
         } else {
-          int any = 0;
           p.ev = e;
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            p.nan[w] = static_cast<uint32_t>(red[w].z);
-            any |= red[w].z;
-          }
+          p.nan[0] = r0.y, p.nan[1] = r0.w, p.nan[2] = r1.y, p.nan[3] = r1.w;
+          const uint32_t any = r0.y | r0.w | r1.y | r1.w;
           p.wide_v = (wide ? 1 : 0) | (any ? 2 : 0);
         }
       }
@@ -505,7 +554,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       float bo = -CUDART_INF_F;  // base of w, at most kSlack below the largest w so far
       float m = -CUDART_INF_F;   // base of l
       float l = 0.f, c = 0.f, ev = 0.f;
-      int flags = 0;  // of the tile: bit 0: by each key's own scales; bit 1: NaN keys
+      int flags = 0;     // of the tile: bit 0: a wide range of scales; bit 1: NaN keys
+      bool far = false;  // its steps are slow ones
       for (int i = 0; i < n_steps; ++i) {
         const int j = i >> 1, buf = i & 1;
         const TileParams& tp = params[j & 3];
@@ -517,43 +567,45 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         tc_fence_after();
         const uint32_t t_mine = t_s[h] + lane_off + kStep * buf;
-        uint32_t sv[64];
-        tmem_ld32(t_mine, *reinterpret_cast<uint32_t(*)[32]>(sv));
-        tmem_ld32(t_mine + 32, *reinterpret_cast<uint32_t(*)[32]>(sv + 32));
         if (buf == 0) {
           ev = static_cast<float>(tp.ev);
           flags = tp.wide_k | tp.wide_v;
+          // (a step leaves bo - ev - m as it is, or less, or at most kSumSlack: this holds for both of the tile)
+          far = __any_sync(0xffffffffu, (flags & 1) || bo - kPBias - ev - m > kSumFactor);
           // (not 0, where a row of zeros or small keys would make it that: masked scores are -infinity)
           c = fmaxf(cr * __uint_as_float(static_cast<uint32_t>(127 + tp.ek) << 23), 0x1p-126f);
         }
         const int k0 = i * kStep;
-        const bool nan = (flags & 2) != 0, wide = (flags & 1) != 0;
-        tmem_ld_wait();
-        if (k0 + kStep - 1 > kmax) {  // the diagonal or the sequence end: keys past this row's last
-#pragma unroll
-          for (int k = 0; k < 64; ++k)
-            if (k0 + k > kmax) sv[k] = __float_as_uint(-CUDART_INF_F);
-        }
-        if (nan) {
-#pragma unroll
-          for (int k = 0; k < 64; ++k)
-            if (((tp.nan[buf * 2 + (k >> 5)] >> (k & 31)) & 1u) && k0 + k <= kmax) sv[k] = 0x7fffffffu;
-        }
-        // row max: four independent three-input chains, then a short tree
-        float mv[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) mv[q] = max3f(__uint_as_float(sv[q]), __uint_as_float(sv[4 + q]), -CUDART_INF_F);
-#pragma unroll
-        for (int k = 8; k < 64; k += 8)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) mv[q] = max3f(mv[q], __uint_as_float(sv[k + q]), __uint_as_float(sv[k + 4 + q]));
-        const float zx = fmaxf(max3f(mv[0], mv[1], mv[2]), mv[3]) * c, mx = zx + ev;
         const float old = bo;
-        const float bn = mx > bo + kSlack ? mx : bo, mn = zx > m + kSumSlack ? zx : m;
-        const float up = bn == -CUDART_INF_F ? 0.f : bn - kPBias - ev - mn;
-        if (!__any_sync(0xffffffffu, wide || up > kSumFactor)) {
-          bo = bn;
-          if (mn > m) l *= ex2(m - mn), m = mn;
+        float sum = 0.f, power = 0.f;  // l gets 2^power sum
+        if (far) {
+          slow_step(t_mine, smem + kScales + (j & 3) * 2 * kTile + buf * kStep, tp.nan + buf * 2, cr, kmax - k0, bo, m, l, sum);
+        } else {
+          uint32_t sv[64];
+          tmem_ld32(t_mine, *reinterpret_cast<uint32_t(*)[32]>(sv));
+          tmem_ld32(t_mine + 32, *reinterpret_cast<uint32_t(*)[32]>(sv + 32));
+          const bool nan = (flags & 2) != 0;
+          tmem_ld_wait();
+          if (k0 + kStep - 1 > kmax) {  // the diagonal or the sequence end: keys past this row's last
+#pragma unroll
+            for (int k = 0; k < 64; ++k)
+              if (k0 + k > kmax) sv[k] = __float_as_uint(-CUDART_INF_F);
+          }
+          if (nan) {
+#pragma unroll
+            for (int k = 0; k < 64; ++k)
+              if (((tp.nan[buf * 2 + (k >> 5)] >> (k & 31)) & 1u) && k0 + k <= kmax) sv[k] = 0x7fffffffu;
+          }
+          // row max: four independent three-input chains, then a short tree
+          float mv[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) mv[q] = max3f(__uint_as_float(sv[q]), __uint_as_float(sv[4 + q]), -CUDART_INF_F);
+#pragma unroll
+          for (int k = 8; k < 64; k += 8)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) mv[q] = max3f(mv[q], __uint_as_float(sv[k + q]), __uint_as_float(sv[k + 4 + q]));
+          const float sx = fmaxf(max3f(mv[0], mv[1], mv[2]), mv[3]), mx = fmaf(sx, c, ev);
+          if (mx > bo + kSlack) bo = mx;
           const float add = bo == -CUDART_INF_F ? 0.f : ev - bo + kPBias;
           float2 rs[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
           const float2 cv = make_float2(c, c), av = make_float2(add, add);
@@ -564,35 +616,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             rs[k & 1] = add2(rs[k & 1], p);
             sv[k] = pack_f16x2(p.x, p.y);
           }
+          tmem_st32(t_mine, *reinterpret_cast<uint32_t(*)[32]>(sv));
           rs[0] = add2(rs[0], rs[1]);
-          l = fmaf(rs[0].x + rs[0].y, ex2(up), l);
-        } else {
-          // each key by its own scales (read a few at a time: all at once, they would push scores out of the registers)
-          const uint8_t* kb = smem + kScales + (j & 3) * 2 * kTile + buf * kStep;
-          const uint8_t* vb = kb + kTile;
-          float zt = -CUDART_INF_F, wt = -CUDART_INF_F;
-#pragma unroll
-          for (int k = 0; k < 64; ++k) {
-            const float x = __uint_as_float(sv[k]);  // (-infinity: not seen, and the factor may be 0)
-            const float z = x == -CUDART_INF_F ? x : x * (cr * kv8_scale(kb[k]));
-            if ((k & 7) == 7) asm volatile("" ::: "memory");
-            sv[k] = __float_as_uint(z);
-            zt = fmaxf(zt, z);
-            wt = fmaxf(wt, z + static_cast<float>(vb[k] - 127));
-          }
-          if (wt > bo + kSlack) bo = wt;
-          if (zt > m + kSumSlack) l *= ex2(m - zt), m = zt;
-          const float zb = m == -CUDART_INF_F ? 0.f : m, wb = (bo == -CUDART_INF_F ? 0.f : bo - kPBias) + 127.f;
-#pragma unroll
-          for (int k = 0; k < 32; ++k) {
-            if ((k & 3) == 0) asm volatile("" ::: "memory");
-            const float z0 = __uint_as_float(sv[2 * k]), z1 = __uint_as_float(sv[2 * k + 1]);
-            l += ex2(z0 - zb) + ex2(z1 - zb);
-            sv[k] = pack_f16x2(ex2(z0 + (static_cast<float>(vb[2 * k]) - wb)), ex2(z1 + (static_cast<float>(vb[2 * k + 1]) - wb)));
-          }
+          sum = rs[0].x + rs[0].y;
+          const float zx = sx * c;
+          if (zx > m + kSumSlack) l *= ex2(m - zx), m = zx;
+          power = bo == -CUDART_INF_F ? 0.f : -add - m;
         }
         const bool grow = bo > old;
-        tmem_st32(t_mine, *reinterpret_cast<uint32_t(*)[32]>(sv));
         // O still holds sums against the old base. tcgen05.ld/st are warp-collective: the whole
         // warp rescales when any of its rows needs it (rows that do not keep alpha = 1).
         if (__any_sync(0xffffffffu, grow && i > 0)) {
@@ -612,6 +643,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_st32(t_o[h] + lane_off + q * 32, ov);
           }
         }
+        l = fmaf(sum, ex2(power), l);
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(&p_full[2 * h + buf]);
