@@ -734,10 +734,13 @@ at::Tensor kv8_prefill(const at::Tensor& q, c10::optional<at::Tensor> out_arg, c
   const c10::cuda::CUDAGuard guard(arena.device());
   // A tile of few rows behind many keys takes less time as columns of the few-row kernel, which cuts its
   // pages evenly over the GPU (17 rows behind 6001 keys, 64 query and 8 KV heads: 43 us), than in a CTA per
-  // KV head of the tcgen05 one, which takes ~2 us per 128 keys. The host does not see the tiles' rows: where
-  // their sum leaves it open that some of several sequences are few (up to 32), both kernels run and find
-  // from the lengths which tiles are whose (kv8_tile_is_few); up to 64 pages the few-row kernel would gain
-  // less than its launches take (five chunks of 78 to 191 rows 13 us in one kernel, 22 in both).
+  // KV head of the tcgen05 one, which takes ~2 us per 128 keys. The host does not see the tiles' rows, and takes
+  // the rows of q for them: where their number leaves it open that some of several sequences are few (up to
+  // 32), both kernels run and find from the lengths which tiles are whose (kv8_tile_is_few); up to 64 pages
+  // the few-row kernel would gain less than its launches take (five chunks of 78 to 191 rows 13 us in one
+  // kernel, 22 in both). Either kernel is right for every tile, so this decides on time alone. Rows of q that
+  // no tile covers (a step's decode rows in front of its chunks) count as the chunks' and may keep a short
+  // chunk with the tcgen05 kernel, and the width of the table stands in for the sequences' pages.
   if (p.num_rows <= 8 * int64_t(p.num_tiles) || (p.num_seqs == 1 && p.num_rows <= kFewRows)) {
     kv8_few_rows(p, q);
   } else {

@@ -22,8 +22,8 @@
 // an equal run of them, whatever the lengths are (all CTAs resident). A segment that lies within one
 // CTA's run goes straight to the output; a CTA has at most two pieces of segments (its first and its
 // last) that go to the workspace, and a second kernel joins them in the order of the CTAs, so results
-// do not depend on timing. A few segments of few pages are not cut (four sequences of 200 tokens: 7.1 us
-// instead of 12.5), and when no block table is wider than kKv8WholePages, none is and there is no second
+// do not depend on timing. A few segments of few pages, of 256 items at most, are not cut (four sequences of
+// 200 tokens: 7.1 us instead of 12.5), and when no block table is wider than kKv8WholePages, none is and there is no second
 // kernel (5.7 us).
 //
 // In a CTA one warp copies pages into a ring (bulk copies of 4128 bytes, page ids fetched 32 at a
@@ -31,8 +31,8 @@
 // once, since a page alone is a chain of dependent products, exponentials and products of ~1400
 // cycles and two cost little more; with more columns the groups fill the chain's gaps.
 //
-// Measured, 32 query and 8 KV heads: 256 sequences of 2304 tokens 200 us, 6.25 TB/s of DRAM reads (0.95
-// of the copy rate): memory. One of 8192 tokens 17 us: start (4.5 us to the first page) and join (2 us of
+// Measured, 32 query and 8 KV heads: 256 sequences of 2304 tokens 200 us for the kernel alone, 6.25 TB/s of
+// DRAM reads (0.95 of the copy rate): memory; 220 us a call with cold caches. One of 8192 tokens 17 us: start (4.5 us to the first page) and join (2 us of
 // waiting, 4 of loads). 16 of 5 rows behind 300 to 2000 tokens 28.5 us: MMAs at 16 cycles, 48 a page for
 // three groups, in 11 us of steps, the rest start, sums of the warps and join.
 #include <algorithm>

@@ -87,7 +87,7 @@ __host__ __device__ __forceinline__ Kv8Packing kv8_packing(int G, int products) 
 // Measured, 64 query and 8 KV heads: chunks of 42 to 1500 rows take 106 us, with one of 17 rows behind 6001
 // keys 131 us in kv8_prefill, 144 in both; two of 32 rows behind 3000 keys 56 us in kv8_prefill, 72 in
 // kv8_attention.
-constexpr int kKv8Ranked = 256;  // tiles that are looked at
+constexpr int kKv8Ranked = 256;  // tiles that are looked at: in a call of more the rest count no work, and tiles run in their order
 constexpr int kKv8CtaCost = 3;
 __device__ __forceinline__ int kv8_tile_keys(const Kv8AttnArgs& a, const int4& t) {
   return max(0, min(min(t.w + t.z, a.seq_lens[t.x]), a.max_blocks * kKv8Page));

@@ -57,7 +57,8 @@ def kv8_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, arena: torc
 def kv8_read(arena: torch.Tensor, layer: int, slots: torch.Tensor, k_out: torch.Tensor | None = None,
              v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """The cached K and V of `slots` (int64 [T]) as dense bf16 rows [T, kv_heads * head_dim]; a
-    negative slot gives a row of zeros (so does one past the arena, which is reported)."""
+    negative slot gives a row of zeros (so does one past the arena, which is reported). On the GPU
+    outputs that are not given are views of one allocation."""
     if arena.is_cuda:
         got = native().kv8_read(arena, layer, slots, k_out, v_out, core.status_word(arena.device))
         core.LAUNCHES[0] += slots.numel() > 0

@@ -1,8 +1,9 @@
 """Tables of an engine step, built on the device from request lengths.
 
-The host keeps one row of page ids per request in a device table and appends to it when a
-request takes a page; a step then needs only which rows it runs and how many tokens each has
-and gets, not every sequence's whole block table again.
+For a caller that keeps one row of page ids per request in a device table, and appends to it when a
+request takes a page: a step then needs only which rows it runs and how many tokens each has
+and gets, not every sequence's whole block table again. (The engine's runner packs its tables on
+the host.)
 """
 from __future__ import annotations
 
@@ -36,7 +37,9 @@ def build_step_tables(pages: torch.Tensor, rows: torch.Tensor, context_lens: tor
     (nothing waits for the device), so a call can be captured into a graph and replayed with other
     lengths. More tokens or tiles than max_tokens / max_tiles, a negative length, a request row
     outside `pages`, or a token whose page is missing (negative, or past the row's end) is reported
-    (the status word on the GPU, ValueError on the CPU); on the GPU such a token gets slot -1."""
+    (the status word on the GPU, ValueError on the CPU); on the GPU such a token gets slot -1.
+
+    On the GPU the seven tables are views of one allocation: keeping one keeps all of them."""
     if pages.is_cuda:
         core.LAUNCHES[0] += 1
         return StepTables._make(native().step_tables(pages, rows, context_lens, new_lens, max_tokens, max_tiles, n_decode,
