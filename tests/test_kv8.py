@@ -696,6 +696,54 @@ def test_scales_over_the_whole_range(cuda_dev, rows, n, case):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv", [(8, 2), (3, 1)])
+def test_wide_and_narrow_tiles_in_turn(cuda_dev, hq, hkv):
+    """Long sequences whose tiles of keys change between far-apart and near scales, NaN rows among them: right, and
+    bit for bit the same when calls follow one another on two streams."""
+    g = torch.Generator().manual_seed(29)
+    n, rows, scale = 2900, 640, 0.09
+    arena, bt, _ = build([n], hq, hkv, 1, 0, g, cuda_dev)
+    j = torch.arange(n)
+    slots = bt[0].cpu().long()[j // PAGE] * PAGE + j % PAGE
+    k, v = torch.randn(n, hkv, 128, generator=g), torch.randn(n, hkv, 128, generator=g)
+    q = torch.randn(rows, hq, 128, generator=g)
+    wide = torch.rand(-(-n // 64), 2, generator=g) < 0.4  # of K, of V, by 64 keys
+    up = torch.exp2(torch.randint(-30, 1, (n, hkv, 2), generator=g).float())
+    up = torch.where(wide[j // 64][:, None, :], up, torch.ones_like(up))
+    k, v = (k * up[..., :1]).to(BF), (v * up[..., 1:]).to(BF)
+    at = n - rows + 77  # seen by the rows from here on
+    v[at, 0, 3] = float("nan")
+    q = q.to(BF)
+    ops.kv8_write(k.view(n, -1).to(cuda_dev), v.view(n, -1).to(cuda_dev), slots.to(cuda_dev), arena, 0)
+    sl = torch.tensor([n], dtype=torch.int32, device=cuda_dev)
+    tiles = ops.build_prefill_tiles([0, rows], [n - rows], device=cuda_dev)
+    qd = q.view(rows, -1).to(cuda_dev)
+    call = lambda: ops.paged_prefill_attention(qd, arena, 0, bt, sl, tiles, None, None, hq, hkv, scale)  # noqa: E731
+    out = call()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    more = []
+    for i in range(16):
+        with torch.cuda.stream(streams[i % 2]):
+            more.append(call())
+    torch.cuda.synchronize()
+    ops.core.check_status(cuda_dev)
+    bits = out.view(torch.int16)
+    assert all(torch.equal(x.view(torch.int16), bits) for x in more)
+    out = out.view(rows, hq, 128)
+    g0 = hq // hkv  # heads of KV head 0
+    assert bool(torch.isnan(out[77:, :g0]).all()) and bool(torch.isfinite(out[:77].float()).all())
+    pick = torch.cat([torch.arange(0, 77, 5), torch.arange(77, rows, 23)])
+    v64 = quantize64(v).nan_to_num(nan=0.0)
+    lim = torch.arange(n - rows + 1, n + 1)
+    args = q.double().to(cuda_dev), quantize64(k).to(cuda_dev), v64.to(cuda_dev)
+    before = pick[pick < 77]
+    check_contributions(out[before], args[0][before], *args[1:], lim[before], scale)
+    if hkv > 1:  # the NaN is KV head 0's alone
+        check_contributions(out[pick][:, g0:], args[0][pick][:, g0:], args[1][:, 1:], args[2][:, 1:], lim[pick], scale)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows", [3, 150])  # both kernels
 def test_scores_too_small_for_their_factor(cuda_dev, rows):
     """Queries of zeros beside keys near fp32's smallest, and a scale of 0: every seen key weighs the same."""
